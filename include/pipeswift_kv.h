@@ -2,7 +2,7 @@
  * pipeswift_kv.h -- C ABI of the MI355X (gfx950) paged KV-cache data path.
  *
  * One shared library, libpipeswift_kv.so, built with hipcc for gfx950 from
- * pipeswift_amd/csrc/{pipeswift_kv,paged_attention,mla_fp8_tiles}.hip.  Every
+ * the .hip files of pipeswift_amd/csrc.  Every
  * entry point takes plain device
  * pointers, element or byte strides and sizes, a dtype code and a HIP stream
  * handle (hipStream_t passed as void*; NULL is the legacy default stream).
@@ -413,6 +413,107 @@ int psk_paged_prefill_attention(const void* q, int64_t q_tok_stride, int64_t q_h
 int64_t psk_paged_prefill_workspace_len(int64_t num_seqs);
 int64_t psk_paged_prefill_step_workspace_len(int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q,
                                              int64_t num_q_heads, int64_t num_kv_heads, int64_t max_seqlen_k);
+
+/*
+ * Attention of drafted trees over the paged FP8 cache (build-defined; the
+ * reference's speculative decode is causal).  Arguments, q~, s_j, out, lse,
+ * descales, page addressing and zero rows for missing pages as
+ * psk_paged_decode_attention, for any number of query tokens and query heads;
+ * the ragged layout as psk_paged_prefill_attention's (rows of q and out past
+ * total_q are never touched, whatever cu_seqlens_q holds).  The n_b query tokens
+ * of sequence b are the last n_b of its seq_lens[b] cached tokens; query token i
+ * sees key j < seq_lens[b] - n_b, and key seq_lens[b] - n_b + t, t < n_b, where
+ * bit t % 64 of tree_mask[(c_b + i) * tree_mask_stride + t / 64] is set.
+ * tree_mask_words words of 64 tokens each hold max_seqlen_q tokens at least.  A
+ * token that sees no key writes zeros and lse = -inf.  max_seq_len, a bound on
+ * seq_lens, only sizes the launch.  out rows need 4-element alignment.
+ * workspace: device floats, psk_paged_tree_workspace_len() of them, no initial
+ * contents needed.
+ */
+int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int q_dtype,
+                             const void* k_cache, const void* v_cache, const int64_t* k_strides,
+                             const int64_t* v_strides, const int32_t* block_table, int64_t block_table_stride,
+                             int64_t block_table_width, const int32_t* seq_lens, int64_t num_seqs, int64_t num_q_heads,
+                             int64_t num_kv_heads, int64_t head_size, int64_t block_size, int64_t num_blocks,
+                             int64_t max_seq_len, int64_t total_q, int64_t max_seqlen_q, const int32_t* cu_seqlens_q,
+                             const int64_t* tree_mask, int64_t tree_mask_stride, int64_t tree_mask_words,
+                             float softmax_scale, const float* q_descale, const float* k_descale,
+                             const float* v_descale, const int64_t* descale_strides, void* out,
+                             int64_t out_tok_stride, int64_t out_head_stride, int out_dtype, float* lse,
+                             int64_t lse_head_stride, float* workspace, int64_t workspace_len, void* stream);
+
+int64_t psk_paged_tree_workspace_len(int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, int64_t num_q_heads,
+                                     int64_t num_kv_heads, int64_t max_seq_len);
+
+/*
+ * The attention weight each cached token received from a step's queries
+ * (build-defined): for sequence b, kv head h and j < min(seq_lens[b], scores_width)
+ *   scores[b * scores_seq_stride + h * scores_head_stride + j] = decay * (the same)
+ *     + sum over its query tokens i that see key j and query heads hq of h of
+ *       exp(s_j - lse[hq * lse_head_stride + c_b + i]),
+ * s_j and the causal rule as psk_paged_decode_attention, any number of query
+ * tokens and heads, in a fixed order of sums.  decay == 0: the old value is not
+ * read.  descale_strides: (b, h) of q and k.  max_seq_len only sizes the launch.
+ * One launch, no workspace.
+ */
+int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, int64_t scores_head_stride,
+                                     int64_t scores_width, const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                                     int q_dtype, const void* k_cache, const int64_t* k_strides, const float* lse,
+                                     int64_t lse_head_stride, const int32_t* block_table, int64_t block_table_stride,
+                                     int64_t block_table_width, const int32_t* seq_lens, int64_t num_seqs,
+                                     int64_t num_q_heads, int64_t num_kv_heads, int64_t head_size, int64_t block_size,
+                                     int64_t num_blocks, int64_t max_seq_len, int64_t total_q, int64_t max_seqlen_q,
+                                     const int32_t* cu_seqlens_q, int causal, float softmax_scale, float decay,
+                                     const float* q_descale, const float* k_descale, const int64_t* descale_strides,
+                                     void* stream);
+
+/*
+ * Eviction of cached tokens to a budget, in two calls (build-defined; the
+ * reference evicts whole pages of idle sequences only).
+ *
+ * psk_select_tokens: for layer l, sequence b and head h, of the n =
+ * min(seq_lens[b], scores_width) scores at scores + l * s[0] + b * s[1] + h * s[2]
+ * (elements): all tokens if n <= budget, else the first `sink`, the last
+ * `recent` and the budget - sink - recent highest scores between (ties to the
+ * lower position, NaN below all).  kept[((l * num_seqs + b) * num_heads + h) *
+ * budget + i]: the i-th kept position, ascending, -1 past the last;
+ * new_lens[b] = min(n, budget).  scores_out (which may be scores itself with the
+ * same strides, and may not overlap it otherwise) receives the kept scores, then
+ * zeros up to n, both up to scores_out_width.
+ *
+ * psk_move_kept_tokens: row kept[..., i] of sequence b, head h (page
+ * block_table[b * stride + kept / block_size], byte strides) goes to row i of
+ * the pages dst_block_table[b]; cache1 (may be NULL) is a second cache of the
+ * same geometry.  A missing source page reads as zeros, a missing destination
+ * is skipped.  kept_heads is num_heads, or 1 for one list for all heads.  No
+ * destination page may be a source page of the call.  At most 65535 layers and
+ * sequences.
+ */
+int psk_select_tokens(const float* scores, const int64_t* scores_strides, int64_t scores_width, float* scores_out,
+                      const int64_t* scores_out_strides, int64_t scores_out_width, const int32_t* seq_lens,
+                      int64_t num_layers, int64_t num_seqs, int64_t num_heads, int64_t budget, int64_t sink,
+                      int64_t recent, int32_t* kept, int32_t* new_lens, void* stream);
+
+int psk_move_kept_tokens(void* cache0, void* cache1, int64_t layer_stride, int64_t block_stride, int64_t row_stride,
+                         int64_t head_stride, int64_t head_bytes, int64_t num_layers, int64_t num_heads,
+                         int64_t block_size, int64_t num_blocks, const int32_t* block_table,
+                         int64_t block_table_stride, int64_t block_table_width, const int32_t* dst_block_table,
+                         int64_t dst_block_table_stride, int64_t dst_block_table_width, const int32_t* kept,
+                         int64_t kept_heads, int64_t budget, int64_t num_seqs, void* stream);
+
+/*
+ * The accepted path of a drafted tree (build-defined): for every layer, sequence
+ * b and i < min(path_lens[b], path_width), the row of position starts[b] +
+ * path[b * path_stride + i] becomes the row of position starts[b] + i, every row
+ * read before any is written.  cache1 (may be NULL): a second cache of the same
+ * geometry (byte strides).  Negative entries and rows on missing pages are
+ * skipped.  path_width is at most 256; at most 65535 layers and sequences.
+ */
+int psk_commit_draft_tokens(void* cache0, void* cache1, int64_t layer_stride, int64_t block_stride, int64_t row_stride,
+                            int64_t row_bytes, int64_t num_layers, int64_t block_size, int64_t num_blocks,
+                            const int32_t* block_table, int64_t block_table_stride, int64_t block_table_width,
+                            const int32_t* starts, const int32_t* path, int64_t path_stride, int64_t path_width,
+                            const int32_t* path_lens, int64_t num_seqs, void* stream);
 
 /*
  * FP8 MLA latent entries with one scale per 128-element tile (build-defined;

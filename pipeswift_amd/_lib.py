@@ -11,6 +11,7 @@ reference's driver-failure path, copy_engine.py:454-457).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -106,6 +107,31 @@ _SIGNATURES = {
     ),
     "psk_paged_prefill_workspace_len": (_i64, [_i64]),
     "psk_paged_prefill_step_workspace_len": (_i64, [_i64] * 6),
+    "psk_paged_tree_attention": (
+        _int,
+        [_vp, _i64, _i64, _int, _vp, _vp, _c_int64_p, _c_int64_p, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, ctypes.c_float, _vp, _vp, _vp, _c_int64_p, _vp, _i64, _i64,
+         _int, _vp, _i64, _vp, _i64, _vp],
+    ),
+    "psk_paged_tree_workspace_len": (_i64, [_i64] * 6),
+    "psk_accumulate_attention_weights": (
+        _int,
+        [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _int, _vp, _c_int64_p, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+         _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _int, ctypes.c_float, ctypes.c_float, _vp, _vp, _c_int64_p,
+         _vp],
+    ),
+    "psk_select_tokens": (
+        _int, [_vp, _c_int64_p, _i64, _vp, _c_int64_p, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp],
+    ),
+    "psk_move_kept_tokens": (
+        _int,
+        [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
+         _i64, _i64, _vp],
+    ),
+    "psk_commit_draft_tokens": (
+        _int,
+        [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp],
+    ),
     "psk_mla_fp8_tile_entry_bytes": (_i64, [_i64, _i64]),
     "psk_concat_and_cache_mla_fp8_tiles": (
         _int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp],
@@ -169,6 +195,14 @@ def stream_handle(device: torch.device) -> int:
         idx = device.index if device.index is not None else torch.cuda.current_device()
         return _raw_stream(idx)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one: the library launches on
+    the current device, and the stream has to be one of its own."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 _I64x4 = ctypes.c_int64 * 4

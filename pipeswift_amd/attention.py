@@ -31,7 +31,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import check, dtype_code, i64_array, lib, ptr, stream_handle
+from ._lib import check, dtype_code, i64_array, lib, on_device, ptr, stream_handle
 
 HEAD_DIM = 128
 MAX_ROWS = 16  # query tokens x query heads per kv head
@@ -289,6 +289,212 @@ def paged_prefill_attention(
     )
     check(st, "paged_prefill_attention")
     return (out, lse) if return_softmax_lse else out
+
+
+def _query_layout(q, cu_seqlens_q, max_seqlen_q, validate):
+    """(sequences, query token bound) of a checked ragged query layout."""
+    n = int(max_seqlen_q)
+    assert n >= 1, f"max_seqlen_q = {n}"
+    if cu_seqlens_q is None:
+        assert q.shape[0] % n == 0, f"{q.shape[0]} query rows are not {n} per sequence"
+        return q.shape[0] // n, n
+    assert cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.is_contiguous() and cu_seqlens_q.dim() == 1
+    assert cu_seqlens_q.device == q.device and cu_seqlens_q.shape[0] >= 1
+    if (validate or _CHECK_ARGS) and not torch.cuda.is_current_stream_capturing():
+        check_cu_seqlens_q(cu_seqlens_q, q.shape[0], n)
+    return cu_seqlens_q.shape[0] - 1, n
+
+
+def _check_paged(q, caches, block_table, seq_lens, num_seqs):
+    """The paged FP8 reader's conditions on its tensors."""
+    assert q.is_cuda and q.dim() == 3 and q.shape[2] == HEAD_DIM and q.stride(2) == 1, \
+        "q must be [T, Hq, 128] with unit last stride"
+    for c in caches:
+        assert c.dtype == torch.float8_e4m3fn, "the cache must be fp8 e4m3fn"
+        assert c.dim() == 4 and c.shape == caches[0].shape and c.shape[3] == HEAD_DIM and c.stride(3) == 1
+    Hq, Hkv = q.shape[1], caches[0].shape[2]
+    assert Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"{Hq} query heads over {Hkv} kv heads"
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
+    assert block_table.shape[0] >= num_seqs
+    assert seq_lens.dtype == torch.int32 and seq_lens.is_contiguous() and seq_lens.numel() >= num_seqs
+    for t in (*caches, block_table, seq_lens):
+        assert t.device == q.device, "all tensors must share the query's device"
+
+
+def tree_mask(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, max_seqlen_q: int) -> torch.Tensor:
+    """``paged_tree_attention``'s mask of drafted trees given by their parents.
+
+    parents: integers [total_q]; a drafted token's parent as an index among its
+    sequence's drafted tokens, negative for a child of the last cached token.
+    Every token sees itself and its ancestors.  Returns int64
+    [total_q, ceil(max_seqlen_q / 64)] on the parents' device, without a host
+    synchronization: log2(max_seqlen_q) rounds, each of which doubles how many
+    ancestors a token has gathered."""
+    assert parents.dim() == 1 and parents.dtype in (torch.int32, torch.int64)
+    n, dev = int(max_seqlen_q), parents.device
+    assert n >= 1
+    words = -(-n // 64)
+    cu = cu_seqlens_q.to(device=dev, dtype=torch.int64)
+    row = torch.arange(parents.shape[0], device=dev)
+    b = (torch.searchsorted(cu, row, right=True) - 1).clamp_(0, max(cu.shape[0] - 2, 0))
+    first = cu[b] if cu.shape[0] > 1 else torch.zeros_like(row)
+    up = torch.where(parents >= 0, first + parents, -1)
+    own = (row - first).clamp_(min=0)
+    mask = torch.zeros(parents.shape[0] + 1, words, dtype=torch.int64, device=dev)  # the last row: no ancestor
+    word = torch.arange(words, device=dev)
+    mask[:-1] = torch.where(own[:, None] // 64 == word, torch.ones_like(own)[:, None] << (own[:, None] % 64), 0)
+    up = torch.cat([torch.where((up >= 0) & (up < parents.shape[0]), up, parents.shape[0]),
+                    torch.full((1,), parents.shape[0], device=dev)])
+    for _ in range(max(n - 1, 1).bit_length()):
+        mask = mask | mask[up]
+        up = up[up]
+    return mask[:-1].contiguous()
+
+
+def paged_tree_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    tree_mask: torch.Tensor,
+    cu_seqlens_q: Optional[torch.Tensor],
+    max_seqlen_q: int,
+    softmax_scale: Optional[float] = None,
+    q_descale: Optional[torch.Tensor] = None,
+    k_descale: Optional[torch.Tensor] = None,
+    v_descale: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    return_softmax_lse: bool = False,
+    max_seq_len: Optional[int] = None,
+    workspace: Optional[torch.Tensor] = None,
+    validate: bool = False,
+):
+    """Attention of drafted trees over the paged FP8 cache: the verification
+    step of tree speculation.
+
+    ``paged_decode_attention``'s tensors and results (q~, scores, descales,
+    zero rows for missing pages, bf16 or float32 ``out``, lse [Hq, total_q]) for
+    any number of drafted tokens and query heads, with a mask of its own: the n
+    query tokens of sequence b are its drafted tokens, the last n of its
+    seq_lens[b] cached ones (appended in tree order), and token i sees every key
+    before the drafted ones and drafted key t where bit t % 64 of
+    ``tree_mask[row, t // 64]`` is set (int64 [total_q, words], or [total_q] for
+    trees of at most 64; bits at or past n are ignored).  ``tree_mask()`` makes
+    it of the tokens' parents.  A token that sees no key gets zeros and
+    lse -inf.  P V runs on the fp16 MFMA with P rounded once to fp16, as in
+    ``paged_prefill_attention``.
+
+    ``max_seq_len``: a bound on seq_lens where the caller has a closer one than
+    the block table's width; it only sizes the launch.  ``workspace``: float32
+    of ``tree_workspace_floats``, for callers that keep one."""
+    B, n = _query_layout(q, cu_seqlens_q, max_seqlen_q, validate)
+    _check_paged(q, (k_cache, v_cache), block_table, seq_lens, B)
+    TQ, Hq, _ = q.shape
+    P, ps, Hkv, _ = k_cache.shape
+    device = q.device
+    if tree_mask.dim() == 1:
+        tree_mask = tree_mask.unsqueeze(1)
+    assert tree_mask.dtype == torch.int64 and tree_mask.dim() == 2 and tree_mask.device == device
+    assert tree_mask.shape[0] >= TQ and (tree_mask.stride(1) == 1 or tree_mask.shape[1] <= 1)
+    assert n <= 64 * tree_mask.shape[1], f"a mask of {tree_mask.shape[1]} words for up to {n} drafted tokens"
+    if softmax_scale is None:
+        softmax_scale = HEAD_DIM ** -0.5
+    bound = block_table.shape[1] * ps
+    bound = bound if max_seq_len is None else min(int(max_seq_len), bound)
+    if out is None:
+        out = torch.empty(TQ, Hq, HEAD_DIM, dtype=torch.bfloat16, device=device)
+    assert out.dtype in _OUT_CODES and out.shape == (TQ, Hq, HEAD_DIM) and out.stride(2) == 1 and out.device == device
+    lse = torch.empty(Hq, TQ, dtype=torch.float32, device=device) if return_softmax_lse else None
+    qd, qsb, qsh = _descale(q_descale, B, Hkv, device)
+    kd, ksb, ksh = _descale(k_descale, B, Hkv, device)
+    vd, vsb, vsh = _descale(v_descale, B, Hkv, device)
+    with on_device(device):
+        need = tree_workspace_floats(B, TQ, n, Hq, Hkv, bound)
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(max(need, 1), dtype=torch.float32, device=device)
+        assert workspace.dtype == torch.float32 and workspace.device == device and workspace.is_contiguous()
+        st = lib().psk_paged_tree_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), dtype_code(q.dtype), k_cache.data_ptr(), v_cache.data_ptr(),
+            i64_array(k_cache.stride()[:3]), i64_array(v_cache.stride()[:3]), block_table.data_ptr(),
+            block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), B, Hq, Hkv, HEAD_DIM, ps, P, bound, TQ, n,
+            ptr(cu_seqlens_q), tree_mask.data_ptr(), tree_mask.stride(0), tree_mask.shape[1], float(softmax_scale),
+            ptr(qd), ptr(kd), ptr(vd), i64_array([qsb, qsh, ksb, ksh, vsb, vsh]), out.data_ptr(), out.stride(0),
+            out.stride(1), _OUT_CODES[out.dtype], ptr(lse), TQ if lse is not None else 0, workspace.data_ptr(),
+            workspace.numel(), stream_handle(device),
+        )
+    check(st, "paged_tree_attention")
+    return (out, lse) if return_softmax_lse else out
+
+
+def tree_workspace_floats(num_seqs: int, total_q: int, max_seqlen_q: int, num_q_heads: int, num_kv_heads: int,
+                          max_seq_len: int) -> int:
+    """float32 elements of ``paged_tree_attention``'s workspace."""
+    n = int(lib().psk_paged_tree_workspace_len(num_seqs, total_q, max_seqlen_q, num_q_heads, num_kv_heads,
+                                                max_seq_len))
+    if n < 0:
+        check(n, "paged tree workspace")
+    return n
+
+
+def accumulate_attention_weights(
+    scores: torch.Tensor,
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    lse: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    max_seqlen_q: int = 1,
+    softmax_scale: Optional[float] = None,
+    q_descale: Optional[torch.Tensor] = None,
+    k_descale: Optional[torch.Tensor] = None,
+    causal: bool = True,
+    decay: float = 1.0,
+    max_seq_len: Optional[int] = None,
+    validate: bool = False,
+) -> torch.Tensor:
+    """Add to ``scores`` the attention weight that every cached token received
+    from a step's queries -- what ``cache_ops.evict_tokens`` goes by.
+
+    For sequence b, kv head h and j < seq_lens[b]:
+    ``scores[b, h, j] = decay * scores[b, h, j] + sum exp(s_ij - lse[hq, i])``
+    over the sequence's query tokens i that see key j and the query heads hq of
+    h, in a fixed order (no atomics: the same inputs give the same bits).
+    q, the cache, the descales, ``causal`` and the ragged layout are those of
+    the attention call (``paged_decode_attention``), and ``lse`` [Hq, total_q]
+    float32 is what it returned; slices of both along the tokens (the last
+    queries of a prompt, with ``cu_seqlens_q`` of their own) give the weights of
+    those queries.  scores: float32 [>= B, Hkv, width], unit last stride;
+    entries at or past seq_lens[b] or the width are left as they are, and new
+    tokens start from what is there (zeros).  ``decay`` 0 does not read the old
+    sums.  ``max_seq_len`` only sizes the launch.  Returns ``scores``."""
+    B, n = _query_layout(q, cu_seqlens_q, max_seqlen_q, validate)
+    _check_paged(q, (k_cache,), block_table, seq_lens, B)
+    TQ, Hq, _ = q.shape
+    P, ps, Hkv, _ = k_cache.shape
+    device = q.device
+    assert scores.dtype == torch.float32 and scores.dim() == 3 and scores.device == device
+    assert scores.shape[0] >= B and scores.shape[1] == Hkv and (scores.stride(2) == 1 or scores.shape[2] <= 1), \
+        f"scores must be [>= {B}, {Hkv}, width] with unit last stride"
+    assert lse.dtype == torch.float32 and lse.shape == (Hq, TQ) and lse.device == device
+    assert lse.stride(1) == 1 or TQ <= 1, "lse must have unit last stride"
+    if softmax_scale is None:
+        softmax_scale = HEAD_DIM ** -0.5
+    bound = block_table.shape[1] * ps
+    bound = bound if max_seq_len is None else min(int(max_seq_len), bound)
+    qd, qsb, qsh = _descale(q_descale, B, Hkv, device)
+    kd, ksb, ksh = _descale(k_descale, B, Hkv, device)
+    with on_device(device):
+        st = lib().psk_accumulate_attention_weights(
+            scores.data_ptr(), scores.stride(0), scores.stride(1), scores.shape[2], q.data_ptr(), q.stride(0),
+            q.stride(1), dtype_code(q.dtype), k_cache.data_ptr(), i64_array(k_cache.stride()[:3]), lse.data_ptr(),
+            lse.stride(0), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), B,
+            Hq, Hkv, HEAD_DIM, ps, P, bound, TQ, n, ptr(cu_seqlens_q), 1 if causal else 0, float(softmax_scale),
+            float(decay), ptr(qd), ptr(kd), i64_array([qsb, qsh, ksb, ksh]), stream_handle(device),
+        )
+    check(st, "accumulate_attention_weights")
+    return scores
 
 
 def _chunked_queries(cu_seqlens_q, total_q, seqused_k, block_table, chunk, causal, descales):

@@ -1,4 +1,5 @@
-"""Block gather, copy_blocks and the per-tensor FP8 scale, on gfx950 HIP kernels.
+"""Block gather, copy_blocks, token eviction and draft commits, and the per-tensor
+FP8 scale, on gfx950 HIP kernels.
 
 None of these has a counterpart in the reference (wsjdsg/PipeSwift):
   * its attention kernels read the paged cache in place through the page table
@@ -8,7 +9,8 @@ None of these has a counterpart in the reference (wsjdsg/PipeSwift):
     so there is no copy_blocks;
   * its FP8 KV cache uses a fixed scale of 1.0 (pipeswift/utils/fp8_kv.py:1-3).
 They follow vLLM's conventions for the same operations and are pinned by the
-closed forms in their docstrings.
+closed forms in their docstrings.  Nor does it evict single tokens or verify
+drafted trees: ``evict_tokens`` and ``commit_draft_tokens`` are this build's own.
 """
 
 from __future__ import annotations
@@ -19,7 +21,7 @@ import threading
 import numpy as np
 import torch
 
-from ._lib import check, dtype_code, lib, ptr, stream_handle
+from ._lib import check, dtype_code, i64_array, lib, on_device, ptr, stream_handle
 
 FP8_E4M3_MAX = 448.0
 
@@ -176,6 +178,172 @@ def copy_blocks(caches, block_mapping: torch.Tensor, validate: bool = True) -> N
     if not block_mapping.is_cuda:
         # keep the staged copy alive until the kernels that read it have run
         dev_map.record_stream(torch.cuda.current_stream(device))
+
+
+# --------------------------------------------------------------------------- #
+# tokens: eviction to a budget, commit of a drafted path
+# --------------------------------------------------------------------------- #
+
+
+def _cache_pairs(caches, first_row_dim):
+    """``caches`` as (cache, second cache of the same geometry or None) pairs, one
+    launch each.  Rows are contiguous from ``first_row_dim`` on."""
+    if isinstance(caches, torch.Tensor):
+        caches = [caches]
+    assert len(caches) > 0
+    for c in caches:
+        assert c.is_cuda and c.device == caches[0].device, "all caches must be on one GPU"
+        assert c.shape[:3] == caches[0].shape[:3], "all caches must have the same layers, pages and page size"
+        expect = 1
+        for dim in range(c.ndim - 1, first_row_dim - 1, -1):
+            assert c.stride(dim) == expect or c.shape[dim] == 1, (
+                f"cache rows must be contiguous beyond dim {first_row_dim - 1} (strides {c.stride()})"
+            )
+            expect *= c.shape[dim]
+    pairs, i = [], 0
+    while i < len(caches):
+        a = caches[i]
+        b = caches[i + 1] if i + 1 < len(caches) else None
+        same = b is not None and (a.shape, a.stride(), a.dtype) == (b.shape, b.stride(), b.dtype)
+        pairs.append((a, b if same else None))
+        i += 2 if same else 1
+    return pairs
+
+
+def _i32(t, device, shape, name):
+    assert t.dtype == torch.int32 and t.device == device, f"{name} must be int32 on the caches' device"
+    assert t.dim() == len(shape) and all(n is None or t.shape[d] >= n for d, n in enumerate(shape)), \
+        f"{name} has shape {tuple(t.shape)}"
+    assert t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name} needs unit last stride"
+
+
+def evict_tokens(
+    caches,
+    scores: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    dst_block_table: torch.Tensor,
+    budget: int,
+    sink: int = 0,
+    recent: int = 0,
+    scores_out: torch.Tensor | None = None,
+):
+    """Keep at most ``budget`` tokens of each sequence and layer, by their
+    scores, in fresh pages.
+
+    caches: one tensor or a list (K and V views), [L, num_blocks, block_size,
+    H, *row] with contiguous head rows, or [L, num_blocks, block_size, row] for
+    a latent cache (H = 1).  scores: float32 [L, B, H, width] (unit last
+    stride), for instance the running sums of
+    ``attention.accumulate_attention_weights``, or [L, B, 1, width] for one
+    choice for all heads.  For each layer, sequence and head, of the n =
+    seq_lens[b] tokens (at most ``width``):
+      * all are kept if n <= budget;
+      * else the first ``sink``, the last ``recent`` and, of those between, the
+        budget - sink - recent of the highest scores; ties go to the lower
+        position, a NaN score counts below every other.
+    Kept token i, in position order, becomes row i of the pages
+    ``dst_block_table[b]`` (int32 [B, W], at least budget rows; entries outside
+    the cache are skipped, a source row on a missing page reads as zeros).
+    Those pages must be none that ``block_table`` names: prefix pages may be
+    shared by sequences, so they are read and left as they are.
+    ``scores_out`` (default: ``scores``, in place) receives the kept tokens'
+    scores, then zeros up to n.
+
+    Returns (kept, new_lens): int32 [L, B, H or 1, budget], each kept token's old
+    position (-1 past the last), and int32 [B], the new lengths.  Two launches
+    per pair of caches of one geometry and a first one in all; no
+    synchronization.
+    """
+    first = caches if isinstance(caches, torch.Tensor) else caches[0]
+    assert first.ndim >= 4, "caches are layered: [L, num_blocks, block_size, heads, ...] or [L, num_blocks, block_size, row]"
+    heads = 1 if first.ndim == 4 else first.shape[3]
+    pairs = _cache_pairs(caches, 3 if first.ndim == 4 else 4)
+    device = first.device
+    layers, num_blocks, page = first.shape[:3]
+    assert all(c.ndim == first.ndim and (1 if c.ndim == 4 else c.shape[3]) == heads for p in pairs for c in p
+               if c is not None), "all caches must have the same heads"
+    assert scores.dtype == torch.float32 and scores.dim() == 4 and scores.device == device
+    assert scores.shape[0] == layers and scores.shape[2] in (1, heads), \
+        f"scores of shape {tuple(scores.shape)} for {layers} layers of {heads} heads"
+    scores_out = scores if scores_out is None else scores_out
+    assert scores_out.dtype == torch.float32 and scores_out.device == device
+    assert scores_out.dim() == 4 and scores_out.shape[:3] == scores.shape[:3]
+    for t in (scores, scores_out):
+        assert t.stride(3) == 1 or t.shape[3] <= 1, "scores need unit last stride"
+    B, kept_heads = scores.shape[1], scores.shape[2]
+    budget, sink, recent = int(budget), int(sink), int(recent)
+    assert budget >= 1 and sink >= 0 and recent >= 0 and sink + recent <= budget, \
+        f"sink {sink} and recent {recent} do not fit a budget of {budget}"
+    _i32(block_table, device, (B, None), "block_table")
+    _i32(dst_block_table, device, (B, None), "dst_block_table")
+    _i32(seq_lens, device, (B,), "seq_lens")
+    assert dst_block_table.shape[1] * page >= budget, \
+        f"{dst_block_table.shape[1]} pages of {page} cannot hold a budget of {budget}"
+    assert block_table.data_ptr() != dst_block_table.data_ptr() or B == 0, "the kept tokens go to pages of their own"
+    kept = torch.empty(layers, B, kept_heads, budget, dtype=torch.int32, device=device)
+    new_lens = torch.empty(B, dtype=torch.int32, device=device)
+    with on_device(device):
+        stream = stream_handle(device)
+        status = lib().psk_select_tokens(
+            ptr(scores), i64_array(scores.stride()[:3]), scores.shape[3], ptr(scores_out),
+            i64_array(scores_out.stride()[:3]), scores_out.shape[3], ptr(seq_lens), layers, B, kept_heads, budget, sink,
+            recent, ptr(kept), ptr(new_lens), stream,
+        )
+        check(status, "evict_tokens")
+        for a, b in pairs:
+            es = a.element_size()
+            head = math.prod(a.shape[3 if a.ndim == 4 else 4:])
+            status = lib().psk_move_kept_tokens(
+                ptr(a), ptr(b), a.stride(0) * es, a.stride(1) * es, a.stride(2) * es,
+                0 if a.ndim == 4 else a.stride(3) * es, head * es, layers, heads, page, num_blocks, ptr(block_table),
+                block_table.stride(0), block_table.shape[1], ptr(dst_block_table), dst_block_table.stride(0),
+                dst_block_table.shape[1], ptr(kept), kept_heads, budget, B, stream,
+            )
+            check(status, "evict_tokens")
+    return kept, new_lens
+
+
+def commit_draft_tokens(
+    caches,
+    block_table: torch.Tensor,
+    starts: torch.Tensor,
+    path: torch.Tensor,
+    path_lens: torch.Tensor,
+) -> None:
+    """Make the accepted path of each drafted tree the sequence's next tokens,
+    in every layer.
+
+    Sequence b's drafted tokens were appended in tree order from position
+    ``starts[b]``; ``path[b, i]`` (int32 [B, M], M at most 256) is the i-th
+    accepted one's index among them, for i < path_lens[b] (int32 [B]).  The row
+    of position starts[b] + path[b, i] becomes the row of position starts[b] +
+    i, as a snapshot: every row is read before any is written, whatever the
+    order of ``path``.  The sequence then has starts[b] + path_lens[b] tokens.
+    caches: one tensor or a list, [L, num_blocks, block_size, *row] with
+    contiguous rows (K and V views of the fused cache, a latent cache); two of
+    one geometry move in one launch.  Negative indices and rows on missing pages
+    are skipped.
+    """
+    pairs = _cache_pairs(caches, 3)
+    first = pairs[0][0]
+    assert first.ndim >= 4, "caches are layered: [L, num_blocks, block_size, ...]"
+    device = first.device
+    layers, num_blocks, page = first.shape[:3]
+    B = path.shape[0]
+    _i32(path, device, (None, None), "path")
+    _i32(block_table, device, (B, None), "block_table")
+    _i32(starts, device, (B,), "starts")
+    _i32(path_lens, device, (B,), "path_lens")
+    with on_device(device):
+        for a, b in pairs:
+            es = a.element_size()
+            status = lib().psk_commit_draft_tokens(
+                ptr(a), ptr(b), a.stride(0) * es, a.stride(1) * es, a.stride(2) * es, math.prod(a.shape[3:]) * es,
+                layers, page, num_blocks, ptr(block_table), block_table.stride(0), block_table.shape[1], ptr(starts),
+                ptr(path), path.stride(0), path.shape[1], ptr(path_lens), B, stream_handle(device),
+            )
+            check(status, "commit_draft_tokens")
 
 
 # --------------------------------------------------------------------------- #
