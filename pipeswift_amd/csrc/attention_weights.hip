@@ -24,6 +24,7 @@ struct WeightArgs {
   int64_t seq_stride, head_stride;  // elements
   int32_t width;
   float decay;
+  double scale_log2;  // softmax_scale * log2(e)
 };
 
 __device__ __forceinline__ float e4m3_value(uint32_t byte) { return e4m3_unpack2(byte, false).x; }
@@ -37,7 +38,7 @@ __global__ void __launch_bounds__(256) attention_weights_kernel(WeightArgs p, in
   const int full = max(a.seq_lens[b], 0);
   const float qd = descale(a.qd, a.qd_b, a.qd_h, b, h);
   const float kd = descale(a.kd, a.kd_b, a.kd_h, b, h);
-  const float sl = a.scale_log2 * qd * kd;
+  const float sl = score_scale(p.scale_log2, qd, kd);
   for (int k0 = int(blockIdx.x) * 256; k0 < L; k0 += int(gridDim.x) * 256) {
     const int key = k0 + int(threadIdx.x);
     const bool in = key < L;
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(256) attention_weights_kernel(WeightArgs p, in
         if (!see) continue;
         float dot = 0.0f;
         for (int j = 0; j < 128; ++j) dot += e4m3_value((kw[j / 4] >> (8 * (j % 4))) & 0xFFu) * s_q[j];
-        const float lse2 = p.lse[int64_t(hq) * p.lse_head_stride + r.first + i] * 1.4426950408889634f;
+        const float lse2 = float(double(p.lse[int64_t(hq) * p.lse_head_stride + r.first + i]) * 1.4426950408889634);
         total += __builtin_amdgcn_exp2f(__builtin_fmaf(dot, sl, -lse2));
       }
     }
@@ -122,6 +123,7 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
   p.head_stride = scores_head_stride;
   p.width = int32_t(scores_width);
   p.decay = decay;
+  p.scale_log2 = double(softmax_scale) * 1.4426950408889634;
   if (num_seqs > 65535 || num_kv_heads > 65535) return fail(PSK_E_ARG, "too many sequences or heads");
   const int64_t keys = max_seq_len < scores_width ? max_seq_len : scores_width;
   const int64_t blocks = ceil_div(keys, 256) < 256 ? ceil_div(keys, 256) : 256;

@@ -81,7 +81,6 @@ inline int check_cached_queries(const CachedQueries& c, DecodeArgs& a, bool* emp
   a.heads = int32_t(group);
   a.q_len = int32_t(c.max_seqlen_q);
   a.cu_q = c.cu_seqlens_q;
-  a.scale_log2 = c.softmax_scale * 1.4426950408889634f;
   a.qd = c.q_descale;
   a.kd = c.k_descale;
   return PSK_OK;
@@ -96,6 +95,114 @@ __device__ __forceinline__ SeqRows seq_rows(const DecodeArgs& a, int32_t total_q
   const int64_t f = q_first(a, b);
   if (f < 0 || f >= total_q) return SeqRows{0, 0};
   return SeqRows{int32_t(f), min(q_count(a, b), total_q - int32_t(f))};
+}
+
+// The scale from a product q~ . K to the exp2 domain, rounded once (each rounding
+// of it is an error of every score in the same direction).
+__device__ __forceinline__ float score_scale(double scale_log2, float qd, float kd) {
+  return float(scale_log2 * double(qd) * double(kd));
+}
+
+// ---------------------------------------------------------------------------
+// a step's work cut into equal runs
+// ---------------------------------------------------------------------------
+//
+// A job is a kv head of a sequence with query tokens; it costs kOver units and
+// one for every kStepKeys keys.  Jobs follow each other by sequence and head, and
+// run j takes the units [j q, (j + 1) q).  Every wave that asks scans the
+// lengths itself, 64 sequences at a time, so that no launch and no memory goes
+// before the kernels and any number of sequences is taken.
+
+constexpr int kStepKeys = 128;
+
+struct JobSpace {
+  int32_t num_seqs, total_q, heads;  // kv heads
+  int32_t over;                      // units a job costs beside its keys
+  int32_t max_runs;
+  int32_t min_run;                   // units a run has at least
+};
+
+// A sequence's length, kept where the arithmetic on whole tiles of it stays in 31 bits.
+__device__ __forceinline__ int32_t cached_len(const DecodeArgs& a, int b) {
+  return min(max(a.seq_lens[b], 0), INT32_MAX - 2 * kStepKeys);
+}
+__device__ __forceinline__ int32_t seq_steps(int32_t len) { return (len + kStepKeys - 1) / kStepKeys; }
+
+// Units of sequence b over all kv heads; 0 without query tokens.
+__device__ __forceinline__ int64_t seq_cost(const DecodeArgs& a, const JobSpace& s, int b) {
+  if (b >= s.num_seqs || seq_rows(a, s.total_q, b).n <= 0) return 0;
+  return int64_t(s.over + seq_steps(cached_len(a, b))) * s.heads;
+}
+
+__device__ __forceinline__ int64_t wave_sum_before(int64_t x, int lane, int64_t& total) {
+  int64_t v = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t y = __shfl_up(v, o);
+    if (lane >= o) v += y;
+  }
+  total = __shfl(v, 63);
+  return v - x;
+}
+
+template <class T>
+__device__ __forceinline__ T wave_uniform(T x) {
+  static_assert(sizeof(T) == 4 || sizeof(T) == 8, "");
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(u))));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(u >> 32))));
+    return __builtin_bit_cast(T, (uint64_t(hi) << 32) | lo);
+  }
+}
+
+// The whole step: its units, and the units of a run.
+struct StepCost {
+  int64_t total, run;
+};
+__device__ __forceinline__ StepCost step_cost(const DecodeArgs& a, const JobSpace& s, int lane) {
+  StepCost c{0, 1};
+  for (int b0 = 0; b0 < s.num_seqs; b0 += 64) {
+    int64_t x = seq_cost(a, s, b0 + lane);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+    c.total += wave_uniform(x);
+  }
+  const int64_t even = (c.total + s.max_runs - 1) / s.max_runs;
+  c.run = even > s.min_run ? even : s.min_run;
+  return c;
+}
+
+// The sequence that unit x < total falls in, and the units before that sequence.
+__device__ __forceinline__ int seq_of_unit(const DecodeArgs& a, const JobSpace& s, int64_t x, int lane, int64_t& before) {
+  before = 0;
+  for (int b0 = 0;; b0 += 64) {
+    const int64_t own = seq_cost(a, s, b0 + lane);
+    int64_t total;
+    const int64_t at = before + wave_sum_before(own, lane, total);
+    const uint64_t m = __ballot(at <= x && x < at + own);
+    if (m) {
+      const int l = __builtin_ctzll(m);
+      before = wave_uniform(int64_t(__shfl(at, l)));
+      return b0 + l;
+    }
+    before += wave_uniform(total);
+    if (b0 + 64 >= s.num_seqs) return s.num_seqs - 1;  // (not reached: x < total)
+  }
+}
+
+// Units before sequence b.
+__device__ __forceinline__ int64_t units_before(const DecodeArgs& a, const JobSpace& s, int b, int lane) {
+  int64_t n = 0;
+  for (int b0 = 0; b0 < b; b0 += 64) {
+    int64_t x = b0 + lane < b ? seq_cost(a, s, b0 + lane) : 0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+    n += wave_uniform(x);
+  }
+  return n;
 }
 
 // The 16-byte chunks of one cached row of a kv head, or nullptr where the page is missing.

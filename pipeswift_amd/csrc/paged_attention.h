@@ -141,6 +141,32 @@ __device__ __forceinline__ void load_query_as(const char* src, float qd, int d0,
   }
 }
 
+// LDS at a byte address
+template <class T>
+__device__ __forceinline__ __attribute__((address_space(3))) T* lds_at(uint32_t at) {
+  return (__attribute__((address_space(3))) T*)size_t(at);
+}
+
+// 16 bytes per lane from global memory straight to LDS: lane i's to at + 16 i.
+// In asm because the compiler, unable to tell which LDS bytes such a load
+// writes, would wait for all of them before every LDS read.  It writes no
+// register and leaves m0 as it was; wait_loads() orders the reads of the bytes.
+__device__ __forceinline__ void load_lds(uint32_t at, const uint8_t* base, uint32_t offset) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "s"(at), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds(uint32_t at, const uint8_t* p) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "s"(at), "v"(p) : "memory");
+}
+// Until at most N of this wave's loads are in flight.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+
 }  // namespace psk_detail
 
 #endif  // PSK_PAGED_ATTENTION_H

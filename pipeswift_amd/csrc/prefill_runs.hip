@@ -243,38 +243,12 @@ __device__ __forceinline__ PfStep pf_step(const RunArgs& p, int64_t* prefix, int
   return PfStep{pf_take(p, uniform(keys), uniform(carry)), uniform(carry)};
 }
 
-// LDS at a byte address
-template <class T>
-__device__ __forceinline__ __attribute__((address_space(3))) T* lds_at(uint32_t at) {
-  return (__attribute__((address_space(3))) T*)size_t(at);
-}
-
 // Workgroup barrier that orders LDS only: the global loads of a coming stage
 // stay in flight across it.
 __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
-// 16 bytes per lane from global memory straight to LDS: lane i's to at + 16 i.
-// In asm because the compiler, unable to tell which LDS bytes such a load
-// writes, would wait for all of them before every LDS read.  It writes no
-// register and leaves m0 as it was; wait_loads() orders the reads of the bytes.
-__device__ __forceinline__ void load_lds(uint32_t at, const uint8_t* base, uint32_t offset) {
-  uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
-               : "=&s"(m0) : "s"(at), "v"(offset), "s"(base) : "memory");
-}
-__device__ __forceinline__ void load_lds(uint32_t at, const uint8_t* p) {
-  uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
-               : "=&s"(m0) : "s"(at), "v"(p) : "memory");
-}
-// Until at most N of this wave's loads are in flight.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
 }
 
 template <int Q_DT, int OUT_DT, bool GEN>
