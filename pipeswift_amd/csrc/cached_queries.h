@@ -107,11 +107,11 @@ __device__ __forceinline__ float score_scale(double scale_log2, float qd, float 
 // a step's work cut into equal runs
 // ---------------------------------------------------------------------------
 //
-// A job is a kv head of a sequence with query tokens; it costs kOver units and
+// A job is a kv head of a sequence with query tokens; it costs `over` units and
 // one for every kStepKeys keys.  Jobs follow each other by sequence and head, and
-// run j takes the units [j q, (j + 1) q).  Every wave that asks scans the
-// lengths itself, 64 sequences at a time, so that no launch and no memory goes
-// before the kernels and any number of sequences is taken.
+// run j takes the units [j q, (j + 1) q).  Every wave scans the lengths itself,
+// 64 sequences at a time and a sequence a lane, so that no launch and no memory
+// goes before the kernels and any number of sequences is taken.
 
 constexpr int kStepKeys = 128;
 
@@ -126,83 +126,98 @@ struct JobSpace {
 __device__ __forceinline__ int32_t cached_len(const DecodeArgs& a, int b) {
   return min(max(a.seq_lens[b], 0), INT32_MAX - 2 * kStepKeys);
 }
-__device__ __forceinline__ int32_t seq_steps(int32_t len) { return (len + kStepKeys - 1) / kStepKeys; }
-
-// Units of sequence b over all kv heads; 0 without query tokens.
-__device__ __forceinline__ int64_t seq_cost(const DecodeArgs& a, const JobSpace& s, int b) {
-  if (b >= s.num_seqs || seq_rows(a, s.total_q, b).n <= 0) return 0;
-  return int64_t(s.over + seq_steps(cached_len(a, b))) * s.heads;
-}
-
-__device__ __forceinline__ int64_t wave_sum_before(int64_t x, int lane, int64_t& total) {
-  int64_t v = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t y = __shfl_up(v, o);
-    if (lane >= o) v += y;
-  }
-  total = __shfl(v, 63);
-  return v - x;
-}
+__device__ __forceinline__ int32_t key_steps(int32_t len) { return (len + kStepKeys - 1) / kStepKeys; }
 
 template <class T>
-__device__ __forceinline__ T wave_uniform(T x) {
+__device__ __forceinline__ T lane_value(T x, int lane) {
   static_assert(sizeof(T) == 4 || sizeof(T) == 8, "");
   if constexpr (sizeof(T) == 4) {
-    return __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
   } else {
     const uint64_t u = __builtin_bit_cast(uint64_t, x);
-    const uint32_t lo = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(u))));
-    const uint32_t hi = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(u >> 32))));
+    const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(u)), lane));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(u >> 32)), lane));
     return __builtin_bit_cast(T, (uint64_t(hi) << 32) | lo);
   }
 }
 
-// The whole step: its units, and the units of a run.
-struct StepCost {
-  int64_t total, run;
-};
-__device__ __forceinline__ StepCost step_cost(const DecodeArgs& a, const JobSpace& s, int lane) {
-  StepCost c{0, 1};
-  for (int b0 = 0; b0 < s.num_seqs; b0 += 64) {
-    int64_t x = seq_cost(a, s, b0 + lane);
+// x / y for 0 <= x, 0 < y, short where both fit 31 bits (they do, but for a huge step).
+__device__ __forceinline__ int64_t uniform_div(int64_t x, int64_t y) {
+  if (((x | y) >> 31) == 0) return int64_t(uint32_t(x) / uint32_t(y));
+  return x / y;
+}
+
+// 64 consecutive sequences, one a lane: the lane's query rows and length, its
+// units over all kv heads, and the units of the window's lanes before it.
+struct SeqWindow {
+  int32_t b0;
+  int32_t first, n, len;
+  int64_t cost, before, total;
+
+  __device__ __forceinline__ void load(const DecodeArgs& a, const JobSpace& s, int from, int lane) {
+    b0 = from;
+    first = n = len = 0;
+    if (from + lane < s.num_seqs) {
+      const SeqRows r = seq_rows(a, s.total_q, from + lane);
+      first = r.first;
+      n = r.n;
+      len = cached_len(a, from + lane);
+    }
+    cost = n > 0 ? int64_t(s.over + key_steps(len)) * s.heads : 0;
+    int64_t v = cost;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-    c.total += wave_uniform(x);
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t y = __shfl_up(v, o);
+      if (lane >= o) v += y;
+    }
+    before = v - cost;
+    total = lane_value(v, 63);
   }
-  const int64_t even = (c.total + s.max_runs - 1) / s.max_runs;
+  __device__ __forceinline__ bool holds(int b) const { return b >= b0 && b < b0 + 64; }
+};
+
+struct StepRuns {
+  int64_t total, run;  // units of the step and of a run
+};
+
+// The step's units.  `w` is left at the window of sequence 0 where there is but one.
+__device__ __forceinline__ StepRuns step_runs(const DecodeArgs& a, const JobSpace& s, SeqWindow& w, int lane) {
+  StepRuns c{0, 1};
+  for (int b0 = 0; b0 < s.num_seqs; b0 += 64) {
+    w.load(a, s, b0, lane);
+    c.total += w.total;
+  }
+  const int64_t even = uniform_div(c.total + s.max_runs - 1, s.max_runs);
   c.run = even > s.min_run ? even : s.min_run;
   return c;
 }
 
-// The sequence that unit x < total falls in, and the units before that sequence.
-__device__ __forceinline__ int seq_of_unit(const DecodeArgs& a, const JobSpace& s, int64_t x, int lane, int64_t& before) {
+// The sequence that unit x (below the total) falls in, and the units before it.
+__device__ __forceinline__ int seq_of_unit(const DecodeArgs& a, const JobSpace& s, int64_t x, SeqWindow& w, int lane,
+                                           int64_t& before) {
   before = 0;
   for (int b0 = 0;; b0 += 64) {
-    const int64_t own = seq_cost(a, s, b0 + lane);
-    int64_t total;
-    const int64_t at = before + wave_sum_before(own, lane, total);
-    const uint64_t m = __ballot(at <= x && x < at + own);
+    if (w.b0 != b0) w.load(a, s, b0, lane);
+    const int64_t at = before + w.before;
+    const uint64_t m = __ballot(at <= x && x < at + w.cost);
     if (m) {
       const int l = __builtin_ctzll(m);
-      before = wave_uniform(int64_t(__shfl(at, l)));
+      before = lane_value(at, l);
       return b0 + l;
     }
-    before += wave_uniform(total);
-    if (b0 + 64 >= s.num_seqs) return s.num_seqs - 1;  // (not reached: x < total)
+    before += w.total;
+    if (b0 + 64 >= s.num_seqs) return s.num_seqs - 1;  // (not reached: x is below the total)
   }
 }
 
-// Units before sequence b.
-__device__ __forceinline__ int64_t units_before(const DecodeArgs& a, const JobSpace& s, int b, int lane) {
+// Units before sequence b; its window is left in `w`.
+__device__ __forceinline__ int64_t units_before(const DecodeArgs& a, const JobSpace& s, int b, SeqWindow& w, int lane) {
   int64_t n = 0;
-  for (int b0 = 0; b0 < b; b0 += 64) {
-    int64_t x = b0 + lane < b ? seq_cost(a, s, b0 + lane) : 0;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-    n += wave_uniform(x);
+  for (int b0 = 0;; b0 += 64) {
+    if (w.b0 != b0) w.load(a, s, b0, lane);
+    if (w.holds(b)) return n + lane_value(w.before, b - b0);
+    n += w.total;
   }
-  return n;
 }
 
 // The 16-byte chunks of one cached row of a kv head, or nullptr where the page is missing.

@@ -70,6 +70,31 @@ __device__ __forceinline__ float* record(const TreeArgs& p, int64_t run, int blo
   return p.records + ((run * p.row_blocks + block) * 2 + slot) * kSlab;
 }
 
+// A tile's eight loads (see load_lds): K rows 8 u .. 8 u + 7 from kp[u] + 1024 u
+// to slot + 1024 u, V rows behind them.  An instruction's offset counts for both
+// its addresses, so the LDS base is set once for K and once for V.
+__device__ __forceinline__ void load_tile(uint32_t slot, const uint8_t* const (&kp)[4], const uint8_t* const (&vp)[4],
+                                          uint32_t off_k, uint32_t off_v) {
+  uint32_t m0;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %3, %5\n\t"
+      "global_load_lds_dwordx4 %3, %6 offset:1024\n\t"
+      "global_load_lds_dwordx4 %3, %7 offset:2048\n\t"
+      "global_load_lds_dwordx4 %3, %8 offset:3072\n\t"
+      "s_mov_b32 m0, %2\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %4, %9\n\t"
+      "global_load_lds_dwordx4 %4, %10 offset:1024\n\t"
+      "global_load_lds_dwordx4 %4, %11 offset:2048\n\t"
+      "global_load_lds_dwordx4 %4, %12 offset:3072\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(m0)
+      : "s"(slot), "s"(slot + kHalfSlot), "v"(off_k), "v"(off_v), "s"(kp[0]), "s"(kp[1]), "s"(kp[2]), "s"(kp[3]),
+        "s"(vp[0]), "s"(vp[1]), "s"(vp[2]), "s"(vp[3])
+      : "memory");
+}
+
 // Steps [from, to) of a job of `steps` that the units [lo, hi) of it pay for.
 struct Piece {
   int32_t from, to;
@@ -122,49 +147,64 @@ __device__ __forceinline__ void finish(const TreeArgs& p, const SeqRows& r, int 
         any ? (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f : -__builtin_inff();
 }
 
-template <int Q_DT, int OUT_DT>
+template <int Q_DT, int OUT_DT, bool GEN>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 tree_attention_kernel(TreeArgs p) {
   const DecodeArgs& a = p.a;
   __shared__ __attribute__((aligned(1024))) char s_ring[kWaves * kRing * kSlot];
   __shared__ int32_t s_pages[kPages];
   __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
+  __shared__ uint32_t s_nan[kHead];  // of each column the rows that see a NaN value
+  __shared__ int s_nans;
   const int tid = int(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, kk = lane & 31;
 
-  // workgroup w runs on XCD w % 8: the row blocks of a run on one, next to each other
+  SeqWindow seqs;
+  const StepRuns step_run = step_runs(a, p.s, seqs, lane);
+  // Workgroup w runs on XCD w % 8.  Each XCD takes consecutive runs, so that its
+  // L2 sees every kv head of a few sequences (a head's rows lie a token apart and
+  // would fall on a part of its channels), and the row blocks of a run, which
+  // read the same keys, are next to each other.
   const int w = int(blockIdx.x);
-  const int64_t j = int64_t(w / (8 * p.row_blocks)) * 8 + (w & 7);
-  const int block = (w >> 3) % p.row_blocks;
-  const StepCost cost = step_cost(a, p.s, lane);
-  int64_t x = j * cost.run;
-  if (j >= p.s.max_runs || x >= cost.total) return;
-  const int64_t x_end = min(x + cost.run, cost.total);
+  const int64_t runs = uniform_div(step_run.total + step_run.run - 1, step_run.run);
+  const int64_t per = (runs + 7) >> 3;
+  const int idx = (w >> 3) / p.row_blocks;
+  const int block = (w >> 3) - idx * p.row_blocks;
+  const int64_t j = (w & 7) * per + idx;
+  if (idx >= per || j >= runs) return;
+  int64_t x = j * step_run.run;
+  const int64_t x_end = min(x + step_run.run, step_run.total);
 
   const uint32_t ring = (uint32_t)(size_t)(lvoid*)s_ring + uint32_t(wave * kRing) * kSlot;
   // loads: lane l takes chunk position l % 8 of keys 8 u + l / 8
   const int lr = lane >> 3, lchunk = 16 * ((lane & 7) ^ lr);
   // reads (see above)
-  const uint32_t rd_k = uint32_t(128 * kk);
-  const int ksw = kk & 7;
+  uint32_t rd_k[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) rd_k[q] = uint32_t(128 * kk + 16 * ((4 * half + q) ^ (kk & 7)));
   const int vr = lane & 15, vg = (lane >> 4) & 1;
   const int vkey = 8 * (vr >> 3) + 4 * half + ((vr >> 1) & 3);  // of each 16
-  const uint32_t rd_v = kHalfSlot + uint32_t(128 * vkey + 8 * (vr & 1));
-  const int vsw = vkey & 7;
+  uint32_t rd_v[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+    rd_v[d] = kHalfSlot + uint32_t(128 * vkey + 16 * ((2 * d + vg) ^ (vkey & 7)) + 8 * (vr & 1));
 
   int64_t before;
-  int b = seq_of_unit(a, p.s, x, lane, before);
+  int b = seq_of_unit(a, p.s, x, seqs, lane, before);
   while (x < x_end) {  // over the run's jobs
-    const SeqRows r = seq_rows(a, p.s.total_q, b);
-    const int L = cached_len(a, b);
-    const int64_t job_cost = p.s.over + seq_steps(L);
-    if (r.n <= 0 || x >= before + job_cost * p.s.heads) {
-      if (r.n > 0) before += job_cost * p.s.heads;
+    if (!seqs.holds(b)) seqs.load(a, p.s, b, lane);
+    const SeqRows r{lane_value(seqs.first, b - seqs.b0), lane_value(seqs.n, b - seqs.b0)};
+    const int L = lane_value(seqs.len, b - seqs.b0);
+    const int steps = key_steps(L);
+    const int64_t job_cost = p.s.over + steps;
+    const int64_t seq_end = before + (r.n > 0 ? job_cost * p.s.heads : 0);
+    if (x >= seq_end) {
+      before = seq_end;
       ++b;
       continue;
     }
-    const int h = int((x - before) / job_cost);
+    const int h = int(uniform_div(x - before, job_cost));
     const int64_t at = before + h * job_cost;
     const int64_t hi = min(x_end, at + job_cost);
     const Piece c = piece_of(p.s, x - at, hi - at);
@@ -199,8 +239,9 @@ tree_attention_kernel(TreeArgs p) {
 #pragma unroll
     for (int d = 0; d < 4; ++d) o[d] = f32x16{};
 
-    const uint8_t* kbase = a.k + int64_t(h) * a.k_head + lchunk;
-    const uint8_t* vbase = a.v + int64_t(h) * a.v_head + lchunk;
+    const uint8_t* kbase = a.k + int64_t(h) * a.k_head;
+    const uint8_t* vbase = a.v + int64_t(h) * a.v_head;
+    const uint32_t off_k = uint32_t(lr * a.k_row) + lchunk, off_v = uint32_t(lr * a.v_row) + lchunk;
     const int n_tiles = (L + kTile - 1) / kTile;
     const int t_mask = max(ctx, 0) / kTile;  // tiles from here on need masks
     const int steps_per_window = int(min(int64_t(kPages - 1) * a.block_size / kStepKeys, int64_t(1) << 24));
@@ -210,7 +251,11 @@ tree_attention_kernel(TreeArgs p) {
       // the pages of the window's keys, missing ones as -1
       const int p0 = page_index(a, s0 * kStepKeys);
       const int p1 = page_index(a, int(min(int64_t(L), int64_t(s1) * kStepKeys)) - 1);
-      __syncthreads();  // readers of the ring (the last piece's merge) and of the ids are done
+      __syncthreads();  // readers of the ring, the marks (the last piece's merge) and the ids are done
+      if (s0 == c.from) {
+        if (tid < kHead) s_nan[tid] = 0;
+        if (tid == 0) s_nans = 0;
+      }
       for (int i = tid; i <= p1 - p0; i += kThreads) {
         int32_t id = -1;
         if (p0 + i < a.bt_width) id = a.block_table[int64_t(b) * a.bt_stride + p0 + i];
@@ -218,87 +263,137 @@ tree_attention_kernel(TreeArgs p) {
       }
       __syncthreads();
 
-      const int t_end = min(4 * s1, n_tiles);
+      const int t_end = min(kWaves * s1, n_tiles);
       bool full = true;  // the newest tile's loads are all in flight
-      auto issue = [&](int t, uint32_t slot) {
-        int32_t id[4], row[4];
-        bool all = true;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int key = t * kTile + 8 * u + lr;
-          const int pi = page_index(a, key);
-          row[u] = key - pi * a.block_size;
-          id[u] = key < L ? s_pages[pi - p0] : -1;
-          all = all && id[u] >= 0;
+      // GEN: every lane looks its four keys' pages up.  Else eight keys of one
+      // load share a page: lane 4 k + u holds where load u of tile win + 4 k
+      // begins, for sixteen tiles at a time, and the addresses are scalar.
+      int win = 0;
+      int64_t at_k = 0, at_v = 0;
+      uint64_t whole8 = 0, some8 = 0;  // loads whose eight keys are all cached; whose first is
+      auto look_up = [&](int t) {
+        win = t;
+        const int key = (t + kWaves * (lane >> 2)) * kTile + 8 * (lane & 3);
+        int32_t id = -1;
+        int pi = 0;
+        if (key < L && t + kWaves * (lane >> 2) < t_end) {
+          pi = page_index(a, key);
+          id = s_pages[pi - p0];
         }
-        full = __all(all);
+        const int64_t row = key - pi * a.block_size;
+        at_k = int64_t(id) * a.k_blk + row * a.k_row - 1024 * (lane & 3);
+        at_v = int64_t(id) * a.v_blk + row * a.v_row - 1024 * (lane & 3);
+        some8 = __ballot(id >= 0);
+        whole8 = __ballot(id >= 0 && key + 8 <= L);
+      };
+      auto issue = [&](int t, uint32_t slot) {
+        if constexpr (GEN) {
+          int32_t id[4], row[4];
+          bool all = true;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (full || id[u] >= 0) {
-            load_lds(slot + 1024 * u, kbase + (int64_t(id[u]) * a.k_blk + int64_t(row[u]) * a.k_row));
-            load_lds(slot + kHalfSlot + 1024 * u, vbase + (int64_t(id[u]) * a.v_blk + int64_t(row[u]) * a.v_row));
+          for (int u = 0; u < 4; ++u) {
+            const int key = t * kTile + 8 * u + lr;
+            const int pi = page_index(a, key);
+            row[u] = key - pi * a.block_size;
+            id[u] = key < L ? s_pages[pi - p0] : -1;
+            all = all && id[u] >= 0;
+          }
+          full = __all(all);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (full || id[u] >= 0) {
+              load_lds(slot + 1024 * u, kbase + lchunk + (int64_t(id[u]) * a.k_blk + int64_t(row[u]) * a.k_row));
+              load_lds(slot + kHalfSlot + 1024 * u, vbase + lchunk + (int64_t(id[u]) * a.v_blk + int64_t(row[u]) * a.v_row));
+            } else {
+              *lds_at<u32x4>(slot + 1024 * u + 16 * lane) = u32x4(0);
+              *lds_at<u32x4>(slot + kHalfSlot + 1024 * u + 16 * lane) = u32x4(0);
+            }
+          }
+        } else {
+          if (t - win >= 16 * kWaves) look_up(t);
+          const int k = t - win;  // lane of the tile's first load
+          const uint8_t* kp[4];
+          const uint8_t* vp[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            kp[u] = kbase + lane_value(at_k, k + u);
+            vp[u] = vbase + lane_value(at_v, k + u);
+          }
+          full = ((whole8 >> k) & 15) == 15;
+          if (__builtin_expect(full, 1)) {
+            load_tile(slot, kp, vp, off_k, off_v);
           } else {
-            *lds_at<u32x4>(slot + 1024 * u + 16 * lane) = u32x4(0);
-            *lds_at<u32x4>(slot + kHalfSlot + 1024 * u + 16 * lane) = u32x4(0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              if (((some8 >> (k + u)) & 1) && t * kTile + 8 * u + lr < L) {
+                load_lds(slot + 1024 * u, kp[u] + 1024 * u, off_k);
+                load_lds(slot + kHalfSlot + 1024 * u, vp[u] + 1024 * u, off_v);
+              } else {
+                *lds_at<u32x4>(slot + 1024 * u + 16 * lane) = u32x4(0);
+                *lds_at<u32x4>(slot + kHalfSlot + 1024 * u + 16 * lane) = u32x4(0);
+              }
+            }
           }
         }
       };
 
-      auto read_v = [&](uint32_t slot, int u, int d) {
-        return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            lds_at<i32x2>(slot + rd_v + uint32_t(2048 * u + 16 * ((2 * d + vg) ^ vsw))));
-      };
       // NaN values of keys that some row does not see (0 x NaN) must not reach
-      // it: they leave the tile, and the rows that do see one become NaN in its
-      // column, by the count of those they see.
-      auto contain_nan = [&](uint32_t slot, uint32_t vis) {
-        auto nan_bytes = [](uint32_t x) { return (((x & 0x7F7F7F7Fu) + 0x01010101u) >> 7) & 0x01010101u; };
-        const uint32_t own = slot + kHalfSlot + uint32_t(16 * lane);
+      // it: they leave the tile, and the (column, row) pairs that do see one are
+      // marked, for the end of the piece.
+      auto contain_nan = [&](i32x2 (&vraw)[8], uint32_t vis) {
+        auto nan_bytes = [](int x) { return (((uint32_t(x) & 0x7F7F7F7Fu) + 0x01010101u) >> 7) & 0x01010101u; };
         uint32_t any = 0;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const u32x4 v = *lds_at<u32x4>(own + 1024 * u);
-          any |= nan_bytes(v[0]) | nan_bytes(v[1]) | nan_bytes(v[2]) | nan_bytes(v[3]);
-        }
+        for (int i = 0; i < 8; ++i) any |= nan_bytes(vraw[i][0]) | nan_bytes(vraw[i][1]);
         if (__builtin_expect(!__any(any != 0), 1)) return;
-#pragma unroll 1
-        for (int u = 0; u < 2; ++u) {
-          f16x8 seen;
+        uint32_t rows[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            seen[i] = ((vis >> (16 * u + 8 * (i >> 2) + (i & 3))) & 1u) ? _Float16(1.0f) : _Float16(0.0f);
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll 1
+          for (int j = 0; j < 8; ++j) {  // byte j: key 16 u + 8 (j / 4) + 4 half + j % 4
+            const uint64_t see = __ballot((vis >> (16 * u + 8 * (j >> 2) + (j & 3))) & 1u);
+            const uint32_t mine = half ? uint32_t(see >> 32) : uint32_t(see);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              const int word = j < 4 ? vraw[4 * u + d][0] : vraw[4 * u + d][1];
+              rows[d] |= ((uint32_t(word) >> (8 * (j & 3))) & 0x7Fu) == 0x7Fu ? mine : 0u;
+            }
           }
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
-            const i32x2 raw = read_v(slot, u, d);
-            const f16x8 bad = e4m3x8_to_f16(nan_bytes(uint32_t(raw[0])) * 0x38u, nan_bytes(uint32_t(raw[1])) * 0x38u);  // 1.0
-            const f32x16 count = __builtin_amdgcn_mfma_f32_32x32x16_f16(bad, seen, f32x16{}, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] = count[i] > 0.0f ? __builtin_nanf("") : o[d][i];
+            vraw[4 * u + d][0] &= int(~(nan_bytes(vraw[4 * u + d][0]) * 0xFFu));
+            vraw[4 * u + d][1] &= int(~(nan_bytes(vraw[4 * u + d][1]) * 0xFFu));
           }
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          u32x4 v = *lds_at<u32x4>(own + 1024 * u);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] &= ~(nan_bytes(v[i]) * 0xFFu);
-          *lds_at<u32x4>(own + 1024 * u) = v;
-        }
+        for (int d = 0; d < 4; ++d)
+          if (rows[d]) atomicOr(&s_nan[32 * d + kk], rows[d]);
+        s_nans = 1;
       };
 
-      auto attend = [&](auto masked_tag, int t, uint32_t slot) {
+      // One tile: its operands leave the slot for registers, the loads of the
+      // tile after the next one start into it, and then it is computed.
+      auto attend = [&](auto masked_tag, int t, uint32_t slot, const auto& refill) {
         constexpr bool MASKED = decltype(masked_tag)::value;
+        u32x4 kraw[4];
+        i32x2 vraw[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) kraw[q] = *lds_at<u32x4>(slot + rd_k[q]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          vraw[i] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(lds_at<i32x2>(slot + rd_v[i & 3] + uint32_t(2048 * (i >> 2))));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        refill();
         f32x16 y = {};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const u32x4 kw = *lds_at<u32x4>(slot + rd_k + uint32_t(16 * ((4 * half + q) ^ ksw)));
-          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16(kw[0], kw[1]), qop[2 * q], y, 0, 0, 0);
-          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16(kw[2], kw[3]), qop[2 * q + 1], y, 0, 0, 0);
+          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16(kraw[q][0], kraw[q][1]), qop[2 * q], y, 0, 0, 0);
+          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16(kraw[q][2], kraw[q][3]), qop[2 * q + 1], y, 0, 0, 0);
         }
         uint32_t vis = 0xFFFFFFFFu;
         if constexpr (MASKED) {
           vis = (live ? visible(mask, ctx, r.n, t * kTile) : 0u) >> (4 * half);
-          contain_nan(slot, vis);
+          contain_nan(vraw, vis);
         }
         auto sees = [&](int i) { return !MASKED || ((vis >> (8 * (i >> 2) + (i & 3))) & 1u); };
         float w[16], sum = 0.0f;
@@ -336,30 +431,32 @@ tree_attention_kernel(TreeArgs p) {
                                        __builtin_convertvector((f32x2{w[8 * u + 2 * i], w[8 * u + 2 * i + 1]}), f16x2));
           const f16x8 pop = __builtin_bit_cast(f16x8, u32x4{pw[0], pw[1], pw[2], pw[3]});
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const i32x2 raw = read_v(slot, u, d);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(e4m3x8_to_f16(uint32_t(raw[0]), uint32_t(raw[1])), pop, o[d], 0, 0,
-                                                          0);
-          }
+          for (int d = 0; d < 4; ++d)
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(e4m3x8_to_f16(uint32_t(vraw[4 * u + d][0]), uint32_t(vraw[4 * u + d][1])),
+                                                          pop, o[d], 0, 0, 0);
         }
       };
 
       int t = kWaves * s0 + wave;
       uint32_t slot = ring;
-      if (t < t_end) issue(t, slot);
       bool next_full = false;
-      if (t + kWaves < t_end) {
-        issue(t + kWaves, slot + kSlot);
-        next_full = full;
+      if (t < t_end) {
+        if constexpr (!GEN) look_up(t);
+        issue(t, slot);
+        if (t + kWaves < t_end) {
+          issue(t + kWaves, slot + kSlot);
+          next_full = full;
+        }
       }
       auto step = [&](auto masked_tag) {
         // the tile's own loads: the next one's eight may stay in flight
         if (t + kWaves < t_end && next_full) wait_loads<8>(); else wait_loads<0>();
-        attend(masked_tag, t, slot);
-        if (t + 2 * kWaves < t_end) {
-          issue(t + 2 * kWaves, slot);
-          next_full = full;
-        }
+        attend(masked_tag, t, slot, [&] {
+          if (t + 2 * kWaves < t_end) {
+            issue(t + 2 * kWaves, slot);
+            next_full = full;
+          }
+        });
         slot = slot == ring ? ring + kSlot : ring;
         t += kWaves;
       };
@@ -374,7 +471,7 @@ tree_attention_kernel(TreeArgs p) {
       s_l[wave][lane] = lt;
     }
     __syncthreads();  // every wave has left its ring, and wrote its maxima
-    const bool whole = c.from == 0 && c.to == int(job_cost) - p.s.over;
+    const bool whole = c.from == 0 && c.to == steps;
     float top = s_m[0][kk];
 #pragma unroll
     for (int v = 1; v < kWaves; ++v) top = __builtin_fmaxf(top, s_m[v][kk]);
@@ -396,6 +493,11 @@ tree_attention_kernel(TreeArgs p) {
       f32x4 v = s_o[q * 64 + lane];
 #pragma unroll
       for (int u = 1; u < kWaves; ++u) v += s_o[(u * 16 + q) * 64 + lane];
+      if (__builtin_expect(s_nans, 0)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if ((s_nan[8 * q + 4 * half + k] >> kk) & 1u) v[k] = __builtin_nanf("");
+      }
       if (whole) finish<OUT_DT>(p, r, b, h, row, q, lane, v, top, sum);
       else *reinterpret_cast<f32x4*>(rec + (q * 64 + lane) * 4) = v;
     }
@@ -424,26 +526,37 @@ __global__ void __launch_bounds__(256) merge_tree_kernel(TreeArgs p) {
   const SeqRows r = seq_rows(a, p.s.total_q, b);
   const int row = kRows * block + kk;
   if (kRows * block >= r.n * a.heads) return;
-  const StepCost cost = step_cost(a, p.s, lane);
-  const int64_t job_cost = p.s.over + seq_steps(cached_len(a, b));
-  const int64_t at = units_before(a, p.s, b, lane) + h * job_cost;
-  const int64_t j0 = at / cost.run, j1 = (at + job_cost - 1) / cost.run;
-  const int32_t steps = int32_t(job_cost) - p.s.over;
+  SeqWindow seqs;
+  const StepRuns cost = step_runs(a, p.s, seqs, lane);
+  const int64_t before = units_before(a, p.s, b, seqs, lane);
+  const int steps = key_steps(lane_value(seqs.len, b - seqs.b0));
+  const int64_t at = before + h * int64_t(p.s.over + steps) + p.s.over;  // the first unit that pays for keys
+  const int64_t j0 = uniform_div(at, cost.run), j1 = steps > 0 ? uniform_div(at + steps - 1, cost.run) : j0 - 1;
+  if (j0 == j1) return;  // one run had all the keys and wrote the rows
 
   float top = kNegBig, sum = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t j = j0; j <= j1; ++j) {
-    const Piece c = piece_of(p.s, max(j * cost.run - at, int64_t(0)), min((j + 1) * cost.run - at, job_cost));
-    if (c.from >= c.to) continue;
-    if (c.from == 0 && c.to == steps) return;  // one run had it all and wrote the rows
-    const float* rec = record(p, j, block, c.from == 0 ? 1 : 0);
-    const float m = rec[4096 + kk], l = rec[4096 + 32 + kk];
-    const f32x4 v = *reinterpret_cast<const f32x4*>(rec + (q * 64 + lane) * 4);
-    const float up = __builtin_fmaxf(top, m);
-    const float f0 = __builtin_amdgcn_exp2f(top - up), f1 = __builtin_amdgcn_exp2f(m - up);
-    top = up;
-    sum = sum * f0 + l * f1;
-    o = o * f0 + v * f1;
+  constexpr int kAhead = 4;  // records read together
+  for (int64_t j = j0; j <= j1; j += kAhead) {
+    float m[kAhead], l[kAhead];
+    f32x4 v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t k = min(j + u, j1);
+      const float* rec = record(p, k, block, k == j0 ? 1 : 0);
+      m[u] = rec[4096 + kk];
+      l[u] = rec[4096 + 32 + kk];
+      v[u] = *reinterpret_cast<const f32x4*>(rec + (q * 64 + lane) * 4);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (j + u > j1) break;
+      const float up = __builtin_fmaxf(top, m[u]);
+      const float f0 = __builtin_amdgcn_exp2f(top - up), f1 = __builtin_amdgcn_exp2f(m[u] - up);
+      top = up;
+      sum = sum * f0 + l[u] * f1;
+      o = o * f0 + v[u] * f1;
+    }
   }
   finish<OUT_DT>(p, r, b, h, row, q, lane, o, top, sum);
 }
@@ -474,9 +587,10 @@ TreeShape tree_shape(int64_t rows, int64_t slots) {
 }
 
 template <int Q_DT, int OUT_DT>
-int launch_tree(const TreeArgs& p, hipStream_t st) {
-  hipLaunchKernelGGL((tree_attention_kernel<Q_DT, OUT_DT>), dim3(unsigned(p.s.max_runs * p.row_blocks)), dim3(kThreads), 0,
-                     st, p);
+int launch_tree(const TreeArgs& p, bool general, hipStream_t st) {
+  const dim3 grid{unsigned(p.s.max_runs * p.row_blocks), 1u, 1u};
+  if (general) hipLaunchKernelGGL((tree_attention_kernel<Q_DT, OUT_DT, true>), grid, dim3(kThreads), 0, st, p);
+  else hipLaunchKernelGGL((tree_attention_kernel<Q_DT, OUT_DT, false>), grid, dim3(kThreads), 0, st, p);
   if (const int e = check_launch("tree_attention_kernel launch"); e != PSK_OK) return e;
   const int64_t tasks = int64_t(p.s.num_seqs) * p.s.heads * p.row_blocks * 16;
   hipLaunchKernelGGL((merge_tree_kernel<OUT_DT>), dim3(unsigned(tasks / 4)), dim3(256), 0, st, p);
@@ -485,7 +599,12 @@ int launch_tree(const TreeArgs& p, hipStream_t st) {
 
 template <int Q_DT>
 int launch_tree_q(const TreeArgs& p, int out_dtype, hipStream_t st) {
-  return out_dtype == PSK_DTYPE_BF16 ? launch_tree<Q_DT, PSK_DTYPE_BF16>(p, st) : launch_tree<Q_DT, PSK_DTYPE_F32>(p, st);
+  const DecodeArgs& a = p.a;
+  // pages of a multiple of 8 keys whose rows lie within 32-bit offsets: the keys of a load share a page
+  const bool general = a.block_size % 8 != 0 || a.k_row < 0 || a.v_row < 0 ||
+                       8 * std::max(a.k_row, a.v_row) >= (int64_t(1) << 31);
+  return out_dtype == PSK_DTYPE_BF16 ? launch_tree<Q_DT, PSK_DTYPE_BF16>(p, general, st)
+                                     : launch_tree<Q_DT, PSK_DTYPE_F32>(p, general, st);
 }
 
 }  // namespace
