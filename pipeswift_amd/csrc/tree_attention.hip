@@ -117,6 +117,39 @@ __device__ __forceinline__ uint32_t visible(const int64_t* m, int ctx, int n, in
   return uint32_t(bits) & in;
 }
 
+// Sixteen elements of a query row, loaded and then quantized to their e4m3 bytes
+// (zeros without a row).
+template <int Q_DT>
+struct QueryBytes {
+  static constexpr int kEsz = Q_DT == PSK_DTYPE_F32 ? 4 : Q_DT == PSK_DTYPE_FP8_E4M3FN ? 1 : 2;
+  u32x4 x[kEsz];
+  bool live;
+  __device__ __forceinline__ void load(const char* src, int d0) {
+    live = src != nullptr;
+#pragma unroll
+    for (int i = 0; i < kEsz; ++i) x[i] = live ? reinterpret_cast<const u32x4*>(src + d0 * kEsz)[i] : u32x4(0);
+  }
+  __device__ __forceinline__ u32x4 quantized(float qd, uint32_t sign) const {
+    u32x4 y;
+    if constexpr (Q_DT == PSK_DTYPE_FP8_E4M3FN) {
+      y = x[0];
+    } else {
+      using QC = QuantConv<Q_DT, 16 / kEsz, kNanTorch>;
+      const QScale qs = make_qscale(qd);
+      uint8_t bytes[16];
+#pragma unroll
+      for (int i = 0; i < kEsz; ++i) {
+        const typename QC::Out z = QC::apply(x[i], qs);
+        __builtin_memcpy(bytes + 16 / kEsz * i, &z, 16 / kEsz);
+      }
+      __builtin_memcpy(&y, bytes, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = live ? y[i] ^ sign : 0u;
+    return y;
+  }
+};
+
 template <int OUT_DT>
 __device__ __forceinline__ void store4(char* dst, f32x4 v) {
   if constexpr (OUT_DT == PSK_DTYPE_F32) {
@@ -153,6 +186,7 @@ tree_attention_kernel(TreeArgs p) {
   const DecodeArgs& a = p.a;
   __shared__ __attribute__((aligned(1024))) char s_ring[kWaves * kRing * kSlot];
   __shared__ int32_t s_pages[kPages];
+  __shared__ u32x4 s_q[kRows * 8];  // the rows' e4m3 queries, chunk c of row r at c ^ (r & 7)
   __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
   __shared__ uint32_t s_nan[kHead];  // of each column the rows that see a NaN value
   __shared__ int s_nans;
@@ -212,32 +246,36 @@ tree_attention_kernel(TreeArgs p) {
     const int row0 = block * kRows;
     if (c.from >= c.to || row0 >= r.n * a.heads) continue;
 
-    // the rows' queries
+    // The queries: every thread quantizes 16 elements of a row, and the waves
+    // read the rows' bytes from LDS.  The pages of the first keys are on their
+    // way meanwhile.
+    const int first_page = page_index(a, c.from * kStepKeys);
+    int32_t page0 = -1;
+    if (first_page + tid < a.bt_width) page0 = a.block_table[int64_t(b) * a.bt_stride + first_page + tid];
     const int ctx = L - r.n;
+    const int row = row0 + kk, i0 = row / a.heads;
+    const bool live = i0 < r.n;
+    const int64_t* mask = p.mask + (int64_t(r.first) + (live ? i0 : 0)) * p.mask_stride;
+    QueryBytes<Q_DT> qb;
+    {
+      const int qr = row0 + (tid >> 3), qi = qr / a.heads;
+      qb.load(qi < r.n ? a.q + (int64_t(r.first) + qi) * a.q_tok_stride +
+                             int64_t(h * a.heads + qr - qi * a.heads) * a.q_head_stride
+                       : nullptr, 16 * (tid & 7));
+    }
     const float qd = descale(a.qd, a.qd_b, a.qd_h, b, h);
     const float sl_signed = score_scale(p.scale_log2, qd, descale(a.kd, a.kd_b, a.kd_h, b, h));
     const float sl = __builtin_fabsf(sl_signed);  // a negative scale is applied as -q~ (exact)
-    const int row = row0 + kk, i0 = row / a.heads;
-    const bool live = i0 < r.n;
-    const int64_t tok = int64_t(r.first) + (live ? i0 : 0);
-    const int64_t* mask = p.mask + tok * p.mask_stride;
-    bf16x8 qop[8];
-    {
-      const char* src = a.q + tok * a.q_tok_stride + int64_t(h * a.heads + (live ? row - i0 * a.heads : 0)) * a.q_head_stride;
-      uint32_t q0[8], q1[8];
-      load_query_as<Q_DT>(src, qd, 64 * half, q0);
-      load_query_as<Q_DT>(src, qd, 64 * half + 32, q1);
-      const uint32_t sign = sl_signed < 0.0f ? 0x80808080u : 0u;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        qop[t] = live ? e4m3x8_to_bf16(q0[2 * t] ^ sign, q0[2 * t + 1] ^ sign) : bf16x8{};
-        qop[4 + t] = live ? e4m3x8_to_bf16(q1[2 * t] ^ sign, q1[2 * t + 1] ^ sign) : bf16x8{};
-      }
-    }
+    __syncthreads();  // readers of the ring, the marks (the last piece's merge), the ids and the queries are done
+    s_q[(tid >> 3) * 8 + ((tid & 7) ^ ((tid >> 3) & 7))] = qb.quantized(qd, sl_signed < 0.0f ? 0x80808080u : 0u);
+    if (tid < kHead) s_nan[tid] = 0;
+    if (tid == 0) s_nans = 0;
+
     float m = live ? kNegBig : -kNegBig, l = 0.0f;  // rows without a token keep every weight at 0
     f32x16 o[4];
 #pragma unroll
     for (int d = 0; d < 4; ++d) o[d] = f32x16{};
+    bf16x8 qop[8];
 
     const uint8_t* kbase = a.k + int64_t(h) * a.k_head;
     const uint8_t* vbase = a.v + int64_t(h) * a.v_head;
@@ -251,17 +289,24 @@ tree_attention_kernel(TreeArgs p) {
       // the pages of the window's keys, missing ones as -1
       const int p0 = page_index(a, s0 * kStepKeys);
       const int p1 = page_index(a, int(min(int64_t(L), int64_t(s1) * kStepKeys)) - 1);
-      __syncthreads();  // readers of the ring, the marks (the last piece's merge) and the ids are done
-      if (s0 == c.from) {
-        if (tid < kHead) s_nan[tid] = 0;
-        if (tid == 0) s_nans = 0;
-      }
+      if (s0 > c.from) __syncthreads();  // the ids before these are done with
       for (int i = tid; i <= p1 - p0; i += kThreads) {
-        int32_t id = -1;
-        if (p0 + i < a.bt_width) id = a.block_table[int64_t(b) * a.bt_stride + p0 + i];
+        int32_t id = page0;
+        if (s0 > c.from || i >= kThreads) {
+          id = -1;
+          if (p0 + i < a.bt_width) id = a.block_table[int64_t(b) * a.bt_stride + p0 + i];
+        }
         s_pages[i] = id < a.num_blocks ? id : -1;
       }
       __syncthreads();
+      if (s0 == c.from) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const u32x4 x = s_q[kk * 8 + ((4 * half + t) ^ (kk & 7))];
+          qop[2 * t] = e4m3x8_to_bf16(x[0], x[1]);
+          qop[2 * t + 1] = e4m3x8_to_bf16(x[2], x[3]);
+        }
+      }
 
       const int t_end = min(kWaves * s1, n_tiles);
       bool full = true;  // the newest tile's loads are all in flight
@@ -683,9 +728,9 @@ int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head
   p.s.num_seqs = int32_t(num_seqs);
   p.s.total_q = int32_t(total_q);
   p.s.heads = int32_t(num_kv_heads);
-  p.s.over = 2;
+  p.s.over = 1;
   p.s.max_runs = int32_t(s.max_runs);
-  p.s.min_run = 3;
+  p.s.min_run = 2;
   p.row_blocks = int32_t(s.row_blocks);
   p.records = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
   if (num_seqs * num_kv_heads * s.row_blocks > INT32_MAX / 16 || s.max_runs * s.row_blocks > INT32_MAX)
