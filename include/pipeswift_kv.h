@@ -454,8 +454,13 @@ int64_t psk_paged_tree_workspace_len(int64_t num_seqs, int64_t total_q, int64_t 
  * s_j and the causal rule as psk_paged_decode_attention, any number of query
  * tokens and heads, in a fixed order of sums.  decay == 0: the old value is not
  * read.  descale_strides: (b, h) of q and k.  max_seq_len only sizes the launch.
- * One launch, no workspace.
+ * workspace: psk_attention_weights_workspace_bytes() bytes of device memory (0
+ * for at most 32 query rows a kv head, max_seqlen_q * num_q_heads / num_kv_heads,
+ * and for an FP8 query; else the queries' e4m3 bytes), no initial contents
+ * needed.  One launch, or two with a workspace.
  */
+int64_t psk_attention_weights_workspace_bytes(int64_t total_q, int64_t max_seqlen_q, int64_t num_q_heads,
+                                              int64_t num_kv_heads, int q_dtype);
 int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, int64_t scores_head_stride,
                                      int64_t scores_width, const void* q, int64_t q_tok_stride, int64_t q_head_stride,
                                      int q_dtype, const void* k_cache, const int64_t* k_strides, const float* lse,
@@ -465,7 +470,7 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
                                      int64_t num_blocks, int64_t max_seq_len, int64_t total_q, int64_t max_seqlen_q,
                                      const int32_t* cu_seqlens_q, int causal, float softmax_scale, float decay,
                                      const float* q_descale, const float* k_descale, const int64_t* descale_strides,
-                                     void* stream);
+                                     void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Eviction of cached tokens to a budget, in two calls (build-defined; the

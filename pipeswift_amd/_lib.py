@@ -118,8 +118,9 @@ _SIGNATURES = {
         _int,
         [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _int, _vp, _c_int64_p, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
          _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _int, ctypes.c_float, ctypes.c_float, _vp, _vp, _c_int64_p,
-         _vp],
+         _vp, _i64, _vp],
     ),
+    "psk_attention_weights_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int]),
     "psk_select_tokens": (
         _int, [_vp, _c_int64_p, _i64, _vp, _c_int64_p, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp],
     ),

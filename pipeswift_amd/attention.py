@@ -452,6 +452,7 @@ def accumulate_attention_weights(
     causal: bool = True,
     decay: float = 1.0,
     max_seq_len: Optional[int] = None,
+    workspace: Optional[torch.Tensor] = None,
     validate: bool = False,
 ) -> torch.Tensor:
     """Add to ``scores`` the attention weight that every cached token received
@@ -468,7 +469,8 @@ def accumulate_attention_weights(
     those queries.  scores: float32 [>= B, Hkv, width], unit last stride;
     entries at or past seq_lens[b] or the width are left as they are, and new
     tokens start from what is there (zeros).  ``decay`` 0 does not read the old
-    sums.  ``max_seq_len`` only sizes the launch.  Returns ``scores``."""
+    sums.  ``max_seq_len`` only sizes the launch.  ``workspace``: uint8 of
+    ``weights_workspace_bytes``, for callers that keep one.  Returns ``scores``."""
     B, n = _query_layout(q, cu_seqlens_q, max_seqlen_q, validate)
     _check_paged(q, (k_cache,), block_table, seq_lens, B)
     TQ, Hq, _ = q.shape
@@ -486,15 +488,32 @@ def accumulate_attention_weights(
     qd, qsb, qsh = _descale(q_descale, B, Hkv, device)
     kd, ksb, ksh = _descale(k_descale, B, Hkv, device)
     with on_device(device):
+        need = weights_workspace_bytes(TQ, n, Hq, Hkv, q.dtype)
+        if need and (workspace is None or workspace.numel() < need):
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        assert workspace is None or (workspace.dtype == torch.uint8 and workspace.device == device
+                                     and workspace.is_contiguous())
         st = lib().psk_accumulate_attention_weights(
             scores.data_ptr(), scores.stride(0), scores.stride(1), scores.shape[2], q.data_ptr(), q.stride(0),
             q.stride(1), dtype_code(q.dtype), k_cache.data_ptr(), i64_array(k_cache.stride()[:3]), lse.data_ptr(),
             lse.stride(0), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), B,
             Hq, Hkv, HEAD_DIM, ps, P, bound, TQ, n, ptr(cu_seqlens_q), 1 if causal else 0, float(softmax_scale),
-            float(decay), ptr(qd), ptr(kd), i64_array([qsb, qsh, ksb, ksh]), stream_handle(device),
+            float(decay), ptr(qd), ptr(kd), i64_array([qsb, qsh, ksb, ksh]), ptr(workspace),
+            0 if workspace is None else workspace.numel(), stream_handle(device),
         )
     check(st, "accumulate_attention_weights")
     return scores
+
+
+def weights_workspace_bytes(total_q: int, max_seqlen_q: int, num_q_heads: int, num_kv_heads: int,
+                            q_dtype: torch.dtype) -> int:
+    """Bytes of ``accumulate_attention_weights``'s workspace: its e4m3 queries
+    where many query rows share a kv head, else none."""
+    n = int(lib().psk_attention_weights_workspace_bytes(total_q, max_seqlen_q, num_q_heads, num_kv_heads,
+                                                         dtype_code(q_dtype)))
+    if n < 0:
+        check(n, "attention weights workspace")
+    return n
 
 
 def _chunked_queries(cu_seqlens_q, total_q, seqused_k, block_table, chunk, causal, descales):

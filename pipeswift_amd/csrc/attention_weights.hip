@@ -1,13 +1,30 @@
 // The attention weight every cached token received, summed over the queries of
-// a step (the scores an eviction goes by):
+// a step (the scores an eviction goes by), for MI355X (gfx950):
 //   A[b, h, j] = decay A[b, h, j] + sum over query tokens i that see j and heads g of
 //                exp(s_ij - lse[h G + g, i]),     j < seq_lens[b],
-// s as the readers compute it and lse as they return it.
+// s as the readers compute it (exactly converted FP8 operands on the bf16 MFMA)
+// and lse as they return it.  V is not read, and no sum of a key leaves its
+// workgroup, so there are no atomics and the order of every sum is fixed.
 //
-// A thread per key: its K row stays in registers and the step's query rows of
-// the kv head pass by it, so no sum leaves the thread.
+// Two kernels, by the query rows n G that share a key:
+//   * few_rows_kernel, at most 32 of them (a decode step): a wave per 32 keys,
+//     S = Q K^T on v_mfma_f32_32x32x16_bf16 leaves lane l key l % 32 and rows
+//     8 (i / 4) + 4 (l / 32) + i % 4, so a key's sum is one lane's registers and
+//     one exchange.  The K rows go from memory to registers, two tiles ahead;
+//     the work is cut into equal runs (cached_queries.h).
+//   * many_rows_kernel, more (the last queries of a prompt, a whole prompt): a
+//     wave holds 64 keys as MFMA operands and the step's e4m3 queries, quantized
+//     once by quantize_queries_kernel, pass by it 32 rows at a time.  S^T = K Q^T
+//     leaves lane l query row l % 32, whose lse is one value, and sixteen sums a
+//     key tile, which are joined over the lanes at the end.  Where there are
+//     too few keys to fill the GPU the waves of a workgroup share its keys and
+//     take the rows in turn.
 //
 // C ABI: include/pipeswift_kv.h.  Nothing here allocates or synchronizes.
+
+#include <algorithm>
+#include <map>
+#include <mutex>
 
 #include "cached_queries.h"
 
@@ -15,75 +32,426 @@ using namespace psk_detail;
 
 namespace {
 
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kTile = 32;    // keys of an MFMA tile
+constexpr int kRows = 32;    // query rows of one
+constexpr int kAhead = 2;    // tiles of K in flight (few rows)
+constexpr int kPages = 1024; // page ids staged at a time (few rows)
+constexpr int kGroup = 2 * kTile;  // keys a wave holds (many rows)
+constexpr int kStepShift = 7;
+constexpr int kStepKeys = kTile * kWaves;  // of a step (few rows): a tile a wave
+static_assert(kStepKeys == 1 << kStepShift, "");
+
 struct WeightArgs {
   DecodeArgs a;
-  int32_t total_q;
+  JobSpace s;
+  double scale_log2;  // softmax_scale * log2(e)
   const float* lse;
   int64_t lse_head_stride;
   float* scores;
   int64_t seq_stride, head_stride;  // elements
-  int32_t width;
   float decay;
-  double scale_log2;  // softmax_scale * log2(e)
+  const uint8_t* q8;  // many rows: e4m3 queries [total_q][Hq][128]
+  int64_t q8_tok, q8_head;
+  int32_t row_tiles;  // many rows: most of any sequence
+  int32_t slots;      // many rows: workgroups that fill the GPU
 };
 
-__device__ __forceinline__ float e4m3_value(uint32_t byte) { return e4m3_unpack2(byte, false).x; }
+__device__ __forceinline__ float* score_row(const WeightArgs& p, int b, int h) {
+  return p.scores + int64_t(b) * p.seq_stride + int64_t(h) * p.head_stride;
+}
 
-__global__ void __launch_bounds__(256) attention_weights_kernel(WeightArgs p, int q_dtype) {
+// lse log2(e) of a query row, rounded once.
+__device__ __forceinline__ float lse_log2(const WeightArgs& p, int hq, int64_t tok) {
+  return float(double(p.lse[int64_t(hq) * p.lse_head_stride + tok]) * 1.4426950408889634);
+}
+
+__device__ __forceinline__ float decayed(const WeightArgs& p, const float* at) {
+  return p.decay == 0.0f ? 0.0f : *at * p.decay;
+}
+
+// ---------------------------------------------------------------------------
+// few rows
+// ---------------------------------------------------------------------------
+
+template <int Q_DT>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(3)))
+few_rows_kernel(WeightArgs p) {
   const DecodeArgs& a = p.a;
-  __shared__ float s_q[kHead];
-  const int h = int(blockIdx.y), b = int(blockIdx.z);
-  const SeqRows r = seq_rows(a, p.total_q, b);
-  const int L = min(max(a.seq_lens[b], 0), p.width);
-  const int full = max(a.seq_lens[b], 0);
-  const float qd = descale(a.qd, a.qd_b, a.qd_h, b, h);
-  const float kd = descale(a.kd, a.kd_b, a.kd_h, b, h);
-  const float sl = score_scale(p.scale_log2, qd, kd);
-  for (int k0 = int(blockIdx.x) * 256; k0 < L; k0 += int(gridDim.x) * 256) {
-    const int key = k0 + int(threadIdx.x);
-    const bool in = key < L;
-    uint32_t kw[32];
-    const uint8_t* row = in ? cached_row(a, a.k + int64_t(h) * a.k_head, a.k_blk, a.k_row, b, key) : nullptr;
-    for (int c = 0; c < 8; ++c) {
-      const u32x4 w = row ? *reinterpret_cast<const u32x4*>(row + 16 * c) : u32x4(0);
-      for (int j = 0; j < 4; ++j) kw[4 * c + j] = w[j];
+  __shared__ int32_t s_pages[kPages];
+  __shared__ u32x4 s_q[kRows * 8];  // the rows' e4m3 queries, chunk c of row r at c ^ (r & 7)
+  __shared__ float s_lse[kRows];    // of each row; +inf for rows without a token
+  __shared__ int32_t s_last[kRows];  // the last key each row sees
+  const int tid = int(threadIdx.x), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, kk = lane & 31;
+  SeqWindow seqs;
+  const StepRuns step_run = step_runs(a, p.s, seqs, lane);
+  int64_t x = int64_t(blockIdx.x) * step_run.run;
+  if (x >= step_run.total) return;
+  const int64_t x_end = min(x + step_run.run, step_run.total);
+  int64_t before;
+  int b = seq_of_unit(a, p.s, x, seqs, lane, before);
+  while (x < x_end) {  // over the run's jobs
+    if (!seqs.holds(b)) seqs.load(a, p.s, b, lane);
+    const SeqRows r{lane_value(seqs.first, b - seqs.b0), lane_value(seqs.n, b - seqs.b0)};
+    const int full = lane_value(seqs.len, b - seqs.b0), L = min(full, p.s.width);
+    const int64_t seq_cost = lane_value(seqs.cost, b - seqs.b0);
+    if (x >= before + seq_cost) {
+      before += seq_cost;
+      ++b;
+      continue;
     }
-    float total = 0.0f;
-    for (int i = 0; i < r.n; ++i) {
-      const bool see = in && (!a.causal || key <= full - r.n + i);
-      for (int g = 0; g < a.heads; ++g) {
-        const int hq = h * a.heads + g;
-        __syncthreads();
-        if (threadIdx.x < 4) {
-          uint32_t qw[8];
-          const int d0 = 32 * int(threadIdx.x);
-          const char* src = a.q + (int64_t(r.first) + i) * a.q_tok_stride + int64_t(hq) * a.q_head_stride;
-          switch (q_dtype) {
-            case PSK_DTYPE_FP8_E4M3FN: load_query_as<PSK_DTYPE_FP8_E4M3FN>(src, qd, d0, qw); break;
-            case PSK_DTYPE_BF16: load_query_as<PSK_DTYPE_BF16>(src, qd, d0, qw); break;
-            case PSK_DTYPE_F16: load_query_as<PSK_DTYPE_F16>(src, qd, d0, qw); break;
-            default: load_query_as<PSK_DTYPE_F32>(src, qd, d0, qw); break;
-          }
-          for (int j = 0; j < 32; ++j) s_q[d0 + j] = e4m3_value((qw[j / 4] >> (8 * (j % 4))) & 0xFFu);
+    const int64_t job_cost = p.s.over + key_steps(p.s, L);
+    const int h = int(uniform_div(x - before, job_cost));
+    const int64_t at = before + h * job_cost;
+    const int64_t hi = min(x_end, at + job_cost);
+    const Piece c = piece_of(p.s, x - at, hi - at);
+    x = hi;
+    if (c.from >= c.to) continue;
+
+    float* scores = score_row(p, b, h);
+    if (r.n <= 0) {  // the old sums decay all the same
+      for (int key = c.from * kStepKeys + tid; key < min(L, c.to * kStepKeys); key += kThreads)
+        scores[key] = decayed(p, scores + key);
+      continue;
+    }
+    const int first_page = page_index(a, c.from * kStepKeys);
+    int32_t page0 = -1;
+    if (first_page + tid < a.bt_width) page0 = a.block_table[int64_t(b) * a.bt_stride + first_page + tid];
+    const int R = r.n * a.heads, ctx = full - r.n;
+    QueryBytes<Q_DT> qb;
+    {
+      const int qr = tid >> 3, qi = qr / a.heads;
+      qb.load(qr < R ? a.q + (int64_t(r.first) + qi) * a.q_tok_stride + int64_t(h * a.heads + qr - qi * a.heads) * a.q_head_stride
+                     : nullptr, 16 * (tid & 7));
+    }
+    float row_lse = __builtin_inff();
+    int row_last = -1;
+    if (tid < R) {  // (R is at most 32)
+      const int qi = tid / a.heads;
+      row_lse = lse_log2(p, h * a.heads + tid - qi * a.heads, int64_t(r.first) + qi);
+      row_last = a.causal ? ctx + qi : full - 1;
+    }
+    const float qd = descale(a.qd, a.qd_b, a.qd_h, b, h);
+    const float sl = score_scale(p.scale_log2, qd, descale(a.kd, a.kd_b, a.kd_h, b, h));
+    __syncthreads();  // readers of the last piece's queries and ids are done
+    s_q[(tid >> 3) * 8 + ((tid & 7) ^ ((tid >> 3) & 7))] = qb.quantized(qd, 0u);
+    if (tid < kRows) {
+      s_lse[tid] = row_lse;
+      s_last[tid] = row_last;
+    }
+    bf16x8 qop[8];
+    float lse[16];
+    const uint8_t* kbase = a.k + int64_t(h) * a.k_head + 64 * half;
+    const int n_tiles = (L + kTile - 1) / kTile;
+    const int t_mask = a.causal ? max(ctx, 0) / kTile : n_tiles;  // tiles below are seen by every row
+    const int groups = (R + 7) >> 3;  // register groups of four that hold rows
+    const int steps_per_window = int(min(int64_t(kPages - 1) * a.block_size / kStepKeys, int64_t(1) << 24));
+    for (int s0 = c.from; s0 < c.to; s0 += steps_per_window) {
+      const int s1 = min(c.to, s0 + steps_per_window);
+      const int p0 = page_index(a, s0 * kStepKeys);
+      const int p1 = page_index(a, int(min(int64_t(L), int64_t(s1) * kStepKeys)) - 1);
+      if (s0 > c.from) __syncthreads();  // the ids before these are done with
+      for (int i = tid; i <= p1 - p0; i += kThreads) {
+        int32_t id = page0;
+        if (s0 > c.from || i >= kThreads) {
+          id = -1;
+          if (p0 + i < a.bt_width) id = a.block_table[int64_t(b) * a.bt_stride + p0 + i];
         }
-        __syncthreads();
-        if (!see) continue;
-        float dot = 0.0f;
-        for (int j = 0; j < 128; ++j) dot += e4m3_value((kw[j / 4] >> (8 * (j % 4))) & 0xFFu) * s_q[j];
-        const float lse2 = float(double(p.lse[int64_t(hq) * p.lse_head_stride + r.first + i]) * 1.4426950408889634);
-        total += __builtin_amdgcn_exp2f(__builtin_fmaf(dot, sl, -lse2));
+        s_pages[i] = id < a.num_blocks ? id : -1;
+      }
+      __syncthreads();
+      if (s0 == c.from) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const u32x4 v = s_q[kk * 8 + ((4 * half + t) ^ (kk & 7))];
+          qop[2 * t] = e4m3x8_to_bf16(v[0], v[1]);
+          qop[2 * t + 1] = e4m3x8_to_bf16(v[2], v[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) lse[i] = s_lse[8 * (i >> 2) + 4 * half + (i & 3)];
+      }
+
+      const int t_end = min(kWaves * s1, n_tiles);
+      u32x4 kraw[kAhead][4];
+      float old[kAhead];
+      // lane l: 64 bytes of key l % 32 at d = 64 (l / 32); missing rows and keys past the end as zeros
+      auto fetch = [&](int t, u32x4 (&k)[4], float& o) {
+        const int key = t * kTile + kk;
+        const bool in = t < t_end && key < L;
+        int32_t id = -1;
+        int pi = 0;
+        if (in) {
+          pi = page_index(a, key);
+          id = s_pages[pi - p0];
+        }
+        o = in && half == 0 ? decayed(p, scores + key) : 0.0f;
+        const uint8_t* row = kbase + (int64_t(id) * a.k_blk + int64_t(key - pi * a.block_size) * a.k_row);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) k[q] = id >= 0 ? *reinterpret_cast<const u32x4*>(row + 16 * q) : u32x4(0);
+      };
+      auto add_up = [&](int t, const u32x4 (&k)[4], float o) {
+        f32x16 y = {};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qop[2 * q], e4m3x8_to_bf16(k[q][0], k[q][1]), y, 0, 0, 0);
+          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qop[2 * q + 1], e4m3x8_to_bf16(k[q][2], k[q][3]), y, 0, 0, 0);
+        }
+        const int key = t * kTile + kk;
+        float sum = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (g < groups) {
+            f32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[4 * g + i], sl, -lse[4 * g + i]));
+            if (t >= t_mask) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[i] = key <= s_last[8 * g + 4 * half + i] ? w[i] : 0.0f;
+            }
+            sum += (w[0] + w[1]) + (w[2] + w[3]);
+          }
+        }
+        sum += __shfl_xor(sum, 32);
+        if (half == 0 && key < L) scores[key] = o + sum;
+      };
+      int t = kWaves * s0 + wave;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) fetch(t + u * kWaves, kraw[u], old[u]);
+      for (; t < t_end; t += kAhead * kWaves) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          if (t + u * kWaves < t_end) add_up(t + u * kWaves, kraw[u], old[u]);
+          fetch(t + (u + kAhead) * kWaves, kraw[u], old[u]);
+        }
       }
     }
-    if (in) {
-      float* dst = p.scores + int64_t(b) * p.seq_stride + int64_t(h) * p.head_stride + key;
-      *dst = p.decay == 0.0f ? total : *dst * p.decay + total;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// many rows
+// ---------------------------------------------------------------------------
+
+// e4m3 queries of all rows, [total_q][Hq][128], sixteen elements a thread.
+template <int Q_DT>
+__global__ void __launch_bounds__(kThreads) quantize_queries_kernel(WeightArgs p, int num_q_heads, uint8_t* q8) {
+  const DecodeArgs& a = p.a;
+  const int64_t x = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t row = x >> 3;
+  const int tok = int(row / num_q_heads), hq = int(row - int64_t(tok) * num_q_heads);
+  if (tok >= p.s.total_q) return;
+  float qd = 1.0f;
+  if (a.qd) {  // the descale of the row's sequence and kv head
+    const int b = a.cu_q ? int(sequence_from(a.cu_q, p.s.num_seqs, 0, tok)) : tok / a.q_len;
+    qd = b < p.s.num_seqs ? descale(a.qd, a.qd_b, a.qd_h, b, hq / a.heads) : 1.0f;
+  }
+  QueryBytes<Q_DT> qb;
+  qb.load(a.q + int64_t(tok) * a.q_tok_stride + int64_t(hq) * a.q_head_stride, 16 * int(x & 7));
+  *reinterpret_cast<u32x4*>(q8 + 16 * x) = qb.quantized(qd, 0u);
+}
+
+// Sixteen values of a lane summed over the 32 lanes of its half, in a fixed
+// order: lane l returns value (l >> 1) & 15.
+__device__ __forceinline__ float sum_lanes(float (&v)[16], int lane) {
+#pragma unroll
+  for (int n = 8; n >= 1; n >>= 1) {
+    const bool up = lane & (2 * n);
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+      v[i] = keep + __shfl_xor(give, 2 * n);
     }
   }
+  return v[0] + __shfl_xor(v[0], 1);
+}
+
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) many_rows_kernel(WeightArgs p) {
+  const DecodeArgs& a = p.a;
+  __shared__ float s_sum[kWaves][kGroup];
+  const int tid = int(threadIdx.x), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, kk = lane & 31;
+  const int G = a.heads;
+  // As many keys to a workgroup as leave `slots` of them; the fewer keys the step
+  // has, the more waves share them (as far as there are row tiles for each).  From
+  // the lengths alone, so that the order of the sums does not depend on a bound.
+  SeqWindow seqs;
+  JobSpace s = p.s;  // (a step of kGroup keys)
+  StepRuns step = step_runs(a, s, seqs, lane);
+  int split = 1;
+  while (split < kWaves && split < p.row_tiles && step.total * split < int64_t(p.slots) * kWaves) split *= 2;
+  s.step_shift += split == 1 ? 2 : split == 2 ? 1 : 0;
+  if (s.num_seqs <= 64) {
+    seqs.price(s, lane);
+    step.total = seqs.total;
+  } else {
+    step = step_runs(a, s, seqs, lane);
+    seqs.b0 = -64;  // (the last window is there, not the first)
+  }
+  // waves w, w + 1 .. of a group of `split` hold the same keys and take the row tiles in turn
+  const int group = wave / split, turn = wave - group * split;
+  for (int64_t x = blockIdx.x; x < step.total; x += gridDim.x) {  // a unit: a workgroup's keys of a kv head
+    int64_t before;
+    const int b = seq_of_unit(a, s, x, seqs, lane, before);
+    const SeqRows r{lane_value(seqs.first, b - seqs.b0), lane_value(seqs.n, b - seqs.b0)};
+    const int full = lane_value(seqs.len, b - seqs.b0), L = min(full, p.s.width);
+    const int units = key_steps(s, L);
+    const int h = int(uniform_div(x - before, units));
+    const int k0 = (int(x - before) - h * units) * (1 << s.step_shift) + group * kGroup;  // the wave's keys
+    const int R = r.n * G, ctx = full - r.n;
+    float* scores = score_row(p, b, h);
+
+    // lane l: 64 bytes of keys l % 32 at d = 64 (l / 32); missing rows and keys past the end as zeros
+    bf16x8 kop[2][8];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int key = k0 + kTile * g + kk;
+      int32_t id = -1;
+      int pi = 0;
+      if (key < L) {
+        pi = page_index(a, key);
+        if (pi < a.bt_width) id = a.block_table[int64_t(b) * a.bt_stride + pi];
+        if (id >= a.num_blocks) id = -1;
+      }
+      const uint8_t* row = a.k + int64_t(h) * a.k_head + 64 * half + int64_t(id) * a.k_blk +
+                           int64_t(key - pi * a.block_size) * a.k_row;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const u32x4 v = id >= 0 ? *reinterpret_cast<const u32x4*>(row + 16 * q) : u32x4(0);
+        kop[g][2 * q] = e4m3x8_to_bf16(v[0], v[1]);
+        kop[g][2 * q + 1] = e4m3x8_to_bf16(v[2], v[3]);
+      }
+    }
+    const float sl = score_scale(p.scale_log2, descale(a.qd, a.qd_b, a.qd_h, b, h), descale(a.kd, a.kd_b, a.kd_h, b, h));
+
+    float acc[2][16];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[g][i] = 0.0f;
+    // row tiles from the first that holds a token that sees the first key
+    const int tiles = (R + kRows - 1) / kRows;
+    const int first = (a.causal && k0 > ctx ? int(min(int64_t(k0 - ctx) * G, int64_t(R))) / kRows : 0) + turn;
+    const int di = kRows * split / G, dg = kRows * split - di * G;
+    int i = (first * kRows + kk) / G, g = first * kRows + kk - i * G;  // the lane's row of the tile fetched next
+    u32x4 qraw[4];
+    float lse = 0.0f;
+    int last = 0;
+    auto fetch = [&](int tile, u32x4 (&q)[4], float& ls, int& lim) {
+      const bool live = tile < tiles && i < r.n;
+      const int64_t tok = int64_t(r.first) + i;
+      const uint8_t* src = p.q8 + tok * p.q8_tok + int64_t(h * G + g) * p.q8_head + 64 * half;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) q[u] = live ? *reinterpret_cast<const u32x4*>(src + 16 * u) : u32x4(0);
+      ls = live ? p.lse[int64_t(h * G + g) * p.lse_head_stride + tok] : __builtin_inff();
+      lim = live ? (a.causal ? ctx + i : full - 1) : -1;
+      i += di;
+      g += dg;
+      if (g >= G) {
+        g -= G;
+        ++i;
+      }
+    };
+    if (first < tiles) fetch(first, qraw, lse, last);
+    for (int tile = first; tile < tiles; tile += split) {
+      u32x4 qnext[4];
+      float lse_next;
+      int last_next;
+      fetch(tile + split, qnext, lse_next, last_next);
+      f32x16 y[2] = {};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bf16x8 q0 = e4m3x8_to_bf16(qraw[q][0], qraw[q][1]), q1 = e4m3x8_to_bf16(qraw[q][2], qraw[q][3]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          y[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[u][2 * q], q0, y[u], 0, 0, 0);
+          y[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[u][2 * q + 1], q1, y[u], 0, 0, 0);
+        }
+      }
+      // lse log2(e), in two parts so that it is rounded once
+      const float lse2 = __builtin_fmaf(lse, 0x1.715476p+0f, lse * 0x1.4ae0cp-26f);
+      const bool masked = !__all(last >= k0 + kGroup - 1);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          float w = __builtin_amdgcn_exp2f(__builtin_fmaf(y[u][n], sl, -lse2));
+          if (masked) w = k0 + kTile * u + 8 * (n >> 2) + 4 * half + (n & 3) <= last ? w : 0.0f;
+          acc[u][n] += w;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) qraw[q] = qnext[q];
+      lse = lse_next;
+      last = last_next;
+    }
+
+    // the key of the lane's sum, two lanes a key
+    const int idx = (lane >> 1) & 15, key_of = 8 * (idx >> 2) + 4 * half + (idx & 3);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float total = sum_lanes(acc[u], lane);
+      const int key = k0 + kTile * u + key_of;
+      if (split > 1) {
+        if ((lane & 1) == 0) s_sum[wave][kTile * u + key_of] = total;
+      } else if ((lane & 1) == 0 && key < L) {
+        scores[key] = decayed(p, scores + key) + total;
+      }
+    }
+    if (split > 1) {
+      __syncthreads();
+      if (turn == 0) {  // the group's first wave joins its waves' sums
+        const int key = k0 + lane;
+        float total = s_sum[wave][lane];
+        for (int w = 1; w < split; ++w) total += s_sum[wave + w][lane];
+        if (key < L) scores[key] = decayed(p, scores + key) + total;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+int64_t weight_cus() {
+  static std::mutex mu;
+  static std::map<int, int64_t> cache;
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = cache.find(dev);
+  if (it != cache.end()) return it->second;
+  int cus = 0;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
+  return cache[dev] = cus;
+}
+
+template <int Q_DT>
+int quantize_queries(const WeightArgs& p, int64_t total_q, int64_t num_q_heads, uint8_t* q8, hipStream_t st) {
+  hipLaunchKernelGGL((quantize_queries_kernel<Q_DT>), dim3(unsigned(ceil_div(total_q * num_q_heads * 8, kThreads))),
+                     dim3(kThreads), 0, st, p, int(num_q_heads), q8);
+  return check_launch("quantize_queries_kernel launch");
+}
+
+template <int Q_DT>
+int launch_few_rows(const WeightArgs& p, hipStream_t st) {
+  hipLaunchKernelGGL((few_rows_kernel<Q_DT>), dim3(unsigned(p.s.max_runs)), dim3(kThreads), 0, st, p);
+  return check_launch("few_rows_kernel launch");
 }
 
 }  // namespace
 
 extern "C" {
+
+int64_t psk_attention_weights_workspace_bytes(int64_t total_q, int64_t max_seqlen_q, int64_t num_q_heads,
+                                              int64_t num_kv_heads, int q_dtype) {
+  if (total_q < 0 || max_seqlen_q <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
+      max_seqlen_q > INT32_MAX / (num_q_heads / num_kv_heads) || total_q > INT32_MAX / num_q_heads)
+    return PSK_E_ARG;
+  const bool few = max_seqlen_q * (num_q_heads / num_kv_heads) <= kRows;
+  return few || q_dtype == PSK_DTYPE_FP8_E4M3FN ? 0 : 16 + total_q * num_q_heads * kHead;
+}
 
 int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, int64_t scores_head_stride,
                                      int64_t scores_width, const void* q, int64_t q_tok_stride, int64_t q_head_stride,
@@ -94,7 +462,7 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
                                      int64_t num_blocks, int64_t max_seq_len, int64_t total_q, int64_t max_seqlen_q,
                                      const int32_t* cu_seqlens_q, int causal, float softmax_scale, float decay,
                                      const float* q_descale, const float* k_descale, const int64_t* descale_strides,
-                                     void* stream) {
+                                     void* workspace, int64_t workspace_bytes, void* stream) {
   begin_device_call();
   const CachedQueries c{q, q_tok_stride, q_head_stride, q_dtype, k_cache, k_strides, block_table, block_table_stride,
                         block_table_width, seq_lens, num_seqs, num_q_heads, num_kv_heads, head_size, block_size,
@@ -115,22 +483,65 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
   a.kd_b = ds[2];
   a.kd_h = ds[3];
   a.causal = causal ? 1 : 0;
-  p.total_q = int32_t(total_q);
+  p.s.num_seqs = int32_t(num_seqs);
+  p.s.total_q = int32_t(total_q);
+  p.s.heads = int32_t(num_kv_heads);
+  p.s.idle = decay != 1.0f;
+  p.s.width = int32_t(std::min<int64_t>(scores_width, INT32_MAX - 1024));
+  p.scale_log2 = double(softmax_scale) * 1.4426950408889634;
   p.lse = lse;
   p.lse_head_stride = lse_head_stride;
   p.scores = scores;
   p.seq_stride = scores_seq_stride;
   p.head_stride = scores_head_stride;
-  p.width = int32_t(scores_width);
   p.decay = decay;
-  p.scale_log2 = double(softmax_scale) * 1.4426950408889634;
-  if (num_seqs > 65535 || num_kv_heads > 65535) return fail(PSK_E_ARG, "too many sequences or heads");
-  const int64_t keys = max_seq_len < scores_width ? max_seq_len : scores_width;
-  const int64_t blocks = ceil_div(keys, 256) < 256 ? ceil_div(keys, 256) : 256;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(attention_weights_kernel, dim3(unsigned(blocks > 0 ? blocks : 1), unsigned(num_kv_heads), unsigned(num_seqs)),
-                     dim3(256), 0, st, p, q_dtype);
-  return check_launch("attention_weights_kernel launch");
+  const int64_t cus = weight_cus();
+  const int64_t rows = max_seqlen_q * a.heads;
+  if (rows <= kRows) {
+    p.s.step_shift = kStepShift;
+    p.s.over = 1;
+    p.s.min_run = 2;
+    p.s.max_runs = int32_t(3 * cus);  // resident at once
+    switch (q_dtype) {
+      case PSK_DTYPE_FP8_E4M3FN: return launch_few_rows<PSK_DTYPE_FP8_E4M3FN>(p, st);
+      case PSK_DTYPE_BF16: return launch_few_rows<PSK_DTYPE_BF16>(p, st);
+      case PSK_DTYPE_F16: return launch_few_rows<PSK_DTYPE_F16>(p, st);
+      default: return launch_few_rows<PSK_DTYPE_F32>(p, st);
+    }
+  }
+  const int64_t need = psk_attention_weights_workspace_bytes(total_q, max_seqlen_q, num_q_heads, num_kv_heads, q_dtype);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(PSK_E_WORKSPACE, "workspace of %lld bytes, need %lld", (long long)workspace_bytes, (long long)need);
+  if (need > 0) {
+    uint8_t* q8 = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
+    p.q8 = q8;
+    p.q8_tok = num_q_heads * kHead;
+    p.q8_head = kHead;
+    int e = PSK_OK;
+    if (total_q > 0) {
+      switch (q_dtype) {
+        case PSK_DTYPE_BF16: e = quantize_queries<PSK_DTYPE_BF16>(p, total_q, num_q_heads, q8, st); break;
+        case PSK_DTYPE_F16: e = quantize_queries<PSK_DTYPE_F16>(p, total_q, num_q_heads, q8, st); break;
+        default: e = quantize_queries<PSK_DTYPE_F32>(p, total_q, num_q_heads, q8, st); break;
+      }
+    }
+    if (e != PSK_OK) return e;
+  } else {
+    p.q8 = reinterpret_cast<const uint8_t*>(a.q);
+    p.q8_tok = a.q_tok_stride;
+    p.q8_head = a.q_head_stride;
+  }
+  const int64_t keys = std::max<int64_t>(1, std::min(max_seq_len, scores_width));
+  p.row_tiles = int32_t(ceil_div(rows, kRows));
+  p.slots = int32_t(2 * cus);  // resident at once
+  p.s.step_shift = log2_exact(kGroup);
+  p.s.over = 0;
+  p.s.min_run = 1;
+  p.s.max_runs = 1;
+  const int64_t most = num_seqs * num_kv_heads * ceil_div(keys, kGroup);
+  hipLaunchKernelGGL(many_rows_kernel, dim3(unsigned(std::min<int64_t>(most, 4 * p.slots))), dim3(kThreads), 0, st, p);
+  return check_launch("many_rows_kernel launch");
 }
 
 }  // extern "C"

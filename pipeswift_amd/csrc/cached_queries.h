@@ -103,30 +103,66 @@ __device__ __forceinline__ float score_scale(double scale_log2, float qd, float 
   return float(scale_log2 * double(qd) * double(kd));
 }
 
+// Sixteen elements of a query row, loaded and then quantized to their e4m3 bytes
+// (zeros without a row).
+template <int Q_DT>
+struct QueryBytes {
+  static constexpr int kEsz = Q_DT == PSK_DTYPE_F32 ? 4 : Q_DT == PSK_DTYPE_FP8_E4M3FN ? 1 : 2;
+  u32x4 x[kEsz];
+  bool live;
+  __device__ __forceinline__ void load(const char* src, int d0) {
+    live = src != nullptr;
+#pragma unroll
+    for (int i = 0; i < kEsz; ++i) x[i] = live ? reinterpret_cast<const u32x4*>(src + d0 * kEsz)[i] : u32x4(0);
+  }
+  __device__ __forceinline__ u32x4 quantized(float qd, uint32_t sign) const {
+    u32x4 y;
+    if constexpr (Q_DT == PSK_DTYPE_FP8_E4M3FN) {
+      y = x[0];
+    } else {
+      using QC = QuantConv<Q_DT, 16 / kEsz, kNanTorch>;
+      const QScale qs = make_qscale(qd);
+      uint8_t bytes[16];
+#pragma unroll
+      for (int i = 0; i < kEsz; ++i) {
+        const typename QC::Out z = QC::apply(x[i], qs);
+        __builtin_memcpy(bytes + 16 / kEsz * i, &z, 16 / kEsz);
+      }
+      __builtin_memcpy(&y, bytes, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = live ? y[i] ^ sign : 0u;
+    return y;
+  }
+};
+
 // ---------------------------------------------------------------------------
 // a step's work cut into equal runs
 // ---------------------------------------------------------------------------
 //
 // A job is a kv head of a sequence with query tokens; it costs `over` units and
-// one for every kStepKeys keys.  Jobs follow each other by sequence and head, and
+// one for every step of 1 << step_shift keys.  Jobs follow each other by sequence and head, and
 // run j takes the units [j q, (j + 1) q).  Every wave scans the lengths itself,
 // 64 sequences at a time and a sequence a lane, so that no launch and no memory
 // goes before the kernels and any number of sequences is taken.
 
-constexpr int kStepKeys = 128;
-
 struct JobSpace {
   int32_t num_seqs, total_q, heads;  // kv heads
+  int32_t step_shift;
   int32_t over;                      // units a job costs beside its keys
   int32_t max_runs;
   int32_t min_run;                   // units a run has at least
+  int32_t idle;                      // sequences without query tokens are jobs too
+  int32_t width;                     // keys past it cost nothing
 };
 
 // A sequence's length, kept where the arithmetic on whole tiles of it stays in 31 bits.
 __device__ __forceinline__ int32_t cached_len(const DecodeArgs& a, int b) {
-  return min(max(a.seq_lens[b], 0), INT32_MAX - 2 * kStepKeys);
+  return min(max(a.seq_lens[b], 0), INT32_MAX - 1024);
 }
-__device__ __forceinline__ int32_t key_steps(int32_t len) { return (len + kStepKeys - 1) / kStepKeys; }
+__device__ __forceinline__ int32_t key_steps(const JobSpace& s, int32_t len) {
+  return (len + (1 << s.step_shift) - 1) >> s.step_shift;
+}
 
 template <class T>
 __device__ __forceinline__ T lane_value(T x, int lane) {
@@ -163,7 +199,10 @@ struct SeqWindow {
       n = r.n;
       len = cached_len(a, from + lane);
     }
-    cost = n > 0 ? int64_t(s.over + key_steps(len)) * s.heads : 0;
+    price(s, lane);
+  }
+  __device__ __forceinline__ void price(const JobSpace& s, int lane) {
+    cost = n > 0 || (s.idle && b0 + lane < s.num_seqs) ? int64_t(s.over + key_steps(s, min(len, s.width))) * s.heads : 0;
     int64_t v = cost;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -220,14 +259,12 @@ __device__ __forceinline__ int64_t units_before(const DecodeArgs& a, const JobSp
   }
 }
 
-// The 16-byte chunks of one cached row of a kv head, or nullptr where the page is missing.
-__device__ __forceinline__ const uint8_t* cached_row(const DecodeArgs& a, const uint8_t* base, int64_t blk, int64_t row,
-                                                     int b, int key) {
-  const int pi = page_index(a, key);
-  if (pi >= a.bt_width) return nullptr;
-  const int32_t id = a.block_table[int64_t(b) * a.bt_stride + pi];
-  if (id < 0 || id >= a.num_blocks) return nullptr;
-  return base + id * blk + int64_t(key - pi * a.block_size) * row;
+// Steps [from, to) of a job of `steps` that the units [lo, hi) of it pay for.
+struct Piece {
+  int32_t from, to;
+};
+__device__ __forceinline__ Piece piece_of(const JobSpace& s, int64_t lo, int64_t hi) {
+  return Piece{int32_t(max(lo - s.over, int64_t(0))), int32_t(max(hi - s.over, int64_t(0)))};
 }
 
 }  // namespace psk_detail

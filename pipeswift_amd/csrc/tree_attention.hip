@@ -46,6 +46,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kRows = 32;                  // query rows of a workgroup
+constexpr int kStepShift = 7;
 constexpr int kTile = 32;                  // keys of a tile
 constexpr uint32_t kHalfSlot = kTile * 128;  // bytes of a tile's K (its V follows)
 constexpr uint32_t kSlot = 2 * kHalfSlot;
@@ -53,7 +54,8 @@ constexpr int kRing = 2;
 constexpr int kPages = 1024;               // page ids a piece stages at a time
 constexpr int kSlab = 4096 + 64;           // floats of 32 rows' partial result: accumulators, maxima, sums
 constexpr int kMaxSlots = 512;             // resident workgroups the workspace is sized for
-static_assert(kStepKeys == kTile * kWaves, "a step is a tile a wave");
+constexpr int kStepKeys = kTile * kWaves;  // of a step: a tile a wave
+static_assert(kStepKeys == 1 << kStepShift, "");
 static_assert(kPages >= kStepKeys + 1, "a step's pages fit, whatever the page size");
 
 struct TreeArgs {
@@ -95,14 +97,6 @@ __device__ __forceinline__ void load_tile(uint32_t slot, const uint8_t* const (&
       : "memory");
 }
 
-// Steps [from, to) of a job of `steps` that the units [lo, hi) of it pay for.
-struct Piece {
-  int32_t from, to;
-};
-__device__ __forceinline__ Piece piece_of(const JobSpace& s, int64_t lo, int64_t hi) {
-  return Piece{int32_t(max(lo - s.over, int64_t(0))), int32_t(max(hi - s.over, int64_t(0)))};
-}
-
 // Visibility of keys key0 .. key0 + 31 (bit k: key0 + k) to a drafted token with mask m, of n after `ctx` keys.
 __device__ __forceinline__ uint32_t visible(const int64_t* m, int ctx, int n, int key0) {
   const int j0 = key0 - ctx;  // the drafted index of key0
@@ -116,39 +110,6 @@ __device__ __forceinline__ uint32_t visible(const int64_t* m, int ctx, int n, in
   if (sh > 32 && left > 64 - sh) bits |= uint64_t(m[w + 1]) << (64 - sh);
   return uint32_t(bits) & in;
 }
-
-// Sixteen elements of a query row, loaded and then quantized to their e4m3 bytes
-// (zeros without a row).
-template <int Q_DT>
-struct QueryBytes {
-  static constexpr int kEsz = Q_DT == PSK_DTYPE_F32 ? 4 : Q_DT == PSK_DTYPE_FP8_E4M3FN ? 1 : 2;
-  u32x4 x[kEsz];
-  bool live;
-  __device__ __forceinline__ void load(const char* src, int d0) {
-    live = src != nullptr;
-#pragma unroll
-    for (int i = 0; i < kEsz; ++i) x[i] = live ? reinterpret_cast<const u32x4*>(src + d0 * kEsz)[i] : u32x4(0);
-  }
-  __device__ __forceinline__ u32x4 quantized(float qd, uint32_t sign) const {
-    u32x4 y;
-    if constexpr (Q_DT == PSK_DTYPE_FP8_E4M3FN) {
-      y = x[0];
-    } else {
-      using QC = QuantConv<Q_DT, 16 / kEsz, kNanTorch>;
-      const QScale qs = make_qscale(qd);
-      uint8_t bytes[16];
-#pragma unroll
-      for (int i = 0; i < kEsz; ++i) {
-        const typename QC::Out z = QC::apply(x[i], qs);
-        __builtin_memcpy(bytes + 16 / kEsz * i, &z, 16 / kEsz);
-      }
-      __builtin_memcpy(&y, bytes, 16);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = live ? y[i] ^ sign : 0u;
-    return y;
-  }
-};
 
 template <int OUT_DT>
 __device__ __forceinline__ void store4(char* dst, f32x4 v) {
@@ -230,7 +191,7 @@ tree_attention_kernel(TreeArgs p) {
     if (!seqs.holds(b)) seqs.load(a, p.s, b, lane);
     const SeqRows r{lane_value(seqs.first, b - seqs.b0), lane_value(seqs.n, b - seqs.b0)};
     const int L = lane_value(seqs.len, b - seqs.b0);
-    const int steps = key_steps(L);
+    const int steps = key_steps(p.s, L);
     const int64_t job_cost = p.s.over + steps;
     const int64_t seq_end = before + (r.n > 0 ? job_cost * p.s.heads : 0);
     if (x >= seq_end) {
@@ -574,7 +535,7 @@ __global__ void __launch_bounds__(256) merge_tree_kernel(TreeArgs p) {
   SeqWindow seqs;
   const StepRuns cost = step_runs(a, p.s, seqs, lane);
   const int64_t before = units_before(a, p.s, b, seqs, lane);
-  const int steps = key_steps(lane_value(seqs.len, b - seqs.b0));
+  const int steps = key_steps(p.s, lane_value(seqs.len, b - seqs.b0));
   const int64_t at = before + h * int64_t(p.s.over + steps) + p.s.over;  // the first unit that pays for keys
   const int64_t j0 = uniform_div(at, cost.run), j1 = steps > 0 ? uniform_div(at + steps - 1, cost.run) : j0 - 1;
   if (j0 == j1) return;  // one run had all the keys and wrote the rows
@@ -728,9 +689,11 @@ int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head
   p.s.num_seqs = int32_t(num_seqs);
   p.s.total_q = int32_t(total_q);
   p.s.heads = int32_t(num_kv_heads);
+  p.s.step_shift = kStepShift;
   p.s.over = 1;
   p.s.max_runs = int32_t(s.max_runs);
   p.s.min_run = 2;
+  p.s.width = INT32_MAX;
   p.row_blocks = int32_t(s.row_blocks);
   p.records = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
   if (num_seqs * num_kv_heads * s.row_blocks > INT32_MAX / 16 || s.max_runs * s.row_blocks > INT32_MAX)
