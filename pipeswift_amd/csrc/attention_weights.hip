@@ -10,8 +10,9 @@
 //   * few_rows_kernel, at most 32 of them (a decode step): a wave per 32 keys,
 //     S = Q K^T on v_mfma_f32_32x32x16_bf16 leaves lane l key l % 32 and rows
 //     8 (i / 4) + 4 (l / 32) + i % 4, so a key's sum is one lane's registers and
-//     one exchange.  The K rows go from memory to registers, two tiles ahead;
-//     the work is cut into equal runs (cached_queries.h).
+//     one exchange.  The K rows go from memory to registers, two tiles ahead, the
+//     kv heads of a token together; the work is cut into equal runs
+//     (cached_queries.h).
 //   * many_rows_kernel, more (the last queries of a prompt, a whole prompt): a
 //     wave holds 64 keys as MFMA operands and the step's e4m3 queries, quantized
 //     once by quantize_queries_kernel, pass by it 32 rows at a time.  S^T = K Q^T
@@ -38,7 +39,10 @@ constexpr int kTile = 32;    // keys of an MFMA tile
 constexpr int kRows = 32;    // query rows of one
 constexpr int kAhead = 2;    // tiles of K in flight (few rows)
 constexpr int kPages = 1024; // page ids staged at a time (few rows)
-constexpr int kGroup = 2 * kTile;  // keys a wave holds (many rows)
+constexpr int kFewRows = 256;  // query rows of a job's heads, each padded to whole groups (few rows)
+constexpr int kManyWaves = 4;  // (many rows)
+constexpr int kHeld = 2;     // tiles of keys a wave holds (many rows)
+constexpr int kGroup = kHeld * kTile;
 constexpr int kStepShift = 7;
 constexpr int kStepKeys = kTile * kWaves;  // of a step (few rows): a tile a wave
 static_assert(kStepKeys == 1 << kStepShift, "");
@@ -54,6 +58,7 @@ struct WeightArgs {
   float decay;
   const uint8_t* q8;  // many rows: e4m3 queries [total_q][Hq][128]
   int64_t q8_tok, q8_head;
+  int32_t hg;         // few rows: kv heads of a job
   int32_t row_tiles;  // many rows: most of any sequence
   int32_t slots;      // many rows: workgroups that fill the GPU
 };
@@ -75,20 +80,24 @@ __device__ __forceinline__ float decayed(const WeightArgs& p, const float* at) {
 // few rows
 // ---------------------------------------------------------------------------
 
+// A job here is a sequence's keys under `hg` kv heads; `heads` of the JobSpace
+// counts its groups of them.  A workgroup's waves take the (tile, head) pairs of
+// a run in turn, heads first, so that the rows of a token's heads, which lie next
+// to each other, are read together.
 template <int Q_DT>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(3)))
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4)))
 few_rows_kernel(WeightArgs p) {
   const DecodeArgs& a = p.a;
   __shared__ int32_t s_pages[kPages];
-  __shared__ u32x4 s_q[kRows * 8];  // the rows' e4m3 queries, chunk c of row r at c ^ (r & 7)
-  __shared__ float s_lse[kRows];    // of each row; +inf for rows without a token
-  __shared__ int32_t s_last[kRows];  // the last key each row sees
+  __shared__ u32x4 s_q[kFewRows * 8];  // e4m3 queries, [head][padded row], chunk c of row r at c ^ (r & 7)
+  __shared__ f32x4 s_lse[kFewRows / 4];  // of each row; +inf for rows without a token
+  __shared__ float s_sl[kFewRows / 8];   // of each head
   const int tid = int(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, kk = lane & 31;
   SeqWindow seqs;
   const StepRuns step_run = step_runs(a, p.s, seqs, lane);
-  int64_t x = int64_t(blockIdx.x) * step_run.run;
+  int64_t x = xcd_run(step_run, int(blockIdx.x) & 7, int(blockIdx.x) >> 3) * step_run.run;
   if (x >= step_run.total) return;
   const int64_t x_end = min(x + step_run.run, step_run.total);
   int64_t before;
@@ -104,50 +113,41 @@ few_rows_kernel(WeightArgs p) {
       continue;
     }
     const int64_t job_cost = p.s.over + key_steps(p.s, L);
-    const int h = int(uniform_div(x - before, job_cost));
-    const int64_t at = before + h * job_cost;
+    const int job = int(uniform_div(x - before, job_cost));
+    const int64_t at = before + job * job_cost;
     const int64_t hi = min(x_end, at + job_cost);
     const Piece c = piece_of(p.s, x - at, hi - at);
     x = hi;
     if (c.from >= c.to) continue;
+    const int h0 = job * p.hg, heads = min(p.hg, a.num_kv_heads - h0);
 
-    float* scores = score_row(p, b, h);
     if (r.n <= 0) {  // the old sums decay all the same
-      for (int key = c.from * kStepKeys + tid; key < min(L, c.to * kStepKeys); key += kThreads)
-        scores[key] = decayed(p, scores + key);
+      for (int h = h0; h < h0 + heads; ++h) {
+        float* scores = score_row(p, b, h);
+        for (int key = c.from * kStepKeys + tid; key < min(L, c.to * kStepKeys); key += kThreads)
+          scores[key] = decayed(p, scores + key);
+      }
       continue;
     }
-    const int first_page = page_index(a, c.from * kStepKeys);
-    int32_t page0 = -1;
-    if (first_page + tid < a.bt_width) page0 = a.block_table[int64_t(b) * a.bt_stride + first_page + tid];
     const int R = r.n * a.heads, ctx = full - r.n;
-    QueryBytes<Q_DT> qb;
-    {
-      const int qr = tid >> 3, qi = qr / a.heads;
-      qb.load(qr < R ? a.q + (int64_t(r.first) + qi) * a.q_tok_stride + int64_t(h * a.heads + qr - qi * a.heads) * a.q_head_stride
-                     : nullptr, 16 * (tid & 7));
+    const int groups = (R + 7) >> 3, padded = 8 * groups;  // register groups of four (of each half) that hold rows
+    __syncthreads();  // readers of the last piece's queries are done
+    for (int i = tid; i < heads * padded * 8; i += kThreads) {
+      const int row = i >> 3, hh = row / padded, rr = row - hh * padded;
+      const int qi = rr / a.heads, h = h0 + hh, hq = h * a.heads + rr - qi * a.heads;
+      const float qd = descale(a.qd, a.qd_b, a.qd_h, b, h);
+      QueryBytes<Q_DT> qb;
+      qb.load(rr < R ? a.q + (int64_t(r.first) + qi) * a.q_tok_stride + int64_t(hq) * a.q_head_stride : nullptr, 16 * (i & 7));
+      s_q[row * 8 + ((i & 7) ^ (row & 7))] = qb.quantized(qd, 0u);
+      if ((i & 7) == 0) {
+        reinterpret_cast<float*>(s_lse)[row] = rr < R ? lse_log2(p, hq, int64_t(r.first) + qi) : __builtin_inff();
+        if (rr == 0) s_sl[hh] = score_scale(p.scale_log2, qd, descale(a.kd, a.kd_b, a.kd_h, b, h));
+      }
     }
-    float row_lse = __builtin_inff();
-    int row_last = -1;
-    if (tid < R) {  // (R is at most 32)
-      const int qi = tid / a.heads;
-      row_lse = lse_log2(p, h * a.heads + tid - qi * a.heads, int64_t(r.first) + qi);
-      row_last = a.causal ? ctx + qi : full - 1;
-    }
-    const float qd = descale(a.qd, a.qd_b, a.qd_h, b, h);
-    const float sl = score_scale(p.scale_log2, qd, descale(a.kd, a.kd_b, a.kd_h, b, h));
-    __syncthreads();  // readers of the last piece's queries and ids are done
-    s_q[(tid >> 3) * 8 + ((tid & 7) ^ ((tid >> 3) & 7))] = qb.quantized(qd, 0u);
-    if (tid < kRows) {
-      s_lse[tid] = row_lse;
-      s_last[tid] = row_last;
-    }
-    bf16x8 qop[8];
-    float lse[16];
-    const uint8_t* kbase = a.k + int64_t(h) * a.k_head + 64 * half;
+    // row of this lane in the query operand (rows past the padded ones: any, their results are not used)
+    const int row_k = min(kk, padded - 1);
     const int n_tiles = (L + kTile - 1) / kTile;
     const int t_mask = a.causal ? max(ctx, 0) / kTile : n_tiles;  // tiles below are seen by every row
-    const int groups = (R + 7) >> 3;  // register groups of four that hold rows
     const int steps_per_window = int(min(int64_t(kPages - 1) * a.block_size / kStepKeys, int64_t(1) << 24));
     for (int s0 = c.from; s0 < c.to; s0 += steps_per_window) {
       const int s1 = min(c.to, s0 + steps_per_window);
@@ -155,76 +155,85 @@ few_rows_kernel(WeightArgs p) {
       const int p1 = page_index(a, int(min(int64_t(L), int64_t(s1) * kStepKeys)) - 1);
       if (s0 > c.from) __syncthreads();  // the ids before these are done with
       for (int i = tid; i <= p1 - p0; i += kThreads) {
-        int32_t id = page0;
-        if (s0 > c.from || i >= kThreads) {
-          id = -1;
-          if (p0 + i < a.bt_width) id = a.block_table[int64_t(b) * a.bt_stride + p0 + i];
-        }
+        int32_t id = -1;
+        if (p0 + i < a.bt_width) id = a.block_table[int64_t(b) * a.bt_stride + p0 + i];
         s_pages[i] = id < a.num_blocks ? id : -1;
       }
       __syncthreads();
-      if (s0 == c.from) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const u32x4 v = s_q[kk * 8 + ((4 * half + t) ^ (kk & 7))];
-          qop[2 * t] = e4m3x8_to_bf16(v[0], v[1]);
-          qop[2 * t + 1] = e4m3x8_to_bf16(v[2], v[3]);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) lse[i] = s_lse[8 * (i >> 2) + 4 * half + (i & 3)];
-      }
 
       const int t_end = min(kWaves * s1, n_tiles);
-      u32x4 kraw[kAhead][4];
-      float old[kAhead];
+      struct Place {
+        int t, hh;  // tile and head of the group
+      };
+      auto next = [&](Place& w, int by) {
+        w.hh += by;
+        while (w.hh >= heads) {
+          w.hh -= heads;
+          ++w.t;
+        }
+      };
       // lane l: 64 bytes of key l % 32 at d = 64 (l / 32); missing rows and keys past the end as zeros
-      auto fetch = [&](int t, u32x4 (&k)[4], float& o) {
-        const int key = t * kTile + kk;
-        const bool in = t < t_end && key < L;
+      auto fetch = [&](const Place& w, u32x4 (&k)[4], float& o) {
+        const int key = w.t * kTile + kk;
+        const bool in = w.t < t_end && key < L;
         int32_t id = -1;
         int pi = 0;
         if (in) {
           pi = page_index(a, key);
           id = s_pages[pi - p0];
         }
-        o = in && half == 0 ? decayed(p, scores + key) : 0.0f;
-        const uint8_t* row = kbase + (int64_t(id) * a.k_blk + int64_t(key - pi * a.block_size) * a.k_row);
+        o = in && half == 0 ? decayed(p, score_row(p, b, h0 + w.hh) + key) : 0.0f;
+        const uint8_t* row = a.k + int64_t(h0 + w.hh) * a.k_head + 64 * half +
+                             (int64_t(id) * a.k_blk + int64_t(key - pi * a.block_size) * a.k_row);
 #pragma unroll
         for (int q = 0; q < 4; ++q) k[q] = id >= 0 ? *reinterpret_cast<const u32x4*>(row + 16 * q) : u32x4(0);
       };
-      auto add_up = [&](int t, const u32x4 (&k)[4], float o) {
+      auto add_up = [&](const Place& w, const u32x4 (&k)[4], float o) {
         f32x16 y = {};
+        const int row = w.hh * padded + row_k;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qop[2 * q], e4m3x8_to_bf16(k[q][0], k[q][1]), y, 0, 0, 0);
-          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qop[2 * q + 1], e4m3x8_to_bf16(k[q][2], k[q][3]), y, 0, 0, 0);
+          const u32x4 v = s_q[row * 8 + ((4 * half + q) ^ (row & 7))];
+          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16(v[0], v[1]), e4m3x8_to_bf16(k[q][0], k[q][1]), y, 0, 0, 0);
+          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16(v[2], v[3]), e4m3x8_to_bf16(k[q][2], k[q][3]), y, 0, 0, 0);
         }
-        const int key = t * kTile + kk;
+        const int key = w.t * kTile + kk;
+        const float sl = s_sl[w.hh];
         float sum = 0.0f;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           if (g < groups) {
-            f32x4 w;
+            const f32x4 lse = s_lse[(w.hh * padded + 8 * g + 4 * half) >> 2];
+            f32x4 e;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[4 * g + i], sl, -lse[4 * g + i]));
-            if (t >= t_mask) {
+            for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[4 * g + i], sl, -lse[i]));
+            if (w.t >= t_mask) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) w[i] = key <= s_last[8 * g + 4 * half + i] ? w[i] : 0.0f;
+              for (int i = 0; i < 4; ++i) e[i] = key <= ctx + (8 * g + 4 * half + i) / a.heads ? e[i] : 0.0f;
             }
-            sum += (w[0] + w[1]) + (w[2] + w[3]);
+            sum += (e[0] + e[1]) + (e[2] + e[3]);
           }
         }
         sum += __shfl_xor(sum, 32);
-        if (half == 0 && key < L) scores[key] = o + sum;
+        if (half == 0 && key < L) score_row(p, b, h0 + w.hh)[key] = o + sum;
       };
-      int t = kWaves * s0 + wave;
+      u32x4 kraw[kAhead][4];
+      float old[kAhead];
+      Place now{kWaves * s0, 0};
+      next(now, wave);
+      Place then = now;  // the pair fetched next
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) fetch(t + u * kWaves, kraw[u], old[u]);
-      for (; t < t_end; t += kAhead * kWaves) {
+      for (int u = 0; u < kAhead; ++u) {
+        fetch(then, kraw[u], old[u]);
+        next(then, kWaves);
+      }
+      while (now.t < t_end) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          if (t + u * kWaves < t_end) add_up(t + u * kWaves, kraw[u], old[u]);
-          fetch(t + (u + kAhead) * kWaves, kraw[u], old[u]);
+          if (now.t < t_end) add_up(now, kraw[u], old[u]);
+          next(now, kWaves);
+          fetch(then, kraw[u], old[u]);
+          next(then, kWaves);
         }
       }
     }
@@ -268,9 +277,9 @@ __device__ __forceinline__ float sum_lanes(float (&v)[16], int lane) {
   return v[0] + __shfl_xor(v[0], 1);
 }
 
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) many_rows_kernel(WeightArgs p) {
+__global__ void __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_per_eu(2))) many_rows_kernel(WeightArgs p) {
   const DecodeArgs& a = p.a;
-  __shared__ float s_sum[kWaves][kGroup];
+  __shared__ float s_sum[kManyWaves][kGroup];
   const int tid = int(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, kk = lane & 31;
@@ -282,8 +291,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
   JobSpace s = p.s;  // (a step of kGroup keys)
   StepRuns step = step_runs(a, s, seqs, lane);
   int split = 1;
-  while (split < kWaves && split < p.row_tiles && step.total * split < int64_t(p.slots) * kWaves) split *= 2;
-  s.step_shift += split == 1 ? 2 : split == 2 ? 1 : 0;
+  while (split < kManyWaves && split < p.row_tiles && step.total * split < int64_t(p.slots) * kManyWaves) split *= 2;
+  for (int w = split; w < kManyWaves; w *= 2) ++s.step_shift;
   if (s.num_seqs <= 64) {
     seqs.price(s, lane);
     step.total = seqs.total;
@@ -305,9 +314,9 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     float* scores = score_row(p, b, h);
 
     // lane l: 64 bytes of keys l % 32 at d = 64 (l / 32); missing rows and keys past the end as zeros
-    bf16x8 kop[2][8];
+    bf16x8 kop[kHeld][8];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < kHeld; ++g) {
       const int key = k0 + kTile * g + kk;
       int32_t id = -1;
       int pi = 0;
@@ -327,72 +336,89 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     }
     const float sl = score_scale(p.scale_log2, descale(a.qd, a.qd_b, a.qd_h, b, h), descale(a.kd, a.kd_b, a.kd_h, b, h));
 
-    float acc[2][16];
+    float acc[kHeld][16];
 #pragma unroll
-    for (int g = 0; g < 2; ++g)
+    for (int g = 0; g < kHeld; ++g)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[g][i] = 0.0f;
     // row tiles from the first that holds a token that sees the first key
     const int tiles = (R + kRows - 1) / kRows;
     const int first = (a.causal && k0 > ctx ? int(min(int64_t(k0 - ctx) * G, int64_t(R))) / kRows : 0) + turn;
+    // The lane's row of the tile fetched next: token i, head g, where its query
+    // and its lse lie, and how far the wave's next tile is (a wrap of the heads
+    // is the next token).
     const int di = kRows * split / G, dg = kRows * split - di * G;
-    int i = (first * kRows + kk) / G, g = first * kRows + kk - i * G;  // the lane's row of the tile fetched next
-    u32x4 qraw[4];
-    float lse = 0.0f;
-    int last = 0;
-    auto fetch = [&](int tile, u32x4 (&q)[4], float& ls, int& lim) {
-      const bool live = tile < tiles && i < r.n;
-      const int64_t tok = int64_t(r.first) + i;
-      const uint8_t* src = p.q8 + tok * p.q8_tok + int64_t(h * G + g) * p.q8_head + 64 * half;
+    int i = (first * kRows + kk) / G, g = first * kRows + kk - i * G;
+    const uint8_t* q_at = p.q8 + (int64_t(r.first) + i) * p.q8_tok + int64_t(h * G + g) * p.q8_head + 64 * half;
+    const float* lse_at = p.lse + int64_t(h * G + g) * p.lse_head_stride + r.first + i;
+    const int64_t q_step = di * p.q8_tok + dg * p.q8_head, q_wrap = p.q8_tok - G * p.q8_head;
+    const int64_t lse_step = di + dg * p.lse_head_stride, lse_wrap = 1 - G * p.lse_head_stride;
+    struct Rows {
+      u32x4 q[4];
+      float lse;
+      int last;  // the last key the row sees, -1 for none
+    };
+    auto fetch = [&](Rows& t) {
+      const bool live = i < r.n;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) q[u] = live ? *reinterpret_cast<const u32x4*>(src + 16 * u) : u32x4(0);
-      ls = live ? p.lse[int64_t(h * G + g) * p.lse_head_stride + tok] : __builtin_inff();
-      lim = live ? (a.causal ? ctx + i : full - 1) : -1;
+      for (int u = 0; u < 4; ++u) t.q[u] = live ? *reinterpret_cast<const u32x4*>(q_at + 16 * u) : u32x4(0);
+      t.lse = live ? *lse_at : __builtin_inff();
+      t.last = live ? (a.causal ? ctx + i : full - 1) : -1;
       i += di;
       g += dg;
+      q_at += q_step;
+      lse_at += lse_step;
       if (g >= G) {
         g -= G;
         ++i;
+        q_at += q_wrap;
+        lse_at += lse_wrap;
       }
     };
-    if (first < tiles) fetch(first, qraw, lse, last);
-    for (int tile = first; tile < tiles; tile += split) {
-      u32x4 qnext[4];
-      float lse_next;
-      int last_next;
-      fetch(tile + split, qnext, lse_next, last_next);
-      f32x16 y[2] = {};
+    auto pass = [&](const Rows& t) {
+      f32x16 y[kHeld] = {};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const bf16x8 q0 = e4m3x8_to_bf16(qraw[q][0], qraw[q][1]), q1 = e4m3x8_to_bf16(qraw[q][2], qraw[q][3]);
+        const bf16x8 q0 = e4m3x8_to_bf16(t.q[q][0], t.q[q][1]), q1 = e4m3x8_to_bf16(t.q[q][2], t.q[q][3]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < kHeld; ++u) {
           y[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[u][2 * q], q0, y[u], 0, 0, 0);
           y[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[u][2 * q + 1], q1, y[u], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
       // lse log2(e), in two parts so that it is rounded once
-      const float lse2 = __builtin_fmaf(lse, 0x1.715476p+0f, lse * 0x1.4ae0cp-26f);
-      const bool masked = !__all(last >= k0 + kGroup - 1);
+      const float lse2 = __builtin_fmaf(t.lse, 0x1.715476p+0f, t.lse * 0x1.4ae0cp-26f);
+      if (__all(t.last >= k0 + kGroup - 1)) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < kHeld; ++u)
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          float w = __builtin_amdgcn_exp2f(__builtin_fmaf(y[u][n], sl, -lse2));
-          if (masked) w = k0 + kTile * u + 8 * (n >> 2) + 4 * half + (n & 3) <= last ? w : 0.0f;
-          acc[u][n] += w;
-        }
+          for (int n = 0; n < 16; ++n) acc[u][n] += __builtin_amdgcn_exp2f(__builtin_fmaf(y[u][n], sl, -lse2));
+      } else {
+        const int limit = t.last - k0 - 4 * half;
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u)
+#pragma unroll
+          for (int n = 0; n < 16; ++n) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(y[u][n], sl, -lse2));
+            acc[u][n] += kTile * u + 8 * (n >> 2) + (n & 3) <= limit ? w : 0.0f;
+          }
       }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) qraw[q] = qnext[q];
-      lse = lse_next;
-      last = last_next;
+    };
+    Rows rows0, rows1;
+    if (first < tiles) fetch(rows0);
+#pragma unroll 1
+    for (int tile = first; tile < tiles; tile += split) {
+      fetch(rows1);
+      __builtin_amdgcn_sched_barrier(0);
+      pass(rows0);
+      rows0 = rows1;
     }
 
     // the key of the lane's sum, two lanes a key
     const int idx = (lane >> 1) & 15, key_of = 8 * (idx >> 2) + 4 * half + (idx & 3);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < kHeld; ++u) {
       const float total = sum_lanes(acc[u], lane);
       const int key = k0 + kTile * u + key_of;
       if (split > 1) {
@@ -405,9 +431,11 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
       __syncthreads();
       if (turn == 0) {  // the group's first wave joins its waves' sums
         const int key = k0 + lane;
-        float total = s_sum[wave][lane];
-        for (int w = 1; w < split; ++w) total += s_sum[wave + w][lane];
-        if (key < L) scores[key] = decayed(p, scores + key) + total;
+        if (lane < kGroup && key < L) {
+          float total = s_sum[wave][lane];
+          for (int w = 1; w < split; ++w) total += s_sum[wave + w][lane];
+          scores[key] = decayed(p, scores + key) + total;
+        }
       }
       __syncthreads();
     }
@@ -502,7 +530,9 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
     p.s.step_shift = kStepShift;
     p.s.over = 1;
     p.s.min_run = 2;
-    p.s.max_runs = int32_t(3 * cus);  // resident at once
+    p.s.max_runs = int32_t(4 * cus);  // resident at once
+    p.hg = int32_t(std::min<int64_t>(num_kv_heads, kFewRows / (8 * ceil_div(rows, 8))));
+    p.s.heads = int32_t(ceil_div(num_kv_heads, p.hg));
     switch (q_dtype) {
       case PSK_DTYPE_FP8_E4M3FN: return launch_few_rows<PSK_DTYPE_FP8_E4M3FN>(p, st);
       case PSK_DTYPE_BF16: return launch_few_rows<PSK_DTYPE_BF16>(p, st);
@@ -540,7 +570,8 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
   p.s.min_run = 1;
   p.s.max_runs = 1;
   const int64_t most = num_seqs * num_kv_heads * ceil_div(keys, kGroup);
-  hipLaunchKernelGGL(many_rows_kernel, dim3(unsigned(std::min<int64_t>(most, 4 * p.slots))), dim3(kThreads), 0, st, p);
+  hipLaunchKernelGGL(many_rows_kernel, dim3(unsigned(std::min<int64_t>(most, 4 * p.slots))),
+                     dim3(64 * kManyWaves), 0, st, p);
   return check_launch("many_rows_kernel launch");
 }
 

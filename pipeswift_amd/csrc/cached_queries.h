@@ -231,6 +231,15 @@ __device__ __forceinline__ StepRuns step_runs(const DecodeArgs& a, const JobSpac
   return c;
 }
 
+// The idx-th run of an XCD.  Workgroup w runs on XCD w % 8, and each XCD takes
+// consecutive runs, so that its L2 sees every kv head of a few sequences (one
+// head's rows lie a token apart and would fall on a part of its channels).  A run
+// past the last comes back as one too.
+__device__ __forceinline__ int64_t xcd_run(const StepRuns& c, int xcd, int idx) {
+  const int64_t runs = uniform_div(c.total + c.run - 1, c.run), per = (runs + 7) >> 3;
+  return idx < per ? xcd * per + idx : runs;
+}
+
 // The sequence that unit x (below the total) falls in, and the units before it.
 __device__ __forceinline__ int seq_of_unit(const DecodeArgs& a, const JobSpace& s, int64_t x, SeqWindow& w, int lane,
                                            int64_t& before) {

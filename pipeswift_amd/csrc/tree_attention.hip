@@ -157,18 +157,11 @@ tree_attention_kernel(TreeArgs p) {
 
   SeqWindow seqs;
   const StepRuns step_run = step_runs(a, p.s, seqs, lane);
-  // Workgroup w runs on XCD w % 8.  Each XCD takes consecutive runs, so that its
-  // L2 sees every kv head of a few sequences (a head's rows lie a token apart and
-  // would fall on a part of its channels), and the row blocks of a run, which
-  // read the same keys, are next to each other.
-  const int w = int(blockIdx.x);
-  const int64_t runs = uniform_div(step_run.total + step_run.run - 1, step_run.run);
-  const int64_t per = (runs + 7) >> 3;
-  const int idx = (w >> 3) / p.row_blocks;
-  const int block = (w >> 3) - idx * p.row_blocks;
-  const int64_t j = (w & 7) * per + idx;
-  if (idx >= per || j >= runs) return;
+  // the row blocks of a run, which read the same keys, are next to each other on its XCD
+  const int w = int(blockIdx.x), idx = (w >> 3) / p.row_blocks, block = (w >> 3) - idx * p.row_blocks;
+  const int64_t j = xcd_run(step_run, w & 7, idx);
   int64_t x = j * step_run.run;
+  if (x >= step_run.total) return;
   const int64_t x_end = min(x + step_run.run, step_run.total);
 
   const uint32_t ring = (uint32_t)(size_t)(lvoid*)s_ring + uint32_t(wave * kRing) * kSlot;
