@@ -10,8 +10,8 @@
 //   * few_rows_kernel, at most 32 of them (a decode step): a wave per 32 keys,
 //     S = Q K^T on v_mfma_f32_32x32x16_bf16 leaves lane l key l % 32 and rows
 //     8 (i / 4) + 4 (l / 32) + i % 4, so a key's sum is one lane's registers and
-//     one exchange.  The K rows go from memory to registers, two tiles ahead, the
-//     kv heads of a token together; the work is cut into equal runs
+//     one exchange.  The K rows go to LDS three tiles ahead, the kv heads of a
+//     token together; the work is cut into equal runs
 //     (cached_queries.h).
 //   * many_rows_kernel, more (the last queries of a prompt, a whole prompt): a
 //     wave holds 64 keys as MFMA operands and the step's e4m3 queries, quantized
@@ -37,9 +37,10 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kTile = 32;    // keys of an MFMA tile
 constexpr int kRows = 32;    // query rows of one
-constexpr int kAhead = 2;    // tiles of K in flight (few rows)
+constexpr uint32_t kHalfSlot = kTile * 128;  // bytes of a tile's K
+constexpr int kFewRing = 4;  // tiles of K a wave has in LDS (few rows)
 constexpr int kPages = 1024; // page ids staged at a time (few rows)
-constexpr int kFewRows = 256;  // query rows of a job's heads, each padded to whole groups (few rows)
+constexpr int kFewRows = 64;   // query rows of a job's heads, each padded to whole groups (few rows)
 constexpr int kManyWaves = 4;  // (many rows)
 constexpr int kHeld = 2;     // tiles of keys a wave holds (many rows)
 constexpr int kGroup = kHeld * kTile;
@@ -84,10 +85,15 @@ __device__ __forceinline__ float decayed(const WeightArgs& p, const float* at) {
 // counts its groups of them.  A workgroup's waves take the (tile, head) pairs of
 // a run in turn, heads first, so that the rows of a token's heads, which lie next
 // to each other, are read together.
-template <int Q_DT>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4)))
+// K goes to LDS by global_load_lds, whole rows at a time (a lane's part of a row
+// read straight to registers makes four requests of every line: 4.0 TB/s against
+// 3.0 without caching), a ring of kFewRing pairs a wave.
+template <int Q_DT, bool OLD, bool GEN>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 few_rows_kernel(WeightArgs p) {
   const DecodeArgs& a = p.a;
+  __shared__ __attribute__((aligned(1024))) char s_ring[kWaves * kFewRing * kHalfSlot];
+  __shared__ float s_old[kWaves * kFewRing * kTile];
   __shared__ int32_t s_pages[kPages];
   __shared__ u32x4 s_q[kFewRows * 8];  // e4m3 queries, [head][padded row], chunk c of row r at c ^ (r & 7)
   __shared__ f32x4 s_lse[kFewRows / 4];  // of each row; +inf for rows without a token
@@ -95,6 +101,11 @@ few_rows_kernel(WeightArgs p) {
   const int tid = int(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, kk = lane & 31;
+  const uint32_t ring = (uint32_t)(size_t)(lvoid*)s_ring + uint32_t(wave * kFewRing) * kHalfSlot;
+  const uint32_t old_at = (uint32_t)(size_t)(lvoid*)s_old + uint32_t(wave * kFewRing * kTile * 4);
+  // loads: lane l takes chunk position l % 8 of keys 8 u + l / 8, chunk c of key t lies at c ^ (t & 7)
+  const int lr = lane >> 3, lchunk = 16 * ((lane & 7) ^ lr);
+  const uint32_t off_k = uint32_t(lr * a.k_row) + lchunk;
   SeqWindow seqs;
   const StepRuns step_run = step_runs(a, p.s, seqs, lane);
   int64_t x = xcd_run(step_run, int(blockIdx.x) & 7, int(blockIdx.x) >> 3) * step_run.run;
@@ -172,30 +183,84 @@ few_rows_kernel(WeightArgs p) {
           ++w.t;
         }
       };
-      // lane l: 64 bytes of key l % 32 at d = 64 (l / 32); missing rows and keys past the end as zeros
-      auto fetch = [&](const Place& w, u32x4 (&k)[4], float& o) {
-        const int key = w.t * kTile + kk;
-        const bool in = w.t < t_end && key < L;
+      // Where the eight keys of a load lie: lane 4 k + u those of load u of tile
+      // win + k, sixteen tiles at a time (GEN: every lane its own key's place).
+      int win = kWaves * s0;
+      int64_t at_k = 0;
+      uint64_t whole8 = 0, some8 = 0;  // loads whose eight keys are all cached; whose first is
+      auto look_up = [&](int t) {
+        win = t;
+        const int key = (t + (lane >> 2)) * kTile + 8 * (lane & 3);
         int32_t id = -1;
         int pi = 0;
-        if (in) {
+        if (t + (lane >> 2) < t_end && key < L) {
           pi = page_index(a, key);
           id = s_pages[pi - p0];
         }
-        o = in && half == 0 ? decayed(p, score_row(p, b, h0 + w.hh) + key) : 0.0f;
-        const uint8_t* row = a.k + int64_t(h0 + w.hh) * a.k_head + 64 * half +
-                             (int64_t(id) * a.k_blk + int64_t(key - pi * a.block_size) * a.k_row);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) k[q] = id >= 0 ? *reinterpret_cast<const u32x4*>(row + 16 * q) : u32x4(0);
+        at_k = int64_t(id) * a.k_blk + int64_t(key - pi * a.block_size) * a.k_row - 1024 * (lane & 3);
+        some8 = __ballot(id >= 0);
+        whole8 = __ballot(id >= 0 && key + 8 <= L);
       };
-      auto add_up = [&](const Place& w, const u32x4 (&k)[4], float o) {
+      // The loads of a pair into a slot: K rows (four), old sums (one).  Pairs whose
+      // loads were not all started are counted out of `sure`, the newest run of
+      // pairs that were.
+      int sure = 0;
+      auto start = [&](const Place& w, int slot_no) {
+        const uint32_t slot = ring + uint32_t(slot_no) * kHalfSlot;
+        const uint8_t* base = a.k + int64_t(h0 + w.hh) * a.k_head;
+        if constexpr (OLD) {
+          const float* sums = reinterpret_cast<const float*>(
+              wave_uniform(int64_t(reinterpret_cast<uintptr_t>(score_row(p, b, h0 + w.hh) + w.t * kTile))));
+          if (half == 0 && w.t * kTile + kk < L) load_lds_dword(old_at + 128 * slot_no, sums, 4 * kk);
+        }
+        bool full;
+        if constexpr (GEN) {
+          const uint8_t* from[4];
+          full = true;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int key = w.t * kTile + 8 * u + lr;
+            const int pi = page_index(a, key);
+            const int32_t id = key < L ? s_pages[pi - p0] : -1;
+            from[u] = id >= 0 ? base + lchunk + (int64_t(id) * a.k_blk + int64_t(key - pi * a.block_size) * a.k_row) : nullptr;
+            full = full && __all(id >= 0);
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (from[u]) load_lds(slot + 1024 * u, from[u]);
+            else *lds_at<u32x4>(slot + 1024 * u + 16 * lane) = u32x4(0);
+          }
+        } else {
+          if (w.t - win >= 16) look_up(w.t);
+          const int k = 4 * (w.t - win);
+          full = ((whole8 >> k) & 15) == 15;
+          if (__builtin_expect(full, 1)) {
+            const uint8_t* from[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) from[u] = base + lane_value(at_k, k + u);
+            load_lds_4k(slot, from, off_k);
+          } else {
+#pragma unroll 1
+            for (int u = 0; u < 4; ++u) {
+              if (((some8 >> (k + u)) & 1) && w.t * kTile + 8 * u + lr < L)
+                load_lds(slot + 1024 * u, base + lane_value(at_k, k + u) + 1024 * u, off_k);
+              else
+                *lds_at<u32x4>(slot + 1024 * u + 16 * lane) = u32x4(0);
+            }
+          }
+        }
+        sure = full ? sure + 1 : 0;
+      };
+      auto add_up = [&](const Place& w, int slot_no) {
+        const uint32_t slot = ring + uint32_t(slot_no) * kHalfSlot;
         f32x16 y = {};
         const int row = w.hh * padded + row_k;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
+          const u32x4 k = *lds_at<u32x4>(slot + uint32_t(128 * kk + 16 * ((4 * half + q) ^ (kk & 7))));
           const u32x4 v = s_q[row * 8 + ((4 * half + q) ^ (row & 7))];
-          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16(v[0], v[1]), e4m3x8_to_bf16(k[q][0], k[q][1]), y, 0, 0, 0);
-          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16(v[2], v[3]), e4m3x8_to_bf16(k[q][2], k[q][3]), y, 0, 0, 0);
+          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16(v[0], v[1]), e4m3x8_to_bf16(k[0], k[1]), y, 0, 0, 0);
+          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e4m3x8_to_bf16(v[2], v[3]), e4m3x8_to_bf16(k[2], k[3]), y, 0, 0, 0);
         }
         const int key = w.t * kTile + kk;
         const float sl = s_sl[w.hh];
@@ -215,26 +280,41 @@ few_rows_kernel(WeightArgs p) {
           }
         }
         sum += __shfl_xor(sum, 32);
+        float o = 0.0f;
+        if constexpr (OLD) o = *lds_at<float>(old_at + 128 * slot_no + 4 * kk) * p.decay;
         if (half == 0 && key < L) score_row(p, b, h0 + w.hh)[key] = o + sum;
+        // every read of the slot is done before its next loads start
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       };
-      u32x4 kraw[kAhead][4];
-      float old[kAhead];
       Place now{kWaves * s0, 0};
       next(now, wave);
-      Place then = now;  // the pair fetched next
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        fetch(then, kraw[u], old[u]);
+      Place then = now;  // the pair whose loads are started next
+      int flying = 0;    // pairs whose loads are in flight
+      if constexpr (!GEN) look_up(win);
+#pragma unroll 1
+      for (int u = 0; u < kFewRing - 1 && then.t < t_end; ++u, ++flying) {
+        start(then, u);
         next(then, kWaves);
       }
+      int slot_no = 0, to = kFewRing - 1;
       while (now.t < t_end) {
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          if (now.t < t_end) add_up(now, kraw[u], old[u]);
-          next(now, kWaves);
-          fetch(then, kraw[u], old[u]);
+        if (then.t < t_end) {
+          start(then, to);
           next(then, kWaves);
+          ++flying;
         }
+        // the pair's own loads: those of the pairs after it may stay in flight
+        // (stores in between count too, and make this wait longer, not shorter)
+        constexpr int kLoads = OLD ? 5 : 4;
+        --flying;
+        if (sure >= flying && flying == 3) wait_loads<3 * kLoads>();
+        else if (sure >= flying && flying == 2) wait_loads<2 * kLoads>();
+        else if (sure >= flying && flying == 1) wait_loads<kLoads>();
+        else wait_loads<0>();
+        add_up(now, slot_no);
+        next(now, kWaves);
+        slot_no = slot_no == kFewRing - 1 ? 0 : slot_no + 1;
+        to = to == kFewRing - 1 ? 0 : to + 1;
       }
     }
   }
@@ -313,7 +393,8 @@ __global__ void __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_p
     const int R = r.n * G, ctx = full - r.n;
     float* scores = score_row(p, b, h);
 
-    // lane l: 64 bytes of keys l % 32 at d = 64 (l / 32); missing rows and keys past the end as zeros
+    // lane l: of keys l % 32 the 16-byte chunks 2 q + l / 32 (the queries' the same);
+    // missing rows and keys past the end as zeros
     bf16x8 kop[kHeld][8];
 #pragma unroll
     for (int g = 0; g < kHeld; ++g) {
@@ -325,11 +406,11 @@ __global__ void __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_p
         if (pi < a.bt_width) id = a.block_table[int64_t(b) * a.bt_stride + pi];
         if (id >= a.num_blocks) id = -1;
       }
-      const uint8_t* row = a.k + int64_t(h) * a.k_head + 64 * half + int64_t(id) * a.k_blk +
+      const uint8_t* row = a.k + int64_t(h) * a.k_head + 16 * half + int64_t(id) * a.k_blk +
                            int64_t(key - pi * a.block_size) * a.k_row;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const u32x4 v = id >= 0 ? *reinterpret_cast<const u32x4*>(row + 16 * q) : u32x4(0);
+        const u32x4 v = id >= 0 ? *reinterpret_cast<const u32x4*>(row + 32 * q) : u32x4(0);
         kop[g][2 * q] = e4m3x8_to_bf16(v[0], v[1]);
         kop[g][2 * q + 1] = e4m3x8_to_bf16(v[2], v[3]);
       }
@@ -349,7 +430,7 @@ __global__ void __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_p
     // is the next token).
     const int di = kRows * split / G, dg = kRows * split - di * G;
     int i = (first * kRows + kk) / G, g = first * kRows + kk - i * G;
-    const uint8_t* q_at = p.q8 + (int64_t(r.first) + i) * p.q8_tok + int64_t(h * G + g) * p.q8_head + 64 * half;
+    const uint8_t* q_at = p.q8 + (int64_t(r.first) + i) * p.q8_tok + int64_t(h * G + g) * p.q8_head + 16 * half;
     const float* lse_at = p.lse + int64_t(h * G + g) * p.lse_head_stride + r.first + i;
     const int64_t q_step = di * p.q8_tok + dg * p.q8_head, q_wrap = p.q8_tok - G * p.q8_head;
     const int64_t lse_step = di + dg * p.lse_head_stride, lse_wrap = 1 - G * p.lse_head_stride;
@@ -361,7 +442,7 @@ __global__ void __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_p
     auto fetch = [&](Rows& t) {
       const bool live = i < r.n;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) t.q[u] = live ? *reinterpret_cast<const u32x4*>(q_at + 16 * u) : u32x4(0);
+      for (int u = 0; u < 4; ++u) t.q[u] = live ? *reinterpret_cast<const u32x4*>(q_at + 32 * u) : u32x4(0);
       t.lse = live ? *lse_at : __builtin_inff();
       t.last = live ? (a.causal ? ctx + i : full - 1) : -1;
       i += di;
@@ -462,10 +543,20 @@ int quantize_queries(const WeightArgs& p, int64_t total_q, int64_t num_q_heads, 
   return check_launch("quantize_queries_kernel launch");
 }
 
+template <int Q_DT, bool OLD>
+int launch_few_rows_old(const WeightArgs& p, hipStream_t st) {
+  const DecodeArgs& a = p.a;
+  // pages of a multiple of 8 keys whose rows lie within 32-bit offsets: the keys of a load share a page
+  const bool general = a.block_size % 8 != 0 || a.k_row < 0 || 8 * a.k_row >= (int64_t(1) << 31);
+  const dim3 grid{unsigned(p.s.max_runs), 1u, 1u};
+  if (general) hipLaunchKernelGGL((few_rows_kernel<Q_DT, OLD, true>), grid, dim3(kThreads), 0, st, p);
+  else hipLaunchKernelGGL((few_rows_kernel<Q_DT, OLD, false>), grid, dim3(kThreads), 0, st, p);
+  return check_launch("few_rows_kernel launch");
+}
+
 template <int Q_DT>
 int launch_few_rows(const WeightArgs& p, hipStream_t st) {
-  hipLaunchKernelGGL((few_rows_kernel<Q_DT>), dim3(unsigned(p.s.max_runs)), dim3(kThreads), 0, st, p);
-  return check_launch("few_rows_kernel launch");
+  return p.decay != 0.0f ? launch_few_rows_old<Q_DT, true>(p, st) : launch_few_rows_old<Q_DT, false>(p, st);
 }
 
 }  // namespace
@@ -530,7 +621,7 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
     p.s.step_shift = kStepShift;
     p.s.over = 1;
     p.s.min_run = 2;
-    p.s.max_runs = int32_t(4 * cus);  // resident at once
+    p.s.max_runs = int32_t(2 * cus);  // resident at once
     p.hg = int32_t(std::min<int64_t>(num_kv_heads, kFewRows / (8 * ceil_div(rows, 8))));
     p.s.heads = int32_t(ceil_div(num_kv_heads, p.hg));
     switch (q_dtype) {

@@ -177,10 +177,13 @@ __device__ __forceinline__ T lane_value(T x, int lane) {
   }
 }
 
+__device__ __forceinline__ int32_t wave_uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t wave_uniform(int64_t x) { return lane_value(x, 0); }
+
 // x / y for 0 <= x, 0 < y, short where both fit 31 bits (they do, but for a huge step).
 __device__ __forceinline__ int64_t uniform_div(int64_t x, int64_t y) {
-  if (((x | y) >> 31) == 0) return int64_t(uint32_t(x) / uint32_t(y));
-  return x / y;
+  if (((x | y) >> 31) == 0) return int64_t(wave_uniform(int32_t(uint32_t(x) / uint32_t(y))));
+  return wave_uniform(x / y);
 }
 
 // 64 consecutive sequences, one a lane: the lane's query rows and length, its
