@@ -161,17 +161,18 @@ __device__ __forceinline__ void load_lds(uint32_t at, const uint8_t* p) {
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
                : "=&s"(m0) : "s"(at), "v"(p) : "memory");
 }
-// Four such loads of 1 KiB: from p[u] + 1024 u to at + 1024 u.  An instruction's
-// offset counts for both its addresses, so the LDS base is set once.
-__device__ __forceinline__ void load_lds_4k(uint32_t at, const uint8_t* const (&p)[4], uint32_t offset) {
+// Four such loads of 1 KiB, of bytes that nothing reads again (nt): from p[u] +
+// 1024 u to at + 1024 u.  An instruction's offset counts for both its addresses,
+// so the LDS base is set once.
+__device__ __forceinline__ void load_lds_4k_once(uint32_t at, const uint8_t* const (&p)[4], uint32_t offset) {
   uint32_t m0;
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
       "s_mov_b32 m0, %1\n\ts_nop 0\n\t"
-      "global_load_lds_dwordx4 %2, %3\n\t"
-      "global_load_lds_dwordx4 %2, %4 offset:1024\n\t"
-      "global_load_lds_dwordx4 %2, %5 offset:2048\n\t"
-      "global_load_lds_dwordx4 %2, %6 offset:3072\n\t"
+      "global_load_lds_dwordx4 %2, %3 nt\n\t"
+      "global_load_lds_dwordx4 %2, %4 offset:1024 nt\n\t"
+      "global_load_lds_dwordx4 %2, %5 offset:2048 nt\n\t"
+      "global_load_lds_dwordx4 %2, %6 offset:3072 nt\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(m0)
       : "s"(at), "v"(offset), "s"(p[0]), "s"(p[1]), "s"(p[2]), "s"(p[3])
