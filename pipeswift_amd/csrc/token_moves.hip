@@ -146,13 +146,22 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(SelectArgs p
 // ---------------------------------------------------------------------------
 // the kept rows to their new pages
 // ---------------------------------------------------------------------------
+//
+// Row (slot, head) by row, heads first, V bytes a lane: the destination is
+// written in order and every source row is read whole.  A thread takes kMoveRows
+// rows at once, so that the chain to a row (kept position, page, row) is waited
+// for once for all of them.
+
+constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = 4;
 
 struct MoveArgs {
   char* cache[2];
   int64_t layer_stride, blk, row, head_stride;  // bytes, of both caches
-  int32_t heads, kept_heads;
-  int32_t chunks;  // vectors of a head's row
-  int32_t block_size, num_blocks;
+  int32_t heads, heads_shift;                   // shifts: log2, or -1
+  int32_t kept_heads;
+  int32_t chunks, chunks_shift;  // vectors of a head's row
+  int32_t block_size, block_shift, num_blocks;
   const int32_t* table;
   int64_t table_stride, table_width;
   const int32_t* dst_table;
@@ -168,26 +177,72 @@ __device__ __forceinline__ int32_t page_of(const int32_t* table, int64_t stride,
   return id >= 0 && id < num_blocks ? id : -1;
 }
 
+__device__ __forceinline__ uint32_t div_by(uint32_t x, int32_t by, int32_t shift) {
+  return shift >= 0 ? x >> shift : x / uint32_t(by);
+}
+
 template <int V>
-__global__ void __launch_bounds__(256) move_kept_kernel(MoveArgs p) {
+__global__ void __launch_bounds__(kMoveThreads) move_kept_kernel(MoveArgs p) {
   const int b = int(blockIdx.y), layer = int(blockIdx.z);
-  const int64_t per = int64_t(p.heads) * p.chunks;  // vectors of a token
-  const int64_t total = per * p.budget;
-  for (int64_t x = int64_t(blockIdx.x) * 256 + threadIdx.x; x < total; x += int64_t(gridDim.x) * 256) {
-    const int i = int(x / per);
-    const int r = int(x - int64_t(i) * per);
-    const int h = r / p.chunks, c = r - h * p.chunks;
-    const int64_t list = (int64_t(layer) * p.num_seqs + b) * p.kept_heads + (p.kept_heads > 1 ? h : 0);
-    const int32_t from = p.kept[list * p.budget + i];
-    if (from < 0) continue;
-    const int32_t dp = page_of(p.dst_table, p.dst_stride, p.dst_width, p.num_blocks, b, i / p.block_size);
-    if (dp < 0) continue;
-    const int32_t sp = page_of(p.table, p.table_stride, p.table_width, p.num_blocks, b, from / p.block_size);
-    const int64_t at = int64_t(layer) * p.layer_stride + int64_t(h) * p.head_stride + int64_t(c) * V;
-    const int64_t so = at + int64_t(sp) * p.blk + int64_t(from % p.block_size) * p.row;
-    const int64_t to = at + int64_t(dp) * p.blk + int64_t(i % p.block_size) * p.row;
-    for (int k = 0; k < 2; ++k)
-      if (p.cache[k]) vstore<V>(p.cache[k] + to, sp >= 0 ? vload<V>(p.cache[k] + so) : typename VecT<V>::T(0));
+  const uint32_t rows = uint32_t(p.budget) * uint32_t(p.heads);  // (host: below 2^31)
+  const uint32_t per = kMoveThreads;                             // vectors of a pass
+  const int64_t items = int64_t(rows) * p.chunks;
+  const int32_t* table = p.table + int64_t(b) * p.table_stride;
+  const int32_t* dst_table = p.dst_table + int64_t(b) * p.dst_stride;
+  const int32_t* lists = p.kept + (int64_t(layer) * p.num_seqs + b) * p.kept_heads * p.budget;
+  char* const k = p.cache[0] + int64_t(layer) * p.layer_stride;
+  char* const v = p.cache[1] ? p.cache[1] + int64_t(layer) * p.layer_stride : nullptr;
+  using T = typename VecT<V>::T;
+  for (int64_t x0 = int64_t(blockIdx.x) * per * kMoveRows; x0 < items; x0 += int64_t(gridDim.x) * per * kMoveRows) {
+    int32_t from[kMoveRows], slot[kMoveRows];
+    int64_t at[kMoveRows];
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) {
+      const int64_t x = x0 + u * int64_t(per) + threadIdx.x;
+      from[u] = -1;
+      slot[u] = 0;
+      at[u] = 0;
+      if (x < items) {
+        // (items fit 32 bits but for budgets of many million tokens)
+        const uint32_t r = items <= INT32_MAX ? div_by(uint32_t(x), p.chunks, p.chunks_shift) : uint32_t(x / p.chunks);
+        const uint32_t c = uint32_t(x - int64_t(r) * p.chunks);
+        const uint32_t i = div_by(r, p.heads, p.heads_shift), h = r - i * uint32_t(p.heads);
+        slot[u] = int32_t(i);
+        at[u] = int64_t(h) * p.head_stride + int64_t(c) * V;
+        from[u] = lists[(p.kept_heads > 1 ? int64_t(h) * p.budget : 0) + i];
+      }
+    }
+    int32_t sp[kMoveRows], dp[kMoveRows];
+    uint32_t si[kMoveRows], di[kMoveRows];
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) {
+      sp[u] = dp[u] = -1;
+      si[u] = di[u] = 0;
+      if (from[u] >= 0) {
+        si[u] = div_by(uint32_t(from[u]), p.block_size, p.block_shift);
+        di[u] = div_by(uint32_t(slot[u]), p.block_size, p.block_shift);
+        if (si[u] < p.table_width) sp[u] = table[si[u]];
+        if (di[u] < p.dst_width) dp[u] = dst_table[di[u]];
+      }
+    }
+    T kv[kMoveRows], vv[kMoveRows];
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) {
+      kv[u] = vv[u] = T(0);
+      if (sp[u] >= 0 && sp[u] < p.num_blocks) {
+        const int64_t src = at[u] + sp[u] * p.blk + int64_t(uint32_t(from[u]) - si[u] * uint32_t(p.block_size)) * p.row;
+        kv[u] = vload_nt<V>(k + src);
+        if (v) vv[u] = vload_nt<V>(v + src);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) {
+      if (dp[u] >= 0 && dp[u] < p.num_blocks) {
+        const int64_t dst = at[u] + dp[u] * p.blk + int64_t(uint32_t(slot[u]) - di[u] * uint32_t(p.block_size)) * p.row;
+        vstore_nt<V>(k + dst, kv[u]);
+        if (v) vstore_nt<V>(v + dst, vv[u]);
+      }
+    }
   }
 }
 
@@ -197,15 +252,19 @@ __global__ void __launch_bounds__(256) move_kept_kernel(MoveArgs p) {
 //
 // Rows starts[b] + path[b, i] become rows starts[b] + i, of every layer, as a
 // snapshot: a workgroup owns some columns of all of a sequence's rows and reads
-// every one of them before it writes any.
+// every one of them before it writes any.  The shorter the paths, the more
+// columns.
 
 constexpr int kCommitRows = 256;  // longest path
 constexpr int kCommitThreads = 256;
+constexpr int kCommitCols = 8;    // fewest vectors of a row a workgroup owns
+constexpr int kCommitItems = kCommitRows * kCommitCols / kCommitThreads;
 
 struct CommitArgs {
   char* cache[2];
   int64_t layer_stride, blk, row;  // bytes
   int32_t chunks;                  // vectors of a row
+  int32_t cols_shift;              // log2 of the vectors of a row a workgroup owns
   int32_t block_size, num_blocks;
   const int32_t* table;
   int64_t table_stride, table_width;
@@ -216,48 +275,72 @@ struct CommitArgs {
   const int32_t* path_lens;
 };
 
-template <int V>
+template <int V, int ITEMS>
 __global__ void __launch_bounds__(kCommitThreads) commit_draft_kernel(CommitArgs p) {
-  constexpr int kItems = kCommitRows / (kCommitThreads / 8);  // eight vectors of a row a workgroup
   __shared__ int64_t s_from[kCommitRows], s_to[kCommitRows];
   const int b = int(blockIdx.y), layer = int(blockIdx.z);
+  const int tid = int(threadIdx.x);
   const int n = min(max(p.path_lens[b], 0), p.path_width);
   const int64_t start = p.starts[b];
-  for (int i = int(threadIdx.x); i < n; i += kCommitThreads) {
-    const int64_t t = p.path[int64_t(b) * p.path_stride + i];
-    const int64_t s = start + t, d = start + i;
+  if (tid < n) {
+    const int64_t t = p.path[int64_t(b) * p.path_stride + tid];
+    const int64_t s = start + t, d = start + tid;
     int64_t from = -1, to = -1;
     if (t >= 0 && start >= 0 && s != d) {
-      const int32_t sp = page_of(p.table, p.table_stride, p.table_width, p.num_blocks, b, s / p.block_size);
-      const int32_t dp = page_of(p.table, p.table_stride, p.table_width, p.num_blocks, b, d / p.block_size);
+      const int64_t si = uint64_t(s) / uint32_t(p.block_size), di = uint64_t(d) / uint32_t(p.block_size);
+      const int32_t sp = page_of(p.table, p.table_stride, p.table_width, p.num_blocks, b, si);
+      const int32_t dp = page_of(p.table, p.table_stride, p.table_width, p.num_blocks, b, di);
       if (sp >= 0 && dp >= 0) {
-        from = sp * p.blk + (s % p.block_size) * p.row;
-        to = dp * p.blk + (d % p.block_size) * p.row;
+        from = sp * p.blk + (s - si * p.block_size) * p.row;
+        to = dp * p.blk + (d - di * p.block_size) * p.row;
       }
     }
-    s_from[i] = from;
-    s_to[i] = to;
+    s_from[tid] = from;
+    s_to[tid] = to;
   }
   __syncthreads();
-  const int c = int(blockIdx.x) * 8 + (int(threadIdx.x) & 7);
-  const int r0 = int(threadIdx.x) >> 3;
-  typename VecT<V>::T v[2][kItems];
+  const int c = (int(blockIdx.x) << p.cols_shift) + (tid & ((1 << p.cols_shift) - 1));
+  const int r0 = tid >> p.cols_shift, step = kCommitThreads >> p.cols_shift;
+  typename VecT<V>::T v[2][ITEMS];
   const int64_t at = int64_t(layer) * p.layer_stride + int64_t(c) * V;
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int i = r0 + k * (kCommitThreads / 8);
+  for (int k = 0; k < ITEMS; ++k) {
+    const int i = r0 + k * step;
     if (c < p.chunks && i < n && s_to[i] >= 0)
       for (int j = 0; j < 2; ++j)
         if (p.cache[j]) v[j][k] = vload<V>(p.cache[j] + at + s_from[i]);
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int i = r0 + k * (kCommitThreads / 8);
+  for (int k = 0; k < ITEMS; ++k) {
+    const int i = r0 + k * step;
     if (c < p.chunks && i < n && s_to[i] >= 0)
       for (int j = 0; j < 2; ++j)
         if (p.cache[j]) vstore<V>(p.cache[j] + at + s_to[i], v[j][k]);
   }
+}
+
+template <int V>
+int launch_commit(CommitArgs p, int64_t num_layers, int64_t num_seqs, hipStream_t st) {
+  // columns: a power of two, as many as the threads can take with a row each (a
+  // row of one pass at least), and no more than the row has
+  int shift = log2_exact(kCommitCols);
+  while ((2 << shift) * int64_t(p.path_width) <= kCommitThreads && (1 << shift) < p.chunks) ++shift;
+  p.cols_shift = shift;
+  const dim3 grid{unsigned(ceil_div(p.chunks, 1 << shift)), unsigned(num_seqs), unsigned(num_layers)};
+  if (int64_t(p.path_width) << shift <= kCommitThreads)
+    hipLaunchKernelGGL((commit_draft_kernel<V, 1>), grid, dim3(kCommitThreads), 0, st, p);
+  else
+    hipLaunchKernelGGL((commit_draft_kernel<V, kCommitItems>), grid, dim3(kCommitThreads), 0, st, p);
+  return check_launch("commit_draft_kernel launch");
+}
+
+template <int V>
+int launch_move(const MoveArgs& p, int64_t num_layers, int64_t num_seqs, hipStream_t st) {
+  const int64_t passes = ceil_div(int64_t(p.budget) * p.heads * p.chunks, kMoveThreads * kMoveRows);
+  const dim3 grid{unsigned(std::min<int64_t>(passes, 65535)), unsigned(num_seqs), unsigned(num_layers)};
+  hipLaunchKernelGGL((move_kept_kernel<V>), grid, dim3(kMoveThreads), 0, st, p);
+  return check_launch("move_kept_kernel launch");
 }
 
 }  // namespace
@@ -347,17 +430,18 @@ int psk_move_kept_tokens(void* cache0, void* cache1, int64_t layer_stride, int64
                              uint64_t(block_stride), uint64_t(row_stride), uint64_t(head_stride), uint64_t(head_bytes)};
   const int v = common_align(align, 7, 16);
   p.chunks = int32_t(head_bytes / v);
-  const int64_t items = budget * num_heads * p.chunks;
-  const dim3 grid{unsigned(std::min<int64_t>(ceil_div(items, 256), 65535)), unsigned(num_seqs), unsigned(num_layers)};
+  p.chunks_shift = log2_exact(p.chunks);
+  p.heads_shift = log2_exact(num_heads);
+  p.block_shift = log2_exact(block_size);
+  if (budget > INT32_MAX / num_heads) return fail(PSK_E_ARG, "budget %lld of %lld heads", (long long)budget, (long long)num_heads);
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (v) {
-    case 16: hipLaunchKernelGGL(move_kept_kernel<16>, grid, dim3(256), 0, st, p); break;
-    case 8: hipLaunchKernelGGL(move_kept_kernel<8>, grid, dim3(256), 0, st, p); break;
-    case 4: hipLaunchKernelGGL(move_kept_kernel<4>, grid, dim3(256), 0, st, p); break;
-    case 2: hipLaunchKernelGGL(move_kept_kernel<2>, grid, dim3(256), 0, st, p); break;
-    default: hipLaunchKernelGGL(move_kept_kernel<1>, grid, dim3(256), 0, st, p); break;
+    case 16: return launch_move<16>(p, num_layers, num_seqs, st);
+    case 8: return launch_move<8>(p, num_layers, num_seqs, st);
+    case 4: return launch_move<4>(p, num_layers, num_seqs, st);
+    case 2: return launch_move<2>(p, num_layers, num_seqs, st);
+    default: return launch_move<1>(p, num_layers, num_seqs, st);
   }
-  return check_launch("move_kept_kernel launch");
 }
 
 int psk_commit_draft_tokens(void* cache0, void* cache1, int64_t layer_stride, int64_t block_stride, int64_t row_stride,
@@ -395,16 +479,14 @@ int psk_commit_draft_tokens(void* cache0, void* cache1, int64_t layer_stride, in
                              uint64_t(block_stride), uint64_t(row_stride), uint64_t(row_bytes)};
   const int v = common_align(align, 6, 16);
   p.chunks = int32_t(row_bytes / v);
-  const dim3 grid{unsigned(ceil_div(p.chunks, 8)), unsigned(num_seqs), unsigned(num_layers)};
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (v) {
-    case 16: hipLaunchKernelGGL(commit_draft_kernel<16>, grid, dim3(kCommitThreads), 0, st, p); break;
-    case 8: hipLaunchKernelGGL(commit_draft_kernel<8>, grid, dim3(kCommitThreads), 0, st, p); break;
-    case 4: hipLaunchKernelGGL(commit_draft_kernel<4>, grid, dim3(kCommitThreads), 0, st, p); break;
-    case 2: hipLaunchKernelGGL(commit_draft_kernel<2>, grid, dim3(kCommitThreads), 0, st, p); break;
-    default: hipLaunchKernelGGL(commit_draft_kernel<1>, grid, dim3(kCommitThreads), 0, st, p); break;
+    case 16: return launch_commit<16>(p, num_layers, num_seqs, st);
+    case 8: return launch_commit<8>(p, num_layers, num_seqs, st);
+    case 4: return launch_commit<4>(p, num_layers, num_seqs, st);
+    case 2: return launch_commit<2>(p, num_layers, num_seqs, st);
+    default: return launch_commit<1>(p, num_layers, num_seqs, st);
   }
-  return check_launch("commit_draft_kernel launch");
 }
 
 }  // extern "C"
