@@ -484,7 +484,9 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
  * budget + i]: the i-th kept position, ascending, -1 past the last;
  * new_lens[b] = min(n, budget).  scores_out (which may be scores itself with the
  * same strides, and may not overlap it otherwise) receives the kept scores, then
- * zeros up to n, both up to scores_out_width.
+ * zeros up to n, both up to scores_out_width.  workspace: device memory of
+ * psk_select_tokens_workspace_bytes() (0 for rows of at most 16384 scores), no
+ * initial contents needed.
  *
  * psk_move_kept_tokens: row kept[..., i] of sequence b, head h (page
  * block_table[b * stride + kept / block_size], byte strides) goes to row i of
@@ -497,7 +499,10 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
 int psk_select_tokens(const float* scores, const int64_t* scores_strides, int64_t scores_width, float* scores_out,
                       const int64_t* scores_out_strides, int64_t scores_out_width, const int32_t* seq_lens,
                       int64_t num_layers, int64_t num_seqs, int64_t num_heads, int64_t budget, int64_t sink,
-                      int64_t recent, int32_t* kept, int32_t* new_lens, void* stream);
+                      int64_t recent, int32_t* kept, int32_t* new_lens, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+int64_t psk_select_tokens_workspace_bytes(int64_t num_layers, int64_t num_seqs, int64_t num_heads, int64_t scores_width,
+                                          int64_t budget);
 
 int psk_move_kept_tokens(void* cache0, void* cache1, int64_t layer_stride, int64_t block_stride, int64_t row_stride,
                          int64_t head_stride, int64_t head_bytes, int64_t num_layers, int64_t num_heads,

@@ -122,8 +122,11 @@ _SIGNATURES = {
     ),
     "psk_attention_weights_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int]),
     "psk_select_tokens": (
-        _int, [_vp, _c_int64_p, _i64, _vp, _c_int64_p, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp],
+        _int,
+        [_vp, _c_int64_p, _i64, _vp, _c_int64_p, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64,
+         _vp],
     ),
+    "psk_select_tokens_workspace_bytes": (_i64, [_i64] * 5),
     "psk_move_kept_tokens": (
         _int,
         [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,

@@ -251,9 +251,9 @@ def evict_tokens(
     scores, then zeros up to n.
 
     Returns (kept, new_lens): int32 [L, B, H or 1, budget], each kept token's old
-    position (-1 past the last), and int32 [B], the new lengths.  Two launches
-    per pair of caches of one geometry and a first one in all; no
-    synchronization.
+    position (-1 past the last), and int32 [B], the new lengths.  One launch for
+    the choice (five for scores of more than 16384 tokens) and one for each pair
+    of caches of one geometry; no synchronization.
     """
     first = caches if isinstance(caches, torch.Tensor) else caches[0]
     assert first.ndim >= 4, "caches are layered: [L, num_blocks, block_size, heads, ...] or [L, num_blocks, block_size, row]"
@@ -285,10 +285,14 @@ def evict_tokens(
     new_lens = torch.empty(B, dtype=torch.int32, device=device)
     with on_device(device):
         stream = stream_handle(device)
+        need = int(lib().psk_select_tokens_workspace_bytes(layers, B, kept_heads, scores.shape[3], budget))
+        if need < 0:
+            check(need, "evict_tokens workspace")
+        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         status = lib().psk_select_tokens(
             ptr(scores), i64_array(scores.stride()[:3]), scores.shape[3], ptr(scores_out),
             i64_array(scores_out.stride()[:3]), scores_out.shape[3], ptr(seq_lens), layers, B, kept_heads, budget, sink,
-            recent, ptr(kept), ptr(new_lens), stream,
+            recent, ptr(kept), ptr(new_lens), ptr(workspace), need, stream,
         )
         check(status, "evict_tokens")
         for a, b in pairs:

@@ -16,13 +16,32 @@ namespace {
 // selection
 // ---------------------------------------------------------------------------
 //
-// One workgroup per row of scores (layer, sequence, head).  The k best of the
-// free tokens are those above the k-th largest key and the first of those at
-// it, found by a radix selection of four 8-bit digits over order-preserving
-// integer keys; a scan in position order then lists the kept tokens.
+// Of a row of scores (layer, sequence, head) the first `sink` and the last
+// `recent` stay, and of the free ones between the `want` largest: those above
+// the want-th largest key and the first of those at it.  The keys are
+// order-preserving integers and that key is found a digit at a time (11, 11 and
+// 10 bits): a histogram of the digit over the keys that agree in the digits
+// before, and the bin that the want-th falls in.  A workgroup holds up to
+// kChunk scores in registers, sixteen a thread, each wave a contiguous part, so
+// that the order is kept with ballots and one exchange between the waves.
+//
+//   * rows of at most kChunk: select_row_kernel, everything in one launch.  8 rows
+//     of 1100: see DESIGN's table; the histogram's barriers bound it.
+//   * longer ones, a workgroup a chunk: three launches of chunk_digit_kernel
+//     leave each chunk's histogram of a digit, and every workgroup of the next
+//     launch adds up those of its row; chunk_emit_kernel then has, from the
+//     histograms of the chunks before its own, where its kept tokens go.  One
+//     workgroup for a row of 131072 took 337 us.
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
+constexpr int kPer = 16;                        // scores of a thread
+constexpr int kChunk = kSelThreads * kPer;
+constexpr int kBins = 2048;                     // of the first two digits; half of the third's are used
+constexpr int kDigits = 3;
+constexpr int kMaxChunks = 4096;                // of one round of launches: bounds the workspace
+
+__device__ __forceinline__ constexpr int digit_shift(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
 
 struct SelectArgs {
   const float* scores;
@@ -36,6 +55,10 @@ struct SelectArgs {
   int32_t budget, sink, recent;
   int32_t* kept;      // [layers, num_seqs, heads, budget]
   int32_t* new_lens;  // [num_seqs]
+  int32_t chunks;     // of a row, at its widest
+  int32_t row0;       // first row of the round of launches
+  uint16_t* hist;     // [rows of a round][chunks][kDigits][kBins]
+  float* staged;      // kept scores where scores_out is scores itself: [rows of a round][budget], else nullptr
 };
 
 // Larger scores have larger keys, -0 and 0 the same one, a NaN the least of all.
@@ -45,102 +68,295 @@ __device__ __forceinline__ uint32_t score_key(float f) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive prefix of `x` over the workgroup and its total.  Two barriers.
-__device__ __forceinline__ uint32_t block_prefix(uint32_t x, uint32_t* s_wave, uint32_t& total) {
-  const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6;
-  uint32_t v = x;
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t y = __shfl_up(v, o);
-    if (lane >= o) v += y;
-  }
-  if (lane == 63) s_wave[wave] = v;
-  __syncthreads();
-  uint32_t before = 0, all = 0;
-  for (int w = 0; w < kSelWaves; ++w) {
-    before += w < wave ? s_wave[w] : 0u;
-    all += s_wave[w];
-  }
-  __syncthreads();
-  total = all;
-  return before + v - x;
+struct SelectRow {
+  const float* src;
+  float* out;
+  int32_t* kept;
+  int32_t len, n;   // tokens, and how many stay
+  int32_t lo, hi;   // the free ones
+  uint32_t want;    // how many of them stay
+};
+
+__device__ __forceinline__ SelectRow select_row(const SelectArgs& p, int row) {
+  const int head = row % p.heads, rest = row / p.heads, b = rest % p.num_seqs, layer = rest / p.num_seqs;
+  SelectRow r;
+  r.src = p.scores + int64_t(layer) * p.s_layer + int64_t(b) * p.s_seq + int64_t(head) * p.s_head;
+  r.out = p.out + int64_t(layer) * p.o_layer + int64_t(b) * p.o_seq + int64_t(head) * p.o_head;
+  r.kept = p.kept + int64_t(row) * p.budget;
+  r.len = min(max(p.seq_lens[b], 0), p.width);
+  r.n = min(r.len, p.budget);
+  const bool all = r.len <= p.budget;
+  r.lo = all ? r.len : p.sink;
+  r.hi = all ? r.len : r.len - p.recent;
+  r.want = all ? 0u : uint32_t(p.budget - p.sink - p.recent);
+  return r;
 }
 
-__global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(SelectArgs p) {
-  __shared__ uint32_t s_hist[256];
-  __shared__ uint32_t s_wave[kSelWaves];
-  __shared__ uint32_t s_pick[2];
-  const int tid = int(threadIdx.x);
-  const int row = int(blockIdx.x);
-  const int head = row % p.heads, b = (row / p.heads) % p.num_seqs, layer = row / p.heads / p.num_seqs;
-  const float* src = p.scores + int64_t(layer) * p.s_layer + int64_t(b) * p.s_seq + int64_t(head) * p.s_head;
-  float* out = p.out + int64_t(layer) * p.o_layer + int64_t(b) * p.o_seq + int64_t(head) * p.o_head;
-  int32_t* kept = p.kept + int64_t(row) * p.budget;
-  const int L = min(max(p.seq_lens[b], 0), p.width);
-  const int n = min(L, p.budget);
-  if (layer == 0 && head == 0 && tid == 0) p.new_lens[b] = n;
+// The scores of positions [c0, c0 + kChunk) of a row: wave w's part is `part`
+// positions long, lane l of it holds positions c0 + w part + 64 k + l.
+struct Held {
+  float f[kPer];
+  int32_t first, part, end;  // the wave's first position, its length, the chunk's end
 
-  // free tokens: [lo, hi); those before and after are kept
-  int lo = L, hi = L;
-  uint32_t want = 0;  // how many of the free tokens stay
-  uint32_t cut = 0, ties = 0;  // keys above `cut` stay, and the first `ties` at it
-  if (L > p.budget) {
-    lo = p.sink;
-    hi = L - p.recent;
-    want = uint32_t(p.budget - p.sink - p.recent);
-    uint32_t left = want, prefix = 0;
-    for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-      if (tid < 256) s_hist[tid] = 0;
-      __syncthreads();
-      for (int i = lo + tid; i < hi; i += kSelThreads) {
-        const uint32_t key = score_key(src[i]);
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(key >> shift) & 255], 1u);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int d = 255;
-        uint32_t above = 0;
-        while (d > 0 && above + s_hist[d] < left) above += s_hist[d--];
-        s_pick[0] = uint32_t(d);
-        s_pick[1] = above;
-      }
-      __syncthreads();
-      prefix |= s_pick[0] << shift;
-      left -= s_pick[1];
-      __syncthreads();
+  __device__ __forceinline__ void load(const SelectRow& r, int c0) {
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = int(threadIdx.x) & 63;
+    end = min(r.len, c0 + kChunk);
+    part = (max(end - c0, 0) + 64 * kSelWaves - 1) / (64 * kSelWaves) * 64;
+    first = c0 + wave * part;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = first + 64 * k + lane;
+      f[k] = 0.0f;
+      if (64 * k < part && i < end) f[k] = r.src[i];
     }
-    cut = prefix;
-    ties = left;
   }
-  uint32_t done = 0, tied = 0;
-  for (int i0 = 0; i0 < L; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    float f = 0.0f;
-    uint32_t above = 0, at = 0;
-    if (i < L) {
-      f = src[i];
-      if (i < lo || i >= hi) {
-        above = 1;
-      } else if (want > 0) {
-        const uint32_t key = score_key(f);
-        above = key > cut;
-        at = key == cut;
-      }
-    }
-    uint32_t tie_total, keep_total;
-    const uint32_t tie_rank = tied + block_prefix(at, s_wave, tie_total);
-    const uint32_t keep = above | (at & uint32_t(tie_rank < ties));
-    const uint32_t rank = done + block_prefix(keep, s_wave, keep_total);
-    // (a kept score moves down at most to its own place: the rows before it are read)
-    if (keep) {
-      kept[rank] = i;
-      if (int(rank) < p.out_width) out[rank] = f;
-    }
-    tied += tie_total;
-    done += keep_total;
+  // fn(k, position) of every place of the wave
+  template <class F>
+  __device__ __forceinline__ void each(const F& fn) const {
+    const int lane = int(threadIdx.x) & 63;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (64 * k < part) fn(k, first + 64 * k + lane);
+  }
+};
+
+// Inclusive prefix over the wave.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t x) {
+  const int lane = int(threadIdx.x) & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// Adds the wave's 64 values to their bins.  All in one bin (equal scores) take one addition.
+__device__ __forceinline__ void count_bins(uint32_t* hist, uint32_t bin, bool in) {
+  const uint64_t m = __ballot(in);
+  if (!m) return;
+  const uint32_t one = uint32_t(__builtin_amdgcn_readlane(int(bin), __builtin_ctzll(m)));
+  if (__ballot(in && bin != one) == 0) {
+    if ((int(threadIdx.x) & 63) == 0) atomicAdd(&hist[one], uint32_t(__popcll(m)));
+  } else if (in) {
+    atomicAdd(&hist[bin], 1u);
+  }
+}
+
+// The digit histogram of the held free keys that agree with `prefix` above it.  Ends with a barrier.
+__device__ __forceinline__ void digit_histogram(const SelectRow& r, const Held& held, int digit, uint32_t prefix,
+                                                uint32_t* hist) {
+  const int shift = digit_shift(digit);
+  for (int i = int(threadIdx.x); i < kBins; i += kSelThreads) hist[i] = 0;
+  __syncthreads();
+  held.each([&](int k, int i) {
+    const uint32_t key = score_key(held.f[k]);
+    const bool in = i >= r.lo && i < r.hi && i < held.end &&
+                    (digit == 0 || (key >> digit_shift(digit - 1)) == (prefix >> digit_shift(digit - 1)));
+    count_bins(hist, (key >> shift) & (digit == 2 ? 1023u : 2047u), in);
+  });
+  __syncthreads();
+}
+
+// The bin, from the top, that the left-th key falls in, and the keys above it;
+// thread t holds bins 2047 - 2 t (`a`) and 2046 - 2 t (`b`).  1 <= left <= all of them.
+struct Digit {
+  uint32_t bin, above;
+};
+__device__ __forceinline__ Digit find_digit(uint32_t a, uint32_t b, uint32_t left, uint32_t* s_wave, uint32_t* s_pick) {
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+  const uint32_t x = wave_prefix(a + b);
+  if (lane == 63) s_wave[wave] = x;
+  __syncthreads();
+  uint32_t before = x - a - b;
+  for (int w = 0; w < kSelWaves; ++w) before += w < wave ? s_wave[w] : 0u;
+  if (before < left && left <= before + a) {
+    s_pick[0] = uint32_t(kBins - 1 - 2 * tid);
+    s_pick[1] = before;
+  } else if (before + a < left && left <= before + a + b) {
+    s_pick[0] = uint32_t(kBins - 2 - 2 * tid);
+    s_pick[1] = before + a;
   }
   __syncthreads();
-  for (int i = n + tid; i < min(L, p.out_width); i += kSelThreads) out[i] = 0.0f;
-  for (int i = n + tid; i < p.budget; i += kSelThreads) kept[i] = -1;
+  return Digit{s_pick[0], s_pick[1]};
+}
+
+// Lists the kept of the held positions: keys above `cut`, the first `ties` at it
+// (of the whole row; `tied` of them and `done` kept tokens come before the chunk)
+// and the forced ones.  Writes kept positions and, if `scores`, their scores.
+__device__ __forceinline__ void emit_kept(const SelectRow& r, const Held& held, uint32_t cut, uint32_t ties, uint32_t tied,
+                                          uint32_t done, float* scores, int32_t scores_width, uint32_t (*s_count)[2]) {
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = int(threadIdx.x) & 63;
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  uint32_t above = 0, at = 0;
+  auto kind = [&](int k, int i, bool& stays, bool& tie) {
+    const bool forced = i < r.lo || i >= r.hi;
+    const uint32_t key = score_key(held.f[k]);
+    stays = i < held.end && (forced || (r.want > 0 && key > cut));
+    tie = i < held.end && !forced && r.want > 0 && key == cut;
+  };
+  held.each([&](int k, int i) {
+    bool stays, tie;
+    kind(k, i, stays, tie);
+    above += __popcll(__ballot(stays));
+    at += __popcll(__ballot(tie));
+  });
+  if (lane == 0) {
+    s_count[wave][0] = above;
+    s_count[wave][1] = at;
+  }
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) {
+    const uint32_t t = s_count[w][1], room = ties > tied ? ties - tied : 0u;
+    done += s_count[w][0] + min(t, room);
+    tied += t;
+  }
+  held.each([&](int k, int i) {
+    bool stays, tie;
+    kind(k, i, stays, tie);
+    const uint64_t t = __ballot(tie);
+    const bool keep = stays || (tie && tied + __popcll(t & below) < ties);
+    tied += __popcll(t);
+    const uint64_t m = __ballot(keep);
+    const uint32_t rank = done + __popcll(m & below);
+    done += __popcll(m);
+    if (keep) {
+      r.kept[rank] = i;
+      if (scores && int64_t(rank) < scores_width) scores[rank] = held.f[k];
+    }
+  });
+}
+
+__global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(8))) select_row_kernel(SelectArgs p) {
+  __shared__ uint32_t s_hist[kBins];
+  __shared__ uint32_t s_wave[kSelWaves], s_count[kSelWaves][2], s_pick[2];
+  const int tid = int(threadIdx.x), row = int(blockIdx.x);
+  const SelectRow r = select_row(p, row);
+  if (row < p.num_seqs * p.heads && row % p.heads == 0 && tid == 0) p.new_lens[row / p.heads] = r.n;
+  Held held;
+  held.load(r, 0);
+  uint32_t prefix = 0, left = r.want;
+  for (int d = 0; d < kDigits && r.want > 0; ++d) {
+    digit_histogram(r, held, d, prefix, s_hist);
+    const Digit g = find_digit(s_hist[kBins - 1 - 2 * tid], s_hist[kBins - 2 - 2 * tid], left, s_wave, s_pick);
+    prefix |= g.bin << digit_shift(d);
+    left -= g.above;
+  }
+  __syncthreads();  // (scores_out may be scores: every score is held by now)
+  emit_kept(r, held, prefix, left, 0, 0, r.out, p.out_width, s_count);
+  for (int i = r.n + tid; i < min(r.len, p.out_width); i += kSelThreads) r.out[i] = 0.0f;
+  for (int i = r.n + tid; i < p.budget; i += kSelThreads) r.kept[i] = -1;
+}
+
+// ---- rows of several chunks
+
+__device__ __forceinline__ uint16_t* chunk_hist(const SelectArgs& p, int row, int chunk, int digit) {
+  return p.hist + ((int64_t(row) * p.chunks + chunk) * kDigits + digit) * kBins;
+}
+
+// Adds up the row's histograms of digit d and finds the bin of the left-th key.
+__device__ __forceinline__ Digit row_digit(const SelectArgs& p, const SelectRow& r, int row, int d, uint32_t left,
+                                           uint32_t* s_wave, uint32_t* s_pick) {
+  uint32_t a = 0, b = 0;
+  const int n = (r.len + kChunk - 1) / kChunk;
+  for (int c = 0; c < n; ++c) {
+    // bins 2046 - 2 t and 2047 - 2 t lie in one word
+    const uint32_t w = reinterpret_cast<const uint32_t*>(chunk_hist(p, row, c, d))[kBins / 2 - 1 - int(threadIdx.x)];
+    a += w >> 16;
+    b += w & 0xFFFFu;
+  }
+  return find_digit(a, b, left, s_wave, s_pick);
+}
+
+template <int DIGIT>
+__global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(8))) chunk_digit_kernel(SelectArgs p) {
+  __shared__ uint32_t s_hist[kBins];
+  __shared__ uint32_t s_wave[kSelWaves], s_pick[2];
+  const int chunk = int(blockIdx.x), row = int(blockIdx.y);
+  const SelectRow r = select_row(p, p.row0 + row);
+  if (r.want == 0 || chunk * kChunk >= r.len) return;
+  Held held;
+  held.load(r, chunk * kChunk);
+  uint32_t prefix = 0, left = r.want;
+#pragma unroll
+  for (int d = 0; d < DIGIT; ++d) {
+    const Digit g = row_digit(p, r, row, d, left, s_wave, s_pick);
+    prefix |= g.bin << digit_shift(d);
+    left -= g.above;
+    __syncthreads();  // the pick is read by all before it is made again
+  }
+  digit_histogram(r, held, DIGIT, prefix, s_hist);
+  const uint32_t w = (s_hist[2 * threadIdx.x + 1] << 16) | s_hist[2 * threadIdx.x];  // (at most kChunk each)
+  reinterpret_cast<uint32_t*>(chunk_hist(p, row, chunk, DIGIT))[threadIdx.x] = w;
+}
+
+__global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(8))) chunk_emit_kernel(SelectArgs p) {
+  __shared__ uint32_t s_wave[kSelWaves], s_count[kSelWaves][2], s_pick[2];
+  const int tid = int(threadIdx.x), chunk = int(blockIdx.x), row = int(blockIdx.y), c0 = chunk * kChunk;
+  const SelectRow r = select_row(p, p.row0 + row);
+  const int whole = p.row0 + row;
+  if (chunk == 0) {
+    if (whole < p.num_seqs * p.heads && whole % p.heads == 0 && tid == 0) p.new_lens[whole / p.heads] = r.n;
+    for (int i = r.n + tid; i < p.budget; i += kSelThreads) r.kept[i] = -1;
+  }
+  if (c0 >= r.len) return;
+  Held held;
+  held.load(r, c0);
+  uint32_t prefix = 0, left = r.want;
+  uint32_t cut_bin[kDigits] = {0, 0, 0};
+  if (r.want > 0) {
+#pragma unroll
+    for (int d = 0; d < kDigits; ++d) {
+      const Digit g = row_digit(p, r, row, d, left, s_wave, s_pick);
+      cut_bin[d] = g.bin;
+      prefix |= g.bin << digit_shift(d);
+      left -= g.above;
+      __syncthreads();  // the pick is read by all before it is made again
+    }
+  }
+  // the chunks before: kept keys above the cut (a digit's bins above its own, of
+  // the keys that agree before it), those at it, and the forced ones
+  uint32_t above = 0, at = 0;
+  if (r.want > 0) {
+    for (int c = 0; c < chunk; ++c) {
+#pragma unroll
+      for (int d = 0; d < kDigits; ++d) {
+        const uint32_t w = reinterpret_cast<const uint32_t*>(chunk_hist(p, row, c, d))[tid];
+        if (uint32_t(2 * tid) > cut_bin[d]) above += w & 0xFFFFu;
+        if (uint32_t(2 * tid + 1) > cut_bin[d]) above += w >> 16;
+        if (d == kDigits - 1 && uint32_t(2 * tid) == cut_bin[d]) at += w & 0xFFFFu;
+        if (d == kDigits - 1 && uint32_t(2 * tid + 1) == cut_bin[d]) at += w >> 16;
+      }
+    }
+  }
+  const int lane = tid & 63, wave = tid >> 6;
+  above = wave_prefix(above);
+  at = wave_prefix(at);
+  if (lane == 63) {
+    s_count[wave][0] = above;
+    s_count[wave][1] = at;
+  }
+  __syncthreads();
+  above = at = 0;
+  for (int w = 0; w < kSelWaves; ++w) {
+    above += s_count[w][0];
+    at += s_count[w][1];
+  }
+  __syncthreads();
+  const uint32_t forced = uint32_t(min(c0, r.lo)) + uint32_t(max(c0 - r.hi, 0));
+  float* scores = p.staged ? p.staged + int64_t(row) * p.budget : r.out;
+  emit_kept(r, held, prefix, left, at, forced + above + min(at, left), scores, p.staged ? p.budget : p.out_width, s_count);
+  if (!p.staged)
+    for (int i = max(r.n, c0) + tid; i < min(held.end, p.out_width); i += kSelThreads) r.out[i] = 0.0f;
+}
+
+// The staged scores to their rows, once every chunk has read its own, and zeros behind them.
+__global__ void __launch_bounds__(256) unstage_scores_kernel(SelectArgs p) {
+  const int row = int(blockIdx.y);
+  const SelectRow r = select_row(p, p.row0 + row);
+  const float* from = p.staged + int64_t(row) * p.budget;
+  for (int i = int(blockIdx.x) * 256 + int(threadIdx.x); i < min(r.len, p.out_width); i += int(gridDim.x) * 256)
+    r.out[i] = i < r.n ? from[i] : 0.0f;
 }
 
 // ---------------------------------------------------------------------------
@@ -347,15 +563,27 @@ int launch_move(const MoveArgs& p, int64_t num_layers, int64_t num_seqs, hipStre
 
 extern "C" {
 
+int64_t psk_select_tokens_workspace_bytes(int64_t num_layers, int64_t num_seqs, int64_t num_heads, int64_t scores_width,
+                                          int64_t budget) {
+  if (num_layers < 0 || num_seqs < 0 || num_heads <= 0 || scores_width < 0 || budget < 1 || budget > INT32_MAX ||
+      scores_width > INT32_MAX || num_layers > INT32_MAX || num_seqs > INT32_MAX || num_heads > INT32_MAX)
+    return PSK_E_ARG;
+  if (scores_width <= kChunk) return 0;
+  const int64_t chunks = ceil_div(scores_width, kChunk);
+  const int64_t rows = std::min(std::max<int64_t>(kMaxChunks / chunks, 1), num_layers * num_seqs * num_heads);
+  return 16 + rows * (chunks * kDigits * kBins * int64_t(sizeof(uint16_t)) + budget * int64_t(sizeof(float)));
+}
+
 int psk_select_tokens(const float* scores, const int64_t* scores_strides, int64_t scores_width, float* scores_out,
                       const int64_t* scores_out_strides, int64_t scores_out_width, const int32_t* seq_lens,
                       int64_t num_layers, int64_t num_seqs, int64_t num_heads, int64_t budget, int64_t sink,
-                      int64_t recent, int32_t* kept, int32_t* new_lens, void* stream) {
+                      int64_t recent, int32_t* kept, int32_t* new_lens, void* workspace, int64_t workspace_bytes,
+                      void* stream) {
   begin_device_call();
-  if (num_layers < 0 || num_seqs < 0 || num_heads <= 0 || scores_width < 0 || scores_width > INT32_MAX - kSelThreads ||
-      scores_out_width < 0 || scores_out_width > INT32_MAX - kSelThreads)
+  if (num_layers < 0 || num_seqs < 0 || num_heads <= 0 || scores_width < 0 || scores_width > INT32_MAX - 2 * kChunk ||
+      scores_out_width < 0 || scores_out_width > INT32_MAX - 2 * kChunk)
     return fail(PSK_E_ARG, "bad sizes");
-  if (budget < 1 || budget > INT32_MAX - kSelThreads) return fail(PSK_E_ARG, "budget %lld", (long long)budget);
+  if (budget < 1 || budget > INT32_MAX - 2 * kChunk) return fail(PSK_E_ARG, "budget %lld", (long long)budget);
   if (sink < 0 || recent < 0 || sink > budget || recent > budget - sink)
     return fail(PSK_E_ARG, "sink %lld and recent %lld do not fit a budget of %lld", (long long)sink, (long long)recent,
                 (long long)budget);
@@ -365,6 +593,9 @@ int psk_select_tokens(const float* scores, const int64_t* scores_strides, int64_
   if (!scores_strides || !scores_out_strides || !seq_lens || !kept || !new_lens ||
       (scores_width > 0 && !scores) || (scores_out_width > 0 && !scores_out))
     return fail(PSK_E_ARG, "NULL pointer");
+  const int64_t need = psk_select_tokens_workspace_bytes(num_layers, num_seqs, num_heads, scores_width, budget);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(PSK_E_WORKSPACE, "workspace of %lld bytes, need %lld", (long long)workspace_bytes, (long long)need);
   SelectArgs p{};
   p.scores = scores;
   p.s_layer = scores_strides[0];
@@ -384,9 +615,30 @@ int psk_select_tokens(const float* scores, const int64_t* scores_strides, int64_
   p.recent = int32_t(recent);
   p.kept = kept;
   p.new_lens = new_lens;
-  hipLaunchKernelGGL(select_tokens_kernel, dim3(unsigned(num_layers * num_seqs * num_heads)), dim3(kSelThreads), 0,
-                     static_cast<hipStream_t>(stream), p);
-  return check_launch("select_tokens_kernel launch");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t rows = num_layers * num_seqs * num_heads;
+  if (need == 0) {
+    hipLaunchKernelGGL(select_row_kernel, dim3(unsigned(rows)), dim3(kSelThreads), 0, st, p);
+    return check_launch("select_row_kernel launch");
+  }
+  p.chunks = int32_t(ceil_div(scores_width, kChunk));
+  const int64_t round = std::min(std::max<int64_t>(kMaxChunks / p.chunks, 1), rows);
+  p.hist = reinterpret_cast<uint16_t*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
+  const bool in_place = scores == scores_out;
+  if (in_place) p.staged = reinterpret_cast<float*>(p.hist + round * p.chunks * kDigits * kBins);
+  for (int64_t row = 0; row < rows; row += round) {
+    const unsigned n = unsigned(std::min(round, rows - row));
+    p.row0 = int32_t(row);
+    const dim3 grid{unsigned(p.chunks), n, 1u};
+    hipLaunchKernelGGL(chunk_digit_kernel<0>, grid, dim3(kSelThreads), 0, st, p);
+    hipLaunchKernelGGL(chunk_digit_kernel<1>, grid, dim3(kSelThreads), 0, st, p);
+    hipLaunchKernelGGL(chunk_digit_kernel<2>, grid, dim3(kSelThreads), 0, st, p);
+    hipLaunchKernelGGL(chunk_emit_kernel, grid, dim3(kSelThreads), 0, st, p);
+    if (in_place)
+      hipLaunchKernelGGL(unstage_scores_kernel, dim3(unsigned(4 * p.chunks), n, 1u), dim3(256), 0, st, p);
+    if (const int e = check_launch("chunked selection launch"); e != PSK_OK) return e;
+  }
+  return PSK_OK;
 }
 
 int psk_move_kept_tokens(void* cache0, void* cache1, int64_t layer_stride, int64_t block_stride, int64_t row_stride,
