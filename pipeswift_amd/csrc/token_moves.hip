@@ -33,10 +33,10 @@ namespace {
 //     histograms of the chunks before its own, where its kept tokens go.  One
 //     workgroup for a row of 131072 took 337 us.
 
-constexpr int kSelThreads = 1024;
-constexpr int kSelWaves = kSelThreads / 64;
+constexpr int kSelThreads = 1024;               // (256 for rows of at most 256 kPer)
 constexpr int kPer = 16;                        // scores of a thread
 constexpr int kChunk = kSelThreads * kPer;
+constexpr int kSmallThreads = 256;
 constexpr int kBins = 2048;                     // of the first two digits; half of the third's are used
 constexpr int kDigits = 3;
 constexpr int kMaxChunks = 4096;                // of one round of launches: bounds the workspace
@@ -94,14 +94,17 @@ __device__ __forceinline__ SelectRow select_row(const SelectArgs& p, int row) {
 
 // The scores of positions [c0, c0 + kChunk) of a row: wave w's part is `part`
 // positions long, lane l of it holds positions c0 + w part + 64 k + l.
+template <int NT>
 struct Held {
+  static constexpr int kWaves = NT / 64;
   float f[kPer];
+  uint32_t key[kPer];
   int32_t first, part, end;  // the wave's first position, its length, the chunk's end
 
   __device__ __forceinline__ void load(const SelectRow& r, int c0) {
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = int(threadIdx.x) & 63;
-    end = min(r.len, c0 + kChunk);
-    part = (max(end - c0, 0) + 64 * kSelWaves - 1) / (64 * kSelWaves) * 64;
+    end = min(r.len, c0 + NT * kPer);
+    part = (max(end - c0, 0) + NT - 1) / NT * 64;
     first = c0 + wave * part;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
@@ -109,6 +112,8 @@ struct Held {
       f[k] = 0.0f;
       if (64 * k < part && i < end) f[k] = r.src[i];
     }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) key[k] = score_key(f[k]);
   }
   // fn(k, position) of every place of the wave
   template <class F>
@@ -144,13 +149,14 @@ __device__ __forceinline__ void count_bins(uint32_t* hist, uint32_t bin, bool in
 }
 
 // The digit histogram of the held free keys that agree with `prefix` above it.  Ends with a barrier.
-__device__ __forceinline__ void digit_histogram(const SelectRow& r, const Held& held, int digit, uint32_t prefix,
+template <int NT>
+__device__ __forceinline__ void digit_histogram(const SelectRow& r, const Held<NT>& held, int digit, uint32_t prefix,
                                                 uint32_t* hist) {
   const int shift = digit_shift(digit);
-  for (int i = int(threadIdx.x); i < kBins; i += kSelThreads) hist[i] = 0;
+  for (int i = int(threadIdx.x); i < kBins; i += NT) hist[i] = 0;
   __syncthreads();
   held.each([&](int k, int i) {
-    const uint32_t key = score_key(held.f[k]);
+    const uint32_t key = held.key[k];
     const bool in = i >= r.lo && i < r.hi && i < held.end &&
                     (digit == 0 || (key >> digit_shift(digit - 1)) == (prefix >> digit_shift(digit - 1)));
     count_bins(hist, (key >> shift) & (digit == 2 ? 1023u : 2047u), in);
@@ -159,23 +165,30 @@ __device__ __forceinline__ void digit_histogram(const SelectRow& r, const Held& 
 }
 
 // The bin, from the top, that the left-th key falls in, and the keys above it;
-// thread t holds bins 2047 - 2 t (`a`) and 2046 - 2 t (`b`).  1 <= left <= all of them.
+// thread t holds the PER bins from kBins - 1 - PER t down.  1 <= left <= all of them.
 struct Digit {
   uint32_t bin, above;
 };
-__device__ __forceinline__ Digit find_digit(uint32_t a, uint32_t b, uint32_t left, uint32_t* s_wave, uint32_t* s_pick) {
+template <int NT>
+__device__ __forceinline__ Digit find_digit(const uint32_t (&n)[kBins / NT], uint32_t left, uint32_t* s_wave,
+                                            uint32_t* s_pick) {
+  constexpr int PER = kBins / NT;
   const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
-  const uint32_t x = wave_prefix(a + b);
+  uint32_t own = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) own += n[i];
+  const uint32_t x = wave_prefix(own);
   if (lane == 63) s_wave[wave] = x;
   __syncthreads();
-  uint32_t before = x - a - b;
-  for (int w = 0; w < kSelWaves; ++w) before += w < wave ? s_wave[w] : 0u;
-  if (before < left && left <= before + a) {
-    s_pick[0] = uint32_t(kBins - 1 - 2 * tid);
-    s_pick[1] = before;
-  } else if (before + a < left && left <= before + a + b) {
-    s_pick[0] = uint32_t(kBins - 2 - 2 * tid);
-    s_pick[1] = before + a;
+  uint32_t before = x - own;
+  for (int w = 0; w < NT / 64; ++w) before += w < wave ? s_wave[w] : 0u;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (before < left && left <= before + n[i]) {
+      s_pick[0] = uint32_t(kBins - 1 - PER * tid - i);
+      s_pick[1] = before;
+    }
+    before += n[i];
   }
   __syncthreads();
   return Digit{s_pick[0], s_pick[1]};
@@ -184,14 +197,15 @@ __device__ __forceinline__ Digit find_digit(uint32_t a, uint32_t b, uint32_t lef
 // Lists the kept of the held positions: keys above `cut`, the first `ties` at it
 // (of the whole row; `tied` of them and `done` kept tokens come before the chunk)
 // and the forced ones.  Writes kept positions and, if `scores`, their scores.
-__device__ __forceinline__ void emit_kept(const SelectRow& r, const Held& held, uint32_t cut, uint32_t ties, uint32_t tied,
+template <int NT>
+__device__ __forceinline__ void emit_kept(const SelectRow& r, const Held<NT>& held, uint32_t cut, uint32_t ties, uint32_t tied,
                                           uint32_t done, float* scores, int32_t scores_width, uint32_t (*s_count)[2]) {
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = int(threadIdx.x) & 63;
   const uint64_t below = (uint64_t(1) << lane) - 1;
   uint32_t above = 0, at = 0;
   auto kind = [&](int k, int i, bool& stays, bool& tie) {
     const bool forced = i < r.lo || i >= r.hi;
-    const uint32_t key = score_key(held.f[k]);
+    const uint32_t key = held.key[k];
     stays = i < held.end && (forced || (r.want > 0 && key > cut));
     tie = i < held.end && !forced && r.want > 0 && key == cut;
   };
@@ -227,25 +241,31 @@ __device__ __forceinline__ void emit_kept(const SelectRow& r, const Held& held, 
   });
 }
 
-__global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(8))) select_row_kernel(SelectArgs p) {
+template <int NT>
+__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) select_row_kernel(SelectArgs p) {
+  constexpr int PER = kBins / NT;
   __shared__ uint32_t s_hist[kBins];
-  __shared__ uint32_t s_wave[kSelWaves], s_count[kSelWaves][2], s_pick[2];
+  __shared__ uint32_t s_wave[NT / 64], s_count[NT / 64][2], s_pick[2];
   const int tid = int(threadIdx.x), row = int(blockIdx.x);
   const SelectRow r = select_row(p, row);
   if (row < p.num_seqs * p.heads && row % p.heads == 0 && tid == 0) p.new_lens[row / p.heads] = r.n;
-  Held held;
+  Held<NT> held;
   held.load(r, 0);
   uint32_t prefix = 0, left = r.want;
+#pragma unroll 1
   for (int d = 0; d < kDigits && r.want > 0; ++d) {
-    digit_histogram(r, held, d, prefix, s_hist);
-    const Digit g = find_digit(s_hist[kBins - 1 - 2 * tid], s_hist[kBins - 2 - 2 * tid], left, s_wave, s_pick);
+    digit_histogram<NT>(r, held, d, prefix, s_hist);
+    uint32_t n[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) n[i] = s_hist[kBins - 1 - PER * tid - i];
+    const Digit g = find_digit<NT>(n, left, s_wave, s_pick);
     prefix |= g.bin << digit_shift(d);
     left -= g.above;
   }
   __syncthreads();  // (scores_out may be scores: every score is held by now)
-  emit_kept(r, held, prefix, left, 0, 0, r.out, p.out_width, s_count);
-  for (int i = r.n + tid; i < min(r.len, p.out_width); i += kSelThreads) r.out[i] = 0.0f;
-  for (int i = r.n + tid; i < p.budget; i += kSelThreads) r.kept[i] = -1;
+  emit_kept<NT>(r, held, prefix, left, 0, 0, r.out, p.out_width, s_count);
+  for (int i = r.n + tid; i < min(r.len, p.out_width); i += NT) r.out[i] = 0.0f;
+  for (int i = r.n + tid; i < p.budget; i += NT) r.kept[i] = -1;
 }
 
 // ---- rows of several chunks
@@ -254,44 +274,58 @@ __device__ __forceinline__ uint16_t* chunk_hist(const SelectArgs& p, int row, in
   return p.hist + ((int64_t(row) * p.chunks + chunk) * kDigits + digit) * kBins;
 }
 
-// Adds up the row's histograms of digit d and finds the bin of the left-th key.
-__device__ __forceinline__ Digit row_digit(const SelectArgs& p, const SelectRow& r, int row, int d, uint32_t left,
-                                           uint32_t* s_wave, uint32_t* s_pick) {
-  uint32_t a = 0, b = 0;
+// Adds up the row's histograms of digit d and finds the bin of the left-th key;
+// above and at: how many keys of the chunks before this one are above that bin
+// and in it.
+__device__ __forceinline__ Digit row_digit(const SelectArgs& p, const SelectRow& r, int row, int chunk, int d, uint32_t left,
+                                           uint32_t* s_wave, uint32_t* s_pick, uint32_t& above, uint32_t& at) {
+  // thread t: bins 2047 - 2 t and 2046 - 2 t, which lie in one word
+  const uint32_t* hist = reinterpret_cast<const uint32_t*>(chunk_hist(p, row, 0, d)) + kBins / 2 - 1 - int(threadIdx.x);
   const int n = (r.len + kChunk - 1) / kChunk;
+  uint32_t all[2] = {0, 0}, mine[2] = {0, 0};
+#pragma unroll 8
   for (int c = 0; c < n; ++c) {
-    // bins 2046 - 2 t and 2047 - 2 t lie in one word
-    const uint32_t w = reinterpret_cast<const uint32_t*>(chunk_hist(p, row, c, d))[kBins / 2 - 1 - int(threadIdx.x)];
-    a += w >> 16;
-    b += w & 0xFFFFu;
+    const uint32_t w = hist[int64_t(c) * (kDigits * kBins / 2)];
+    all[0] += w >> 16;
+    all[1] += w & 0xFFFFu;
+    mine[0] += c < chunk ? w >> 16 : 0u;
+    mine[1] += c < chunk ? w & 0xFFFFu : 0u;
   }
-  return find_digit(a, b, left, s_wave, s_pick);
+  const Digit g = find_digit<kSelThreads>(all, left, s_wave, s_pick);
+  at = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t bin = uint32_t(kBins - 1 - 2 * int(threadIdx.x) - i);
+    above += bin > g.bin ? mine[i] : 0u;
+    at += bin == g.bin ? mine[i] : 0u;
+  }
+  __syncthreads();  // the pick is read by all before it is made again
+  return g;
 }
 
 template <int DIGIT>
-__global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(8))) chunk_digit_kernel(SelectArgs p) {
+__global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))) chunk_digit_kernel(SelectArgs p) {
   __shared__ uint32_t s_hist[kBins];
-  __shared__ uint32_t s_wave[kSelWaves], s_pick[2];
+  __shared__ uint32_t s_wave[kSelThreads / 64], s_pick[2];
   const int chunk = int(blockIdx.x), row = int(blockIdx.y);
   const SelectRow r = select_row(p, p.row0 + row);
   if (r.want == 0 || chunk * kChunk >= r.len) return;
-  Held held;
+  Held<kSelThreads> held;
   held.load(r, chunk * kChunk);
-  uint32_t prefix = 0, left = r.want;
+  uint32_t prefix = 0, left = r.want, above = 0, at;
 #pragma unroll
   for (int d = 0; d < DIGIT; ++d) {
-    const Digit g = row_digit(p, r, row, d, left, s_wave, s_pick);
+    const Digit g = row_digit(p, r, row, chunk, d, left, s_wave, s_pick, above, at);
     prefix |= g.bin << digit_shift(d);
     left -= g.above;
-    __syncthreads();  // the pick is read by all before it is made again
   }
-  digit_histogram(r, held, DIGIT, prefix, s_hist);
+  digit_histogram<kSelThreads>(r, held, DIGIT, prefix, s_hist);
   const uint32_t w = (s_hist[2 * threadIdx.x + 1] << 16) | s_hist[2 * threadIdx.x];  // (at most kChunk each)
   reinterpret_cast<uint32_t*>(chunk_hist(p, row, chunk, DIGIT))[threadIdx.x] = w;
 }
 
-__global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(8))) chunk_emit_kernel(SelectArgs p) {
-  __shared__ uint32_t s_wave[kSelWaves], s_count[kSelWaves][2], s_pick[2];
+__global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))) chunk_emit_kernel(SelectArgs p) {
+  __shared__ uint32_t s_wave[kSelThreads / 64], s_count[kSelThreads / 64][2], s_pick[2];
   const int tid = int(threadIdx.x), chunk = int(blockIdx.x), row = int(blockIdx.y), c0 = chunk * kChunk;
   const SelectRow r = select_row(p, p.row0 + row);
   const int whole = p.row0 + row;
@@ -300,33 +334,17 @@ __global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_e
     for (int i = r.n + tid; i < p.budget; i += kSelThreads) r.kept[i] = -1;
   }
   if (c0 >= r.len) return;
-  Held held;
+  Held<kSelThreads> held;
   held.load(r, c0);
-  uint32_t prefix = 0, left = r.want;
-  uint32_t cut_bin[kDigits] = {0, 0, 0};
+  // The cut, and of the chunks before this one the keys above it (in each digit
+  // those of higher bins that agree before it) and at it.
+  uint32_t prefix = 0, left = r.want, above = 0, at = 0;
   if (r.want > 0) {
 #pragma unroll
     for (int d = 0; d < kDigits; ++d) {
-      const Digit g = row_digit(p, r, row, d, left, s_wave, s_pick);
-      cut_bin[d] = g.bin;
+      const Digit g = row_digit(p, r, row, chunk, d, left, s_wave, s_pick, above, at);
       prefix |= g.bin << digit_shift(d);
       left -= g.above;
-      __syncthreads();  // the pick is read by all before it is made again
-    }
-  }
-  // the chunks before: kept keys above the cut (a digit's bins above its own, of
-  // the keys that agree before it), those at it, and the forced ones
-  uint32_t above = 0, at = 0;
-  if (r.want > 0) {
-    for (int c = 0; c < chunk; ++c) {
-#pragma unroll
-      for (int d = 0; d < kDigits; ++d) {
-        const uint32_t w = reinterpret_cast<const uint32_t*>(chunk_hist(p, row, c, d))[tid];
-        if (uint32_t(2 * tid) > cut_bin[d]) above += w & 0xFFFFu;
-        if (uint32_t(2 * tid + 1) > cut_bin[d]) above += w >> 16;
-        if (d == kDigits - 1 && uint32_t(2 * tid) == cut_bin[d]) at += w & 0xFFFFu;
-        if (d == kDigits - 1 && uint32_t(2 * tid + 1) == cut_bin[d]) at += w >> 16;
-      }
     }
   }
   const int lane = tid & 63, wave = tid >> 6;
@@ -338,14 +356,15 @@ __global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_e
   }
   __syncthreads();
   above = at = 0;
-  for (int w = 0; w < kSelWaves; ++w) {
+  for (int w = 0; w < kSelThreads / 64; ++w) {
     above += s_count[w][0];
     at += s_count[w][1];
   }
   __syncthreads();
   const uint32_t forced = uint32_t(min(c0, r.lo)) + uint32_t(max(c0 - r.hi, 0));
   float* scores = p.staged ? p.staged + int64_t(row) * p.budget : r.out;
-  emit_kept(r, held, prefix, left, at, forced + above + min(at, left), scores, p.staged ? p.budget : p.out_width, s_count);
+  emit_kept<kSelThreads>(r, held, prefix, left, at, forced + above + min(at, left), scores,
+                         p.staged ? p.budget : p.out_width, s_count);
   if (!p.staged)
     for (int i = max(r.n, c0) + tid; i < min(held.end, p.out_width); i += kSelThreads) r.out[i] = 0.0f;
 }
@@ -618,7 +637,11 @@ int psk_select_tokens(const float* scores, const int64_t* scores_strides, int64_
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t rows = num_layers * num_seqs * num_heads;
   if (need == 0) {
-    hipLaunchKernelGGL(select_row_kernel, dim3(unsigned(rows)), dim3(kSelThreads), 0, st, p);
+    // (fewer threads wait less at the barriers, more hold more scores)
+    if (scores_width <= kSmallThreads * kPer)
+      hipLaunchKernelGGL(select_row_kernel<kSmallThreads>, dim3(unsigned(rows)), dim3(kSmallThreads), 0, st, p);
+    else
+      hipLaunchKernelGGL(select_row_kernel<kSelThreads>, dim3(unsigned(rows)), dim3(kSelThreads), 0, st, p);
     return check_launch("select_row_kernel launch");
   }
   p.chunks = int32_t(ceil_div(scores_width, kChunk));
