@@ -206,12 +206,7 @@ struct SeqWindow {
   }
   __device__ __forceinline__ void price(const JobSpace& s, int lane) {
     cost = n > 0 || (s.idle && b0 + lane < s.num_seqs) ? int64_t(s.over + key_steps(s, min(len, s.width))) * s.heads : 0;
-    int64_t v = cost;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t y = __shfl_up(v, o);
-      if (lane >= o) v += y;
-    }
+    const int64_t v = int64_t(wave_prefix(uint64_t(cost)));
     before = v - cost;
     total = lane_value(v, 63);
   }

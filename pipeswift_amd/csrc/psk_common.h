@@ -233,6 +233,27 @@ __device__ __forceinline__ void find_rows(const int32_t* cu, const int32_t* star
   }
 }
 
+// Inclusive prefix sum over the wave (all 64 lanes active), by DPP: within rows
+// of 16, then each row's last lane to the rows after it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_zero(uint32_t x) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_or_zero(uint64_t x) {
+  return uint64_t(dpp_or_zero<CTRL, ROWS>(uint32_t(x >> 32))) << 32 | dpp_or_zero<CTRL, ROWS>(uint32_t(x));
+}
+template <class T>
+__device__ __forceinline__ T wave_prefix(T x) {
+  x += dpp_or_zero<0x111, 0xF>(x);  // row_shr:1, 2, 4, 8
+  x += dpp_or_zero<0x112, 0xF>(x);
+  x += dpp_or_zero<0x114, 0xF>(x);
+  x += dpp_or_zero<0x118, 0xF>(x);
+  x += dpp_or_zero<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
+  x += dpp_or_zero<0x143, 0xC>(x);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
 template <int DT> struct Elt;
 template <> struct Elt<PSK_DTYPE_F32> {
   using Bits = uint32_t;

@@ -16,17 +16,19 @@ namespace {
 // selection
 // ---------------------------------------------------------------------------
 //
-// Of a row of scores (layer, sequence, head) the first `sink` and the last
-// `recent` stay, and of the free ones between the `want` largest: those above
-// the want-th largest key and the first of those at it.  The keys are
-// order-preserving integers and that key is found a digit at a time (11, 11 and
-// 10 bits): a histogram of the digit over the keys that agree in the digits
-// before, and the bin that the want-th falls in.  A workgroup holds up to
-// kChunk scores in registers, sixteen a thread, each wave a contiguous part, so
+// Of a row of scores (layer, sequence, head) the n = `budget` tokens of the
+// largest keys stay: those above the n-th largest key and the first of those at
+// it.  The keys are order-preserving integers, the first `sink` and the last
+// `recent` tokens have the greatest of all, and the n-th is found a digit at a
+// time (11, 11 and 10 bits): a histogram of the digit over the keys that agree
+// in the digits before, and the bin that it falls in.  A workgroup holds up to
+// kChunk keys in registers, sixteen a thread, each wave a contiguous part, so
 // that the order is kept with ballots and one exchange between the waves.
 //
-//   * rows of at most kChunk: select_row_kernel, everything in one launch.  8 rows
-//     of 1100: see DESIGN's table; the histogram's barriers bound it.
+//   * rows of at most kChunk: select_row_kernel, everything in one launch, with 64
+//     registers so that two workgroups of 1024 threads share a CU (73 registers,
+//     one of them: 56 us).  512 rows of 12288: 27 us, bound by the histograms'
+//     additions; 8 rows of 1100: 7.8 us, the barriers between the digits.
 //   * longer ones, a workgroup a chunk: three launches of chunk_digit_kernel
 //     leave each chunk's histogram of a digit, and every workgroup of the next
 //     launch adds up those of its row; chunk_emit_kernel then has, from the
@@ -61,11 +63,13 @@ struct SelectArgs {
   float* staged;      // kept scores where scores_out is scores itself: [rows of a round][budget], else nullptr
 };
 
-// Larger scores have larger keys, -0 and 0 the same one, a NaN the least of all.
+// Larger scores have larger keys, -0 and 0 the same one, a NaN the least of all;
+// between 1 and 0xFF800001.  0: no token there; kForced: one that stays in any case.
+constexpr uint32_t kForced = 0xFFFFFFFFu;
 __device__ __forceinline__ uint32_t score_key(float f) {
-  if (__builtin_isnan(f)) return 0u;
+  if (__builtin_isnan(f)) return 1u;
   const uint32_t u = __float_as_uint(f + 0.0f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return (u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u)) + 1u;
 }
 
 struct SelectRow {
@@ -74,7 +78,7 @@ struct SelectRow {
   int32_t* kept;
   int32_t len, n;   // tokens, and how many stay
   int32_t lo, hi;   // the free ones
-  uint32_t want;    // how many of them stay
+  uint32_t want;    // n where there is a choice, else 0
 };
 
 __device__ __forceinline__ SelectRow select_row(const SelectArgs& p, int row) {
@@ -88,7 +92,7 @@ __device__ __forceinline__ SelectRow select_row(const SelectArgs& p, int row) {
   const bool all = r.len <= p.budget;
   r.lo = all ? r.len : p.sink;
   r.hi = all ? r.len : r.len - p.recent;
-  r.want = all ? 0u : uint32_t(p.budget - p.sink - p.recent);
+  r.want = all ? 0u : uint32_t(p.budget);
   return r;
 }
 
@@ -113,7 +117,10 @@ struct Held {
       if (64 * k < part && i < end) f[k] = r.src[i];
     }
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) key[k] = score_key(f[k]);
+    for (int k = 0; k < kPer; ++k) {
+      const int i = first + 64 * k + lane;
+      key[k] = 64 * k < part && i < end ? (i < r.lo || i >= r.hi ? kForced : score_key(f[k])) : 0u;
+    }
   }
   // fn(k, position) of every place of the wave
   template <class F>
@@ -125,41 +132,17 @@ struct Held {
   }
 };
 
-// Inclusive prefix over the wave.
-__device__ __forceinline__ uint32_t wave_prefix(uint32_t x) {
-  const int lane = int(threadIdx.x) & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  return x;
-}
-
-// Adds the wave's 64 values to their bins.  All in one bin (equal scores) take one addition.
-__device__ __forceinline__ void count_bins(uint32_t* hist, uint32_t bin, bool in) {
-  const uint64_t m = __ballot(in);
-  if (!m) return;
-  const uint32_t one = uint32_t(__builtin_amdgcn_readlane(int(bin), __builtin_ctzll(m)));
-  if (__ballot(in && bin != one) == 0) {
-    if ((int(threadIdx.x) & 63) == 0) atomicAdd(&hist[one], uint32_t(__popcll(m)));
-  } else if (in) {
-    atomicAdd(&hist[bin], 1u);
-  }
-}
-
-// The digit histogram of the held free keys that agree with `prefix` above it.  Ends with a barrier.
+// The digit histogram of the held keys that agree with `prefix` above it (places
+// without a token have the least key, which is never reached).  Ends with a barrier.
 template <int NT>
-__device__ __forceinline__ void digit_histogram(const SelectRow& r, const Held<NT>& held, int digit, uint32_t prefix,
-                                                uint32_t* hist) {
-  const int shift = digit_shift(digit);
+__device__ __forceinline__ void digit_histogram(const Held<NT>& held, int digit, uint32_t prefix, uint32_t* hist) {
+  const int shift = digit_shift(digit), over = digit == 0 ? 31 : digit_shift(digit - 1);
+  const uint32_t mask = digit == 2 ? 1023u : 2047u;
   for (int i = int(threadIdx.x); i < kBins; i += NT) hist[i] = 0;
   __syncthreads();
-  held.each([&](int k, int i) {
+  held.each([&](int k, int) {
     const uint32_t key = held.key[k];
-    const bool in = i >= r.lo && i < r.hi && i < held.end &&
-                    (digit == 0 || (key >> digit_shift(digit - 1)) == (prefix >> digit_shift(digit - 1)));
-    count_bins(hist, (key >> shift) & (digit == 2 ? 1023u : 2047u), in);
+    if (digit == 0 || ((key ^ prefix) >> over) == 0) atomicAdd(&hist[(key >> shift) & mask], 1u);
   });
   __syncthreads();
 }
@@ -169,19 +152,23 @@ __device__ __forceinline__ void digit_histogram(const SelectRow& r, const Held<N
 struct Digit {
   uint32_t bin, above;
 };
+// The sum of lanes 0 .. wave - 1's values.
+__device__ __forceinline__ uint32_t waves_before(uint32_t x, int wave) {
+  const uint32_t v = wave_prefix(x);
+  return wave > 0 ? uint32_t(__builtin_amdgcn_readlane(int(v), wave - 1)) : 0u;
+}
 template <int NT>
 __device__ __forceinline__ Digit find_digit(const uint32_t (&n)[kBins / NT], uint32_t left, uint32_t* s_wave,
                                             uint32_t* s_pick) {
   constexpr int PER = kBins / NT;
-  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint32_t own = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) own += n[i];
   const uint32_t x = wave_prefix(own);
   if (lane == 63) s_wave[wave] = x;
   __syncthreads();
-  uint32_t before = x - own;
-  for (int w = 0; w < NT / 64; ++w) before += w < wave ? s_wave[w] : 0u;
+  uint32_t before = x - own + waves_before(lane < NT / 64 ? s_wave[lane] : 0u, wave);
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     if (before < left && left <= before + n[i]) {
@@ -194,58 +181,55 @@ __device__ __forceinline__ Digit find_digit(const uint32_t (&n)[kBins / NT], uin
   return Digit{s_pick[0], s_pick[1]};
 }
 
-// Lists the kept of the held positions: keys above `cut`, the first `ties` at it
-// (of the whole row; `tied` of them and `done` kept tokens come before the chunk)
-// and the forced ones.  Writes kept positions and, if `scores`, their scores.
+// Lists the kept of the held positions: keys above `cut` and the first `ties` at
+// it (of the whole row; `tied` of them and `done` kept tokens come before the
+// chunk).  Writes kept positions and their scores.
 template <int NT>
 __device__ __forceinline__ void emit_kept(const SelectRow& r, const Held<NT>& held, uint32_t cut, uint32_t ties, uint32_t tied,
-                                          uint32_t done, float* scores, int32_t scores_width, uint32_t (*s_count)[2]) {
+                                          uint32_t done, float* scores, int32_t scores_width, uint32_t (*s_count)[NT / 64]) {
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = int(threadIdx.x) & 63;
-  const uint64_t below = (uint64_t(1) << lane) - 1;
   uint32_t above = 0, at = 0;
-  auto kind = [&](int k, int i, bool& stays, bool& tie) {
-    const bool forced = i < r.lo || i >= r.hi;
-    const uint32_t key = held.key[k];
-    stays = i < held.end && (forced || (r.want > 0 && key > cut));
-    tie = i < held.end && !forced && r.want > 0 && key == cut;
-  };
-  held.each([&](int k, int i) {
-    bool stays, tie;
-    kind(k, i, stays, tie);
-    above += __popcll(__ballot(stays));
-    at += __popcll(__ballot(tie));
+  held.each([&](int k, int) {
+    above += held.key[k] > cut;
+    at += held.key[k] == cut;
   });
-  if (lane == 0) {
-    s_count[wave][0] = above;
-    s_count[wave][1] = at;
+  above = wave_prefix(above);
+  at = wave_prefix(at);
+  if (lane == 63) {
+    s_count[0][wave] = above;
+    s_count[1][wave] = at;
   }
   __syncthreads();
-  for (int w = 0; w < wave; ++w) {
-    const uint32_t t = s_count[w][1], room = ties > tied ? ties - tied : 0u;
-    done += s_count[w][0] + min(t, room);
-    tied += t;
-  }
+  // the waves before: all their keys above the cut, and as many at it as there is room for
+  const uint32_t room = ties > tied ? ties - tied : 0u;
+  const uint32_t before = waves_before(lane < NT / 64 ? s_count[1][lane] : 0u, wave);
+  done += waves_before(lane < NT / 64 ? s_count[0][lane] : 0u, wave) + min(before, room);
+  tied += before;
+  const uint64_t below = (uint64_t(1) << lane) - 1;
   held.each([&](int k, int i) {
-    bool stays, tie;
-    kind(k, i, stays, tie);
-    const uint64_t t = __ballot(tie);
-    const bool keep = stays || (tie && tied + __popcll(t & below) < ties);
-    tied += __popcll(t);
+    const uint32_t key = held.key[k];
+    const uint64_t t = __ballot(key == cut);
+    bool keep = key > cut;
+    if (t) {
+      keep = keep || (key == cut && tied + __popcll(t & below) < ties);
+      tied += __popcll(t);
+    }
     const uint64_t m = __ballot(keep);
     const uint32_t rank = done + __popcll(m & below);
     done += __popcll(m);
     if (keep) {
       r.kept[rank] = i;
-      if (scores && int64_t(rank) < scores_width) scores[rank] = held.f[k];
+      if (int64_t(rank) < scores_width) scores[rank] = held.f[k];
     }
   });
 }
 
 template <int NT>
-__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) select_row_kernel(SelectArgs p) {
+__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == kSelThreads ? 8 : 6)))
+select_row_kernel(SelectArgs p) {
   constexpr int PER = kBins / NT;
   __shared__ uint32_t s_hist[kBins];
-  __shared__ uint32_t s_wave[NT / 64], s_count[NT / 64][2], s_pick[2];
+  __shared__ uint32_t s_wave[NT / 64], s_count[2][NT / 64], s_pick[2];
   const int tid = int(threadIdx.x), row = int(blockIdx.x);
   const SelectRow r = select_row(p, row);
   if (row < p.num_seqs * p.heads && row % p.heads == 0 && tid == 0) p.new_lens[row / p.heads] = r.n;
@@ -254,7 +238,7 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) se
   uint32_t prefix = 0, left = r.want;
 #pragma unroll 1
   for (int d = 0; d < kDigits && r.want > 0; ++d) {
-    digit_histogram<NT>(r, held, d, prefix, s_hist);
+    digit_histogram<NT>(held, d, prefix, s_hist);
     uint32_t n[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) n[i] = s_hist[kBins - 1 - PER * tid - i];
@@ -319,13 +303,13 @@ __global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_e
     prefix |= g.bin << digit_shift(d);
     left -= g.above;
   }
-  digit_histogram<kSelThreads>(r, held, DIGIT, prefix, s_hist);
+  digit_histogram<kSelThreads>(held, DIGIT, prefix, s_hist);
   const uint32_t w = (s_hist[2 * threadIdx.x + 1] << 16) | s_hist[2 * threadIdx.x];  // (at most kChunk each)
   reinterpret_cast<uint32_t*>(chunk_hist(p, row, chunk, DIGIT))[threadIdx.x] = w;
 }
 
 __global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))) chunk_emit_kernel(SelectArgs p) {
-  __shared__ uint32_t s_wave[kSelThreads / 64], s_count[kSelThreads / 64][2], s_pick[2];
+  __shared__ uint32_t s_wave[kSelThreads / 64], s_count[2][kSelThreads / 64], s_pick[2];
   const int tid = int(threadIdx.x), chunk = int(blockIdx.x), row = int(blockIdx.y), c0 = chunk * kChunk;
   const SelectRow r = select_row(p, p.row0 + row);
   const int whole = p.row0 + row;
@@ -347,23 +331,20 @@ __global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_e
       left -= g.above;
     }
   }
-  const int lane = tid & 63, wave = tid >> 6;
+  const int lane = tid & 63;
   above = wave_prefix(above);
   at = wave_prefix(at);
   if (lane == 63) {
-    s_count[wave][0] = above;
-    s_count[wave][1] = at;
+    s_count[0][tid >> 6] = above;
+    s_count[1][tid >> 6] = at;
   }
   __syncthreads();
-  above = at = 0;
-  for (int w = 0; w < kSelThreads / 64; ++w) {
-    above += s_count[w][0];
-    at += s_count[w][1];
-  }
+  above = waves_before(lane < kSelThreads / 64 ? s_count[0][lane] : 0u, kSelThreads / 64);
+  at = waves_before(lane < kSelThreads / 64 ? s_count[1][lane] : 0u, kSelThreads / 64);
   __syncthreads();
-  const uint32_t forced = uint32_t(min(c0, r.lo)) + uint32_t(max(c0 - r.hi, 0));
+  if (r.want == 0) above = uint32_t(c0);  // every token before stays
   float* scores = p.staged ? p.staged + int64_t(row) * p.budget : r.out;
-  emit_kept<kSelThreads>(r, held, prefix, left, at, forced + above + min(at, left), scores,
+  emit_kept<kSelThreads>(r, held, prefix, left, at, above + min(at, left), scores,
                          p.staged ? p.budget : p.out_width, s_count);
   if (!p.staged)
     for (int i = max(r.n, c0) + tid; i < min(held.end, p.out_width); i += kSelThreads) r.out[i] = 0.0f;
