@@ -14,7 +14,7 @@
 //     token together; the work is cut into equal runs
 //     (cached_queries.h).
 //   * many_rows_kernel, more (the last queries of a prompt, a whole prompt): a
-//     wave holds 64 keys as MFMA operands and the step's e4m3 queries, quantized
+//     wave holds 32 keys as MFMA operands and the step's e4m3 queries, quantized
 //     once by quantize_queries_kernel, pass by it 32 rows at a time.  S^T = K Q^T
 //     leaves lane l query row l % 32, whose lse is one value, and sixteen sums a
 //     key tile, which are joined over the lanes at the end.  Where there are
@@ -41,9 +41,8 @@ constexpr uint32_t kHalfSlot = kTile * 128;  // bytes of a tile's K
 constexpr int kFewRing = 4;  // tiles of K a wave has in LDS (few rows)
 constexpr int kPages = 1024; // page ids staged at a time (few rows)
 constexpr int kFewRows = 64;   // query rows of a job's heads, each padded to whole groups (few rows)
-constexpr int kManyWaves = 4;  // (many rows)
-constexpr int kHeld = 2;     // tiles of keys a wave holds (many rows)
-constexpr int kGroup = kHeld * kTile;
+constexpr int kManyWaves = 8;  // (many rows)
+constexpr int kManyRing = 2;   // row tiles a wave has in LDS (many rows)
 constexpr int kStepShift = 7;
 constexpr int kStepKeys = kTile * kWaves;  // of a step (few rows): a tile a wave
 static_assert(kStepKeys == 1 << kStepShift, "");
@@ -62,6 +61,8 @@ struct WeightArgs {
   int32_t hg;         // few rows: kv heads of a job
   int32_t row_tiles;  // many rows: most of any sequence
   int32_t slots;      // many rows: workgroups that fill the GPU
+  int32_t cus;
+  int32_t near;       // many rows: the rows of a tile lie within 32-bit offsets
 };
 
 __device__ __forceinline__ float* score_row(const WeightArgs& p, int b, int h) {
@@ -359,48 +360,71 @@ __device__ __forceinline__ float sum_lanes(float (&v)[16], int lane) {
   return v[0] + __shfl_xor(v[0], 1);
 }
 
-__global__ void __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_per_eu(2))) many_rows_kernel(WeightArgs p) {
-  const DecodeArgs& a = p.a;
-  __shared__ float s_sum[kManyWaves][kGroup];
+// The rows go to LDS two tiles ahead, whole 128-byte rows by global_load_lds, so
+// that the loop's registers let four waves share a SIMD: 38 us for the last 64
+// queries of 4 contexts of 8000 to 32000 tokens (32 query heads over 4), 77 % of it
+// VALU time (per score an fma, a quarter-rate exp2 and an addition).  Rows read
+// straight to registers, 64 keys a wave and two waves a SIMD: 48; 64 keys from LDS:
+// 49.  Units go keys first and the CUs take them forwards and backwards in turn, so
+// that under a causal mask a CU's long and short ones add up alike: 28 us for a
+// prompt of 2000 tokens (32 over 8), MANY_FWD.
+//
+// The unit of workgroup w, which runs on XCD w % 8: forwards over the CUs in even
+// rounds, backwards in odd ones.
+__device__ __forceinline__ int64_t unit_of(int64_t w, int cus) {
+  const int64_t round = uniform_div(w, cus);
+  if ((round & 1) == 0) return w;
+  const int64_t q = (w >> 3) - round * (cus >> 3);
+  return 8 * (round * (cus >> 3) + (cus >> 3) - 1 - q) + (w & 7);
+}
+
+__global__ void __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_per_eu(4))) many_rows_kernel(WeightArgs args) {
+  __shared__ __attribute__((aligned(1024))) char s_ring[kManyWaves * kManyRing * kHalfSlot];
+  __shared__ float s_lse[kManyWaves * kManyRing * kRows];
+  __shared__ float s_sum[kManyWaves][kTile];
   const int tid = int(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, kk = lane & 31;
-  const int G = a.heads;
+  const uint32_t ring = (uint32_t)(size_t)(lvoid*)s_ring + uint32_t(wave * kManyRing) * kHalfSlot;
+  const uint32_t lse_ring = (uint32_t)(size_t)(lvoid*)s_lse + uint32_t(wave * kManyRing * kRows * 4);
   // As many keys to a workgroup as leave `slots` of them; the fewer keys the step
   // has, the more waves share them (as far as there are row tiles for each).  From
   // the lengths alone, so that the order of the sums does not depend on a bound.
   SeqWindow seqs;
-  JobSpace s = p.s;  // (a step of kGroup keys)
-  StepRuns step = step_runs(a, s, seqs, lane);
+  JobSpace s = args.s;  // (a step of kTile keys)
+  StepRuns step = step_runs(args.a, s, seqs, lane);
   int split = 1;
-  while (split < kManyWaves && split < p.row_tiles && step.total * split < int64_t(p.slots) * kManyWaves) split *= 2;
+  while (split < kManyWaves && split < args.row_tiles && step.total * split < int64_t(args.slots) * kManyWaves) split *= 2;
   for (int w = split; w < kManyWaves; w *= 2) ++s.step_shift;
   if (s.num_seqs <= 64) {
     seqs.price(s, lane);
     step.total = seqs.total;
   } else {
-    step = step_runs(a, s, seqs, lane);
+    step = step_runs(args.a, s, seqs, lane);
     seqs.b0 = -64;  // (the last window is there, not the first)
   }
   // waves w, w + 1 .. of a group of `split` hold the same keys and take the row tiles in turn
   const int group = wave / split, turn = wave - group * split;
-  for (int64_t x = blockIdx.x; x < step.total; x += gridDim.x) {  // a unit: a workgroup's keys of a kv head
+  const int64_t places = uniform_div(step.total + args.cus - 1, args.cus) * args.cus;
+  for (int64_t w = blockIdx.x; w < places; w += gridDim.x) {  // a unit: a workgroup's keys of a kv head
+    const WeightArgs& p = args_again<WeightArgs>();
+    const DecodeArgs& a = p.a;
+    const int G = a.heads;
+    const int64_t x = unit_of(w, p.cus);
+    if (x >= step.total) continue;
     int64_t before;
     const int b = seq_of_unit(a, s, x, seqs, lane, before);
     const SeqRows r{lane_value(seqs.first, b - seqs.b0), lane_value(seqs.n, b - seqs.b0)};
     const int full = lane_value(seqs.len, b - seqs.b0), L = min(full, p.s.width);
-    const int units = key_steps(s, L);
-    const int h = int(uniform_div(x - before, units));
-    const int k0 = (int(x - before) - h * units) * (1 << s.step_shift) + group * kGroup;  // the wave's keys
+    const int unit = int(uniform_div(x - before, s.heads)), h = int(x - before) - unit * s.heads;
+    const int k0 = unit * (1 << s.step_shift) + group * kTile;  // the wave's keys
     const int R = r.n * G, ctx = full - r.n;
-    float* scores = score_row(p, b, h);
 
     // lane l: of keys l % 32 the 16-byte chunks 2 q + l / 32 (the queries' the same);
     // missing rows and keys past the end as zeros
-    bf16x8 kop[kHeld][8];
-#pragma unroll
-    for (int g = 0; g < kHeld; ++g) {
-      const int key = k0 + kTile * g + kk;
+    bf16x8 kop[8];
+    {
+      const int key = k0 + kk;
       int32_t id = -1;
       int pi = 0;
       if (key < L) {
@@ -413,111 +437,156 @@ __global__ void __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_p
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const u32x4 v = id >= 0 ? *reinterpret_cast<const u32x4*>(row + 32 * q) : u32x4(0);
-        kop[g][2 * q] = e4m3x8_to_bf16(v[0], v[1]);
-        kop[g][2 * q + 1] = e4m3x8_to_bf16(v[2], v[3]);
+        kop[2 * q] = e4m3x8_to_bf16(v[0], v[1]);
+        kop[2 * q + 1] = e4m3x8_to_bf16(v[2], v[3]);
       }
     }
     const float sl = score_scale(p.scale_log2, descale(a.qd, a.qd_b, a.qd_h, b, h), descale(a.kd, a.kd_b, a.kd_h, b, h));
 
-    float acc[kHeld][16];
+    float acc[16];
 #pragma unroll
-    for (int g = 0; g < kHeld; ++g)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[g][i] = 0.0f;
-    // row tiles from the first that holds a token that sees the first key
-    const int tiles = (R + kRows - 1) / kRows;
-    const int first = (a.causal && k0 > ctx ? int(min(int64_t(k0 - ctx) * G, int64_t(R))) / kRows : 0) + turn;
-    // The lane's row of the tile fetched next: token i, head g, where its query
-    // and its lse lie, and how far the wave's next tile is (a wrap of the heads
-    // is the next token).
-    const int di = kRows * split / G, dg = kRows * split - di * G;
-    int i = (first * kRows + kk) / G, g = first * kRows + kk - i * G;
-    const uint8_t* q_at = p.q8 + (int64_t(r.first) + i) * p.q8_tok + int64_t(h * G + g) * p.q8_head + 16 * half;
-    const float* lse_at = p.lse + int64_t(h * G + g) * p.lse_head_stride + r.first + i;
-    const int64_t q_step = di * p.q8_tok + dg * p.q8_head, q_wrap = p.q8_tok - G * p.q8_head;
-    const int64_t lse_step = di + dg * p.lse_head_stride, lse_wrap = 1 - G * p.lse_head_stride;
-    struct Rows {
-      u32x4 q[4];
-      float lse;
-      int last;  // the last key the row sees, -1 for none
+    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+    // A row tile is 2^hs heads of 32 >> hs consecutive tokens, the shape that needs
+    // the fewest of them; row r is token r >> hs, head r & (2^hs - 1).
+    int hs = 0, fewest = INT32_MAX;
+    for (int e = 0; e <= 5 && (1 << e) < 2 * G; ++e) {
+      const int n = ((r.n + (kRows >> e) - 1) >> (5 - e)) * ((G + (1 << e) - 1) >> e);
+      if (n < fewest) {
+        fewest = n;
+        hs = e;
+      }
+    }
+    const int toks = kRows >> hs, mask = (1 << hs) - 1;
+    const int hgroups = (G + mask) >> hs, hend = hgroups << hs, tiles = ((r.n + toks - 1) >> (5 - hs)) * hgroups;
+    // tiles from the first that holds a token that sees the first key
+    const bool causal = a.causal;
+    const int skip = causal ? min(max(k0 - ctx, 0), r.n) >> (5 - hs) : 0;
+    int tile = skip * hgroups + turn;
+    // tokens and heads that `t` < 9 tiles are (a wrap of the heads is the next tokens)
+    auto apart = [&](int t, int& tok, int& hd) {
+      tok = 0;
+      for (; t >= hgroups; t -= hgroups) tok += toks;
+      hd = t << hs;
     };
-    auto fetch = [&](Rows& t) {
-      const bool live = i < r.n;
+    int tok, hd, dt, dh;
+    apart(turn, tok, hd);
+    apart(split, dt, dh);
+    tok += skip * toks;          // tok, hd: the tile computed next
+    int tok_a = tok, hd_a = hd;  // the tile loaded next
+    const uint8_t* q0 = p.q8 + int64_t(r.first) * p.q8_tok + int64_t(h) * G * p.q8_head;
+    const float* lse0 = p.lse + int64_t(h) * G * p.lse_head_stride + r.first;
+    const uint8_t* q_at = q0 + tok * p.q8_tok + hd * p.q8_head;
+    const float* lse_at = lse0 + tok + hd * p.lse_head_stride;
+    const int64_t q_step = dt * p.q8_tok + dh * p.q8_head, q_wrap = toks * p.q8_tok - hend * p.q8_head;
+    const int64_t lse_step = dt + dh * p.lse_head_stride, lse_wrap = toks - hend * p.lse_head_stride;
+    // loads: lane l takes chunk position l % 8 of rows 8 u + l / 8, chunk c of row t lies at c ^ (t & 7)
+    const int lr = lane >> 3, lchunk = 16 * ((lane & 7) ^ lr);
+    // (rows no closer than 128 bytes: offsets less their 1024 u, see load_lds_4k, stay positive)
+    const bool near = p.near && p.q8_tok >= int64_t(kHead) << hs;
+    uint32_t off_q[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) t.q[u] = live ? *reinterpret_cast<const u32x4*>(q_at + 32 * u) : u32x4(0);
-      t.lse = live ? *lse_at : __builtin_inff();
-      t.last = live ? (a.causal ? ctx + i : full - 1) : -1;
-      i += di;
-      g += dg;
+    for (int u = 0; u < 4; ++u) {
+      const int row = 8 * u + lr;
+      off_q[u] = uint32_t((row >> hs) * p.q8_tok + (row & mask) * p.q8_head) + lchunk - 1024 * u;
+    }
+    const uint32_t off_lse = 4 * uint32_t((kk >> hs) + (kk & mask) * p.lse_head_stride);
+    auto start = [&](int slot_no) {  // five loads: the rows, their lse
+      const uint32_t slot = ring + uint32_t(slot_no) * kHalfSlot, lse_slot = lse_ring + uint32_t(slot_no * kRows * 4);
+      if (__builtin_expect(near && tok_a + toks <= r.n && hd_a + mask < G, 1)) {
+        load_lds_4k(slot, q_at, off_q);
+        if (half == 0) load_lds_dword(lse_slot, lse_at, off_lse);
+      } else {  // rows that are not there: any that is, they count for nothing
+#pragma unroll 1
+        for (int u = 0; u < 4; ++u) {
+          const int row = 8 * u + lr;
+          load_lds(slot + 1024 * u, q0 + min(tok_a + (row >> hs), r.n - 1) * p.q8_tok +
+                                        min(hd_a + (row & mask), G - 1) * p.q8_head + lchunk);
+        }
+        if (half == 0)
+          load_lds_dword(lse_slot, lse0 + min(hd_a + (kk & mask), G - 1) * p.lse_head_stride + min(tok_a + (kk >> hs), r.n - 1));
+      }
+      tok_a += dt;
+      hd_a += dh;
       q_at += q_step;
       lse_at += lse_step;
-      if (g >= G) {
-        g -= G;
-        ++i;
+      if (hd_a >= hend) {
+        hd_a -= hend;
+        tok_a += toks;
         q_at += q_wrap;
         lse_at += lse_wrap;
       }
     };
-    auto pass = [&](const Rows& t) {
-      f32x16 y[kHeld] = {};
+    auto pass = [&](int slot_no) {
+      const uint32_t slot = ring + uint32_t(slot_no) * kHalfSlot;
+      f32x16 y = {};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const bf16x8 q0 = e4m3x8_to_bf16(t.q[q][0], t.q[q][1]), q1 = e4m3x8_to_bf16(t.q[q][2], t.q[q][3]);
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u) {
-          y[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[u][2 * q], q0, y[u], 0, 0, 0);
-          y[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[u][2 * q + 1], q1, y[u], 0, 0, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        const u32x4 v = *lds_at<u32x4>(slot + uint32_t(128 * kk + 16 * ((2 * q + half) ^ (kk & 7))));
+        const bf16x8 v0 = e4m3x8_to_bf16(v[0], v[1]), v1 = e4m3x8_to_bf16(v[2], v[3]);
+        y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[2 * q], v0, y, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[2 * q + 1], v1, y, 0, 0, 0);
       }
       // lse log2(e), in two parts so that it is rounded once
-      const float lse2 = __builtin_fmaf(t.lse, 0x1.715476p+0f, t.lse * 0x1.4ae0cp-26f);
-      if (__all(t.last >= k0 + kGroup - 1)) {
+      const float lse = *lds_at<float>(lse_ring + uint32_t(slot_no * kRows * 4) + 4 * kk);
+      const float lse2 = __builtin_fmaf(lse, 0x1.715476p+0f, lse * 0x1.4ae0cp-26f);
 #pragma unroll
-        for (int u = 0; u < kHeld; ++u)
+      for (int n = 0; n < 16; ++n) y[n] = __builtin_fmaf(y[n], sl, -lse2);
+      if (!(tok + toks <= r.n && hd + mask < G && (!causal || ctx + tok >= k0 + kTile - 1))) {
+        // the last key the row sees, -1 for none
+        const int i = tok + (kk >> hs), last = i < r.n && hd + (kk & mask) < G ? (causal ? ctx + i : full - 1) : -1;
+        const int limit = last - k0 - 4 * half;
 #pragma unroll
-          for (int n = 0; n < 16; ++n) acc[u][n] += __builtin_amdgcn_exp2f(__builtin_fmaf(y[u][n], sl, -lse2));
-      } else {
-        const int limit = t.last - k0 - 4 * half;
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-#pragma unroll
-          for (int n = 0; n < 16; ++n) {
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(y[u][n], sl, -lse2));
-            acc[u][n] += kTile * u + 8 * (n >> 2) + (n & 3) <= limit ? w : 0.0f;
-          }
+        for (int n = 0; n < 16; ++n) y[n] = 8 * (n >> 2) + (n & 3) <= limit ? y[n] : -__builtin_inff();
       }
+#pragma unroll
+      for (int n = 0; n < 16; ++n) acc[n] += __builtin_amdgcn_exp2f(y[n]);
+      tok += dt;
+      hd += dh;
+      if (hd >= hend) {
+        hd -= hend;
+        tok += toks;
+      }
+      // every read of the slot is done before its next loads start
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
-    Rows rows0, rows1;
-    if (first < tiles) fetch(rows0);
+    int ahead = tile, slot_no = 0, to = 0;
 #pragma unroll 1
-    for (int tile = first; tile < tiles; tile += split) {
-      fetch(rows1);
-      __builtin_amdgcn_sched_barrier(0);
-      pass(rows0);
-      rows0 = rows1;
+    for (; ahead < tiles && to < kManyRing - 1; ahead += split, ++to) {
+      start(to);
+    }
+    to = kManyRing - 1;
+#pragma unroll 1
+    for (; tile < tiles; tile += split) {
+      if (ahead < tiles) {
+        start(to);
+        ahead += split;
+        wait_loads<5 * (kManyRing - 1)>();
+      } else {
+        wait_loads<0>();
+      }
+      pass(slot_no);
+      slot_no = slot_no == kManyRing - 1 ? 0 : slot_no + 1;
+      to = to == kManyRing - 1 ? 0 : to + 1;
     }
 
+    const WeightArgs& o = args_again<WeightArgs>();
+    float* scores = score_row(o, b, h);
     // the key of the lane's sum, two lanes a key
     const int idx = (lane >> 1) & 15, key_of = 8 * (idx >> 2) + 4 * half + (idx & 3);
-#pragma unroll
-    for (int u = 0; u < kHeld; ++u) {
-      const float total = sum_lanes(acc[u], lane);
-      const int key = k0 + kTile * u + key_of;
-      if (split > 1) {
-        if ((lane & 1) == 0) s_sum[wave][kTile * u + key_of] = total;
-      } else if ((lane & 1) == 0 && key < L) {
-        scores[key] = decayed(p, scores + key) + total;
-      }
+    const float total = sum_lanes(acc, lane);
+    if (split > 1) {
+      if ((lane & 1) == 0) s_sum[wave][key_of] = total;
+    } else if ((lane & 1) == 0 && k0 + key_of < L) {
+      scores[k0 + key_of] = decayed(o, scores + k0 + key_of) + total;
     }
     if (split > 1) {
       __syncthreads();
       if (turn == 0) {  // the group's first wave joins its waves' sums
         const int key = k0 + lane;
-        if (lane < kGroup && key < L) {
-          float total = s_sum[wave][lane];
-          for (int w = 1; w < split; ++w) total += s_sum[wave + w][lane];
-          scores[key] = decayed(p, scores + key) + total;
+        if (lane < kTile && key < L) {
+          float sum = s_sum[wave][lane];
+          for (int i = 1; i < split; ++i) sum += s_sum[wave + i][lane];
+          scores[key] = decayed(o, scores + key) + sum;
         }
       }
       __syncthreads();
@@ -655,14 +724,18 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
     p.q8_tok = a.q_tok_stride;
     p.q8_head = a.q_head_stride;
   }
+  const int64_t reach = INT32_MAX / (2 * kRows);
+  p.near = p.q8_tok >= kHead && p.q8_tok <= reach && p.q8_head >= kHead && p.q8_head <= reach && lse_head_stride >= 0 &&
+           lse_head_stride <= reach / 4;
   const int64_t keys = std::max<int64_t>(1, std::min(max_seq_len, scores_width));
   p.row_tiles = int32_t(ceil_div(rows, kRows));
   p.slots = int32_t(2 * cus);  // resident at once
-  p.s.step_shift = log2_exact(kGroup);
+  p.cus = int32_t(std::max<int64_t>(cus & ~7, 8));
+  p.s.step_shift = log2_exact(kTile);
   p.s.over = 0;
   p.s.min_run = 1;
   p.s.max_runs = 1;
-  const int64_t most = num_seqs * num_kv_heads * ceil_div(keys, kGroup);
+  const int64_t most = ceil_div(num_seqs * num_kv_heads * ceil_div(keys, kTile), p.cus) * p.cus;
   hipLaunchKernelGGL(many_rows_kernel, dim3(unsigned(std::min<int64_t>(most, 4 * p.slots))),
                      dim3(64 * kManyWaves), 0, st, p);
   return check_launch("many_rows_kernel launch");

@@ -136,6 +136,15 @@ struct QueryBytes {
   }
 };
 
+// A kernel's only argument, read again from where the launch put it: what is used
+// between two such calls alone takes no scalar registers outside.
+template <class Args>
+__device__ __forceinline__ const Args& args_again() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Args*)p;
+}
+
 // ---------------------------------------------------------------------------
 // a step's work cut into equal runs
 // ---------------------------------------------------------------------------

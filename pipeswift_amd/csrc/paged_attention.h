@@ -161,9 +161,23 @@ __device__ __forceinline__ void load_lds(uint32_t at, const uint8_t* p) {
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
                : "=&s"(m0) : "s"(at), "v"(p) : "memory");
 }
-// Four such loads of 1 KiB, of bytes that nothing reads again (nt): from p[u] +
-// 1024 u to at + 1024 u.  An instruction's offset counts for both its addresses,
-// so the LDS base is set once.
+// Four such loads of 1 KiB, to at + 1024 u.  An instruction's offset counts for
+// both its addresses, so the LDS base is set once: from base + offset[u] + 1024 u.
+__device__ __forceinline__ void load_lds_4k(uint32_t at, const uint8_t* base, const uint32_t (&offset)[4]) {
+  uint32_t m0;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %3, %2\n\t"
+      "global_load_lds_dwordx4 %4, %2 offset:1024\n\t"
+      "global_load_lds_dwordx4 %5, %2 offset:2048\n\t"
+      "global_load_lds_dwordx4 %6, %2 offset:3072\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(m0)
+      : "s"(at), "s"(base), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3])
+      : "memory");
+}
+// From p[u] + 1024 u, bytes that nothing reads again (nt).
 __device__ __forceinline__ void load_lds_4k_once(uint32_t at, const uint8_t* const (&p)[4], uint32_t offset) {
   uint32_t m0;
   asm volatile(
@@ -183,6 +197,11 @@ __device__ __forceinline__ void load_lds_dword(uint32_t at, const void* base, ui
   uint32_t m0;
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %2, %3\n\ts_mov_b32 m0, %0"
                : "=&s"(m0) : "s"(at), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds_dword(uint32_t at, const void* p) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "s"(at), "v"(p) : "memory");
 }
 // Until at most N of this wave's loads are in flight.
 template <int N>
