@@ -93,8 +93,7 @@ __device__ __forceinline__ float decayed(const WeightArgs& p, const float* at) {
 // every line.  Runs of one kv head instead of all of a token's: 164.
 template <int Q_DT, bool OLD, bool GEN>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
-few_rows_kernel(WeightArgs p) {
-  const DecodeArgs& a = p.a;
+few_rows_kernel(WeightArgs args) {
   __shared__ __attribute__((aligned(1024))) char s_ring[kWaves * kFewRing * kHalfSlot];
   __shared__ float s_old[kWaves * kFewRing * kTile];
   __shared__ int32_t s_pages[kPages];
@@ -108,15 +107,17 @@ few_rows_kernel(WeightArgs p) {
   const uint32_t old_at = (uint32_t)(size_t)(lvoid*)s_old + uint32_t(wave * kFewRing * kTile * 4);
   // loads: lane l takes chunk position l % 8 of keys 8 u + l / 8, chunk c of key t lies at c ^ (t & 7)
   const int lr = lane >> 3, lchunk = 16 * ((lane & 7) ^ lr);
-  const uint32_t off_k = uint32_t(lr * a.k_row) + lchunk;
+  const uint32_t off_k = uint32_t(lr * args.a.k_row) + lchunk;
   SeqWindow seqs;
-  const StepRuns step_run = step_runs(a, p.s, seqs, lane);
+  const StepRuns step_run = step_runs(args.a, args.s, seqs, lane);
   int64_t x = xcd_run(step_run, int(blockIdx.x) & 7, int(blockIdx.x) >> 3) * step_run.run;
   if (x >= step_run.total) return;
   const int64_t x_end = min(x + step_run.run, step_run.total);
   int64_t before;
-  int b = seq_of_unit(a, p.s, x, seqs, lane, before);
+  int b = seq_of_unit(args.a, args.s, x, seqs, lane, before);
   while (x < x_end) {  // over the run's jobs
+    const WeightArgs& p = args_again<WeightArgs>();
+    const DecodeArgs& a = p.a;
     if (!seqs.holds(b)) seqs.load(a, p.s, b, lane);
     const SeqRows r{lane_value(seqs.first, b - seqs.b0), lane_value(seqs.n, b - seqs.b0)};
     const int full = lane_value(seqs.len, b - seqs.b0), L = min(full, p.s.width);

@@ -76,24 +76,24 @@ __device__ __forceinline__ float* record(const TreeArgs& p, int64_t run, int blo
 // to slot + 1024 u, V rows behind them.  An instruction's offset counts for both
 // its addresses, so the LDS base is set once for K and once for V.
 __device__ __forceinline__ void load_tile(uint32_t slot, const uint8_t* const (&kp)[4], const uint8_t* const (&vp)[4],
-                                          uint32_t off_k, uint32_t off_v) {
+                                          uint32_t offset) {
   uint32_t m0;
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
       "s_mov_b32 m0, %1\n\ts_nop 0\n\t"
-      "global_load_lds_dwordx4 %3, %5\n\t"
-      "global_load_lds_dwordx4 %3, %6 offset:1024\n\t"
-      "global_load_lds_dwordx4 %3, %7 offset:2048\n\t"
-      "global_load_lds_dwordx4 %3, %8 offset:3072\n\t"
+      "global_load_lds_dwordx4 %3, %4\n\t"
+      "global_load_lds_dwordx4 %3, %5 offset:1024\n\t"
+      "global_load_lds_dwordx4 %3, %6 offset:2048\n\t"
+      "global_load_lds_dwordx4 %3, %7 offset:3072\n\t"
       "s_mov_b32 m0, %2\n\ts_nop 0\n\t"
-      "global_load_lds_dwordx4 %4, %9\n\t"
-      "global_load_lds_dwordx4 %4, %10 offset:1024\n\t"
-      "global_load_lds_dwordx4 %4, %11 offset:2048\n\t"
-      "global_load_lds_dwordx4 %4, %12 offset:3072\n\t"
+      "global_load_lds_dwordx4 %3, %8\n\t"
+      "global_load_lds_dwordx4 %3, %9 offset:1024\n\t"
+      "global_load_lds_dwordx4 %3, %10 offset:2048\n\t"
+      "global_load_lds_dwordx4 %3, %11 offset:3072\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(m0)
-      : "s"(slot), "s"(slot + kHalfSlot), "v"(off_k), "v"(off_v), "s"(kp[0]), "s"(kp[1]), "s"(kp[2]), "s"(kp[3]),
-        "s"(vp[0]), "s"(vp[1]), "s"(vp[2]), "s"(vp[3])
+      : "s"(slot), "s"(slot + kHalfSlot), "v"(offset), "s"(kp[0]), "s"(kp[1]), "s"(kp[2]), "s"(kp[3]), "s"(vp[0]),
+        "s"(vp[1]), "s"(vp[2]), "s"(vp[3])
       : "memory");
 }
 
@@ -143,8 +143,7 @@ __device__ __forceinline__ void finish(const TreeArgs& p, const SeqRows& r, int 
 
 template <int Q_DT, int OUT_DT, bool GEN>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
-tree_attention_kernel(TreeArgs p) {
-  const DecodeArgs& a = p.a;
+tree_attention_kernel(TreeArgs args) {
   __shared__ __attribute__((aligned(1024))) char s_ring[kWaves * kRing * kSlot];
   __shared__ int32_t s_pages[kPages];
   __shared__ u32x4 s_q[kRows * 8];  // the rows' e4m3 queries, chunk c of row r at c ^ (r & 7)
@@ -156,9 +155,9 @@ tree_attention_kernel(TreeArgs p) {
   const int half = lane >> 5, kk = lane & 31;
 
   SeqWindow seqs;
-  const StepRuns step_run = step_runs(a, p.s, seqs, lane);
+  const StepRuns step_run = step_runs(args.a, args.s, seqs, lane);
   // the row blocks of a run, which read the same keys, are next to each other on its XCD
-  const int w = int(blockIdx.x), idx = (w >> 3) / p.row_blocks, block = (w >> 3) - idx * p.row_blocks;
+  const int w = int(blockIdx.x), idx = (w >> 3) / args.row_blocks, block = (w >> 3) - idx * args.row_blocks;
   const int64_t j = xcd_run(step_run, w & 7, idx);
   int64_t x = j * step_run.run;
   if (x >= step_run.total) return;
@@ -179,8 +178,10 @@ tree_attention_kernel(TreeArgs p) {
     rd_v[d] = kHalfSlot + uint32_t(128 * vkey + 16 * ((2 * d + vg) ^ (vkey & 7)) + 8 * (vr & 1));
 
   int64_t before;
-  int b = seq_of_unit(a, p.s, x, seqs, lane, before);
+  int b = seq_of_unit(args.a, args.s, x, seqs, lane, before);
   while (x < x_end) {  // over the run's jobs
+    const TreeArgs& p = args_again<TreeArgs>();
+    const DecodeArgs& a = p.a;
     if (!seqs.holds(b)) seqs.load(a, p.s, b, lane);
     const SeqRows r{lane_value(seqs.first, b - seqs.b0), lane_value(seqs.n, b - seqs.b0)};
     const int L = lane_value(seqs.len, b - seqs.b0);
@@ -233,7 +234,8 @@ tree_attention_kernel(TreeArgs p) {
 
     const uint8_t* kbase = a.k + int64_t(h) * a.k_head;
     const uint8_t* vbase = a.v + int64_t(h) * a.v_head;
-    const uint32_t off_k = uint32_t(lr * a.k_row) + lchunk, off_v = uint32_t(lr * a.v_row) + lchunk;
+    const int64_t v_from_k = vbase - kbase;
+    const uint32_t off = uint32_t(lr * a.k_row) + lchunk;
     const int n_tiles = (L + kTile - 1) / kTile;
     const int t_mask = max(ctx, 0) / kTile;  // tiles from here on need masks
     const int steps_per_window = int(min(int64_t(kPages - 1) * a.block_size / kStepKeys, int64_t(1) << 24));
@@ -266,11 +268,12 @@ tree_attention_kernel(TreeArgs p) {
       bool full = true;  // the newest tile's loads are all in flight
       // GEN: every lane looks its four keys' pages up.  Else eight keys of one
       // load share a page: lane 4 k + u holds where load u of tile win + 4 k
-      // begins, for sixteen tiles at a time, and the addresses are scalar.
+      // begins in a kv head's K, for sixteen tiles at a time, and the addresses are scalar.
       int win = 0;
-      int64_t at_k = 0, at_v = 0;
+      int64_t at = 0;
       uint64_t whole8 = 0, some8 = 0;  // loads whose eight keys are all cached; whose first is
       auto look_up = [&](int t) {
+        const DecodeArgs& a = args_again<TreeArgs>().a;
         win = t;
         const int key = (t + kWaves * (lane >> 2)) * kTile + 8 * (lane & 3);
         int32_t id = -1;
@@ -280,8 +283,7 @@ tree_attention_kernel(TreeArgs p) {
           id = s_pages[pi - p0];
         }
         const int64_t row = key - pi * a.block_size;
-        at_k = int64_t(id) * a.k_blk + row * a.k_row - 1024 * (lane & 3);
-        at_v = int64_t(id) * a.v_blk + row * a.v_row - 1024 * (lane & 3);
+        at = int64_t(id) * a.k_blk + row * a.k_row - 1024 * (lane & 3);
         some8 = __ballot(id >= 0);
         whole8 = __ballot(id >= 0 && key + 8 <= L);
       };
@@ -315,18 +317,18 @@ tree_attention_kernel(TreeArgs p) {
           const uint8_t* vp[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            kp[u] = kbase + lane_value(at_k, k + u);
-            vp[u] = vbase + lane_value(at_v, k + u);
+            kp[u] = kbase + lane_value(at, k + u);
+            vp[u] = kp[u] + v_from_k;
           }
           full = ((whole8 >> k) & 15) == 15;
           if (__builtin_expect(full, 1)) {
-            load_tile(slot, kp, vp, off_k, off_v);
+            load_tile(slot, kp, vp, off);
           } else {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               if (((some8 >> (k + u)) & 1) && t * kTile + 8 * u + lr < L) {
-                load_lds(slot + 1024 * u, kp[u] + 1024 * u, off_k);
-                load_lds(slot + kHalfSlot + 1024 * u, vp[u] + 1024 * u, off_v);
+                load_lds(slot + 1024 * u, kp[u] + 1024 * u, off);
+                load_lds(slot + kHalfSlot + 1024 * u, vp[u] + 1024 * u, off);
               } else {
                 *lds_at<u32x4>(slot + 1024 * u + 16 * lane) = u32x4(0);
                 *lds_at<u32x4>(slot + kHalfSlot + 1024 * u + 16 * lane) = u32x4(0);
@@ -463,6 +465,7 @@ tree_attention_kernel(TreeArgs p) {
       while (t < t_end) step(std::true_type{});
     }
 
+    const TreeArgs& rest = args_again<TreeArgs>();
     // the four waves' results, joined in the order of the waves
     const float lt = l + __shfl_xor(l, 32);
     if (lane < 32) {
@@ -485,7 +488,7 @@ tree_attention_kernel(TreeArgs p) {
       s_o[(wave * 16 + q) * 64 + lane] =
           f32x4{o[q >> 2][4 * (q & 3)], o[q >> 2][4 * (q & 3) + 1], o[q >> 2][4 * (q & 3) + 2], o[q >> 2][4 * (q & 3) + 3]} * f;
     __syncthreads();
-    float* rec = record(p, j, block, c.from == 0 ? 1 : 0);
+    float* rec = record(rest, j, block, c.from == 0 ? 1 : 0);
 #pragma unroll
     for (int i = 0; i < 16 / kWaves; ++i) {
       const int q = wave + kWaves * i;
@@ -497,7 +500,7 @@ tree_attention_kernel(TreeArgs p) {
         for (int k = 0; k < 4; ++k)
           if ((s_nan[8 * q + 4 * half + k] >> kk) & 1u) v[k] = __builtin_nanf("");
       }
-      if (whole) finish<OUT_DT>(p, r, b, h, row, q, lane, v, top, sum);
+      if (whole) finish<OUT_DT>(rest, r, b, h, row, q, lane, v, top, sum);
       else *reinterpret_cast<f32x4*>(rec + (q * 64 + lane) * 4) = v;
     }
     if (!whole && wave == 0 && lane < 32) {
@@ -599,9 +602,10 @@ int launch_tree(const TreeArgs& p, bool general, hipStream_t st) {
 template <int Q_DT>
 int launch_tree_q(const TreeArgs& p, int out_dtype, hipStream_t st) {
   const DecodeArgs& a = p.a;
-  // pages of a multiple of 8 keys whose rows lie within 32-bit offsets: the keys of a load share a page
-  const bool general = a.block_size % 8 != 0 || a.k_row < 0 || a.v_row < 0 ||
-                       8 * std::max(a.k_row, a.v_row) >= (int64_t(1) << 31);
+  // pages of a multiple of 8 keys whose rows lie within 32-bit offsets (the keys of a
+  // load share a page), K and V laid out alike
+  const bool general = a.block_size % 8 != 0 || a.k_row < 0 || 8 * a.k_row >= (int64_t(1) << 31) || a.k_row != a.v_row ||
+                       a.k_blk != a.v_blk;
   return out_dtype == PSK_DTYPE_BF16 ? launch_tree<Q_DT, PSK_DTYPE_BF16>(p, general, st)
                                      : launch_tree<Q_DT, PSK_DTYPE_F32>(p, general, st);
 }
