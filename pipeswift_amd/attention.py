@@ -411,17 +411,18 @@ def paged_tree_attention(
     vd, vsb, vsh = _descale(v_descale, B, Hkv, device)
     with on_device(device):
         need = tree_workspace_floats(B, TQ, n, Hq, Hkv, bound)
-        if workspace is None or workspace.numel() < need:
-            workspace = torch.empty(max(need, 1), dtype=torch.float32, device=device)
-        assert workspace.dtype == torch.float32 and workspace.device == device and workspace.is_contiguous()
+        if need and (workspace is None or workspace.numel() < need):
+            workspace = torch.empty(need, dtype=torch.float32, device=device)
+        assert workspace is None or (workspace.dtype == torch.float32 and workspace.device == device
+                                     and workspace.is_contiguous())
         st = lib().psk_paged_tree_attention(
             q.data_ptr(), q.stride(0), q.stride(1), dtype_code(q.dtype), k_cache.data_ptr(), v_cache.data_ptr(),
             i64_array(k_cache.stride()[:3]), i64_array(v_cache.stride()[:3]), block_table.data_ptr(),
             block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), B, Hq, Hkv, HEAD_DIM, ps, P, bound, TQ, n,
             ptr(cu_seqlens_q), tree_mask.data_ptr(), tree_mask.stride(0), tree_mask.shape[1], float(softmax_scale),
             ptr(qd), ptr(kd), ptr(vd), i64_array([qsb, qsh, ksb, ksh, vsb, vsh]), out.data_ptr(), out.stride(0),
-            out.stride(1), _OUT_CODES[out.dtype], ptr(lse), TQ if lse is not None else 0, workspace.data_ptr(),
-            workspace.numel(), stream_handle(device),
+            out.stride(1), _OUT_CODES[out.dtype], ptr(lse), TQ if lse is not None else 0, ptr(workspace),
+            0 if workspace is None else workspace.numel(), stream_handle(device),
         )
     check(st, "paged_tree_attention")
     return (out, lse) if return_softmax_lse else out

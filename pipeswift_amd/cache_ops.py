@@ -191,15 +191,17 @@ def _cache_pairs(caches, first_row_dim):
     if isinstance(caches, torch.Tensor):
         caches = [caches]
     assert len(caches) > 0
+    device, outer = caches[0].device, caches[0].shape[:3]
     for c in caches:
-        assert c.is_cuda and c.device == caches[0].device, "all caches must be on one GPU"
-        assert c.shape[:3] == caches[0].shape[:3], "all caches must have the same layers, pages and page size"
+        shape, strides = c.shape, c.stride()
+        assert c.is_cuda and c.device == device, "all caches must be on one GPU"
+        assert shape[:3] == outer, "all caches must have the same layers, pages and page size"
         expect = 1
-        for dim in range(c.ndim - 1, first_row_dim - 1, -1):
-            assert c.stride(dim) == expect or c.shape[dim] == 1, (
-                f"cache rows must be contiguous beyond dim {first_row_dim - 1} (strides {c.stride()})"
+        for dim in range(len(shape) - 1, first_row_dim - 1, -1):
+            assert strides[dim] == expect or shape[dim] == 1, (
+                f"cache rows must be contiguous beyond dim {first_row_dim - 1} (strides {strides})"
             )
-            expect *= c.shape[dim]
+            expect *= shape[dim]
     pairs, i = [], 0
     while i < len(caches):
         a = caches[i]
@@ -210,11 +212,11 @@ def _cache_pairs(caches, first_row_dim):
     return pairs
 
 
-def _i32(t, device, shape, name):
+def _i32(t, device, dims, rows, name):
+    shape = t.shape
     assert t.dtype == torch.int32 and t.device == device, f"{name} must be int32 on the caches' device"
-    assert t.dim() == len(shape) and all(n is None or t.shape[d] >= n for d, n in enumerate(shape)), \
-        f"{name} has shape {tuple(t.shape)}"
-    assert t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name} needs unit last stride"
+    assert len(shape) == dims and shape[0] >= rows, f"{name} has shape {tuple(shape)}, want {dims} dimensions and {rows} rows"
+    assert shape[-1] <= 1 or t.stride(-1) == 1, f"{name} needs unit last stride"
 
 
 def evict_tokens(
@@ -275,9 +277,9 @@ def evict_tokens(
     budget, sink, recent = int(budget), int(sink), int(recent)
     assert budget >= 1 and sink >= 0 and recent >= 0 and sink + recent <= budget, \
         f"sink {sink} and recent {recent} do not fit a budget of {budget}"
-    _i32(block_table, device, (B, None), "block_table")
-    _i32(dst_block_table, device, (B, None), "dst_block_table")
-    _i32(seq_lens, device, (B,), "seq_lens")
+    _i32(block_table, device, 2, B, "block_table")
+    _i32(dst_block_table, device, 2, B, "dst_block_table")
+    _i32(seq_lens, device, 1, B, "seq_lens")
     assert dst_block_table.shape[1] * page >= budget, \
         f"{dst_block_table.shape[1]} pages of {page} cannot hold a budget of {budget}"
     assert block_table.data_ptr() != dst_block_table.data_ptr() or B == 0, "the kept tokens go to pages of their own"
@@ -335,10 +337,10 @@ def commit_draft_tokens(
     device = first.device
     layers, num_blocks, page = first.shape[:3]
     B = path.shape[0]
-    _i32(path, device, (None, None), "path")
-    _i32(block_table, device, (B, None), "block_table")
-    _i32(starts, device, (B,), "starts")
-    _i32(path_lens, device, (B,), "path_lens")
+    _i32(path, device, 2, 0, "path")
+    _i32(block_table, device, 2, B, "block_table")
+    _i32(starts, device, 1, B, "starts")
+    _i32(path_lens, device, 1, B, "path_lens")
     with on_device(device):
         for a, b in pairs:
             es = a.element_size()

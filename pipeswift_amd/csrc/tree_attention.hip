@@ -51,6 +51,11 @@ constexpr int kTile = 32;                  // keys of a tile
 constexpr uint32_t kHalfSlot = kTile * 128;  // bytes of a tile's K (its V follows)
 constexpr uint32_t kSlot = 2 * kHalfSlot;
 constexpr int kRing = 2;
+constexpr int kOver = 6;                   // units (of kStepKeys keys) that a piece costs beside its keys
+// Up to this many keys a workgroup takes all of a job's and nothing is merged: four
+// sequences of 8 tokens (32 query heads over 8), us, whole / cut: 1000 keys 17 / 19, 1600
+// 19 / 19, 2500 24 / 21; 64 sequences of 1000, 32 / 38.
+constexpr int kWholeKeys = 1536;
 constexpr int kPages = 1024;               // page ids a piece stages at a time
 constexpr int kSlab = 4096 + 64;           // floats of 32 rows' partial result: accumulators, maxima, sums
 constexpr int kMaxSlots = 512;             // resident workgroups the workspace is sized for
@@ -65,6 +70,7 @@ struct TreeArgs {
   const int64_t* mask;
   int64_t mask_stride;   // words from a query token's mask to the next one's
   int32_t row_blocks;    // workgroups that share a run's keys
+  int32_t whole;         // a workgroup takes all of a job's keys, and nothing is merged
   float* records;        // [max_runs][row_blocks][2][kSlab]
 };
 
@@ -154,14 +160,29 @@ tree_attention_kernel(TreeArgs args) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, kk = lane & 31;
 
-  SeqWindow seqs;
-  const StepRuns step_run = step_runs(args.a, args.s, seqs, lane);
   // the row blocks of a run, which read the same keys, are next to each other on its XCD
   const int w = int(blockIdx.x), idx = (w >> 3) / args.row_blocks, block = (w >> 3) - idx * args.row_blocks;
-  const int64_t j = xcd_run(step_run, w & 7, idx);
-  int64_t x = j * step_run.run;
-  if (x >= step_run.total) return;
-  const int64_t x_end = min(x + step_run.run, step_run.total);
+  SeqWindow seqs;
+  int64_t j = 0, x, x_end, before = 0;  // the run, its units, the units before the sequence
+  int b;
+  if (args.whole) {  // a workgroup a job
+    const int jobs = args.s.num_seqs * args.s.heads, per = (jobs + 7) >> 3;
+    const int job = (w & 7) * per + idx;
+    if (job >= jobs) return;
+    b = job / args.s.heads;
+    seqs.load(args.a, args.s, b & ~63, lane);
+    if (lane_value(seqs.n, b - seqs.b0) == 0) return;
+    const int64_t cost = args.s.over + key_steps(args.s, lane_value(seqs.len, b - seqs.b0));
+    x = (job - b * args.s.heads) * cost;
+    x_end = x + cost;
+  } else {
+    const StepRuns step_run = step_runs(args.a, args.s, seqs, lane);
+    j = xcd_run(step_run, w & 7, idx);
+    x = j * step_run.run;
+    if (x >= step_run.total) return;
+    x_end = min(x + step_run.run, step_run.total);
+    b = seq_of_unit(args.a, args.s, x, seqs, lane, before);
+  }
 
   const uint32_t ring = (uint32_t)(size_t)(lvoid*)s_ring + uint32_t(wave * kRing) * kSlot;
   // loads: lane l takes chunk position l % 8 of keys 8 u + l / 8
@@ -177,8 +198,6 @@ tree_attention_kernel(TreeArgs args) {
   for (int d = 0; d < 4; ++d)
     rd_v[d] = kHalfSlot + uint32_t(128 * vkey + 16 * ((2 * d + vg) ^ (vkey & 7)) + 8 * (vr & 1));
 
-  int64_t before;
-  int b = seq_of_unit(args.a, args.s, x, seqs, lane, before);
   while (x < x_end) {  // over the run's jobs
     const TreeArgs& p = args_again<TreeArgs>();
     const DecodeArgs& a = p.a;
@@ -199,7 +218,7 @@ tree_attention_kernel(TreeArgs args) {
     const Piece c = piece_of(p.s, x - at, hi - at);
     x = hi;
     const int row0 = block * kRows;
-    if (c.from >= c.to || row0 >= r.n * a.heads) continue;
+    if ((c.from >= c.to && !p.whole) || row0 >= r.n * a.heads) continue;
 
     // The queries: every thread quantizes 16 elements of a row, and the waves
     // read the rows' bytes from LDS.  The pages of the first keys are on their
@@ -590,11 +609,12 @@ TreeShape tree_shape(int64_t rows, int64_t slots) {
 
 template <int Q_DT, int OUT_DT>
 int launch_tree(const TreeArgs& p, bool general, hipStream_t st) {
-  const dim3 grid{unsigned(p.s.max_runs * p.row_blocks), 1u, 1u};
+  const int64_t jobs = int64_t(p.s.num_seqs) * p.s.heads;
+  const dim3 grid{unsigned((p.whole ? ceil_div(jobs, 8) * 8 : p.s.max_runs) * p.row_blocks), 1u, 1u};
   if (general) hipLaunchKernelGGL((tree_attention_kernel<Q_DT, OUT_DT, true>), grid, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((tree_attention_kernel<Q_DT, OUT_DT, false>), grid, dim3(kThreads), 0, st, p);
-  if (const int e = check_launch("tree_attention_kernel launch"); e != PSK_OK) return e;
-  const int64_t tasks = int64_t(p.s.num_seqs) * p.s.heads * p.row_blocks * 16;
+  if (const int e = check_launch("tree_attention_kernel launch"); e != PSK_OK || p.whole) return e;
+  const int64_t tasks = jobs * p.row_blocks * 16;
   hipLaunchKernelGGL((merge_tree_kernel<OUT_DT>), dim3(unsigned(tasks / 4)), dim3(256), 0, st, p);
   return check_launch("merge_tree_kernel launch");
 }
@@ -619,6 +639,7 @@ int64_t psk_paged_tree_workspace_len(int64_t num_seqs, int64_t total_q, int64_t 
   if (num_seqs < 0 || total_q < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
       max_seqlen_q <= 0 || max_seqlen_q > INT32_MAX / (num_q_heads / num_kv_heads) || max_seq_len < 0)
     return PSK_E_ARG;
+  if (max_seq_len <= kWholeKeys) return 0;
   const TreeShape s = tree_shape(max_seqlen_q * (num_q_heads / num_kv_heads), kMaxSlots);
   return 4 + s.max_runs * s.row_blocks * 2 * kSlab;
 }
@@ -649,7 +670,7 @@ int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head
   if (max_seq_len < 0) return fail(PSK_E_ARG, "max_seq_len %lld", (long long)max_seq_len);
   if (const int st = check_cached_queries(c, a, &empty); st != PSK_OK) return st;
   if (empty || total_q == 0) return PSK_OK;
-  if (!v_cache || !v_strides || !tree_mask || !out || !workspace) return fail(PSK_E_ARG, "NULL pointer");
+  if (!v_cache || !v_strides || !tree_mask || !out) return fail(PSK_E_ARG, "NULL pointer");
   const uint64_t v_align[4] = {uint64_t(uintptr_t(v_cache)), uint64_t(v_strides[0]), uint64_t(v_strides[1]),
                                uint64_t(v_strides[2])};
   if (common_align(v_align, 4, 16) < 16) return fail(PSK_E_ARG, "K/V caches need 16-byte aligned bases and strides");
@@ -659,7 +680,7 @@ int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head
   if (common_align(o_align, 3, 4 * osz) < 4 * osz)
     return fail(PSK_E_ARG, "output rows need %d-byte alignment", 4 * osz);
   const int64_t need = psk_paged_tree_workspace_len(num_seqs, total_q, max_seqlen_q, num_q_heads, num_kv_heads, max_seq_len);
-  if (workspace_len < need)
+  if (workspace_len < need || (need > 0 && !workspace))
     return fail(PSK_E_WORKSPACE, "workspace of %lld floats, need %lld", (long long)workspace_len, (long long)need);
   a.v = static_cast<const uint8_t*>(v_cache);
   a.v_blk = v_strides[0];
@@ -687,11 +708,12 @@ int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head
   p.s.total_q = int32_t(total_q);
   p.s.heads = int32_t(num_kv_heads);
   p.s.step_shift = kStepShift;
-  p.s.over = 1;
+  p.s.over = kOver;
   p.s.max_runs = int32_t(s.max_runs);
   p.s.min_run = 2;
   p.s.width = INT32_MAX;
   p.row_blocks = int32_t(s.row_blocks);
+  p.whole = max_seq_len <= kWholeKeys;
   p.records = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
   if (num_seqs * num_kv_heads * s.row_blocks > INT32_MAX / 16 || s.max_runs * s.row_blocks > INT32_MAX)
     return fail(PSK_E_ARG, "too many rows (%lld sequences of up to %lld drafted tokens)", (long long)num_seqs,
