@@ -1,6 +1,6 @@
 // What the kernels that read queries against the paged FP8 cache and take a
 // whole batch's lengths from the device share (tree_attention.hip,
-// attention_weights.hip): the argument checks of their C entries.
+// prefill_runs.hip's trees, attention_weights.hip).
 #pragma once
 
 #include <cmath>
@@ -97,10 +97,34 @@ __device__ __forceinline__ SeqRows seq_rows(const DecodeArgs& a, int32_t total_q
   return SeqRows{int32_t(f), min(q_count(a, b), total_q - int32_t(f))};
 }
 
+// A sequence's length, kept where the arithmetic on whole tiles of it stays in 31 bits.
+__device__ __forceinline__ int32_t cached_len(const DecodeArgs& a, int b) {
+  return min(max(a.seq_lens[b], 0), INT32_MAX - 1024);
+}
+
 // The scale from a product q~ . K to the exp2 domain, rounded once (each rounding
 // of it is an error of every score in the same direction).
 __device__ __forceinline__ float score_scale(double scale_log2, float qd, float kd) {
   return float(scale_log2 * double(qd) * double(kd));
+}
+
+// Visibility of keys key0 .. key0 + 31 (bit k: key0 + k) to a drafted token with mask m, of n after `ctx` keys.
+__device__ __forceinline__ uint32_t visible(const int64_t* m, int ctx, int n, int key0) {
+  const int j0 = key0 - ctx;  // the drafted index of key0
+  if (j0 <= -32) return 0xFFFFFFFFu;
+  if (j0 >= n) return 0u;
+  const int left = n - j0;  // keys before the tree's end
+  const uint32_t in = left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u;
+  if (j0 < 0) return ((uint32_t(m[0]) << -j0) | ((1u << -j0) - 1u)) & in;
+  const int w = j0 >> 6, sh = j0 & 63;
+  uint64_t bits = uint64_t(m[w]) >> sh;
+  if (sh > 32 && left > 64 - sh) bits |= uint64_t(m[w + 1]) << (64 - sh);
+  return uint32_t(bits) & in;
+}
+
+// Bit 0 of every byte of x that is an e4m3 NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {
+  return (((x & 0x7F7F7F7Fu) + 0x01010101u) >> 7) & 0x01010101u;
 }
 
 // Sixteen elements of a query row, loaded and then quantized to their e4m3 bytes
@@ -165,10 +189,6 @@ struct JobSpace {
   int32_t width;                     // keys past it cost nothing
 };
 
-// A sequence's length, kept where the arithmetic on whole tiles of it stays in 31 bits.
-__device__ __forceinline__ int32_t cached_len(const DecodeArgs& a, int b) {
-  return min(max(a.seq_lens[b], 0), INT32_MAX - 1024);
-}
 __device__ __forceinline__ int32_t key_steps(const JobSpace& s, int32_t len) {
   return (len + (1 << s.step_shift) - 1) >> s.step_shift;
 }

@@ -163,8 +163,8 @@ __device__ __forceinline__ void store_cols4<PSK_DTYPE_BF16>(char* dst, f32x4 v) 
 // Row lane % 32 of a wave's 32 of a block of ni query tokens from row `first`
 // of q: columns 32 d + 8 q + 4 (lane / 32) .. + 3 of O^T in o[4 (d - d0) + q]
 // for d0 <= d < d0 + ND, the sum lt and the maximum m, times vd to the output
-// and (with d0 = 0) to the lse.
-template <int OUT_DT, int ND>
+// and (with d0 = 0) to the lse.  A NaN sum counts where NANS.
+template <int OUT_DT, int ND, bool NANS = false>
 __device__ __forceinline__ void write_row(const DecodeArgs& a, int64_t first, int ni, int h, float vd, int wave, int lane,
                                           int d0, const f32x4 (&o)[4 * ND], float m, float lt) {
   const int G = a.heads;
@@ -172,7 +172,8 @@ __device__ __forceinline__ void write_row(const DecodeArgs& a, int64_t first, in
   const int ti = r / G, g = r - ti * G;
   if (ti >= ni) return;
   const int64_t tok = first + ti;
-  const float inv = lt > 0.0f ? vd / lt : 0.0f;  // no key seen: zeros, lse = -inf
+  const bool any = NANS ? lt != 0.0f : lt > 0.0f;
+  const float inv = any ? vd / lt : 0.0f;  // no key seen: zeros, lse = -inf
   char* dst = a.out + tok * a.out_tok_stride + int64_t(h * G + g) * a.out_head_stride;
   constexpr int kEsz = Elt<OUT_DT>::kSize;
 #pragma unroll
@@ -180,7 +181,7 @@ __device__ __forceinline__ void write_row(const DecodeArgs& a, int64_t first, in
     store_cols4<OUT_DT>(dst + (32 * (d0 + (c >> 2)) + 8 * (c & 3) + 4 * (lane >> 5)) * kEsz, o[c] * inv);
   if (lane < 32 && d0 == 0 && a.lse)
     a.lse[int64_t(h * G + g) * a.lse_head_stride + tok] =
-        lt > 0.0f ? (m + __builtin_log2f(lt)) * 0.6931471805599453f : -__builtin_inff();
+        any ? (m + __builtin_log2f(lt)) * 0.6931471805599453f : -__builtin_inff();
 }
 
 // LDS of merge_records.
@@ -202,8 +203,10 @@ struct MergeLds {
 // 2 kv heads, the whole call with this merge in the launch the device chooses for:
 // 54.7 us with the tasks on the first workgroups, 50.6-52.2 spread over all of them
 // (R = 4 and 8), 42.1 (R = 4) and 39.3 (R = 8) with the maxima 16 a round as well.
-template <int OUT_DT, int R>
-__device__ __forceinline__ void merge_records(const DecodeArgs& a, int tq, const RunSpace& s, MergeLds& lds) {
+// first_row(b): the row of q that sequence b begins with.
+template <int OUT_DT, int R, bool NANS = false, class First>
+__device__ __forceinline__ void merge_records(const DecodeArgs& a, int tq, const RunSpace& s, MergeLds& lds,
+                                              const First& first_row) {
   const int tid = int(threadIdx.x), lane = tid & 63, wave = uniform(tid >> 6);
   const int Hkv = a.num_kv_heads;
   static_assert(kRunMaxWgs <= kRunThreads, "a run per thread");
@@ -236,7 +239,7 @@ __device__ __forceinline__ void merge_records(const DecodeArgs& a, int tq, const
     const int b = uniform(lds.last[j].b), i = uniform(lds.last[j].i);
     const int ni = min(tq, uniform(lds.last[j].n) - i * tq);
     if (row_wave * 32 >= ni * a.heads) continue;  // no query rows
-    const int64_t first = q_first(a, b) + i * tq;
+    const int64_t first = first_row(b) + i * tq;
     const float vd = descale(a.vd, a.vd_b, a.vd_h, b, h);
     // how many of the following runs' first pieces are of the same block
     int n = 0;
@@ -291,8 +294,12 @@ __device__ __forceinline__ void merge_records(const DecodeArgs& a, int tq, const
       for (int r = R; r <= n; ++r) m = __builtin_fmaxf(m, max_of(r));
       for (int r0 = 0; r0 <= n; r0 += R) add(std::integral_constant<int, R>{}, r0);
     }
-    write_row<OUT_DT, 1>(a, first, ni, h, vd, row_wave, lane, d0, o, m, l);
+    write_row<OUT_DT, 1, NANS>(a, first, ni, h, vd, row_wave, lane, d0, o, m, l);
   }
+}
+template <int OUT_DT, int R>
+__device__ __forceinline__ void merge_records(const DecodeArgs& a, int tq, const RunSpace& s, MergeLds& lds) {
+  merge_records<OUT_DT, R>(a, tq, s, lds, [&](int b) { return q_first(a, b); });
 }
 
 // prefill_runs.hip.  `a` as the decode reader's, with a.q_len the most query
@@ -307,6 +314,19 @@ int64_t prefill_runs_words();  // int32 words of a RunSpace, no initial contents
 // `workspace`.
 int launch_prefill_runs(const DecodeArgs& a, int64_t num_seqs, int64_t wgs, bool sure, int q_dtype, int out_dtype,
                         int32_t* workspace, int32_t* blocks, int32_t* order, RunSpace* space, hipStream_t st);
+// Trees of drafted tokens (tree_attention.hip), a step that is sure to be cut into
+// runs: a.causal is 0, token i of a sequence sees of its drafted keys those of its
+// mask, rows [first, first + n) of a sequence lie inside total_q, and a NaN value
+// reaches the rows that see it alone.  Pages of a multiple of 8 keys whose rows lie
+// within 32-bit offsets.
+struct TreeStep {
+  const int64_t* mask;
+  int64_t mask_stride;
+  double scale_log2;
+  int32_t total_q;
+};
+int launch_tree_runs(const DecodeArgs& a, const TreeStep& t, int64_t num_seqs, int q_dtype, int out_dtype,
+                     int32_t* workspace, hipStream_t st);
 
 }  // namespace psk_detail
 

@@ -10,6 +10,7 @@
 #include <mutex>
 #include <type_traits>
 
+#include "cached_queries.h"
 #include "prefill_runs.h"
 
 using namespace psk_detail;
@@ -86,7 +87,25 @@ struct RunArgs {
   int32_t sure;      // the step is cut into runs whatever its lengths
   int32_t* blocks;   // the launch order of the blocks, where they are not run here
   int32_t* order;
+  TreeStep tree;
 };
+
+// A sequence's query tokens: how many, their first row of q, and its length.
+template <bool TREE>
+__device__ __forceinline__ int pf_count(const RunArgs& p, int b) {
+  if constexpr (TREE) return seq_rows(p.a, p.tree.total_q, b).n;
+  return q_count(p.a, b);
+}
+template <bool TREE>
+__device__ __forceinline__ int64_t pf_first(const DecodeArgs& a, int32_t total_q, int b) {
+  if constexpr (TREE) return seq_rows(a, total_q, b).first;
+  return q_first(a, b);
+}
+template <bool TREE>
+__device__ __forceinline__ int pf_len(const RunArgs& p, int b) {
+  if constexpr (TREE) return cached_len(p.a, b);
+  return max(p.a.seq_lens[b], 0);
+}
 
 // A sequence's blocks: nb of them, block i costs base + i * step.
 struct PfSeq {
@@ -129,6 +148,7 @@ struct PfBlock {
 };
 
 // The block that cost x (0 <= x < prefix[num_seqs]) falls in.
+template <bool TREE>
 __device__ __forceinline__ PfBlock pf_block(const RunArgs& p, const int64_t* prefix, int64_t x) {
   int lo = 0, hi = p.num_seqs - 1;  // the last sequence with prefix <= x (those without blocks share the next one's)
   while (lo < hi) {
@@ -136,7 +156,7 @@ __device__ __forceinline__ PfBlock pf_block(const RunArgs& p, const int64_t* pre
     if (prefix[mid] <= x) lo = mid; else hi = mid - 1;
   }
   lo = uniform(lo);
-  const PfSeq s = pf_seq(p.a, p.tq, q_count(p.a, lo), max(p.a.seq_lens[lo], 0));
+  const PfSeq s = pf_seq(p.a, p.tq, pf_count<TREE>(p, lo), pf_len<TREE>(p, lo));
   const int64_t before = lo > 0 ? int64_t(prefix[lo]) : 0;  // prefix[0] is not stored
   const int64_t y = x - before;
   int i = 0, last = s.nb - 1;  // the last block with upto(i) <= y
@@ -189,13 +209,13 @@ __device__ __forceinline__ bool pf_take(const RunArgs& p, int keys, int64_t T) {
 // of the sequences (prefix[b + 1]: up to b), else their query tokens and
 // lengths in `seqs`.  Up to 64 sequences every wave does it for itself, a
 // sequence a lane, without a barrier.
-template <int NT>
+template <int NT, bool TREE>
 __device__ __forceinline__ PfStep pf_step(const RunArgs& p, int64_t* prefix, int64_t* s_wave, OrderLds& seqs) {
   const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
   const DecodeArgs& a = p.a;
   if (p.num_seqs <= 64) {
     const bool in = lane < p.num_seqs;
-    const int n = in ? q_count(a, lane) : 0, len = in ? max(a.seq_lens[lane], 0) : 0;
+    const int n = in ? pf_count<TREE>(p, lane) : 0, len = in ? pf_len<TREE>(p, lane) : 0;
     const int keys = wave_longest(n > 0 ? len : 0, p.num_seqs);
     PfStep found{false, 0};
     if (p.sure || keys >= kRunsLeast) {  // else the costs do not matter
@@ -216,7 +236,7 @@ __device__ __forceinline__ PfStep pf_step(const RunArgs& p, int64_t* prefix, int
     const int b = c0 + tid;
     int64_t own = 0;
     if (b < p.num_seqs) {
-      const int n = q_count(a, b), len = max(a.seq_lens[b], 0);
+      const int n = pf_count<TREE>(p, b), len = pf_len<TREE>(p, b);
       put_sequence(seqs, b, n, len);
       const PfSeq s = pf_seq(a, p.tq, n, len);
       own = s.upto(s.nb);
@@ -251,26 +271,31 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <int Q_DT, int OUT_DT, bool GEN>
+// TREE: see launch_tree_runs.  The drafted keys' visibility is a lane's 32 mask bits
+// a tile, in place of the row's limit.
+template <int Q_DT, int OUT_DT, bool GEN, bool TREE = false>
 __global__ void __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2)))
 prefill_runs_kernel(RunArgs p) {
   const DecodeArgs& a = p.a;
   __shared__ __attribute__((aligned(1024))) char s_lds[kPfRaws * kPfRaw + kPfBufs * kPfStage];
   __shared__ int64_t s_prefix[kOrderMax + 1];  // every workgroup scans the sequences' costs
   __shared__ int64_t s_wave[kPfWaves];
+  __shared__ int32_t s_nans[3];  // TREE: a piece met NaN values in masked stages (pieces in turn)
   const int tid = int(threadIdx.x);
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int Hkv = a.num_kv_heads;
   OrderLds& seqs = *reinterpret_cast<OrderLds*>(s_lds);
   static_assert(sizeof(OrderLds) <= sizeof(s_lds), "the stages hold it until the first one");
-  const PfStep found = pf_step<kPfThreads>(p, s_prefix, s_wave, seqs);
-  if (!found.take) {
-    __syncthreads();
-    if (blockIdx.x == 0) order_blocks<kPfThreads>(a, p.num_seqs, p.tq, p.blocks, p.order, seqs);
-    return;
+  const PfStep found = pf_step<kPfThreads, TREE>(p, s_prefix, s_wave, seqs);
+  if constexpr (!TREE) {  // (a tree step is cut into runs whatever its lengths: no launch order, no `blocks`)
+    if (!found.take) {
+      __syncthreads();
+      if (blockIdx.x == 0) order_blocks<kPfThreads>(a, p.num_seqs, p.tq, p.blocks, p.order, seqs);
+      return;
+    }
+    if (blockIdx.x == 0 && tid == 0) p.blocks[p.num_seqs] = -1;
   }
-  if (blockIdx.x == 0 && tid == 0) p.blocks[p.num_seqs] = -1;
   const int64_t T = found.T;
   const int M = uniform(pf_runs(p, T));
   // Workgroup w runs on XCD w % 8: a kv head's runs, in order, on as few XCDs
@@ -292,7 +317,8 @@ prefill_runs_kernel(RunArgs p) {
   if (T == 0) return;
   const int64_t x_begin = uniform(pf_run_start(T, j, M));
   const int64_t x_end = uniform(pf_run_start(T, j + 1, M));
-  const PfBlock k_first = pf_block(p, s_prefix, x_begin);
+  const PfBlock k_first = pf_block<TREE>(p, s_prefix, x_begin);
+  if (TREE && tid < 3) s_nans[tid] = 0;
   __syncthreads();  // the descriptors' initial stores come before run j's own
 
   // staging: thread t moves 16-byte chunk t & 7 of key t >> 3 of a stage, of K and of V
@@ -334,7 +360,7 @@ prefill_runs_kernel(RunArgs p) {
           k_last.at += k_last.cost;
           k_last.cost += k_last.step;
         } else {
-          k_last = pf_block(p, s_prefix, x);
+          k_last = pf_block<TREE>(p, s_prefix, x);
         }
         c.k = k_last;
         lo = x;
@@ -438,21 +464,22 @@ prefill_runs_kernel(RunArgs p) {
   Piece c;
   if (!next_piece(c)) return;
   open(c, look_up(c, c.sa));
+  int nans = 0;  // the piece's place in s_nans
   for (;;) {  // over the pieces
     const PfBlock& k = c.k;
     const int sa = c.sa, sb = c.sb, ns = c.ns, key_end = c.key_end;
     const int b = k.b, i0 = k.i * p.tq;
     const int n = k.n, L = k.len;
     const int ni = min(p.tq, n - i0);
-    const int64_t qf = q_first(a, b);
+    const int64_t qf = pf_first<TREE>(a, p.tree.total_q, b);
     const int G = a.heads;
     // causal: query token i sees keys below base + i (FA's bottom-right alignment)
     const int base = a.causal ? L - n + 1 : L;
-    const int mask_from = a.causal ? min(max(base + i0, 0), L) : L;  // keys every row sees
+    const int mask_from = TREE ? max(L - n, 0) : a.causal ? min(max(base + i0, 0), L) : L;  // keys every row sees
     const float qd = descale(a.qd, a.qd_b, a.qd_h, b, h);
     const float kd = descale(a.kd, a.kd_b, a.kd_h, b, h);
     // exp2-domain score scale; a negative one is applied as -q~ (exact) times |sl|
-    const float sl_signed = a.scale_log2 * qd * kd;
+    const float sl_signed = TREE ? score_scale(p.tree.scale_log2, qd, kd) : a.scale_log2 * qd * kd;
     const float sl = __int_as_float(uniform(__float_as_int(__builtin_fabsf(sl_signed))));
 
     const int r = wave * 32 + kk;
@@ -460,6 +487,11 @@ prefill_runs_kernel(RunArgs p) {
     const bool live = ti < ni;
     // this lane's scores are of keys 4 half + const: the row's limit less that
     const int row_lim = (live ? (a.causal ? min(max(base + i0 + ti, 0), L) : L) : 0) - 4 * half;
+
+    // TREE: the 32 keys from key0 that the lane's row sees, and of them the lane's (key_of's bits)
+    const int64_t* mask = TREE ? p.tree.mask + (qf + i0 + (live ? ti : 0)) * p.tree.mask_stride : nullptr;
+    auto seen = [&](int key0) { return live ? visible(mask, L - n, n, key0) : 0u; };
+    uint32_t vis = 0xFFFFFFFFu;
 
     bf16x8 qop[8];
     {
@@ -498,9 +530,24 @@ prefill_runs_kernel(RunArgs p) {
 
     // K as bf16 and V as fp16 (both exact), converted once here for every
     // wave, from the raw bytes this thread loaded
-    auto stage_read = [&](uint32_t slot, u32x4& kr, u32x4& vr) {
+    const int t_open = min(sb, mask_from / kPfKeys);  // stages below need no mask
+    auto stage_read = [&](uint32_t slot, int t, u32x4& kr, u32x4& vr) {
       kr = *lds_at<u32x4>(raw0 + slot + uint32_t(16 * tid));
       vr = *lds_at<u32x4>(raw0 + slot + kPfRaw / 2 + uint32_t(16 * tid));
+      if constexpr (TREE) {
+        // a NaN value of a key that some row does not see (0 x NaN) must not reach
+        // it: it leaves the stage, and the rows that see one have it at the end
+        if (t >= t_open && t < sb) {
+          uint32_t any = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = nan_bytes(vr[i]);
+            any |= x;
+            vr[i] &= ~(x * 0xFFu);
+          }
+          if (any) s_nans[nans] = 1;
+        }
+      }
     };
     auto stage_store = [&](uint32_t buf, const u32x4& kr, const u32x4& vr, int quarter) {
       switch (quarter) {
@@ -541,11 +588,14 @@ prefill_runs_kernel(RunArgs p) {
     };
     // the lane's key i of a tile, before its 4 half
     auto key_of = [](int i) { return 8 * (i >> 2) + (i & 3); };
+    auto sees = [&](int key0, int i) {
+      return TREE ? ((vis >> key_of(i)) & 1u) != 0 : key0 + key_of(i) < row_lim;
+    };
     // the row's largest scaled score of a tile (sl >= 0: max(y) * sl)
     auto tile_max = [&](const f32x16& y, int key0) {
       float v = -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v = __builtin_fmaxf(v, key0 + key_of(i) < row_lim ? y[i] : -__builtin_inff());
+      for (int i = 0; i < 16; ++i) v = __builtin_fmaxf(v, sees(key0, i) ? y[i] : -__builtin_inff());
       v *= sl;
       v = __builtin_fmaxf(v, __shfl_xor(v, 32));
       return live ? __builtin_fmaxf(v, kNegBig) : kBig;
@@ -555,8 +605,8 @@ prefill_runs_kernel(RunArgs p) {
     auto weigh = [&](auto masked_tag, const f32x16& y, int key0, int i, float& s0, float& s1, uint32_t (&pw)[8]) {
       constexpr bool MASKED = decltype(masked_tag)::value;
       float e0 = __builtin_fmaf(y[i], sl, -m), e1 = __builtin_fmaf(y[i + 1], sl, -m);
-      if (MASKED && key0 + key_of(i) >= row_lim) e0 = -__builtin_inff();
-      if (MASKED && key0 + key_of(i + 1) >= row_lim) e1 = -__builtin_inff();
+      if (MASKED && !sees(key0, i)) e0 = -__builtin_inff();
+      if (MASKED && !sees(key0, i + 1)) e1 = -__builtin_inff();
       const float p0 = __builtin_amdgcn_exp2f(e0), p1 = __builtin_amdgcn_exp2f(e1);
       s0 += p0;
       s1 += p1;
@@ -578,6 +628,7 @@ prefill_runs_kernel(RunArgs p) {
         kw[c] = *lds_at<u32x4>(rd_k[c] + uint32_t(8192 * k_tile));
         vw[c] = load_v(v_tile, c >> 2, c & 3);
       };
+      if constexpr (TREE) vis = decltype(masked_tag)::value ? seen(key0) >> (4 * half) : 0xFFFFFFFFu;
       float s0 = 0.0f, s1 = 0.0f;
       f32x16 yn = {};
       read(0);
@@ -621,7 +672,6 @@ prefill_runs_kernel(RunArgs p) {
     // load counter is all it waits for: two loads each of the two later
     // stages may be in flight.  Past the run's last stage stale bytes are
     // converted, and the scores of stale bytes taken, and neither is used.
-    const int t_open = min(sb, mask_from / kPfKeys);  // stages below need no mask
     // the next piece and its first pages, while this one's first loads fly
     Piece c_next;
     const bool more = next_piece(c_next);
@@ -630,10 +680,11 @@ prefill_runs_kernel(RunArgs p) {
     {
       u32x4 kr, vr;
       wait_loads<0>();
+      if (TREE && tid == 0) s_nans[nans == 2 ? 0 : nans + 1] = 0;  // (the piece before may still read its own)
       lds_barrier();  // the buffers' previous readers are done
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        stage_read(i * kPfRaw, kr, vr);
+        stage_read(i * kPfRaw, sa + i, kr, vr);
 #pragma unroll
         for (int q = 0; q < 4; ++q) stage_store(i * kPfStage, kr, vr, q);
       }
@@ -652,6 +703,7 @@ prefill_runs_kernel(RunArgs p) {
       for (int c = 0; c < 8; ++c)
         y0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, *lds_at<u32x4>(rd_k[c])), qop[c], y0, 0,
                                                      0, 0);
+      if constexpr (TREE) vis = seen(sa * kPfKeys) >> (4 * half);
       m = tile_max(y0, sa * kPfKeys);
     }
     uint32_t from_last = 0;  // from the buffer of stage t - 1 to that of stage t
@@ -668,7 +720,7 @@ prefill_runs_kernel(RunArgs p) {
       lds_barrier();
       u32x4 kr, vr;
       if (t + 4 < sb && !holes) wait_loads<4>(); else wait_loads<0>();
-      stage_read(raw, kr, vr);
+      stage_read(raw, t + 2, kr, vr);
       if (busy) {
         y0 = tile_step(masked_tag, y1, t * kPfKeys + 32, 0, 0, p0, p1, [&](int c) {
           if (c >= 4) stage_store(to, kr, vr, c - 4);
@@ -696,6 +748,27 @@ prefill_runs_kernel(RunArgs p) {
       }
     }
 
+    if constexpr (TREE) {
+      if (__builtin_expect(busy && s_nans[nans], 0)) {  // the NaN values that the lane's row sees, from the cache again
+#pragma unroll 1
+        for (int key = max(t_open, sa) * kPfKeys; key < min(sb * kPfKeys, L); ++key) {
+          const int pi = page_index(a, key);
+          int32_t id = -1;
+          if (pi < a.bt_width) id = a.block_table[int64_t(b) * a.bt_stride + pi];
+          if (id < 0 || id >= a.num_blocks || !(seen(key) & 1u)) continue;
+          const uint8_t* row = vbase + int64_t(id) * a.v_blk + int64_t(key - pi * a.block_size) * a.v_row + 4 * half;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const uint32_t x = nan_bytes(*reinterpret_cast<const uint32_t*>(row + 8 * c));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((x >> (8 * i)) & 1u) o[c >> 2][4 * (c & 3) + i] = __builtin_nanf("");
+          }
+        }
+      }
+      nans = nans == 2 ? 0 : nans + 1;
+    }
+
     // the next piece's first loads fly while this one's result is written
     if (more) open(c_next, pages_next);
     const float lt = l + __shfl_xor(l, 32);
@@ -705,10 +778,10 @@ prefill_runs_kernel(RunArgs p) {
       frag[c] = f32x4{o[c >> 2][4 * (c & 3)], o[c >> 2][4 * (c & 3) + 1], o[c >> 2][4 * (c & 3) + 2],
                       o[c >> 2][4 * (c & 3) + 3]};
     if (sa == 0 && sb == ns) {
-      write_row<OUT_DT, 4>(a, q_first(a, b) + i0, ni, h, descale(a.vd, a.vd_b, a.vd_h, b, h), wave, lane, 0, frag, m, lt);
+      write_row<OUT_DT, 4, TREE>(a, pf_first<TREE>(a, p.tree.total_q, b) + i0, ni, h, descale(a.vd, a.vd_b, a.vd_h, b, h), wave, lane, 0, frag, m, lt);
     } else {
       const int slot = sa == 0 ? 1 : 0;
-      if (h == 0 && tid == 0) p.s.desc[2 * j + slot] = RunDesc{1, b, k.i, q_count(a, b)};
+      if (h == 0 && tid == 0) p.s.desc[2 * j + slot] = RunDesc{1, b, k.i, pf_count<TREE>(p, b)};
       if (busy) {
         float* rec = p.s.records + ((int64_t(j) * Hkv + h) * 2 + slot) * kRunRecord + wave * kRunSlab;
 #pragma unroll
@@ -729,6 +802,19 @@ template <int OUT_DT>
 __global__ void __launch_bounds__(kRunThreads) prefill_merge_kernel(DecodeArgs a, int tq, RunSpace s) {
   __shared__ MergeLds lds;
   merge_records<OUT_DT, 4>(a, tq, s, lds);
+}
+
+template <int OUT_DT>
+__global__ void __launch_bounds__(kRunThreads) tree_runs_merge_kernel(DecodeArgs a, int tq, RunSpace s, int32_t total_q) {
+  __shared__ MergeLds lds;
+  merge_records<OUT_DT, 4, true>(a, tq, s, lds, [&](int b) { return pf_first<true>(a, total_q, b); });
+}
+
+template <int Q_DT, int OUT_DT>
+void launch_tree_step(const RunArgs& p, dim3 grid, hipStream_t st) {
+  hipLaunchKernelGGL((prefill_runs_kernel<Q_DT, OUT_DT, false, true>), grid, dim3(kPfThreads), 0, st, p);
+  hipLaunchKernelGGL((tree_runs_merge_kernel<OUT_DT>), dim3(4 * grid.x), dim3(kRunThreads), 0, st, p.a, p.tq, p.s,
+                     p.tree.total_q);
 }
 
 template <int Q_DT, bool GEN>
@@ -802,6 +888,42 @@ int launch_prefill_runs(const DecodeArgs& a, int64_t num_seqs, int64_t wgs, bool
   else
     hipLaunchKernelGGL((prefill_merge_kernel<PSK_DTYPE_F32>), grid2, dim3(kRunThreads), 0, st, a, p.tq, p.s);
   return check_launch("prefill_merge_kernel launch");
+}
+
+int launch_tree_runs(const DecodeArgs& a, const TreeStep& t, int64_t num_seqs, int q_dtype, int out_dtype,
+                     int32_t* workspace, hipStream_t st) {
+  RunArgs p{};
+  p.a = a;
+  p.a.causal = 0;
+  p.tree = t;
+  p.num_seqs = int32_t(num_seqs);
+  p.tq = kPfRows / a.heads;
+  p.cus = int32_t(prefill_cus());
+  p.sure = 1;
+  p.s.max_runs = p.cus / a.num_kv_heads;
+  p.s.desc = reinterpret_cast<RunDesc*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
+  p.s.records = reinterpret_cast<float*>(p.s.desc + 2 * p.s.max_runs);
+  const dim3 grid{unsigned(p.s.max_runs * a.num_kv_heads), 1u, 1u};
+  const bool bf16 = out_dtype == PSK_DTYPE_BF16;
+  switch (q_dtype) {
+    case PSK_DTYPE_FP8_E4M3FN:
+      bf16 ? launch_tree_step<PSK_DTYPE_FP8_E4M3FN, PSK_DTYPE_BF16>(p, grid, st)
+           : launch_tree_step<PSK_DTYPE_FP8_E4M3FN, PSK_DTYPE_F32>(p, grid, st);
+      break;
+    case PSK_DTYPE_BF16:
+      bf16 ? launch_tree_step<PSK_DTYPE_BF16, PSK_DTYPE_BF16>(p, grid, st)
+           : launch_tree_step<PSK_DTYPE_BF16, PSK_DTYPE_F32>(p, grid, st);
+      break;
+    case PSK_DTYPE_F16:
+      bf16 ? launch_tree_step<PSK_DTYPE_F16, PSK_DTYPE_BF16>(p, grid, st)
+           : launch_tree_step<PSK_DTYPE_F16, PSK_DTYPE_F32>(p, grid, st);
+      break;
+    default:
+      bf16 ? launch_tree_step<PSK_DTYPE_F32, PSK_DTYPE_BF16>(p, grid, st)
+           : launch_tree_step<PSK_DTYPE_F32, PSK_DTYPE_F32>(p, grid, st);
+      break;
+  }
+  return check_launch("prefill_runs_kernel launch");
 }
 
 }  // namespace psk_detail

@@ -38,6 +38,7 @@
 #include <mutex>
 
 #include "cached_queries.h"
+#include "prefill_runs.h"
 
 using namespace psk_detail;
 
@@ -56,6 +57,15 @@ constexpr int kOver = 6;                   // units (of kStepKeys keys) that a p
 // sequences of 8 tokens (32 query heads over 8), us, whole / cut: 1000 keys 17 / 19, 1600
 // 19 / 19, 2500 24 / 21; 64 sequences of 1000, 32 / 38.
 constexpr int kWholeKeys = 1536;
+// Wide trees over much work go to prefill_runs.hip, whose waves share each key's
+// conversion (here every 32 rows convert it again) at 15 us more for its start and
+// end: from kWideRows rows a sequence on average, and kWideWork query rows x keys at
+// most.  This kernel / that one, us (32 query heads): 4 sequences of 30000 keys over
+// 4 kv heads, 24 tokens each 75 / 80, 32: 88 / 87, 48: 126 / 120, 64: 157 / 134; 16 of
+// 8000 over 8, 32 tokens 95 / 110, 48: 157 / 138; 32 of 2000, 32 tokens 64 / 60, 48:
+// 100 / 74; one of 16000, 64 tokens 38 / 55.
+constexpr int kWideRows = 192;
+constexpr int64_t kWideWork = 80000000;
 constexpr int kPages = 1024;               // page ids a piece stages at a time
 constexpr int kSlab = 4096 + 64;           // floats of 32 rows' partial result: accumulators, maxima, sums
 constexpr int kMaxSlots = 512;             // resident workgroups the workspace is sized for
@@ -101,20 +111,6 @@ __device__ __forceinline__ void load_tile(uint32_t slot, const uint8_t* const (&
       : "s"(slot), "s"(slot + kHalfSlot), "v"(offset), "s"(kp[0]), "s"(kp[1]), "s"(kp[2]), "s"(kp[3]), "s"(vp[0]),
         "s"(vp[1]), "s"(vp[2]), "s"(vp[3])
       : "memory");
-}
-
-// Visibility of keys key0 .. key0 + 31 (bit k: key0 + k) to a drafted token with mask m, of n after `ctx` keys.
-__device__ __forceinline__ uint32_t visible(const int64_t* m, int ctx, int n, int key0) {
-  const int j0 = key0 - ctx;  // the drafted index of key0
-  if (j0 <= -32) return 0xFFFFFFFFu;
-  if (j0 >= n) return 0u;
-  const int left = n - j0;  // keys before the tree's end
-  const uint32_t in = left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u;
-  if (j0 < 0) return ((uint32_t(m[0]) << -j0) | ((1u << -j0) - 1u)) & in;
-  const int w = j0 >> 6, sh = j0 & 63;
-  uint64_t bits = uint64_t(m[w]) >> sh;
-  if (sh > 32 && left > 64 - sh) bits |= uint64_t(m[w + 1]) << (64 - sh);
-  return uint32_t(bits) & in;
 }
 
 template <int OUT_DT>
@@ -361,10 +357,9 @@ tree_attention_kernel(TreeArgs args) {
       // it: they leave the tile, and the (column, row) pairs that do see one are
       // marked, for the end of the piece.
       auto contain_nan = [&](i32x2 (&vraw)[8], uint32_t vis) {
-        auto nan_bytes = [](int x) { return (((uint32_t(x) & 0x7F7F7F7Fu) + 0x01010101u) >> 7) & 0x01010101u; };
         uint32_t any = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) any |= nan_bytes(vraw[i][0]) | nan_bytes(vraw[i][1]);
+        for (int i = 0; i < 8; ++i) any |= nan_bytes(uint32_t(vraw[i][0])) | nan_bytes(uint32_t(vraw[i][1]));
         if (__builtin_expect(!__any(any != 0), 1)) return;
         uint32_t rows[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -381,8 +376,8 @@ tree_attention_kernel(TreeArgs args) {
           }
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
-            vraw[4 * u + d][0] &= int(~(nan_bytes(vraw[4 * u + d][0]) * 0xFFu));
-            vraw[4 * u + d][1] &= int(~(nan_bytes(vraw[4 * u + d][1]) * 0xFFu));
+            vraw[4 * u + d][0] &= int(~(nan_bytes(uint32_t(vraw[4 * u + d][0])) * 0xFFu));
+            vraw[4 * u + d][1] &= int(~(nan_bytes(uint32_t(vraw[4 * u + d][1])) * 0xFFu));
           }
         }
 #pragma unroll
@@ -607,6 +602,12 @@ TreeShape tree_shape(int64_t rows, int64_t slots) {
   return s;
 }
 
+bool wide_step(int64_t num_seqs, int64_t total_q, int64_t num_q_heads, int64_t num_kv_heads, int64_t max_seq_len) {
+  return total_q * (num_q_heads / num_kv_heads) >= kWideRows * num_seqs &&
+         double(total_q) * double(num_q_heads) * double(max_seq_len) >= double(kWideWork) && num_seqs <= kOrderMax &&
+         num_q_heads / num_kv_heads <= kBlockRows;
+}
+
 template <int Q_DT, int OUT_DT>
 int launch_tree(const TreeArgs& p, bool general, hipStream_t st) {
   const int64_t jobs = int64_t(p.s.num_seqs) * p.s.heads;
@@ -619,13 +620,15 @@ int launch_tree(const TreeArgs& p, bool general, hipStream_t st) {
   return check_launch("merge_tree_kernel launch");
 }
 
+// Pages of a multiple of 8 keys whose rows lie within 32-bit offsets (the keys of a
+// load share a page), K and V laid out alike.
+bool shares_pages(const DecodeArgs& a) {
+  return a.block_size % 8 == 0 && a.k_row >= 0 && 8 * a.k_row < (int64_t(1) << 31) && a.k_row == a.v_row && a.k_blk == a.v_blk;
+}
+
 template <int Q_DT>
 int launch_tree_q(const TreeArgs& p, int out_dtype, hipStream_t st) {
-  const DecodeArgs& a = p.a;
-  // pages of a multiple of 8 keys whose rows lie within 32-bit offsets (the keys of a
-  // load share a page), K and V laid out alike
-  const bool general = a.block_size % 8 != 0 || a.k_row < 0 || 8 * a.k_row >= (int64_t(1) << 31) || a.k_row != a.v_row ||
-                       a.k_blk != a.v_blk;
+  const bool general = !shares_pages(p.a);
   return out_dtype == PSK_DTYPE_BF16 ? launch_tree<Q_DT, PSK_DTYPE_BF16>(p, general, st)
                                      : launch_tree<Q_DT, PSK_DTYPE_F32>(p, general, st);
 }
@@ -641,7 +644,8 @@ int64_t psk_paged_tree_workspace_len(int64_t num_seqs, int64_t total_q, int64_t 
     return PSK_E_ARG;
   if (max_seq_len <= kWholeKeys) return 0;
   const TreeShape s = tree_shape(max_seqlen_q * (num_q_heads / num_kv_heads), kMaxSlots);
-  return 4 + s.max_runs * s.row_blocks * 2 * kSlab;
+  const int64_t own = 4 + s.max_runs * s.row_blocks * 2 * kSlab;
+  return wide_step(num_seqs, total_q, num_q_heads, num_kv_heads, max_seq_len) ? std::max(own, prefill_runs_words()) : own;
 }
 
 int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int q_dtype,
@@ -714,6 +718,10 @@ int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head
   p.s.width = INT32_MAX;
   p.row_blocks = int32_t(s.row_blocks);
   p.whole = max_seq_len <= kWholeKeys;
+  if (!p.whole && wide_step(num_seqs, total_q, num_q_heads, num_kv_heads, max_seq_len) && shares_pages(a) &&
+      2 * num_kv_heads <= prefill_cus())
+    return launch_tree_runs(a, TreeStep{tree_mask, tree_mask_stride, p.scale_log2, int32_t(total_q)}, num_seqs, q_dtype,
+                            out_dtype, reinterpret_cast<int32_t*>(workspace), static_cast<hipStream_t>(stream));
   p.records = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
   if (num_seqs * num_kv_heads * s.row_blocks > INT32_MAX / 16 || s.max_runs * s.row_blocks > INT32_MAX)
     return fail(PSK_E_ARG, "too many rows (%lld sequences of up to %lld drafted tokens)", (long long)num_seqs,

@@ -264,3 +264,143 @@ def test_refusals(dev):
             attention.paged_tree_attention(**{**good, **change})
     with pytest.raises(AssertionError, match="query rows"):
         attention.paged_tree_attention(**{**good, "max_seqlen_q": 3}, validate=True)
+
+
+# --------------------------------------------------------------------------- #
+# steps cut into runs: tables that could name more than 1536 keys
+# --------------------------------------------------------------------------- #
+
+
+def _room(ps, counts=(), Hq=0):
+    """Pages past a table's own that make it one of more than 1536 keys, and the step (drafted
+    tokens `counts`, Hq heads) at most 2^27 query rows x keys."""
+    return -(-max(1600, 2 ** 27 // max(sum(counts) * Hq, 1) if Hq else 0) // ps)
+
+
+@pytest.mark.parametrize("ps", [16, 24, 7])
+@pytest.mark.parametrize("Hq,Hkv", [(32, 8), (8, 1), (4, 4), (6, 2), (40, 1)])
+def test_ragged_trees_cut(dev, Hq, Hkv, ps):
+    """As test_ragged_trees; 40 and 8 heads over one make blocks of 256 rows and more."""
+    rng = np.random.default_rng(Hq + Hkv + ps)
+    counts = [int(x) for x in rng.integers(1, 34, 8)]
+    counts[3], counts[7] = 0, 33
+    lens = [n + int(x) for n, x in zip(counts, rng.integers(0, 900, 8))]
+    lens[1] = counts[1]
+    lens[5] = max(counts[5] - 2, 0)
+    lens[6] = 0
+    lens[2] += 2500
+    case = Case(dev, 11, lens, counts, Hq, Hkv, ps, spare_rows=3, spare_table=_room(ps, counts, Hq))
+    mask = _trees(case, 5)
+    _check(case, mask, *_run(case, mask, dev))
+
+
+@pytest.mark.parametrize("n", [7, 8, 31, 32, 33, 64, 65, 130, 200])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 1), (64, 2), (5, 1)])
+def test_wide_trees(dev, n, Hq, Hkv):
+    """Around blocks of 256 rows and mask words; arbitrary masks with bits past the tree."""
+    case = Case(dev, n, [n + 100, n, n + 31, n + 4000], [n, n, max(1, n - 1), n], Hq, Hkv, 16,
+                spare_table=_room(16, [n] * 4, Hq))
+    mask = _trees(case, 7, words=-(-n // 64) + 1, arbitrary=True)
+    _check(case, mask, *_run(case, mask, dev))
+
+
+@pytest.mark.parametrize("q_dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_wide_types_and_strides(dev, q_dtype, out_dtype):
+    case = Case(dev, 3, [300, 61, 1025], [33, 40, 37], 16, 2, 16, q_dtype=q_dtype, strided_q=True, head_major=True,
+                spare_table=_room(16, [33, 40, 37], 16), spare_rows=2)
+    mask = _trees(case, 6)
+    _check(case, mask, *_run(case, mask, dev, out_dtype))
+
+
+@pytest.mark.parametrize("n", [4, 40])
+def test_cut_rows_that_see_nothing(dev, n):
+    case = Case(dev, 21, [n, 40 + n, n // 2, 0], [n, n, n, n], 8, 1, 16, spare_table=_room(16, [n] * 4, 8))
+    mask = _trees(case, 1, arbitrary=True)
+    mask[1] = 0          # no context and an empty mask
+    mask[n + 1] = 0      # its context alone
+    out, lse = _run(case, mask, dev)
+    _check(case, mask, out, lse)
+    assert bool((out[1] == 0).all()) and bool(torch.isneginf(lse[:, 1]).all())
+    assert bool((out[3 * n:] == 0).all()) and bool(torch.isneginf(lse[:, 3 * n:]).all())
+
+
+@pytest.mark.parametrize("n", [6, 40])
+def test_cut_missing_pages(dev, n):
+    case = Case(dev, 31, [200 + n, 90 + n, 33 + n], [n, n, n], 8, 1, 16, holes=[(0, 1), (0, 12), (1, 0), (2, 2)],
+                spare_table=_room(16, [n] * 3, 8))
+    mask = _trees(case, 2)
+    _check(case, mask, *_run(case, mask, dev))
+
+
+@pytest.mark.parametrize("n", [6, 40, 70])
+def test_cut_nan_in_places_that_a_row_does_not_see(dev, n):
+    case = Case(dev, 51, [50 + n, 70 + n, 2000 + n], [n, n, n], 16, 2, 16, descales=False,
+                spare_table=_room(16, [n] * 3, 16))
+    mask = _trees(case, 4)
+    for b, i, kind, h, d in ((0, 2, 0, 0, 5), (1, 4, 1, 1, 9), (1, n - 1, 1, 0, 127), (2, 0, 1, 1, 64), (2, 3, 0, 1, 0)):
+        pos = case.lens[b] - n + i
+        page, row = int(case.bt[b, pos // 16]), pos % 16
+        (case.k, case.v)[kind].view(torch.uint8)[page, row, h, d] = 0x7F if d % 2 else 0xFF
+        case.fused.view(torch.uint8)[page, kind, row, h, d] = 0x7F if d % 2 else 0xFF
+    for b, L in enumerate(case.lens):  # rows past the lengths hold NaN as well
+        if L % 16:
+            p = int(case.bt[b, L // 16])
+            for t in (case.k, case.v):
+                t.view(torch.uint8)[p, L % 16:] = 0x7F
+            case.fused.view(torch.uint8)[p, :, L % 16:] = 0x7F
+    got, lse = _run(case, mask, dev)
+    assert bool(torch.isnan(got).any()) and not bool(torch.isnan(got).all())
+    _check(case, mask, got, lse, nan=True)
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_cut_scores_far_apart_and_negative_scales(dev, n):
+    case = Case(dev, 41, [1900 + n, 260 + n], [n, n], 8, 1, 16, k_sign=-1.0, spare_table=_room(16, [n] * 2, 8))
+    case.fused[:, 0] = (case.fused[:, 0].float() * torch.linspace(0.05, 3.0, case.fused.shape[0]).view(-1, 1, 1, 1)
+                        ).to(torch.float8_e4m3fn)
+    case.k.copy_(case.fused[:, 0].to(dev))
+    mask = _trees(case, 3)
+    _check(case, mask, *_run(case, mask, dev, scale=0.4), scale=0.4)
+
+
+@pytest.mark.parametrize("n,spare", [(2, 0), (2, 200), (70, 800)])
+def test_many_sequences(dev, n, spare):
+    """More than one window of 64 sequences, some without drafted tokens."""
+    rng = np.random.default_rng(3)
+    counts = [int(x) for x in rng.integers(0, n + 1, 150)]
+    lens = [c + int(x) for c, x in zip(counts, rng.integers(0, 120, 150))]
+    case = Case(dev, 91, lens, counts, 8, 1, 8, spare_table=spare)
+    mask = _trees(case, 3)
+    _check(case, mask, *_run(case, mask, dev))
+
+
+@pytest.mark.parametrize("n", [2, 40])
+def test_pages_of_one_token(dev, n):
+    """More page ids than are staged at a time, eight tables' worth of keys in one row."""
+    case = Case(dev, 95, [5000, 1030], [n, n], 8, 1, 1)
+    mask = _trees(case, 3)
+    _check(case, mask, *_run(case, mask, dev))
+
+
+def test_wide_other_stream_and_graph_replay(dev):
+    case = Case(dev, 81, [2500, 133], [40, 37], 8, 1, 16, spare_table=_room(16, [40, 37], 8))
+    mask = _trees(case, 9).to(dev)
+    want, lse_want = _run(case, mask, dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got, lse = _run(case, mask, dev)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(lse, lse_want)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out, lse = _run(case, mask, dev)
+    for r in range(3):
+        case.qd.copy_((case.q.float() * (1 + r)).to(case.q.dtype))
+        want, lse_want = _run(case, mask, dev)
+        torch.cuda.synchronize()
+        out.fill_(7.0)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, lse_want)
