@@ -201,21 +201,35 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_HERE = contextlib.nullcontext()
+
+
 def on_device(device: torch.device):
     """A context in which ``device`` is the current one: the library launches on
     the current device, and the stream has to be one of its own."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index is None or device.index == _current_device():
+        return _HERE
     return torch.cuda.device(device)
 
 
 _I64x4 = ctypes.c_int64 * 4
+_I64x3, _I64x6 = ctypes.c_int64 * 3, ctypes.c_int64 * 6
 
 
 def i64_array(values) -> ctypes.Array:
-    if len(values) == 4:
+    n = len(values)
+    if n == 4:
         return _I64x4(*values)
-    return (ctypes.c_int64 * len(values))(*values)
+    if n == 3:
+        return _I64x3(*values)
+    return (_I64x6 if n == 6 else ctypes.c_int64 * n)(*values)
+
+
+def distinct(t) -> bool:
+    """Whether a tensor that is written has no two elements in one place by a broadcast."""
+    strides = t.stride()
+    return 0 not in strides or all(s != 0 or n <= 1 for s, n in zip(strides, t.shape))
 
 
 def ptr(t) -> int:

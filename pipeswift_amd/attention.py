@@ -31,7 +31,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import check, dtype_code, i64_array, lib, on_device, ptr, stream_handle
+from ._lib import check, distinct, dtype_code, i64_array, lib, on_device, ptr, stream_handle
 
 HEAD_DIM = 128
 MAX_ROWS = 16  # query tokens x query heads per kv head
@@ -307,18 +307,19 @@ def _query_layout(q, cu_seqlens_q, max_seqlen_q, validate):
 
 def _check_paged(q, caches, block_table, seq_lens, num_seqs):
     """The paged FP8 reader's conditions on its tensors."""
-    assert q.is_cuda and q.dim() == 3 and q.shape[2] == HEAD_DIM and q.stride(2) == 1, \
+    shape, device, first = q.shape, q.device, caches[0].shape
+    assert q.is_cuda and len(shape) == 3 and shape[2] == HEAD_DIM and q.stride(2) == 1, \
         "q must be [T, Hq, 128] with unit last stride"
     for c in caches:
         assert c.dtype == torch.float8_e4m3fn, "the cache must be fp8 e4m3fn"
-        assert c.dim() == 4 and c.shape == caches[0].shape and c.shape[3] == HEAD_DIM and c.stride(3) == 1
-    Hq, Hkv = q.shape[1], caches[0].shape[2]
+        assert c.device == device, "all tensors must share the query's device"
+        assert len(first) == 4 and c.shape == first and first[3] == HEAD_DIM and c.stride(3) == 1
+    Hq, Hkv = shape[1], first[2]
     assert Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"{Hq} query heads over {Hkv} kv heads"
     assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
     assert block_table.shape[0] >= num_seqs
     assert seq_lens.dtype == torch.int32 and seq_lens.is_contiguous() and seq_lens.numel() >= num_seqs
-    for t in (*caches, block_table, seq_lens):
-        assert t.device == q.device, "all tensors must share the query's device"
+    assert block_table.device == device and seq_lens.device == device, "all tensors must share the query's device"
 
 
 def tree_mask(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, max_seqlen_q: int) -> torch.Tensor:
@@ -405,6 +406,7 @@ def paged_tree_attention(
     if out is None:
         out = torch.empty(TQ, Hq, HEAD_DIM, dtype=torch.bfloat16, device=device)
     assert out.dtype in _OUT_CODES and out.shape == (TQ, Hq, HEAD_DIM) and out.stride(2) == 1 and out.device == device
+    assert distinct(out), "out is a broadcast"
     lse = torch.empty(Hq, TQ, dtype=torch.float32, device=device) if return_softmax_lse else None
     qd, qsb, qsh = _descale(q_descale, B, Hkv, device)
     kd, ksb, ksh = _descale(k_descale, B, Hkv, device)
@@ -480,6 +482,7 @@ def accumulate_attention_weights(
     assert scores.dtype == torch.float32 and scores.dim() == 3 and scores.device == device
     assert scores.shape[0] >= B and scores.shape[1] == Hkv and (scores.stride(2) == 1 or scores.shape[2] <= 1), \
         f"scores must be [>= {B}, {Hkv}, width] with unit last stride"
+    assert distinct(scores), "scores are a broadcast"
     assert lse.dtype == torch.float32 and lse.shape == (Hq, TQ) and lse.device == device
     assert lse.stride(1) == 1 or TQ <= 1, "lse must have unit last stride"
     if softmax_scale is None:

@@ -21,7 +21,7 @@ import threading
 import numpy as np
 import torch
 
-from ._lib import check, dtype_code, i64_array, lib, on_device, ptr, stream_handle
+from ._lib import check, distinct, dtype_code, i64_array, lib, on_device, ptr, stream_handle
 
 FP8_E4M3_MAX = 448.0
 
@@ -191,10 +191,14 @@ def _cache_pairs(caches, first_row_dim):
     if isinstance(caches, torch.Tensor):
         caches = [caches]
     assert len(caches) > 0
-    device, outer = caches[0].device, caches[0].shape[:3]
-    for c in caches:
-        shape, strides = c.shape, c.stride()
-        assert c.is_cuda and c.device == device, "all caches must be on one GPU"
+    first = caches[0]
+    device, outer = first.device, first.shape[:3]
+    assert first.is_cuda, "all caches must be on one GPU"
+    pairs, i = [], 0
+    while i < len(caches):
+        a = caches[i]
+        shape, strides = a.shape, a.stride()
+        assert a.device == device, "all caches must be on one GPU"
         assert shape[:3] == outer, "all caches must have the same layers, pages and page size"
         expect = 1
         for dim in range(len(shape) - 1, first_row_dim - 1, -1):
@@ -202,13 +206,13 @@ def _cache_pairs(caches, first_row_dim):
                 f"cache rows must be contiguous beyond dim {first_row_dim - 1} (strides {strides})"
             )
             expect *= shape[dim]
-    pairs, i = [], 0
-    while i < len(caches):
-        a = caches[i]
         b = caches[i + 1] if i + 1 < len(caches) else None
-        same = b is not None and (a.shape, a.stride(), a.dtype) == (b.shape, b.stride(), b.dtype)
-        pairs.append((a, b if same else None))
-        i += 2 if same else 1
+        if b is not None and b.device == device and b.shape == shape and b.stride() == strides and b.dtype == a.dtype:
+            pairs.append((a, b))
+            i += 2
+        else:
+            pairs.append((a, None))
+            i += 1
     return pairs
 
 
@@ -247,10 +251,10 @@ def evict_tokens(
     Kept token i, in position order, becomes row i of the pages
     ``dst_block_table[b]`` (int32 [B, W], at least budget rows; entries outside
     the cache are skipped, a source row on a missing page reads as zeros).
-    Those pages must be none that ``block_table`` names: prefix pages may be
-    shared by sequences, so they are read and left as they are.
-    ``scores_out`` (default: ``scores``, in place) receives the kept tokens'
-    scores, then zeros up to n.
+    Those pages must be none that ``block_table`` names, each named once: prefix
+    pages may be shared by sequences, so they are read and left as they are.
+    ``scores_out`` (default: ``scores``, in place; else it shares no element with
+    it) receives the kept tokens' scores, then zeros up to n.
 
     Returns (kept, new_lens): int32 [L, B, H or 1, budget], each kept token's old
     position (-1 past the last), and int32 [B], the new lengths.  One launch for
@@ -263,23 +267,34 @@ def evict_tokens(
     pairs = _cache_pairs(caches, 3 if first.ndim == 4 else 4)
     device = first.device
     layers, num_blocks, page = first.shape[:3]
-    assert all(c.ndim == first.ndim and (1 if c.ndim == 4 else c.shape[3]) == heads for p in pairs for c in p
-               if c is not None), "all caches must have the same heads"
-    assert scores.dtype == torch.float32 and scores.dim() == 4 and scores.device == device
-    assert scores.shape[0] == layers and scores.shape[2] in (1, heads), \
-        f"scores of shape {tuple(scores.shape)} for {layers} layers of {heads} heads"
-    scores_out = scores if scores_out is None else scores_out
-    assert scores_out.dtype == torch.float32 and scores_out.device == device
-    assert scores_out.dim() == 4 and scores_out.shape[:3] == scores.shape[:3]
-    for t in (scores, scores_out):
-        assert t.stride(3) == 1 or t.shape[3] <= 1, "scores need unit last stride"
-    B, kept_heads = scores.shape[1], scores.shape[2]
+    for a, _ in pairs:
+        assert a.ndim == first.ndim and (a.ndim == 4 or a.shape[3] == heads), "all caches must have the same heads"
+    shape, strides = scores.shape, scores.stride()
+    assert scores.dtype == torch.float32 and len(shape) == 4 and scores.device == device
+    B, kept_heads, width = shape[1:]
+    assert shape[0] == layers and kept_heads in (1, heads), \
+        f"scores of shape {tuple(shape)} for {layers} layers of {heads} heads"
+    assert strides[3] == 1 or width <= 1, "scores need unit last stride"
+    out_strides, out_width = strides, width
+    if scores_out is None:
+        scores_out = scores
+    else:
+        out_strides, out_width = scores_out.stride(), scores_out.shape[-1]
+        assert scores_out.dtype == torch.float32 and scores_out.device == device
+        assert scores_out.dim() == 4 and scores_out.shape[:3] == shape[:3]
+        assert out_strides[3] == 1 or out_width <= 1, "scores need unit last stride"
+    assert distinct(scores_out) and (out_strides == strides or scores_out.data_ptr() != scores.data_ptr()), \
+        "scores_out must be scores itself or share no element with it, and be no broadcast"
     budget, sink, recent = int(budget), int(sink), int(recent)
     assert budget >= 1 and sink >= 0 and recent >= 0 and sink + recent <= budget, \
         f"sink {sink} and recent {recent} do not fit a budget of {budget}"
     _i32(block_table, device, 2, B, "block_table")
     _i32(dst_block_table, device, 2, B, "dst_block_table")
     _i32(seq_lens, device, 1, B, "seq_lens")
+    # (all that a launch would refuse, so that none follows one that has written)
+    assert 1 <= layers <= 65535 and B <= 65535 and budget * heads < 2 ** 31, \
+        f"{layers} layers, {B} sequences, a budget of {budget} for {heads} heads"
+    assert num_blocks >= 1 and page >= 1 and (block_table.shape[1] >= 1 or B == 0), "an empty cache or block table"
     assert dst_block_table.shape[1] * page >= budget, \
         f"{dst_block_table.shape[1]} pages of {page} cannot hold a budget of {budget}"
     assert block_table.data_ptr() != dst_block_table.data_ptr() or B == 0, "the kept tokens go to pages of their own"
@@ -287,22 +302,22 @@ def evict_tokens(
     new_lens = torch.empty(B, dtype=torch.int32, device=device)
     with on_device(device):
         stream = stream_handle(device)
-        need = int(lib().psk_select_tokens_workspace_bytes(layers, B, kept_heads, scores.shape[3], budget))
+        need = int(lib().psk_select_tokens_workspace_bytes(layers, B, kept_heads, width, budget))
         if need < 0:
             check(need, "evict_tokens workspace")
         workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         status = lib().psk_select_tokens(
-            ptr(scores), i64_array(scores.stride()[:3]), scores.shape[3], ptr(scores_out),
-            i64_array(scores_out.stride()[:3]), scores_out.shape[3], ptr(seq_lens), layers, B, kept_heads, budget, sink,
-            recent, ptr(kept), ptr(new_lens), ptr(workspace), need, stream,
+            ptr(scores), i64_array(strides[:3]), width, ptr(scores_out), i64_array(out_strides[:3]), out_width,
+            ptr(seq_lens), layers, B, kept_heads, budget, sink, recent, ptr(kept), ptr(new_lens), ptr(workspace), need,
+            stream,
         )
         check(status, "evict_tokens")
-        for a, b in pairs:
-            es = a.element_size()
+        for a, b in pairs if B else ():
+            es, st = a.element_size(), a.stride()
             head = math.prod(a.shape[3 if a.ndim == 4 else 4:])
             status = lib().psk_move_kept_tokens(
-                ptr(a), ptr(b), a.stride(0) * es, a.stride(1) * es, a.stride(2) * es,
-                0 if a.ndim == 4 else a.stride(3) * es, head * es, layers, heads, page, num_blocks, ptr(block_table),
+                ptr(a), ptr(b), st[0] * es, st[1] * es, st[2] * es, 0 if a.ndim == 4 else st[3] * es, head * es, layers,
+                heads, page, num_blocks, ptr(block_table),
                 block_table.stride(0), block_table.shape[1], ptr(dst_block_table), dst_block_table.stride(0),
                 dst_block_table.shape[1], ptr(kept), kept_heads, budget, B, stream,
             )
@@ -329,7 +344,7 @@ def commit_draft_tokens(
     caches: one tensor or a list, [L, num_blocks, block_size, *row] with
     contiguous rows (K and V views of the fused cache, a latent cache); two of
     one geometry move in one launch.  Negative indices and rows on missing pages
-    are skipped.
+    are skipped.  The pages of drafted tokens are a sequence's own.
     """
     pairs = _cache_pairs(caches, 3)
     first = pairs[0][0]
@@ -343,10 +358,9 @@ def commit_draft_tokens(
     _i32(path_lens, device, 1, B, "path_lens")
     with on_device(device):
         for a, b in pairs:
-            es = a.element_size()
+            es, st = a.element_size(), a.stride()
             status = lib().psk_commit_draft_tokens(
-                ptr(a), ptr(b), a.stride(0) * es, a.stride(1) * es, a.stride(2) * es, math.prod(a.shape[3:]) * es,
-                layers, page, num_blocks, ptr(block_table), block_table.stride(0), block_table.shape[1], ptr(starts),
+                ptr(a), ptr(b), st[0] * es, st[1] * es, st[2] * es, math.prod(a.shape[3:]) * es, layers, page, num_blocks, ptr(block_table), block_table.stride(0), block_table.shape[1], ptr(starts),
                 ptr(path), path.stride(0), path.shape[1], ptr(path_lens), B, stream_handle(device),
             )
             check(status, "commit_draft_tokens")

@@ -202,3 +202,101 @@ def test_refusals(dev):
     for match, change in bad:
         with pytest.raises(AssertionError, match=match):
             attention.accumulate_attention_weights(**{**good, **change})
+
+
+# --------------------------------------------------------------------------- #
+# many query rows a key
+# --------------------------------------------------------------------------- #
+
+
+@pytest.mark.parametrize("n", [1, 7, 8, 9, 20, 33, 64, 100])
+@pytest.mark.parametrize("Hq,Hkv", [(40, 1), (5, 1), (12, 4), (9, 3), (64, 1), (2, 2)])
+def test_shapes_of_row_tiles(dev, n, Hq, Hkv):
+    """Tiles of 32 rows as heads by tokens, neither a multiple of the tile."""
+    case = Case(dev, n + Hq, [n + 200, n, max(n - 2, 0), n + 1], [n, n, n, max(n // 2, 1)], Hq, Hkv, 16, spare_rows=1)
+    lse, scores = _lse(case), _scores(case)
+    _check(case, lse, scores, _run(case, dev, lse, scores, decay=0.5), decay=0.5)
+
+
+@pytest.mark.parametrize("strided", [True, False])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_rows_of_fp8_queries(dev, strided, causal):
+    """Read where they lie, without a workspace."""
+    case = Case(dev, 6, [300, 61, 1025], [30, 16, 50], 15, 3, 24, q_dtype=torch.float8_e4m3fn, strided_q=strided)
+    assert attention.weights_workspace_bytes(case.TQ, case.max_q, 15, 3, case.qd.dtype) == 0
+    lse, scores = _lse(case, causal), _scores(case)
+    _check(case, lse, scores, _run(case, dev, lse, scores, causal), causal)
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_many_sequences(dev, n):
+    """More than one window of 64 sequences, some without query tokens, whose sums decay all the same."""
+    rng = np.random.default_rng(2)
+    counts = [int(x) for x in rng.integers(0, n + 1, 150)]
+    lens = [c + int(x) for c, x in zip(counts, rng.integers(0, 90, 150))]
+    case = Case(dev, 14, lens, counts, 8, 2, 8)
+    lse, scores = _lse(case), _scores(case)
+    _check(case, lse, scores, _run(case, dev, lse, scores, decay=0.25), decay=0.25)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_pages_of_one_token_and_long_rows(dev, n):
+    case = Case(dev, 15, [4100, 1030], [n, n], 4, 2, 1)
+    lse, scores = _lse(case), _scores(case)
+    _check(case, lse, scores, _run(case, dev, lse, scores))
+
+
+@pytest.mark.parametrize("n", [2, 40])
+def test_nan_keys_that_a_row_does_not_see(dev, n):
+    """A NaN key gives its own column NaN and no other; one that no query sees, none."""
+    case = Case(dev, 16, [60 + n, 30 + n], [n, n], 8, 2, 16)
+    lse, scores = _lse(case), _scores(case)
+    want = _run(case, dev, lse, scores)
+    page, row = int(case.bt[0, 1]), 3
+    case.k.view(torch.uint8)[page, row, 1, 7] = 0x7F
+    for b, L in enumerate(case.lens):
+        if L % 16:
+            case.k.view(torch.uint8)[int(case.bt[b, L // 16]), L % 16:] = 0x7F
+    got = _run(case, dev, lse, scores)
+    assert bool(torch.isnan(got[0, 1, 19]))
+    got[0, 1, 19] = want[0, 1, 19]
+    assert torch.equal(got, want)
+
+
+def test_a_query_row_of_nan_reaches_the_keys_it_sees(dev):
+    n = 20
+    case = Case(dev, 17, [70], [n], 4, 1, 16, descales=False)
+    lse, scores = _lse(case), _scores(case)
+    want = _run(case, dev, lse, scores)
+    case.qd[5, 2, 9] = float("nan")
+    got = _run(case, dev, lse, scores)
+    assert bool(torch.isnan(got[0, 0, :56]).all())
+    assert torch.equal(got[0, 0, 56:], want[0, 0, 56:])
+
+
+def test_scores_that_are_a_broadcast_are_refused(dev):
+    case = Case(dev, 1, [20, 30], [3, 4], 8, 2, 16)
+    lse = torch.from_numpy(_lse(case)).to(dev)
+    with pytest.raises(AssertionError, match="broadcast"):
+        attention.accumulate_attention_weights(torch.zeros(1, 2, 32, device=dev).expand(2, 2, 32), case.qd, case.k, lse,
+                                               case.btd, case.lensd, case.cud, 4)
+
+
+def test_many_rows_replayed_in_a_graph(dev):
+    case = Case(dev, 18, [500, 133], [40, 30], 8, 2, 16)
+    lse = torch.from_numpy(_lse(case)).to(dev)
+    kw = dict(softmax_scale=case.scale, q_descale=case.dd[0], k_descale=case.dd[1], decay=0.5)
+    args = (case.qd, case.k, lse, case.btd, case.lensd, case.cud, 40)
+    total, want = torch.zeros(2, 2, 512, device=dev), torch.zeros(2, 2, 512, device=dev)
+    attention.accumulate_attention_weights(total.clone(), *args, **kw)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        attention.accumulate_attention_weights(total, *args, **kw)
+    for r in range(4):
+        case.qd.copy_((case.q.float() * (1 + r)).to(case.q.dtype))
+        gr.replay()
+        torch.cuda.synchronize()
+        attention.accumulate_attention_weights(want, *args, **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(total, want)

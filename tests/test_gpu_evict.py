@@ -289,3 +289,55 @@ def test_commit_replayed_in_a_graph(dev):
         torch.cuda.synchronize()
         T.commit_draft_tokens(host, bt.numpy(), [20, 5], path.cpu().numpy(), [4 - r, 3])
         assert np.array_equal(cache.cpu().numpy(), host), r
+
+
+# --------------------------------------------------------------------------- #
+# equal scores, rounds of long rows, refusals before anything is written
+# --------------------------------------------------------------------------- #
+
+
+@pytest.mark.parametrize("n,budget,sink,recent", [(40, 12, 0, 0), (5000, 700, 4, 64), (20000, 3000, 4, 64), (40000, 64, 32, 32),
+                                                  (16384, 16383, 0, 0), (16385, 1, 0, 0), (4096, 4096, 7, 9), (4097, 4096, 1, 0)])
+@pytest.mark.parametrize("value", [0.0, float("nan"), float("-inf"), -1.5])
+def test_equal_scores_keep_the_first(dev, n, budget, sink, recent, value):
+    e = Evict(3, 1, [n, n // 2], budget, 16, heads=1, row=16)
+    e.scores.fill_(value)
+    e.check(dev, sink, recent)
+
+
+def test_many_long_rows(dev):
+    """More chunks than one round of launches takes, lengths apart."""
+    lens = [17000, 1, 0, 16385, 900, 65540]
+    e = Evict(4, 2, lens, 64, 64, heads=69, row=16, dtype=torch.uint8)
+    assert 2 * 6 * 69 * 5 > 4096
+    e.check(dev, 4, 8)
+
+
+def test_eviction_refuses_before_it_writes(dev):
+    e = Evict(10, 1, [50, 60], 20, 16)
+    cache = e.cache.to(dev)
+    k, v = e.views(cache)
+    scores = e.scores.to(dev)
+    good = dict(caches=[k, v], scores=scores, block_table=e.bt.to(dev),
+                seq_lens=torch.tensor(e.lens, dtype=torch.int32, device=dev), dst_block_table=e.dst.to(dev), budget=20)
+    bad = [
+        ("scores_out", dict(scores_out=scores.transpose(1, 2).contiguous().transpose(1, 2).transpose(0, 0)[:, :, :1]
+                            .expand(1, 2, 2, scores.shape[3]))),
+        ("scores_out", dict(scores_out=torch.as_strided(scores, scores.shape, (0, scores.stride(2), scores.stride(1), 1)))),
+        ("block table", dict(block_table=good["block_table"][:, :0])),
+        ("layers", dict(caches=[k[:0], v[:0]], scores=scores[:0])),
+    ]
+    for match, change in bad:
+        with pytest.raises(AssertionError, match=match):
+            cache_ops.evict_tokens(**{**good, **change})
+    torch.cuda.synchronize()
+    assert np.array_equal(_bits(scores), _bits(e.scores)) and np.array_equal(_bits(cache), _bits(e.cache))
+    none = dict(scores=scores[:, :0], block_table=good["block_table"][:0], seq_lens=good["seq_lens"][:0],
+                dst_block_table=good["dst_block_table"][:0])
+    kept, lens = cache_ops.evict_tokens(**{**good, **none})
+    assert kept.shape == (1, 0, 2, 20) and lens.shape == (0,)
+
+
+def test_a_path_that_names_a_token_twice(dev):
+    """Both rows get the token's; one that stays where it is, is left."""
+    _commit(dev, 5, (2, 40, 2, 16, 2, 128), torch.float8_e4m3fn, [5, 33], [[3, 3, 0, 2], [0, 1, 1, 7]], [4, 3], _FUSED)
