@@ -29,11 +29,14 @@ namespace {
 //     registers so that two workgroups of 1024 threads share a CU (73 registers,
 //     one of them: 56 us).  512 rows of 12288: 27 us, bound by the histograms'
 //     additions; 8 rows of 1100: 7.8 us, the barriers between the digits.
+//     Rows of at most 4096 take 256 threads, which wait less at them: 512 rows of
+//     4000 and their moves 29 us against 31 with 1024, 2048 of 2000, 74 against 95.
 //   * longer ones, a workgroup a chunk: three launches of chunk_digit_kernel
 //     leave each chunk's histogram of a digit, and every workgroup of the next
 //     launch adds up those of its row; chunk_emit_kernel then has, from the
-//     histograms of the chunks before its own, where its kept tokens go.  One
-//     workgroup for a row of 131072 took 337 us.
+//     histograms of the chunks before its own, where its kept tokens go.  Four rows
+//     of 131072: 34 us, bound by the launches and the histograms; with one workgroup
+//     a row 337.  Chunks of 8192: the same, but 15 us more for a row of a million.
 
 constexpr int kSelThreads = 1024;               // (256 for rows of at most 256 kPer)
 constexpr int kPer = 16;                        // scores of a thread
@@ -366,7 +369,9 @@ __global__ void __launch_bounds__(256) unstage_scores_kernel(SelectArgs p) {
 // Row (slot, head) by row, heads first, V bytes a lane: the destination is
 // written in order and every source row is read whole.  A thread takes kMoveRows
 // rows at once, so that the chain to a row (kept position, page, row) is waited
-// for once for all of them.
+// for once for all of them.  Bound by HBM: 2048 rows of 8 heads in each of 64
+// (layer, sequence) pairs, 537 MB moved, 97 us, 5.5 TB/s (a row a thread through the
+// caches: 20 us more).
 
 constexpr int kMoveThreads = 256;
 constexpr int kMoveRows = 4;
@@ -469,7 +474,8 @@ __global__ void __launch_bounds__(kMoveThreads) move_kept_kernel(MoveArgs p) {
 // Rows starts[b] + path[b, i] become rows starts[b] + i, of every layer, as a
 // snapshot: a workgroup owns some columns of all of a sequence's rows and reads
 // every one of them before it writes any.  The shorter the paths, the more
-// columns.
+// columns.  Bound by the chain of its three loads: paths of 6 in 32 sequences and 32
+// layers (1 KB rows) 4.8 us, of 9 in 8 sequences and 61 layers the same.
 
 constexpr int kCommitRows = 256;  // longest path
 constexpr int kCommitThreads = 256;
@@ -618,7 +624,6 @@ int psk_select_tokens(const float* scores, const int64_t* scores_strides, int64_
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t rows = num_layers * num_seqs * num_heads;
   if (need == 0) {
-    // (fewer threads wait less at the barriers, more hold more scores)
     if (scores_width <= kSmallThreads * kPer)
       hipLaunchKernelGGL(select_row_kernel<kSmallThreads>, dim3(unsigned(rows)), dim3(kSmallThreads), 0, st, p);
     else

@@ -29,7 +29,16 @@
 // The work is cut into equal runs over sequences and kv heads (cached_queries.h).
 // A run's piece that is not all of a job's keys leaves a partial record (maxima,
 // sums, float32 accumulators); merge_tree_kernel joins a job's records in the
-// order of its keys.
+// order of its keys.  Short contexts are not cut (kWholeKeys), and wide trees over
+// much work run in prefill_runs.hip (kWideRows).
+//
+// What bounds it, and what it measured: 32 trees of 16 tokens over contexts of 512 to
+// 16384 (32 query heads over 8), 113 us, the loads' latency (3.2 TB/s; the row blocks'
+// second reads come from L2); 48 ragged trees over up to 6000 keys (8 heads over one)
+// 27 us and one of 8 over 1000 15 us, the chain lengths - page ids - keys and the
+// merge.  A tile of 32 keys and 32 rows costs 512 matrix cycles and 156 vector
+// instructions, 64 of them the conversion of K and V to bf16 and fp16; the two hardly
+// overlap at two waves a SIMD (1400 cycles a tile), and three do not fit the registers.
 //
 // C ABI: include/pipeswift_kv.h.  Nothing here allocates or synchronizes.
 
@@ -52,7 +61,9 @@ constexpr int kTile = 32;                  // keys of a tile
 constexpr uint32_t kHalfSlot = kTile * 128;  // bytes of a tile's K (its V follows)
 constexpr uint32_t kSlot = 2 * kHalfSlot;
 constexpr int kRing = 2;
-constexpr int kOver = 6;                   // units (of kStepKeys keys) that a piece costs beside its keys
+// units (of kStepKeys keys) that a piece costs beside its keys: 1, 4, 6, 12 gave 35.5,
+// 29.7, 28.4, 27.4 us for the ragged trees above and 113, 114, 114, 120 for the 32
+constexpr int kOver = 6;
 // Up to this many keys a workgroup takes all of a job's and nothing is merged: four
 // sequences of 8 tokens (32 query heads over 8), us, whole / cut: 1000 keys 17 / 19, 1600
 // 19 / 19, 2500 24 / 21; 64 sequences of 1000, 32 / 38.
@@ -621,7 +632,8 @@ int launch_tree(const TreeArgs& p, bool general, hipStream_t st) {
 }
 
 // Pages of a multiple of 8 keys whose rows lie within 32-bit offsets (the keys of a
-// load share a page), K and V laid out alike.
+// load share a page), K and V laid out alike.  16 trees of 16 tokens over 8000: pages
+// of 16 take 72 us, of 12 with a look-up a lane 85.
 bool shares_pages(const DecodeArgs& a) {
   return a.block_size % 8 == 0 && a.k_row >= 0 && 8 * a.k_row < (int64_t(1) << 31) && a.k_row == a.v_row && a.k_blk == a.v_blk;
 }
