@@ -387,8 +387,9 @@ def paged_tree_attention(
     ``paged_prefill_attention``.
 
     ``max_seq_len``: a bound on seq_lens where the caller has a closer one than
-    the block table's width; it only sizes the launch.  ``workspace``: float32
-    of ``tree_workspace_floats``, for callers that keep one."""
+    the block table's width; it sizes the launch and chooses its form, and a
+    longer sequence is read whole all the same.  ``workspace``: float32 of
+    ``tree_workspace_floats``, for callers that keep one."""
     B, n = _query_layout(q, cu_seqlens_q, max_seqlen_q, validate)
     _check_paged(q, (k_cache, v_cache), block_table, seq_lens, B)
     TQ, Hq, _ = q.shape

@@ -710,6 +710,7 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
   if (workspace_bytes < need || (need > 0 && !workspace))
     return fail(PSK_E_WORKSPACE, "workspace of %lld bytes, need %lld", (long long)workspace_bytes, (long long)need);
   if (need > 0) {
+    if (total_q * num_q_heads >= int64_t(1) << 29) return fail(PSK_E_ARG, "%lld query rows", (long long)(total_q * num_q_heads));
     uint8_t* q8 = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
     p.q8 = q8;
     p.q8_tok = num_q_heads * kHead;

@@ -233,7 +233,7 @@ select_row_kernel(SelectArgs p) {
   constexpr int PER = kBins / NT;
   __shared__ uint32_t s_hist[kBins];
   __shared__ uint32_t s_wave[NT / 64], s_count[2][NT / 64], s_pick[2];
-  const int tid = int(threadIdx.x), row = int(blockIdx.x);
+  const int tid = int(threadIdx.x), row = p.row0 + int(blockIdx.x);
   const SelectRow r = select_row(p, row);
   if (row < p.num_seqs * p.heads && row % p.heads == 0 && tid == 0) p.new_lens[row / p.heads] = r.n;
   Held<NT> held;
@@ -624,10 +624,15 @@ int psk_select_tokens(const float* scores, const int64_t* scores_strides, int64_
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t rows = num_layers * num_seqs * num_heads;
   if (need == 0) {
-    if (scores_width <= kSmallThreads * kPer)
-      hipLaunchKernelGGL(select_row_kernel<kSmallThreads>, dim3(unsigned(rows)), dim3(kSmallThreads), 0, st, p);
-    else
-      hipLaunchKernelGGL(select_row_kernel<kSelThreads>, dim3(unsigned(rows)), dim3(kSelThreads), 0, st, p);
+    constexpr int64_t kMostRows = 1 << 20;  // of a launch
+    for (int64_t row = 0; row < rows; row += kMostRows) {
+      p.row0 = int32_t(row);
+      const dim3 grid{unsigned(std::min(kMostRows, rows - row)), 1u, 1u};
+      if (scores_width <= kSmallThreads * kPer)
+        hipLaunchKernelGGL(select_row_kernel<kSmallThreads>, grid, dim3(kSmallThreads), 0, st, p);
+      else
+        hipLaunchKernelGGL(select_row_kernel<kSelThreads>, grid, dim3(kSelThreads), 0, st, p);
+    }
     return check_launch("select_row_kernel launch");
   }
   p.chunks = int32_t(ceil_div(scores_width, kChunk));

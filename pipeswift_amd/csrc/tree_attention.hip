@@ -535,57 +535,57 @@ tree_attention_kernel(TreeArgs args) {
   }
 }
 
-// The records of a job joined: a wave per (job, 32 rows, 8 columns).
+// The records of a job joined: a wave per task (job, 32 rows, 8 columns).
 template <int OUT_DT>
 __global__ void __launch_bounds__(256) merge_tree_kernel(TreeArgs p) {
   const DecodeArgs& a = p.a;
   const int lane = int(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
   const int kk = lane & 31;
-  // the wave's task: column group q of row block `block` of job (b, h)
-  const int64_t task = int64_t(blockIdx.x) * 4 + wave;
-  const int q = int(task & 15);
-  const int64_t rest = task >> 4;
-  const int block = int(rest % p.row_blocks);
-  const int64_t job = rest / p.row_blocks;
-  const int h = int(job % p.s.heads), b = int(job / p.s.heads);
-  if (b >= p.s.num_seqs) return;
-  const SeqRows r = seq_rows(a, p.s.total_q, b);
-  const int row = kRows * block + kk;
-  if (kRows * block >= r.n * a.heads) return;
-  SeqWindow seqs;
-  const StepRuns cost = step_runs(a, p.s, seqs, lane);
-  const int64_t before = units_before(a, p.s, b, seqs, lane);
-  const int steps = key_steps(p.s, lane_value(seqs.len, b - seqs.b0));
-  const int64_t at = before + h * int64_t(p.s.over + steps) + p.s.over;  // the first unit that pays for keys
-  const int64_t j0 = uniform_div(at, cost.run), j1 = steps > 0 ? uniform_div(at + steps - 1, cost.run) : j0 - 1;
-  if (j0 == j1) return;  // one run had all the keys and wrote the rows
+  const uint32_t tasks = uint32_t(p.s.num_seqs) * uint32_t(p.s.heads) * uint32_t(p.row_blocks) * 16;  // (host: below 2^28)
+  for (uint32_t task = blockIdx.x * 4 + wave; task < tasks; task += gridDim.x * 4) {
+    // column group q of row block `block` of job (b, h)
+    const int q = int(task & 15);
+    const uint32_t rest = task >> 4, job = rest / uint32_t(p.row_blocks);
+    const int block = int(rest - job * uint32_t(p.row_blocks));
+    const int b = int(job / uint32_t(p.s.heads)), h = int(job - uint32_t(b) * uint32_t(p.s.heads));
+    const SeqRows r = seq_rows(a, p.s.total_q, b);
+    const int row = kRows * block + kk;
+    if (kRows * block >= r.n * a.heads) continue;
+    SeqWindow seqs;
+    const StepRuns cost = step_runs(a, p.s, seqs, lane);
+    const int64_t before = units_before(a, p.s, b, seqs, lane);
+    const int steps = key_steps(p.s, lane_value(seqs.len, b - seqs.b0));
+    const int64_t at = before + h * int64_t(p.s.over + steps) + p.s.over;  // the first unit that pays for keys
+    const int64_t j0 = uniform_div(at, cost.run), j1 = steps > 0 ? uniform_div(at + steps - 1, cost.run) : j0 - 1;
+    if (j0 == j1) continue;  // one run had all the keys and wrote the rows
 
-  float top = kNegBig, sum = 0.0f;
-  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr int kAhead = 4;  // records read together
-  for (int64_t j = j0; j <= j1; j += kAhead) {
-    float m[kAhead], l[kAhead];
-    f32x4 v[kAhead];
+    float top = kNegBig, sum = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kAhead = 4;  // records read together
+    for (int64_t j = j0; j <= j1; j += kAhead) {
+      float m[kAhead], l[kAhead];
+      f32x4 v[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int64_t k = min(j + u, j1);
-      const float* rec = record(p, k, block, k == j0 ? 1 : 0);
-      m[u] = rec[4096 + kk];
-      l[u] = rec[4096 + 32 + kk];
-      v[u] = *reinterpret_cast<const f32x4*>(rec + (q * 64 + lane) * 4);
-    }
+      for (int u = 0; u < kAhead; ++u) {
+        const int64_t k = min(j + u, j1);
+        const float* rec = record(p, k, block, k == j0 ? 1 : 0);
+        m[u] = rec[4096 + kk];
+        l[u] = rec[4096 + 32 + kk];
+        v[u] = *reinterpret_cast<const f32x4*>(rec + (q * 64 + lane) * 4);
+      }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (j + u > j1) break;
-      const float up = __builtin_fmaxf(top, m[u]);
-      const float f0 = __builtin_amdgcn_exp2f(top - up), f1 = __builtin_amdgcn_exp2f(m[u] - up);
-      top = up;
-      sum = sum * f0 + l[u] * f1;
-      o = o * f0 + v[u] * f1;
+      for (int u = 0; u < kAhead; ++u) {
+        if (j + u > j1) break;
+        const float up = __builtin_fmaxf(top, m[u]);
+        const float f0 = __builtin_amdgcn_exp2f(top - up), f1 = __builtin_amdgcn_exp2f(m[u] - up);
+        top = up;
+        sum = sum * f0 + l[u] * f1;
+        o = o * f0 + v[u] * f1;
+      }
     }
+    finish<OUT_DT>(p, r, b, h, row, q, lane, o, top, sum);
   }
-  finish<OUT_DT>(p, r, b, h, row, q, lane, o, top, sum);
 }
 
 // Workgroups resident at once: two per CU (LDS and registers).
@@ -626,8 +626,8 @@ int launch_tree(const TreeArgs& p, bool general, hipStream_t st) {
   if (general) hipLaunchKernelGGL((tree_attention_kernel<Q_DT, OUT_DT, true>), grid, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((tree_attention_kernel<Q_DT, OUT_DT, false>), grid, dim3(kThreads), 0, st, p);
   if (const int e = check_launch("tree_attention_kernel launch"); e != PSK_OK || p.whole) return e;
-  const int64_t tasks = jobs * p.row_blocks * 16;
-  hipLaunchKernelGGL((merge_tree_kernel<OUT_DT>), dim3(unsigned(tasks / 4)), dim3(256), 0, st, p);
+  const int64_t groups = std::min<int64_t>(jobs * p.row_blocks * 4, 1 << 20);  // of four tasks
+  hipLaunchKernelGGL((merge_tree_kernel<OUT_DT>), dim3(unsigned(groups)), dim3(256), 0, st, p);
   return check_launch("merge_tree_kernel launch");
 }
 
@@ -735,7 +735,8 @@ int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head
     return launch_tree_runs(a, TreeStep{tree_mask, tree_mask_stride, p.scale_log2, int32_t(total_q)}, num_seqs, q_dtype,
                             out_dtype, reinterpret_cast<int32_t*>(workspace), static_cast<hipStream_t>(stream));
   p.records = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
-  if (num_seqs * num_kv_heads * s.row_blocks > INT32_MAX / 16 || s.max_runs * s.row_blocks > INT32_MAX)
+  constexpr int64_t kMost = (int64_t(1) << 24) - 8;  // workgroups of a launch
+  if (std::max(num_seqs * num_kv_heads, s.max_runs) > kMost / s.row_blocks)
     return fail(PSK_E_ARG, "too many rows (%lld sequences of up to %lld drafted tokens)", (long long)num_seqs,
                 (long long)max_seqlen_q);
   hipStream_t st = static_cast<hipStream_t>(stream);
