@@ -334,9 +334,9 @@ few_rows_kernel(WeightArgs args) {
 template <int Q_DT>
 __global__ void __launch_bounds__(kThreads) quantize_queries_kernel(WeightArgs p, int num_q_heads, uint8_t* q8) {
   const DecodeArgs& a = p.a;
-  const int64_t x = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t row = x >> 3;
-  const int tok = int(row / num_q_heads), hq = int(row - int64_t(tok) * num_q_heads);
+  const uint32_t x = blockIdx.x * kThreads + threadIdx.x;  // (host: below 2^32)
+  const uint32_t row = x >> 3, token = row / uint32_t(num_q_heads);
+  const int tok = int(token), hq = int(row - token * uint32_t(num_q_heads));
   if (tok >= p.s.total_q) return;
   float qd = 1.0f;
   if (a.qd) {  // the descale of the row's sequence and kv head
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) quantize_queries_kernel(WeightArgs p
   }
   QueryBytes<Q_DT> qb;
   qb.load(a.q + int64_t(tok) * a.q_tok_stride + int64_t(hq) * a.q_head_stride, 16 * int(x & 7));
-  *reinterpret_cast<u32x4*>(q8 + 16 * x) = qb.quantized(qd, 0u);
+  *reinterpret_cast<u32x4*>(q8 + 16 * int64_t(x)) = qb.quantized(qd, 0u);
 }
 
 // Sixteen values of a lane summed over the 32 lanes of its half, in a fixed
