@@ -261,34 +261,46 @@ __device__ __forceinline__ uint16_t* chunk_hist(const SelectArgs& p, int row, in
   return p.hist + ((int64_t(row) * p.chunks + chunk) * kDigits + digit) * kBins;
 }
 
-// Adds up the row's histograms of digit d and finds the bin of the left-th key;
-// above and at: how many keys of the chunks before this one are above that bin
-// and in it.
-__device__ __forceinline__ Digit row_digit(const SelectArgs& p, const SelectRow& r, int row, int chunk, int d, uint32_t left,
-                                           uint32_t* s_wave, uint32_t* s_pick, uint32_t& above, uint32_t& at) {
-  // thread t: bins 2047 - 2 t and 2046 - 2 t, which lie in one word
-  const uint32_t* hist = reinterpret_cast<const uint32_t*>(chunk_hist(p, row, 0, d)) + kBins / 2 - 1 - int(threadIdx.x);
-  const int n = (r.len + kChunk - 1) / kChunk;
-  uint32_t all[2] = {0, 0}, mine[2] = {0, 0};
-#pragma unroll 8
-  for (int c = 0; c < n; ++c) {
-    const uint32_t w = hist[int64_t(c) * (kDigits * kBins / 2)];
-    all[0] += w >> 16;
-    all[1] += w & 0xFFFFu;
-    mine[0] += c < chunk ? w >> 16 : 0u;
-    mine[1] += c < chunk ? w & 0xFFFFu : 0u;
-  }
-  const Digit g = find_digit<kSelThreads>(all, left, s_wave, s_pick);
-  at = 0;
+// The row's histograms of its first N digits added up, all of them and those of the
+// chunks before this one; thread t has bins 2047 - 2 t and 2046 - 2 t, which lie in
+// one word.  (The loads of all the digits are in flight together.)
+template <int N>
+struct RowBins {
+  uint32_t all[N][2], mine[N][2];
+
+  __device__ __forceinline__ void load(const SelectArgs& p, const SelectRow& r, int row, int chunk) {
+    const uint32_t* hist = reinterpret_cast<const uint32_t*>(chunk_hist(p, row, 0, 0)) + kBins / 2 - 1 - int(threadIdx.x);
+    const int n = (r.len + kChunk - 1) / kChunk;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t bin = uint32_t(kBins - 1 - 2 * int(threadIdx.x) - i);
-    above += bin > g.bin ? mine[i] : 0u;
-    at += bin == g.bin ? mine[i] : 0u;
+    for (int d = 0; d < N; ++d) all[d][0] = all[d][1] = mine[d][0] = mine[d][1] = 0;
+#pragma unroll 8
+    for (int c = 0; c < n; ++c) {
+#pragma unroll
+      for (int d = 0; d < N; ++d) {
+        const uint32_t w = hist[(int64_t(c) * kDigits + d) * (kBins / 2)];
+        all[d][0] += w >> 16;
+        all[d][1] += w & 0xFFFFu;
+        mine[d][0] += c < chunk ? w >> 16 : 0u;
+        mine[d][1] += c < chunk ? w & 0xFFFFu : 0u;
+      }
+    }
   }
-  __syncthreads();  // the pick is read by all before it is made again
-  return g;
-}
+  // Finds digit d's bin of the left-th key; above and at: how many keys of the
+  // chunks before this one are above that bin (added) and in it.
+  __device__ __forceinline__ Digit find(int d, uint32_t left, uint32_t* s_wave, uint32_t* s_pick, uint32_t& above,
+                                        uint32_t& at) const {
+    const Digit g = find_digit<kSelThreads>(all[d], left, s_wave, s_pick);
+    at = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t bin = uint32_t(kBins - 1 - 2 * int(threadIdx.x) - i);
+      above += bin > g.bin ? mine[d][i] : 0u;
+      at += bin == g.bin ? mine[d][i] : 0u;
+    }
+    __syncthreads();  // the pick is read by all before it is made again
+    return g;
+  }
+};
 
 template <int DIGIT>
 __global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))) chunk_digit_kernel(SelectArgs p) {
@@ -299,12 +311,17 @@ __global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_e
   if (r.want == 0 || chunk * kChunk >= r.len) return;
   Held<kSelThreads> held;
   held.load(r, chunk * kChunk);
-  uint32_t prefix = 0, left = r.want, above = 0, at;
+  uint32_t prefix = 0;
+  if constexpr (DIGIT > 0) {
+    RowBins<DIGIT> bins;
+    bins.load(p, r, row, chunk);
+    uint32_t left = r.want, above = 0, at;
 #pragma unroll
-  for (int d = 0; d < DIGIT; ++d) {
-    const Digit g = row_digit(p, r, row, chunk, d, left, s_wave, s_pick, above, at);
-    prefix |= g.bin << digit_shift(d);
-    left -= g.above;
+    for (int d = 0; d < DIGIT; ++d) {
+      const Digit g = bins.find(d, left, s_wave, s_pick, above, at);
+      prefix |= g.bin << digit_shift(d);
+      left -= g.above;
+    }
   }
   digit_histogram<kSelThreads>(held, DIGIT, prefix, s_hist);
   const uint32_t w = (s_hist[2 * threadIdx.x + 1] << 16) | s_hist[2 * threadIdx.x];  // (at most kChunk each)
@@ -327,9 +344,11 @@ __global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_e
   // those of higher bins that agree before it) and at it.
   uint32_t prefix = 0, left = r.want, above = 0, at = 0;
   if (r.want > 0) {
+    RowBins<kDigits> bins;
+    bins.load(p, r, row, chunk);
 #pragma unroll
     for (int d = 0; d < kDigits; ++d) {
-      const Digit g = row_digit(p, r, row, chunk, d, left, s_wave, s_pick, above, at);
+      const Digit g = bins.find(d, left, s_wave, s_pick, above, at);
       prefix |= g.bin << digit_shift(d);
       left -= g.above;
     }
