@@ -44,6 +44,8 @@ constexpr int kChunk = kSelThreads * kPer;
 constexpr int kSmallThreads = 256;
 constexpr int kBins = 2048;                     // of the first two digits; half of the third's are used
 constexpr int kDigits = 3;
+constexpr int kCopies = 2;                      // counters of a bin in LDS (see digit_histogram)
+using Copies = uint32_t __attribute__((ext_vector_type(kCopies)));
 constexpr int kMaxChunks = 4096;                // of one round of launches: bounds the workspace
 
 __device__ __forceinline__ constexpr int digit_shift(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
@@ -136,18 +138,28 @@ struct Held {
 };
 
 // The digit histogram of the held keys that agree with `prefix` above it (places
-// without a token have the least key, which is never reached).  Ends with a barrier.
+// without a token have the least key, which is never reached), kCopies counters a
+// bin, lanes in turn: additions to one place wait for each other.  512 rows of 12288
+// and their moves, scores apart / all equal, us: one counter 123 / 188, two 123 / 152,
+// four 125 / 136, eight 134 / 137.  Ends with a barrier.
 template <int NT>
-__device__ __forceinline__ void digit_histogram(const Held<NT>& held, int digit, uint32_t prefix, uint32_t* hist) {
+__device__ __forceinline__ void digit_histogram(const Held<NT>& held, int digit, uint32_t prefix, Copies* hist) {
   const int shift = digit_shift(digit), over = digit == 0 ? 31 : digit_shift(digit - 1);
-  const uint32_t mask = digit == 2 ? 1023u : 2047u;
-  for (int i = int(threadIdx.x); i < kBins; i += NT) hist[i] = 0;
+  const uint32_t mask = digit == 2 ? 1023u : 2047u, copy = threadIdx.x & (kCopies - 1);
+  for (int i = int(threadIdx.x); i < kBins; i += NT) hist[i] = Copies(0);
   __syncthreads();
   held.each([&](int k, int) {
     const uint32_t key = held.key[k];
-    if (digit == 0 || ((key ^ prefix) >> over) == 0) atomicAdd(&hist[(key >> shift) & mask], 1u);
+    if (digit == 0 || ((key ^ prefix) >> over) == 0)
+      atomicAdd(reinterpret_cast<uint32_t*>(hist) + ((key >> shift) & mask) * kCopies + copy, 1u);
   });
   __syncthreads();
+}
+__device__ __forceinline__ uint32_t bin_count(const Copies& c) {
+  uint32_t n = c[0];
+#pragma unroll
+  for (int i = 1; i < kCopies; ++i) n += c[i];
+  return n;
 }
 
 // The bin, from the top, that the left-th key falls in, and the keys above it;
@@ -231,7 +243,7 @@ template <int NT>
 __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == kSelThreads ? 8 : 6)))
 select_row_kernel(SelectArgs p) {
   constexpr int PER = kBins / NT;
-  __shared__ uint32_t s_hist[kBins];
+  __shared__ Copies s_hist[kBins];
   __shared__ uint32_t s_wave[NT / 64], s_count[2][NT / 64], s_pick[2];
   const int tid = int(threadIdx.x), row = p.row0 + int(blockIdx.x);
   const SelectRow r = select_row(p, row);
@@ -244,7 +256,7 @@ select_row_kernel(SelectArgs p) {
     digit_histogram<NT>(held, d, prefix, s_hist);
     uint32_t n[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) n[i] = s_hist[kBins - 1 - PER * tid - i];
+    for (int i = 0; i < PER; ++i) n[i] = bin_count(s_hist[kBins - 1 - PER * tid - i]);
     const Digit g = find_digit<NT>(n, left, s_wave, s_pick);
     prefix |= g.bin << digit_shift(d);
     left -= g.above;
@@ -304,7 +316,7 @@ struct RowBins {
 
 template <int DIGIT>
 __global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(4))) chunk_digit_kernel(SelectArgs p) {
-  __shared__ uint32_t s_hist[kBins];
+  __shared__ Copies s_hist[kBins];
   __shared__ uint32_t s_wave[kSelThreads / 64], s_pick[2];
   const int chunk = int(blockIdx.x), row = int(blockIdx.y);
   const SelectRow r = select_row(p, p.row0 + row);
@@ -324,7 +336,7 @@ __global__ void __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_e
     }
   }
   digit_histogram<kSelThreads>(held, DIGIT, prefix, s_hist);
-  const uint32_t w = (s_hist[2 * threadIdx.x + 1] << 16) | s_hist[2 * threadIdx.x];  // (at most kChunk each)
+  const uint32_t w = (bin_count(s_hist[2 * threadIdx.x + 1]) << 16) | bin_count(s_hist[2 * threadIdx.x]);  // (at most kChunk each)
   reinterpret_cast<uint32_t*>(chunk_hist(p, row, chunk, DIGIT))[threadIdx.x] = w;
 }
 
