@@ -429,8 +429,8 @@ int64_t psk_paged_prefill_step_workspace_len(int64_t num_seqs, int64_t total_q, 
  * seq_lens, sizes the launch and chooses its form (the results' last bits may
  * differ between forms; a longer sequence is read whole all the same).  out rows
  * need 4-element alignment.  workspace: device floats,
- * psk_paged_tree_workspace_len() of them (0 for a max_seq_len of at most 1536), no
- * initial contents needed.
+ * psk_paged_tree_workspace_len() of them (0 where a max_seq_len of at most 1536
+ * leaves nothing to merge), no initial contents needed.
  */
 int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int q_dtype,
                              const void* k_cache, const void* v_cache, const int64_t* k_strides,

@@ -74,7 +74,8 @@ constexpr int kWholeKeys = 1536;
 // most.  This kernel / that one, us (32 query heads): 4 sequences of 30000 keys over
 // 4 kv heads, 24 tokens each 75 / 80, 32: 88 / 87, 48: 126 / 120, 64: 157 / 134; 16 of
 // 8000 over 8, 32 tokens 95 / 110, 48: 157 / 138; 32 of 2000, 32 tokens 64 / 60, 48:
-// 100 / 74; one of 16000, 64 tokens 38 / 55.
+// 100 / 74; one of 16000, 64 tokens 38 / 55; uncut (kWholeKeys), 64 of 1500 over 4 kv
+// heads, 24 tokens 73 / 74, 32: 87 / 72; 128 of 500 over 8, 60 tokens 216 / 141.
 constexpr int kWideRows = 192;
 constexpr int64_t kWideWork = 80000000;
 constexpr int kPages = 1024;               // page ids a piece stages at a time
@@ -654,10 +655,11 @@ int64_t psk_paged_tree_workspace_len(int64_t num_seqs, int64_t total_q, int64_t 
   if (num_seqs < 0 || total_q < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
       max_seqlen_q <= 0 || max_seqlen_q > INT32_MAX / (num_q_heads / num_kv_heads) || max_seq_len < 0)
     return PSK_E_ARG;
-  if (max_seq_len <= kWholeKeys) return 0;
+  const bool wide = wide_step(num_seqs, total_q, num_q_heads, num_kv_heads, max_seq_len);
+  if (max_seq_len <= kWholeKeys) return wide ? prefill_runs_words() : 0;
   const TreeShape s = tree_shape(max_seqlen_q * (num_q_heads / num_kv_heads), kMaxSlots);
   const int64_t own = 4 + s.max_runs * s.row_blocks * 2 * kSlab;
-  return wide_step(num_seqs, total_q, num_q_heads, num_kv_heads, max_seq_len) ? std::max(own, prefill_runs_words()) : own;
+  return wide ? std::max(own, prefill_runs_words()) : own;
 }
 
 int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int q_dtype,
@@ -730,7 +732,7 @@ int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head
   p.s.width = INT32_MAX;
   p.row_blocks = int32_t(s.row_blocks);
   p.whole = max_seq_len <= kWholeKeys;
-  if (!p.whole && wide_step(num_seqs, total_q, num_q_heads, num_kv_heads, max_seq_len) && shares_pages(a) &&
+  if (wide_step(num_seqs, total_q, num_q_heads, num_kv_heads, max_seq_len) && shares_pages(a) &&
       2 * num_kv_heads <= prefill_cus())
     return launch_tree_runs(a, TreeStep{tree_mask, tree_mask_stride, p.scale_log2, int32_t(total_q)}, num_seqs, q_dtype,
                             out_dtype, reinterpret_cast<int32_t*>(workspace), static_cast<hipStream_t>(stream));

@@ -404,3 +404,17 @@ def test_wide_other_stream_and_graph_replay(dev):
         gr.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(lse, lse_want)
+
+
+def test_wide_trees_over_short_contexts(dev):
+    """A table of at most 1536 keys, and enough query rows for the wide form."""
+    rng = np.random.default_rng(8)
+    counts = [int(x) for x in rng.integers(50, 70, 16)]
+    counts[4] = 0
+    lens = [c + int(x) for c, x in zip(counts, rng.integers(0, 60, 16))]
+    lens[7] = counts[7] - 5
+    case = Case(dev, 97, lens, counts, 64, 2, 16, spare_table=96 - -(-max(lens) // 16))
+    assert sum(counts) * 64 * 1536 >= 8e7
+    assert attention.tree_workspace_floats(16, case.TQ, case.max_q, 64, 2, 1536) > 0
+    mask = _trees(case, 3)
+    _check(case, mask, *_run(case, mask, dev))
