@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_p
     const int full = lane_value(seqs.len, b - seqs.b0), L = min(full, p.s.width);
     const int unit = int(uniform_div(x - before, s.heads)), h = int(x - before) - unit * s.heads;
     const int k0 = unit * (1 << s.step_shift) + group * kTile;  // the wave's keys
-    const int R = r.n * G, ctx = full - r.n;
+    const int ctx = full - r.n;
 
     // lane l: of keys l % 32 the 16-byte chunks 2 q + l / 32 (the queries' the same);
     // missing rows and keys past the end as zeros
