@@ -45,9 +45,8 @@ constexpr int kPages = 1024; // page ids staged at a time (few rows)
 constexpr int kFewRows = 64;   // query rows of a job's heads, each padded to whole groups (few rows)
 constexpr int kManyWaves = 8;  // (many rows)
 constexpr int kManyRing = 2;   // row tiles a wave has in LDS (many rows)
-constexpr int kStepShift = 7;
-constexpr int kStepKeys = kTile * kWaves;  // of a step (few rows): a tile a wave
-static_assert(kStepKeys == 1 << kStepShift, "");
+constexpr int kStepTiles = 4;  // of a step (few rows)
+constexpr int kStepKeys = kTile * kStepTiles;
 
 struct WeightArgs {
   DecodeArgs a;
@@ -178,7 +177,7 @@ few_rows_kernel(WeightArgs args) {
       }
       __syncthreads();
 
-      const int t_end = min(kWaves * s1, n_tiles);
+      const int t_end = min(kStepTiles * s1, n_tiles);
       struct Place {
         int t, hh;  // tile and head of the group
       };
@@ -191,7 +190,7 @@ few_rows_kernel(WeightArgs args) {
       };
       // Where the eight keys of a load lie: lane 4 k + u those of load u of tile
       // win + k, sixteen tiles at a time (GEN: every lane its own key's place).
-      int win = kWaves * s0;
+      int win = kStepTiles * s0;
       int64_t at_k = 0;
       uint64_t whole8 = 0, some8 = 0;  // loads whose eight keys are all cached; whose first is
       auto look_up = [&](int t) {
@@ -292,7 +291,7 @@ few_rows_kernel(WeightArgs args) {
         // every read of the slot is done before its next loads start
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       };
-      Place now{kWaves * s0, 0};
+      Place now{kStepTiles * s0, 0};
       next(now, wave);
       Place then = now;  // the pair whose loads are started next
       int flying = 0;    // pairs whose loads are in flight
@@ -693,9 +692,11 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
   const int64_t cus = weight_cus();
   const int64_t rows = max_seqlen_q * a.heads;
   if (rows <= kRows) {
-    p.s.step_shift = kStepShift;
+    p.s.step_shift = log2_exact(kStepKeys);
+    // (64 / 16 sequences of 500 / 2000, us: runs of at least one unit 17 / 16, two 22 / 21;
+    // 256 of 300, a job's start priced as one 27, two 33)
     p.s.over = 1;
-    p.s.min_run = 2;
+    p.s.min_run = 1;
     p.s.max_runs = int32_t(2 * cus);  // resident at once
     p.hg = int32_t(std::min<int64_t>(num_kv_heads, kFewRows / (8 * ceil_div(rows, 8))));
     p.s.heads = int32_t(ceil_div(num_kv_heads, p.hg));
