@@ -64,6 +64,10 @@ constexpr int kRing = 2;
 // units (of kStepKeys keys) that a piece costs beside its keys: 1, 4, 6, 12 gave 35.5,
 // 29.7, 28.4, 27.4 us for the ragged trees above and 113, 114, 114, 120 for the 32
 constexpr int kOver = 6;
+// units a run has at least: a shorter one is another record to merge.  2, 4, 8, 12 gave
+// 20, 19, 20, 22 us for 8 tokens over 4000 keys (8 heads over one), 36, 30, 26, 26 over
+// 16000 (32 over 8) and 43, 43, 31, 29 for 30 tokens over 30000 (8 over one)
+constexpr int kMinRun = 8;
 // Up to this many keys a workgroup takes all of a job's and nothing is merged: four
 // sequences of 8 tokens (32 query heads over 8), us, whole / cut: 1000 keys 17 / 19, 1600
 // 19 / 19, 2500 24 / 21; 64 sequences of 1000, 32 / 38.
@@ -728,7 +732,7 @@ int psk_paged_tree_attention(const void* q, int64_t q_tok_stride, int64_t q_head
   p.s.step_shift = kStepShift;
   p.s.over = kOver;
   p.s.max_runs = int32_t(s.max_runs);
-  p.s.min_run = 2;
+  p.s.min_run = kMinRun;
   p.s.width = INT32_MAX;
   p.row_blocks = int32_t(s.row_blocks);
   p.whole = max_seq_len <= kWholeKeys;
