@@ -64,10 +64,11 @@ constexpr int kRing = 2;
 // units (of kStepKeys keys) that a piece costs beside its keys: 1, 4, 6, 12 gave 35.5,
 // 29.7, 28.4, 27.4 us for the ragged trees above and 113, 114, 114, 120 for the 32
 constexpr int kOver = 6;
-// units a run has at least: a shorter one is another record to merge.  2, 4, 8, 12 gave
-// 20, 19, 20, 22 us for 8 tokens over 4000 keys (8 heads over one), 36, 30, 26, 26 over
-// 16000 (32 over 8) and 43, 43, 31, 29 for 30 tokens over 30000 (8 over one)
-constexpr int kMinRun = 8;
+// units a run has at least: a shorter one is another record to merge.  4, 6, 8 gave 19,
+// 20, 20 us for 8 tokens over 4000 keys (8 heads over one), 21, 21, 22 over 16000 (32
+// over 8), 26, 25, 23 for 30 tokens over 30000 (8 over one) and 22, 28, 23 for 16
+// trees of 8 over 100 to 4000
+constexpr int kMinRun = 4;
 // Up to this many keys a workgroup takes all of a job's and nothing is merged: four
 // sequences of 8 tokens (32 query heads over 8), us, whole / cut: 1000 keys 17 / 19, 1600
 // 19 / 19, 2500 24 / 21; 64 sequences of 1000, 32 / 38.
@@ -540,18 +541,22 @@ tree_attention_kernel(TreeArgs args) {
   }
 }
 
-// The records of a job joined: a wave per task (job, 32 rows, 8 columns).
+// The records of a job joined: a workgroup per 32 rows and 32 columns of a job.  Its
+// waves take the records in turn, so that as many as possible are in flight, and
+// then a group of 8 columns each, over the four parts in order.
 template <int OUT_DT>
 __global__ void __launch_bounds__(256) merge_tree_kernel(TreeArgs p) {
   const DecodeArgs& a = p.a;
+  __shared__ f32x4 s_o[4][4][64];
+  __shared__ float s_m[4][kRows], s_l[4][kRows];
   const int lane = int(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
   const int kk = lane & 31;
-  const uint32_t tasks = uint32_t(p.s.num_seqs) * uint32_t(p.s.heads) * uint32_t(p.row_blocks) * 16;  // (host: below 2^28)
-  for (uint32_t task = blockIdx.x * 4 + wave; task < tasks; task += gridDim.x * 4) {
-    // column group q of row block `block` of job (b, h)
-    const int q = int(task & 15);
-    const uint32_t rest = task >> 4, job = rest / uint32_t(p.row_blocks);
+  const uint32_t tasks = uint32_t(p.s.num_seqs) * uint32_t(p.s.heads) * uint32_t(p.row_blocks) * 4;  // (host: below 2^26)
+  for (uint32_t task = blockIdx.x; task < tasks; task += gridDim.x) {
+    // column groups 4 c .. 4 c + 3 of row block `block` of job (b, h)
+    const int c = int(task & 3);
+    const uint32_t rest = task >> 2, job = rest / uint32_t(p.row_blocks);
     const int block = int(rest - job * uint32_t(p.row_blocks));
     const int b = int(job / uint32_t(p.s.heads)), h = int(job - uint32_t(b) * uint32_t(p.s.heads));
     const SeqRows r = seq_rows(a, p.s.total_q, b);
@@ -566,30 +571,53 @@ __global__ void __launch_bounds__(256) merge_tree_kernel(TreeArgs p) {
     if (j0 == j1) continue;  // one run had all the keys and wrote the rows
 
     float top = kNegBig, sum = 0.0f;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int kAhead = 4;  // records read together
-    for (int64_t j = j0; j <= j1; j += kAhead) {
+    f32x4 o[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kAhead = 2;  // records of a wave read together
+    for (int64_t j = j0 + wave; j <= j1; j += 4 * kAhead) {
       float m[kAhead], l[kAhead];
-      f32x4 v[kAhead];
+      f32x4 v[kAhead][4];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int64_t k = min(j + u, j1);
+        const int64_t k = min(j + 4 * u, j1);
         const float* rec = record(p, k, block, k == j0 ? 1 : 0);
         m[u] = rec[4096 + kk];
         l[u] = rec[4096 + 32 + kk];
-        v[u] = *reinterpret_cast<const f32x4*>(rec + (q * 64 + lane) * 4);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[u][q] = *reinterpret_cast<const f32x4*>(rec + ((4 * c + q) * 64 + lane) * 4);
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        if (j + u > j1) break;
+        if (j + 4 * u > j1) break;
         const float up = __builtin_fmaxf(top, m[u]);
         const float f0 = __builtin_amdgcn_exp2f(top - up), f1 = __builtin_amdgcn_exp2f(m[u] - up);
         top = up;
         sum = sum * f0 + l[u] * f1;
-        o = o * f0 + v[u] * f1;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[q] = o[q] * f0 + v[u][q] * f1;
       }
     }
-    finish<OUT_DT>(p, r, b, h, row, q, lane, o, top, sum);
+    __syncthreads();  // the last task's readers are done
+    if (lane < kRows) {
+      s_m[wave][lane] = top;
+      s_l[wave][lane] = sum;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) s_o[wave][q][lane] = o[q];
+    __syncthreads();
+    top = s_m[0][kk];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = __builtin_fmaxf(top, s_m[w][kk]);
+    sum = 0.0f;
+    o[0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(s_m[w][kk] - top);
+      sum += s_l[w][kk] * f;
+      o[0] += s_o[w][wave][lane] * f;
+    }
+    finish<OUT_DT>(p, r, b, h, row, 4 * c + wave, lane, o[0], top, sum);
   }
 }
 
@@ -631,7 +659,7 @@ int launch_tree(const TreeArgs& p, bool general, hipStream_t st) {
   if (general) hipLaunchKernelGGL((tree_attention_kernel<Q_DT, OUT_DT, true>), grid, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((tree_attention_kernel<Q_DT, OUT_DT, false>), grid, dim3(kThreads), 0, st, p);
   if (const int e = check_launch("tree_attention_kernel launch"); e != PSK_OK || p.whole) return e;
-  const int64_t groups = std::min<int64_t>(jobs * p.row_blocks * 4, 1 << 20);  // of four tasks
+  const int64_t groups = std::min<int64_t>(jobs * p.row_blocks * 4, 1 << 20);
   hipLaunchKernelGGL((merge_tree_kernel<OUT_DT>), dim3(unsigned(groups)), dim3(256), 0, st, p);
   return check_launch("merge_tree_kernel launch");
 }
