@@ -249,8 +249,9 @@ def evict_tokens(
         budget - sink - recent of the highest scores; ties go to the lower
         position, a NaN score counts below every other.
     Kept token i, in position order, becomes row i of the pages
-    ``dst_block_table[b]`` (int32 [B, W], at least budget rows; entries outside
-    the cache are skipped, a source row on a missing page reads as zeros).
+    ``dst_block_table[b]`` (int32 [B, W], rows for the budget or for ``width``
+    tokens, whichever are fewer; entries outside the cache are skipped, a source
+    row on a missing page reads as zeros).
     Those pages must be none that ``block_table`` names, each named once: prefix
     pages may be shared by sequences, so they are read and left as they are.
     ``scores_out`` (default: ``scores``, in place; else it shares no element with
@@ -294,8 +295,9 @@ def evict_tokens(
     # (all that a launch would refuse, so that none follows one that has written)
     assert 1 <= layers <= 65535 and B <= 65535 and budget * heads < 2 ** 31, \
         f"{layers} layers, {B} sequences, a budget of {budget} for {heads} heads"
-    assert num_blocks >= 1 and page >= 1 and (block_table.shape[1] >= 1 or B == 0), "an empty cache or block table"
-    assert dst_block_table.shape[1] * page >= budget, \
+    assert num_blocks >= 1 and page >= 1 and (B == 0 or block_table.shape[1] >= 1 and dst_block_table.shape[1] >= 1), \
+        "an empty cache or block table"
+    assert dst_block_table.shape[1] * page >= min(budget, width), \
         f"{dst_block_table.shape[1]} pages of {page} cannot hold a budget of {budget}"
     assert block_table.data_ptr() != dst_block_table.data_ptr() or B == 0, "the kept tokens go to pages of their own"
     kept = torch.empty(layers, B, kept_heads, budget, dtype=torch.int32, device=device)

@@ -341,3 +341,13 @@ def test_eviction_refuses_before_it_writes(dev):
 def test_a_path_that_names_a_token_twice(dev):
     """Both rows get the token's; one that stays where it is, is left."""
     _commit(dev, 5, (2, 40, 2, 16, 2, 128), torch.float8_e4m3fn, [5, 33], [[3, 3, 0, 2], [0, 1, 1, 7]], [4, 3], _FUSED)
+
+
+@pytest.mark.parametrize("shared", [True, False])
+def test_a_budget_past_every_length_needs_pages_for_the_tokens_alone(dev, shared):
+    e = Evict(12, 2, [30, 20, 0], 100, 16, shared=shared)  # scores of 33 places
+    e.dst = e.dst[:, :3].contiguous()
+    e.check(dev, 4, 8)
+    e.dst = e.dst[:, :2].contiguous()
+    with pytest.raises(AssertionError, match="cannot hold"):
+        e.check(dev, 4, 8)
