@@ -122,6 +122,11 @@ __device__ __forceinline__ uint32_t visible(const int64_t* m, int ctx, int n, in
   return uint32_t(bits) & in;
 }
 
+// A tree row's running maximum is raised to this much (log2) below the largest weight:
+// its weights have to stay below 2^16 only, and those of keys far below count in fp16
+// down to 2^-33 of the largest, not 2^-25 (the sum counts them all).
+constexpr float kHeadRoom = 8.0f;
+
 // Bit 0 of every byte of x that is an e4m3 NaN.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {
   return (((x & 0x7F7F7F7Fu) + 0x01010101u) >> 7) & 0x01010101u;

@@ -598,7 +598,7 @@ prefill_runs_kernel(RunArgs p) {
       for (int i = 0; i < 16; ++i) v = __builtin_fmaxf(v, sees(key0, i) ? y[i] : -__builtin_inff());
       v *= sl;
       v = __builtin_fmaxf(v, __shfl_xor(v, 32));
-      return live ? __builtin_fmaxf(v, kNegBig) : kBig;
+      return live ? __builtin_fmaxf(TREE ? v - kHeadRoom : v, kNegBig) : kBig;
     };
     // P of two keys (elements i, i + 1) of a tile in fp16 (RNE, relative error
     // <= 2^-11 from 2^-14 up), and their sums

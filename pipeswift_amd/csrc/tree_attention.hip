@@ -24,7 +24,8 @@
 //   * a key's 128 bytes lie in a slot as eight 16-byte chunks, chunk c of key t at
 //     c ^ (t & 7), which spreads both kinds of reads over the banks.
 // A row's maximum is raised only when the weights of a tile pass 2^15 in sum, so
-// that every weight is a finite fp16 value and the common path has no rescale.
+// that every weight is a finite fp16 value and the common path has no rescale, and to
+// kHeadRoom below the tile's largest.
 //
 // The work is cut into equal runs over sequences and kv heads (cached_queries.h).
 // A run's piece that is not all of a job's keys leaves a partial record (maxima,
@@ -444,7 +445,7 @@ tree_attention_kernel(TreeArgs args) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, sees(i) ? y[i] : -__builtin_inff());
           top *= sl;
-          top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+          top = __builtin_fmaxf(top, __shfl_xor(top, 32)) - kHeadRoom;
           const float mn = live ? __builtin_fmaxf(m, top) : m;
           const float f = __builtin_amdgcn_exp2f(m - mn);
           m = mn;

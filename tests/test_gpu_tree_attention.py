@@ -418,3 +418,60 @@ def test_wide_trees_over_short_contexts(dev):
     assert attention.tree_workspace_floats(16, case.TQ, case.max_q, 64, 2, 1536) > 0
     mask = _trees(case, 3)
     _check(case, mask, *_run(case, mask, dev))
+
+
+# --------------------------------------------------------------------------- #
+# what P V loses of the weights
+# --------------------------------------------------------------------------- #
+#
+# A weight is rounded once to fp16 (r = 2^-11 of itself), whose least step is 2^-24; a
+# row's largest weight is at least 2^8 where its maximum was last raised, so a weight is
+# also off by 2^-25 of 2^-8 times the largest: 2^-33 of the row's sum.  With S = sum
+# p |V| vd and vmax the largest |V vd|,
+#   |out - exact| <= S (2 d + r + (K + 64) eps) + K 2^-33 vmax,
+# beside the output's own rounding.  Where every q~ . K is an exact float32 (small
+# integers), d = eps (8 max(|s|, 1) + 4 (1 + 2 max|s|) + K).
+
+
+def _check_weights(case, mask, got, scale, most, r=2.0 ** -11):
+    q, k, v = case.host()
+    args = (case.bt.numpy(), case.lens, mask.numpy(), case.cu, scale, *case.ds)
+    want, _, _ = T.tree_attention(q, case.name, k, v, *args)
+    size, _, _ = T.tree_attention(q, case.name, k, v & 0x7F, *args)
+    K = max([1, *case.lens])
+    d = EPS * (8 * max(most, 1.0) + 4 * (1 + 2 * most) + K)
+    vmax = float(np.abs(O.e4m3fn_to_f32(v)).max())
+    tol = size * (2 * d + r + (K + 64) * EPS) + K * 2.0 ** -33 * vmax
+    tol = tol + np.abs(want) * (2.0 ** -8 if got.dtype == torch.bfloat16 else 4 * EPS)
+    o = got.double().cpu().numpy()
+    assert np.isfinite(o[:case.rows]).all()
+    err = np.abs(o - want)[:case.rows]
+    assert (err <= tol[:case.rows]).all(), f"{(err / tol[:case.rows]).max():.3g} of the bound"
+
+
+# (drafted tokens, Hq, Hkv, page, wide): uncut, cut (pages shared by a load or not), the prefill kernel's form
+_FORMS = [(3, 8, 2, 16, False), (3, 8, 1, 16, True), (3, 8, 1, 24, True), (40, 8, 1, 16, True)]
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,Hq,Hkv,ps,wide", _FORMS)
+def test_weights_far_below_the_largest_add_up(dev, n, Hq, Hkv, ps, wide, out_dtype):
+    """A first key 2^26 above all others, whose values alone are not zero."""
+    L = 1400 if not wide else 3000
+    spare = _room(ps, [n] * 2, Hq) if wide else 0
+    case = Case(dev, 6, [L + n, L + n + 45], [n, n], Hq, Hkv, ps, descales=False, spare_table=spare)
+    case.q = torch.zeros_like(case.q)
+    case.q[:, :, 0] = 1
+    case.fused = torch.zeros_like(case.fused, dtype=torch.float32)
+    case.fused[:, 1] = 1.0
+    for b in range(2):
+        case.fused[int(case.bt[b, 0]), 0, 0, :, 0] = 1.0
+        case.fused[int(case.bt[b, 0]), 1, 0] = 0.0
+    case.fused = case.fused.to(torch.float8_e4m3fn)
+    case.qd.copy_(case.q)
+    case.k.copy_(case.fused[:, 0].to(dev))
+    case.v.copy_(case.fused[:, 1].to(dev))
+    mask = _trees(case, 2)
+    scale = 26 * np.log(2.0)
+    got, _ = _run(case, mask, dev, out_dtype=out_dtype, scale=scale)
+    _check_weights(case, mask, got, scale, scale)
