@@ -427,8 +427,9 @@ int64_t psk_paged_prefill_step_workspace_len(int64_t num_seqs, int64_t total_q, 
  * tree_mask_words words of 64 tokens each hold max_seqlen_q tokens at least.  A
  * token that sees no key writes zeros and lse = -inf.  max_seq_len, a bound on
  * seq_lens, sizes the launch and chooses its form (the results' last bits may
- * differ between forms; a longer sequence is read whole all the same).  out rows
- * need 4-element alignment.  workspace: device floats,
+ * differ between forms; a longer sequence is read whole all the same).  P V has
+ * a weight rounded once to fp16 for a bf16 out, and as the sum of two fp16 for a
+ * float32 one.  out rows need 4-element alignment.  workspace: device floats,
  * psk_paged_tree_workspace_len() of them (0 where a max_seq_len of at most 1536
  * leaves nothing to merge), no initial contents needed.
  */

@@ -383,8 +383,9 @@ def paged_tree_attention(
     ``tree_mask[row, t // 64]`` is set (int64 [total_q, words], or [total_q] for
     trees of at most 64; bits at or past n are ignored).  ``tree_mask()`` makes
     it of the tokens' parents.  A token that sees no key gets zeros and
-    lse -inf.  P V runs on the fp16 MFMA with P rounded once to fp16, as in
-    ``paged_prefill_attention``.
+    lse -inf.  P V runs on the fp16 MFMA: for a bf16 ``out`` with P rounded once
+    to fp16, as in ``paged_prefill_attention``; for a float32 one with P as the
+    sum of two fp16 (2^-22 of a weight).
 
     ``max_seq_len``: a bound on seq_lens where the caller has a closer one than
     the block table's width; it sizes the launch and chooses its form, and a

@@ -276,6 +276,8 @@ __device__ __forceinline__ void lds_barrier() {
 template <int Q_DT, int OUT_DT, bool GEN, bool TREE = false>
 __global__ void __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2)))
 prefill_runs_kernel(RunArgs p) {
+  constexpr bool kPairs = TREE && OUT_DT == PSK_DTYPE_F32;  // P as the sum of two fp16 (tree_attention.hip)
+  constexpr int kPWords = kPairs ? 16 : 8;                  // of a tile's weights
   const DecodeArgs& a = p.a;
   __shared__ __attribute__((aligned(1024))) char s_lds[kPfRaws * kPfRaw + kPfBufs * kPfStage];
   __shared__ int64_t s_prefix[kOrderMax + 1];  // every workgroup scans the sequences' costs
@@ -602,7 +604,7 @@ prefill_runs_kernel(RunArgs p) {
     };
     // P of two keys (elements i, i + 1) of a tile in fp16 (RNE, relative error
     // <= 2^-11 from 2^-14 up), and their sums
-    auto weigh = [&](auto masked_tag, const f32x16& y, int key0, int i, float& s0, float& s1, uint32_t (&pw)[8]) {
+    auto weigh = [&](auto masked_tag, const f32x16& y, int key0, int i, float& s0, float& s1, uint32_t (&pw)[kPWords]) {
       constexpr bool MASKED = decltype(masked_tag)::value;
       float e0 = __builtin_fmaf(y[i], sl, -m), e1 = __builtin_fmaf(y[i + 1], sl, -m);
       if (MASKED && !sees(key0, i)) e0 = -__builtin_inff();
@@ -610,7 +612,17 @@ prefill_runs_kernel(RunArgs p) {
       const float p0 = __builtin_amdgcn_exp2f(e0), p1 = __builtin_amdgcn_exp2f(e1);
       s0 += p0;
       s1 += p1;
-      pw[i / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{p0, p1}), f16x2));
+      const f16x2 ph = __builtin_convertvector((f32x2{p0, p1}), f16x2);
+      pw[i / 2] = __builtin_bit_cast(uint32_t, ph);
+      if constexpr (kPairs)
+        pw[8 + i / 2] = __builtin_bit_cast(uint32_t, f16x2{_Float16(__builtin_fmaf(float(ph[0]), -1.0f, p0)),
+                                                           _Float16(__builtin_fmaf(float(ph[1]), -1.0f, p1))});
+    };
+    // o += V^T P^T of step u of a tile (pv: its weights)
+    auto add_pv = [&](f16x8 v, const uint32_t (&pv)[kPWords], int u, f32x16& o) {
+      auto weights = [&](int i) { return __builtin_bit_cast(f16x8, u32x4{pv[i], pv[i + 1], pv[i + 2], pv[i + 3]}); };
+      if constexpr (kPairs) o = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, weights(8 + 4 * u), o, 0, 0, 0);
+      o = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, weights(4 * u), o, 0, 0, 0);
     };
     // One tile's step of the wave's pipeline, three independent strands that
     // fill the matrix and vector units together: the softmax of a tile (scores
@@ -620,8 +632,8 @@ prefill_runs_kernel(RunArgs p) {
     // reads of two groups on.  The order is fixed (sched_barrier): left alone,
     // the compiler reads each operand right before its MFMA and waits for it.
     // extra(c): more work for group c.
-    auto tile_step = [&](auto masked_tag, const f32x16& y, int key0, int k_tile, int v_tile, const uint32_t (&pv)[8],
-                         uint32_t (&pw)[8], const auto& extra) {
+    auto tile_step = [&](auto masked_tag, const f32x16& y, int key0, int k_tile, int v_tile, const uint32_t (&pv)[kPWords],
+                         uint32_t (&pw)[kPWords], const auto& extra) {
       u32x4 kw[8];
       f16x8 vw[8];
       auto read = [&](int c) {
@@ -643,8 +655,7 @@ prefill_runs_kernel(RunArgs p) {
         yn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kw[c]), qop[c], yn, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
         if (c < 7) weigh(masked_tag, y, key0, 2 * c + 2, s0, s1, pw);
-        const f16x8 pop = __builtin_bit_cast(f16x8, u32x4{pv[4 * u], pv[4 * u + 1], pv[4 * u + 2], pv[4 * u + 3]});
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vw[c], pop, o[d], 0, 0, 0);
+        add_pv(vw[c], pv, u, o[d]);
         extra(c);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -695,9 +706,9 @@ prefill_runs_kernel(RunArgs p) {
     uint32_t to = 2 * kPfStage;   // the buffer that stage t + 2 goes to
     uint32_t to_next = kPfStage;  // from the buffer of stage t to that of stage t + 1
     f32x16 y0 = {};
-    uint32_t p0[8], p1[8];  // weights of the stage's two tiles
+    uint32_t p0[kPWords], p1[kPWords];  // weights of the stage's two tiles
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p1[i] = 0u;  // before the first tile: zero weights (on that stage's own V)
+    for (int i = 0; i < kPWords; ++i) p1[i] = 0u;  // before the first tile: zero weights (on that stage's own V)
     if (busy) {
 #pragma unroll
       for (int c = 0; c < 8; ++c)
@@ -743,8 +754,7 @@ prefill_runs_kernel(RunArgs p) {
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         const int u = c >> 2, d = c & 3;
-        const f16x8 pop = __builtin_bit_cast(f16x8, u32x4{p1[4 * u], p1[4 * u + 1], p1[4 * u + 2], p1[4 * u + 3]});
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(load_v(1, u, d), pop, o[d], 0, 0, 0);
+        add_pv(load_v(1, u, d), p1, u, o[d]);
       }
     }
 

@@ -6,7 +6,10 @@
 // set.  Otherwise as the readers of paged_attention.hip and prefill_runs.hip:
 // q~ = e4m3(q / qd), s = softmax_scale qd kd (q~ . K), out = vd softmax(s) V,
 // lse = log sum exp s, Q K^T on the bf16 MFMA over exactly converted FP8
-// operands, P V on the fp16 MFMA with V exact and P rounded once, float32 sums.
+// operands, P V on the fp16 MFMA with V exact, float32 sums.  For a bf16 out P is
+// rounded once (2^-11, below what the output's own rounding leaves); for a float32 one
+// it is the sum of two fp16 (2^-22) and P V runs twice: 102 / 109 us for the 32 trees
+// below, 148 / 201 for four wide ones (prefill_runs.hip).
 //
 // The n G query rows of a kv head (G query heads each) are rows of MFMA tiles,
 // 32 to a workgroup.  Its four waves hold all of them and take the 32-key
@@ -164,6 +167,7 @@ __device__ __forceinline__ void finish(const TreeArgs& p, const SeqRows& r, int 
 template <int Q_DT, int OUT_DT, bool GEN>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 tree_attention_kernel(TreeArgs args) {
+  constexpr bool kPairs = OUT_DT == PSK_DTYPE_F32;  // P as fp16 pairs
   __shared__ __attribute__((aligned(1024))) char s_ring[kWaves * kRing * kSlot];
   __shared__ int32_t s_pages[kPages];
   __shared__ u32x4 s_q[kRows * 8];  // the rows' e4m3 queries, chunk c of row r at c ^ (r & 7)
@@ -457,16 +461,19 @@ tree_attention_kernel(TreeArgs args) {
         l += sum;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          uint32_t pw[4];
+          f16x8 pop, rest;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            pw[i] = __builtin_bit_cast(uint32_t,
-                                       __builtin_convertvector((f32x2{w[8 * u + 2 * i], w[8 * u + 2 * i + 1]}), f16x2));
-          const f16x8 pop = __builtin_bit_cast(f16x8, u32x4{pw[0], pw[1], pw[2], pw[3]});
+          for (int i = 0; i < 8; ++i) pop[i] = _Float16(w[8 * u + i]);
+          if constexpr (kPairs) {
 #pragma unroll
-          for (int d = 0; d < 4; ++d)
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(e4m3x8_to_f16(uint32_t(vraw[4 * u + d][0]), uint32_t(vraw[4 * u + d][1])),
-                                                          pop, o[d], 0, 0, 0);
+            for (int i = 0; i < 8; ++i) rest[i] = _Float16(__builtin_fmaf(float(pop[i]), -1.0f, w[8 * u + i]));
+          }
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const f16x8 v = e4m3x8_to_f16(uint32_t(vraw[4 * u + d][0]), uint32_t(vraw[4 * u + d][1]));
+            if constexpr (kPairs) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, rest, o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pop, o[d], 0, 0, 0);
+          }
         }
       };
 

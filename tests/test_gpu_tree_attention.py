@@ -475,3 +475,27 @@ def test_weights_far_below_the_largest_add_up(dev, n, Hq, Hkv, ps, wide, out_dty
     scale = 26 * np.log(2.0)
     got, _ = _run(case, mask, dev, out_dtype=out_dtype, scale=scale)
     _check_weights(case, mask, got, scale, scale)
+
+
+def _integers(case, dev, seed):
+    """Integer queries and keys: every q~ . K is an exact float32."""
+    g = torch.Generator().manual_seed(seed)
+    case.q = torch.randint(-1, 2, case.q.shape, generator=g).to(case.q.dtype)
+    case.fused[:, 0] = torch.randint(-2, 3, case.fused[:, 0].shape, generator=g).float().to(torch.float8_e4m3fn)
+    case.qd.copy_(case.q)
+    case.k.copy_(case.fused[:, 0].to(dev))
+    case.v.copy_(case.fused[:, 1].to(dev))
+
+
+@pytest.mark.parametrize("n,Hq,Hkv,ps,wide", _FORMS)
+def test_a_float32_out_has_both_halves_of_the_weights(dev, n, Hq, Hkv, ps, wide):
+    """P as the sum of two fp16, r = 2^-22; few keys a row, so that no rounding averages out."""
+    spare = _room(ps, [n] * 3, Hq) if wide else 0
+    case = Case(dev, 5, [n + 5, n + 2, n + 9], [n, n, n], Hq, Hkv, ps, descales=False, spare_table=spare)
+    _integers(case, dev, 1)
+    mask = torch.zeros(case.TQ, -(-n // 64), dtype=torch.int64)  # their contexts alone
+    scale = 0.02
+    most = float(np.abs(case.q.double().numpy()).sum(-1).max()) * 2 * scale
+    for dtype in (torch.float32, torch.bfloat16):
+        got, _ = _run(case, mask, dev, out_dtype=dtype, scale=scale)
+        _check_weights(case, mask, got, scale, most, r=2.0 ** -22 if dtype == torch.float32 else 2.0 ** -11)
