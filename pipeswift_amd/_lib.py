@@ -16,6 +16,7 @@ import ctypes
 import os
 import threading
 
+import numpy as np
 import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpipeswift_kv.so")
@@ -226,10 +227,46 @@ def i64_array(values) -> ctypes.Array:
     return (_I64x6 if n == 6 else ctypes.c_int64 * n)(*values)
 
 
-def distinct(t) -> bool:
-    """Whether a tensor that is written has no two elements in one place by a broadcast."""
-    strides = t.stride()
-    return 0 not in strides or all(s != 0 or n <= 1 for s, n in zip(strides, t.shape))
+def _row_starts(t):
+    """(first elements of a tensor's rows, sorted, by their places in memory; elements of a row).
+    A row is the last dimension where its stride is one, else a single element."""
+    shape, strides = list(t.shape), list(t.stride())
+    width = shape.pop() if shape and strides[-1] == 1 else 1
+    at = np.zeros(1, dtype=np.int64)
+    for n, s in zip(shape, strides):
+        at = (at[:, None] + np.arange(n, dtype=np.int64) * s).reshape(-1)
+    return np.sort(at), width
+
+
+def distinct(t, width: int = 0) -> bool:
+    """Whether no two elements of a tensor lie in one place (a broadcast, rows that
+    overlap); ``width``: with rows of at least as many elements."""
+    if t.is_contiguous() and (not width or width <= t.shape[-1]):
+        return True
+    inner = 0  # places that the dimensions so far span, less one
+    for s, n in sorted((s, n if s != 1 else max(n, width)) for s, n in zip(t.stride(), t.shape) if n > 1 or s == 1):
+        if n > 1 and s <= inner:
+            break
+        inner += s * (n - 1)
+    else:
+        return True
+    starts, own = _row_starts(t)
+    return len(starts) < 2 or int(np.diff(starts).min()) >= max(own, width)
+
+
+def overlap(a, b) -> bool:
+    """Whether two tensors of one element size share an element."""
+    apart = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if a.is_contiguous() and b.is_contiguous():
+        return -b.numel() < apart < a.numel() and 0 not in a.shape and 0 not in b.shape
+    if 0 in a.shape or 0 in b.shape:
+        return False
+    ends = [sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)) for t in (a, b)]
+    if apart > ends[0] or apart + ends[1] < 0:
+        return False
+    (x, wx), (y, wy) = _row_starts(a), _row_starts(b)
+    y = y + apart  # a row of b at y overlaps those of a at y - wx < x < y + wy
+    return bool((np.searchsorted(x, y - wx, "right") < np.searchsorted(x, y + wy, "left")).any())
 
 
 def ptr(t) -> int:

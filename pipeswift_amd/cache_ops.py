@@ -21,7 +21,7 @@ import threading
 import numpy as np
 import torch
 
-from ._lib import check, distinct, dtype_code, i64_array, lib, on_device, ptr, stream_handle
+from ._lib import check, distinct, dtype_code, i64_array, lib, on_device, overlap, ptr, stream_handle
 
 FP8_E4M3_MAX = 448.0
 
@@ -284,7 +284,8 @@ def evict_tokens(
         assert scores_out.dtype == torch.float32 and scores_out.device == device
         assert scores_out.dim() == 4 and scores_out.shape[:3] == shape[:3]
         assert out_strides[3] == 1 or out_width <= 1, "scores need unit last stride"
-    assert distinct(scores_out) and (out_strides == strides or scores_out.data_ptr() != scores.data_ptr()), \
+    in_place = scores_out is scores or (scores_out.data_ptr() == scores.data_ptr() and out_strides == strides)
+    assert distinct(scores_out, max(width, out_width)) if in_place else distinct(scores_out) and not overlap(scores, scores_out), \
         "scores_out must be scores itself or share no element with it, and be no broadcast"
     budget, sink, recent = int(budget), int(sink), int(recent)
     assert budget >= 1 and sink >= 0 and recent >= 0 and sink + recent <= budget, \

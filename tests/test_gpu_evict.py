@@ -351,3 +351,36 @@ def test_a_budget_past_every_length_needs_pages_for_the_tokens_alone(dev, shared
     e.dst = e.dst[:, :2].contiguous()
     with pytest.raises(AssertionError, match="cannot hold"):
         e.check(dev, 4, 8)
+
+
+@pytest.mark.parametrize("n", [300, 20000])
+def test_scores_out_beside_or_over_the_scores(dev, n):
+    """Rows between the scores' own are another tensor; views that share elements are refused."""
+    e = Evict(13, 2, [n, n // 2], 64, 16)
+    w = e.scores.shape[3]
+    buf = torch.full((16 * w + 8,), 9.0, device=dev)[:16 * w].view(2, 2, 2, 2 * w)
+    scores, other = buf[..., :w], buf[..., w:]
+    scores.copy_(e.scores)
+    cache = e.cache.to(dev)
+    args = dict(block_table=e.bt.to(dev), seq_lens=torch.tensor(e.lens, dtype=torch.int32, device=dev),
+                dst_block_table=e.dst.to(dev), budget=64, sink=4, recent=8)
+    kept, _ = cache_ops.evict_tokens(e.views(cache), scores, scores_out=other, **args)
+    ek, _ = T.select_tokens(e.scores.numpy(), e.lens, 64, 4, 8)
+    assert np.array_equal(kept.cpu().numpy(), ek)
+    assert torch.equal(scores.cpu(), e.scores)
+    for b, k in enumerate(e.lens):
+        got = other[:, b, :, :k].cpu()
+        want = torch.zeros_like(got)
+        want[..., :min(k, 64)] = torch.gather(e.scores[:, b], 2, torch.from_numpy(ek[:, b, :, :min(k, 64)]).long())
+        assert torch.equal(got, want)
+    before = buf.clone()
+    over = [buf[..., 1:w + 1], buf[..., w - 1:], scores.transpose(0, 1), torch.as_strided(buf, (2, 2, 2, w), (4 * w, 2 * w, w, 1), 8 * w - 1),
+            torch.as_strided(buf, (2, 2, 2, 2 * w + 1), scores.stride())]  # the same first elements, rows too wide
+    over += [torch.as_strided(buf, (2, 2, 2, w), (2 * w, w, w - 1, 1), 0)]
+    for out in over:
+        with pytest.raises(AssertionError, match="scores_out"):
+            cache_ops.evict_tokens(e.views(cache), scores, scores_out=out, **args)
+    with pytest.raises(AssertionError, match="scores_out"):  # rows of the scores over each other, in place
+        cache_ops.evict_tokens(e.views(cache), over[-1], **args)
+    torch.cuda.synchronize()
+    assert torch.equal(buf, before)

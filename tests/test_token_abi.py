@@ -202,3 +202,30 @@ def test_tensors_on_the_host_are_refused():
 def test_a_broadcast_is_not_written():
     assert _lib.distinct(torch.zeros(3, 4)) and _lib.distinct(torch.zeros(1, 4).expand(1, 4)[:, ::2])
     assert _lib.distinct(torch.zeros(4).expand(1, 4)) and not _lib.distinct(torch.zeros(4).expand(2, 4))
+
+
+def test_tensors_whose_elements_share_a_place():
+    t = torch.zeros(4000)
+    at = lambda shape, strides, first=0: torch.as_strided(t, shape, strides, first)  # noqa: E731
+    for shape, strides in (((3, 4), (4, 1)), ((3, 4), (9, 1)), ((3, 4), (1, 3)), ((2, 3, 4), (4, 8, 1)), ((2, 3), (3, 2)),
+                           ((2, 2, 3), (3, 9, 1)), ((2, 2, 2), (5, 3, 1)), ((0, 4), (1, 1)), ((1, 4), (0, 1)), ((5,), (1,)),
+                           ((), ()), ((4, 1), (1, 7))):
+        x = at(shape, strides)
+        seen = (torch.arange(4000).as_strided(shape, strides)).reshape(-1).tolist()
+        assert _lib.distinct(x) and len(set(seen)) == len(seen), (shape, strides)
+    for shape, strides in (((3, 4), (3, 1)), ((3, 4), (0, 1)), ((2, 3, 4), (2, 8, 1)), ((2, 2, 2), (3, 2, 1)), ((4, 4), (1, 1)),
+                           ((3, 3), (2, 2))):
+        assert not _lib.distinct(at(shape, strides)), (shape, strides)
+    # rows counted wider than they are
+    assert _lib.distinct(at((3, 4), (9, 1)), 9) and not _lib.distinct(at((3, 4), (9, 1)), 10)
+    assert _lib.distinct(at((1, 4), (4, 1)), 100) and not _lib.distinct(at((3, 4), (4, 1)), 5)
+
+
+def test_tensors_that_share_elements():
+    t = torch.zeros(2, 3, 2, 100)
+    for a, b in ((t, t), (t, t[..., 5:]), (t[..., :60], t[..., 59:]), (t[:1], t), (t[:, 1:], t[:, :2]),
+                 (t.view(-1)[:50], t.view(-1)[49:52]), (t[..., ::2], t[..., 2:3])):
+        assert _lib.overlap(a, b) and _lib.overlap(b, a)
+    for a, b in ((t, t.clone()), (t[..., :50], t[..., 50:]), (t[:, :1], t[:, 1:]), (t[:, ::2], t[:, 1:2]), (t[..., ::2], t[..., 1::2]),
+                 (t[:, :, 0], t[:, :, 1]), (t[:0], t), (t.view(-1)[:50], t.view(-1)[50:])):
+        assert not _lib.overlap(a, b) and not _lib.overlap(b, a)
