@@ -206,6 +206,8 @@ def _cache_pairs(caches, first_row_dim):
                 f"cache rows must be contiguous beyond dim {first_row_dim - 1} (strides {strides})"
             )
             expect *= shape[dim]
+        # (all that a launch would refuse of a cache, so that none follows one that has written)
+        assert 1 <= expect * a.element_size() < 2 ** 31, f"cache rows of {expect} elements"
         b = caches[i + 1] if i + 1 < len(caches) else None
         if b is not None and b.device == device and b.shape == shape and b.stride() == strides and b.dtype == a.dtype:
             pairs.append((a, b))
@@ -294,7 +296,7 @@ def evict_tokens(
     _i32(dst_block_table, device, 2, B, "dst_block_table")
     _i32(seq_lens, device, 1, B, "seq_lens")
     # (all that a launch would refuse, so that none follows one that has written)
-    assert 1 <= layers <= 65535 and B <= 65535 and budget * heads < 2 ** 31, \
+    assert 1 <= layers <= 65535 and B <= 65535 and heads >= 1 and budget * heads < 2 ** 31, \
         f"{layers} layers, {B} sequences, a budget of {budget} for {heads} heads"
     assert num_blocks >= 1 and page >= 1 and (B == 0 or block_table.shape[1] >= 1 and dst_block_table.shape[1] >= 1), \
         "an empty cache or block table"

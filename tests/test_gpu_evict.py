@@ -384,3 +384,29 @@ def test_scores_out_beside_or_over_the_scores(dev, n):
         cache_ops.evict_tokens(e.views(cache), over[-1], **args)
     torch.cuda.synchronize()
     assert torch.equal(buf, before)
+
+
+@pytest.mark.parametrize("heads,row", [(2, 0), (0, 16), (0, 0)])
+def test_caches_without_rows_are_refused_before_a_write(dev, heads, row):
+    e = Evict(10, 1, [50, 60], 20, 16, shared=True)
+    k, v = e.views(e.cache.to(dev))
+    scores = e.scores.to(dev)
+    none = torch.empty(k.shape[:3] + (heads, row), dtype=k.dtype, device=dev)
+    args = (scores, e.bt.to(dev), torch.tensor(e.lens, dtype=torch.int32, device=dev), e.dst.to(dev), 20)
+    with pytest.raises(AssertionError, match="rows|heads"):
+        cache_ops.evict_tokens([none, none.clone()], *args)
+    torch.cuda.synchronize()
+    assert np.array_equal(_bits(scores), _bits(e.scores))
+
+
+@pytest.mark.parametrize("row", [(0,), (2, 0), (0, 16)])
+def test_a_cache_without_rows_beside_a_commit(dev, row):
+    """Refused before the caches in front of it are written."""
+    cache = torch.randint(0, 255, (2, 10, 16, 2, 64), dtype=torch.uint8, device=dev)
+    before = cache.clone()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    none = torch.empty(cache.shape[:3] + row, dtype=torch.uint8, device=dev)
+    with pytest.raises(AssertionError, match="rows"):
+        cache_ops.commit_draft_tokens([cache, none], i32([[1, 2], [3, 4]]), i32([3, 4]), i32([[1, 2], [2, 3]]), i32([2, 2]))
+    torch.cuda.synchronize()
+    assert torch.equal(cache, before)
