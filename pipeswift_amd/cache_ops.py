@@ -194,6 +194,7 @@ def _cache_pairs(caches, first_row_dim):
     first = caches[0]
     device, outer = first.device, first.shape[:3]
     assert first.is_cuda, "all caches must be on one GPU"
+    assert first.ndim < 6 or outer[2] != 2, "a fused [L, num_blocks, 2, block_size, ...] cache goes as its K and V views"
     pairs, i = [], 0
     while i < len(caches):
         a = caches[i]
@@ -347,8 +348,9 @@ def commit_draft_tokens(
     i, as a snapshot: every row is read before any is written, whatever the
     order of ``path``.  The sequence then has starts[b] + path_lens[b] tokens.
     caches: one tensor or a list, [L, num_blocks, block_size, *row] with
-    contiguous rows (K and V views of the fused cache, a latent cache); two of
-    one geometry move in one launch.  Negative indices and rows on missing pages
+    contiguous rows (K and V views of the fused cache, a latent cache; the fused
+    [L, num_blocks, 2, block_size, ...] one itself is refused); two of one
+    geometry move in one launch.  Negative indices and rows on missing pages
     are skipped.  The pages of drafted tokens are a sequence's own.
     """
     pairs = _cache_pairs(caches, 3)

@@ -410,3 +410,18 @@ def test_a_cache_without_rows_beside_a_commit(dev, row):
         cache_ops.commit_draft_tokens([cache, none], i32([[1, 2], [3, 4]]), i32([3, 4]), i32([[1, 2], [2, 3]]), i32([2, 2]))
     torch.cuda.synchronize()
     assert torch.equal(cache, before)
+
+
+def test_a_fused_cache_goes_as_its_views(dev):
+    """Its two halves are no page of two tokens."""
+    e = Evict(14, 1, [50, 60], 20, 16, shared=True)
+    cache = e.cache.to(dev)
+    scores = e.scores.to(dev)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    for caches in (cache, [cache]):
+        with pytest.raises(AssertionError, match="K and V views"):
+            cache_ops.commit_draft_tokens(caches, i32([[1, 2], [3, 4]]), i32([0, 1]), i32([[1, 2], [2, 3]]), i32([2, 2]))
+        with pytest.raises(AssertionError, match="K and V views"):
+            cache_ops.evict_tokens(caches, scores, e.bt.to(dev), i32(e.lens), e.dst[:, :1].repeat(1, 20).to(dev), 20)
+    torch.cuda.synchronize()
+    assert np.array_equal(_bits(cache), _bits(e.cache)) and np.array_equal(_bits(scores), _bits(e.scores))
