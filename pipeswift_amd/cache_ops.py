@@ -356,6 +356,8 @@ def commit_draft_tokens(
     pairs = _cache_pairs(caches, 3)
     first = pairs[0][0]
     assert first.ndim >= 4, "caches are layered: [L, num_blocks, block_size, ...]"
+    # (a launch moves what the one before it has left)
+    assert len(pairs) == 1 or len({c.data_ptr() for c in caches}) == len(caches), "a cache is named twice"
     device = first.device
     layers, num_blocks, page = first.shape[:3]
     B = path.shape[0]

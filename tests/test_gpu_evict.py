@@ -425,3 +425,21 @@ def test_a_fused_cache_goes_as_its_views(dev):
             cache_ops.evict_tokens(caches, scores, e.bt.to(dev), i32(e.lens), e.dst[:, :1].repeat(1, 20).to(dev), 20)
     torch.cuda.synchronize()
     assert np.array_equal(_bits(cache), _bits(e.cache)) and np.array_equal(_bits(scores), _bits(e.scores))
+
+
+def test_a_commit_moves_every_cache_once(dev):
+    cache = torch.randint(0, 255, (2, 10, 2, 16, 2, 64), dtype=torch.uint8, device=dev)
+    other = torch.randint(0, 255, (2, 10, 16, 64), dtype=torch.uint8, device=dev)
+    k, v = cache[:, :, 0], cache[:, :, 1]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    args = (i32([[1, 2], [3, 4]]), i32([3, 4]), i32([[1, 2], [2, 3]]), i32([2, 2]))
+    before, left = cache.clone(), other.clone()
+    for caches in ([k, v, k], [k, other, k], [other, k, v, other]):
+        with pytest.raises(AssertionError, match="twice"):
+            cache_ops.commit_draft_tokens(caches, *args)
+    torch.cuda.synchronize()
+    assert torch.equal(cache, before) and torch.equal(other, left)
+    cache_ops.commit_draft_tokens([k, k], *args)  # one launch
+    once = before.clone()
+    cache_ops.commit_draft_tokens(once[:, :, 0], *args)
+    assert torch.equal(cache, once)
