@@ -326,7 +326,7 @@ def tree_mask(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, max_seqlen_q: i
     """``paged_tree_attention``'s mask of drafted trees given by their parents.
 
     parents: integers [total_q]; a drafted token's parent as an index among its
-    sequence's drafted tokens, negative for a child of the last cached token.
+    sequence's drafted tokens; negative, or not one of them, for a child of the last cached token.
     Every token sees itself and its ancestors.  Returns int64
     [total_q, ceil(max_seqlen_q / 64)] on the parents' device, without a host
     synchronization: log2(max_seqlen_q) rounds, each of which doubles how many
@@ -338,8 +338,8 @@ def tree_mask(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, max_seqlen_q: i
     cu = cu_seqlens_q.to(device=dev, dtype=torch.int64)
     row = torch.arange(parents.shape[0], device=dev)
     b = (torch.searchsorted(cu, row, right=True) - 1).clamp_(0, max(cu.shape[0] - 2, 0))
-    first = cu[b] if cu.shape[0] > 1 else torch.zeros_like(row)
-    up = torch.where(parents >= 0, first + parents, -1)
+    first, end = (cu[b], cu[b + 1]) if cu.shape[0] > 1 else (torch.zeros_like(row), torch.zeros_like(row))
+    up = torch.where((parents >= 0) & (parents < end - first), first + parents, -1)
     own = (row - first).clamp_(min=0)
     mask = torch.zeros(parents.shape[0] + 1, words, dtype=torch.int64, device=dev)  # the last row: no ancestor
     word = torch.arange(words, device=dev)

@@ -110,3 +110,13 @@ def test_moves_by_hand():
     T.commit_draft_tokens(rows, np.array([[3, 1, 0]]), [1], np.array([[2, 0, 3]]), [3])
     # positions 1..4 hold rows 7, 2, 3, 0: position 1 <- 3, 2 <- 1, 3 <- 4
     assert rows[0].tolist() == [[0, 1], [7, 0], [4, 5], [6, 3]]
+
+
+def test_a_parent_outside_its_sequence_is_none():
+    """An index at or past a sequence's tokens names no token of the next one."""
+    cu = torch.tensor([0, 3, 3, 5, 7], dtype=torch.int32)
+    parents = [-1, 0, 3, 2, 0, 9, -7]
+    want = [0b001, 0b011, 0b100, 0b01, 0b11, 0b01, 0b10]
+    for dtype in (torch.int32, torch.int64):
+        made = tree_mask(torch.tensor(parents + [0, 2], dtype=dtype), cu, 3)  # (two rows that no sequence owns)
+        assert made[:7, 0].tolist() == want
