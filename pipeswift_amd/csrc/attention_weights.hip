@@ -697,7 +697,7 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
     // 256 of 300, a job's start priced as one 27, two 33)
     p.s.over = 1;
     p.s.min_run = 1;
-    p.s.max_runs = int32_t(2 * cus);  // resident at once
+    p.s.max_runs = int32_t(xcd_rounds(2 * cus));  // resident at once
     p.hg = int32_t(std::min<int64_t>(num_kv_heads, kFewRows / (8 * ceil_div(rows, 8))));
     p.s.heads = int32_t(ceil_div(num_kv_heads, p.hg));
     switch (q_dtype) {

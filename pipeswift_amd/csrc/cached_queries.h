@@ -6,6 +6,7 @@
 #include <cmath>
 
 #include "paged_attention.h"
+#include "xcd_runs.h"
 
 namespace psk_detail {
 
@@ -266,10 +267,9 @@ __device__ __forceinline__ StepRuns step_runs(const DecodeArgs& a, const JobSpac
 // The idx-th run of an XCD.  Workgroup w runs on XCD w % 8, and each XCD takes
 // consecutive runs, so that its L2 sees every kv head of a few sequences (one
 // head's rows lie a token apart and would fall on a part of its channels).  A run
-// past the last comes back as one too.
+// past the last comes back as one too.  max_runs is xcd_rounds() of something.
 __device__ __forceinline__ int64_t xcd_run(const StepRuns& c, int xcd, int idx) {
-  const int64_t runs = uniform_div(c.total + c.run - 1, c.run), per = (runs + 7) >> 3;
-  return idx < per ? xcd * per + idx : runs;
+  return run_of_xcd(uniform_div(c.total + c.run - 1, c.run), xcd, idx);
 }
 
 // The sequence that unit x (below the total) falls in, and the units before it.

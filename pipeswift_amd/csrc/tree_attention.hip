@@ -649,8 +649,7 @@ struct TreeShape {
 TreeShape tree_shape(int64_t rows, int64_t slots) {
   TreeShape s;
   s.row_blocks = ceil_div(rows, kRows);
-  // runs in whole rounds of the eight XCDs
-  s.max_runs = std::max<int64_t>(8, slots / s.row_blocks / 8 * 8);
+  s.max_runs = xcd_rounds(slots / s.row_blocks);
   return s;
 }
 
