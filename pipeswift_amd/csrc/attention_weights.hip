@@ -26,8 +26,6 @@
 // C ABI: include/pipeswift_kv.h.  Nothing here allocates or synchronizes.
 
 #include <algorithm>
-#include <map>
-#include <mutex>
 
 #include "cached_queries.h"
 
@@ -596,19 +594,6 @@ __global__ void __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_p
   }
 }
 
-int64_t weight_cus() {
-  static std::mutex mu;
-  static std::map<int, int64_t> cache;
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return 256;
-  std::lock_guard<std::mutex> lock(mu);
-  auto it = cache.find(dev);
-  if (it != cache.end()) return it->second;
-  int cus = 0;
-  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
-  return cache[dev] = cus;
-}
-
 template <int Q_DT>
 int quantize_queries(const WeightArgs& p, int64_t total_q, int64_t num_q_heads, uint8_t* q8, hipStream_t st) {
   hipLaunchKernelGGL((quantize_queries_kernel<Q_DT>), dim3(unsigned(ceil_div(total_q * num_q_heads * 8, kThreads))),
@@ -689,7 +674,7 @@ int psk_accumulate_attention_weights(float* scores, int64_t scores_seq_stride, i
   p.head_stride = scores_head_stride;
   p.decay = decay;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t cus = weight_cus();
+  const int64_t cus = device_cus();
   const int64_t rows = max_seqlen_q * a.heads;
   if (rows <= kRows) {
     p.s.step_shift = log2_exact(kStepKeys);

@@ -3,6 +3,7 @@
 // prefill_runs.hip's trees, attention_weights.hip).
 #pragma once
 
+#include <atomic>
 #include <cmath>
 
 #include "paged_attention.h"
@@ -85,6 +86,18 @@ inline int check_cached_queries(const CachedQueries& c, DecodeArgs& a, bool* emp
   a.qd = c.q_descale;
   a.kd = c.k_descale;
   return PSK_OK;
+}
+
+// CUs of the current device, asked for once each; 256 where it is not known.
+inline int64_t device_cus() {
+  static std::atomic<int> known[64];
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  const bool kept = dev >= 0 && dev < 64;
+  if (kept && (cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
+  if (kept) known[dev].store(cus, std::memory_order_relaxed);
+  return cus;
 }
 
 // Sequence b's query rows: [first, first + n), inside the total_q rows of q

@@ -47,8 +47,6 @@
 // C ABI: include/pipeswift_kv.h.  Nothing here allocates or synchronizes.
 
 #include <algorithm>
-#include <map>
-#include <mutex>
 
 #include "cached_queries.h"
 #include "prefill_runs.h"
@@ -630,18 +628,7 @@ __global__ void __launch_bounds__(256) merge_tree_kernel(TreeArgs p) {
 }
 
 // Workgroups resident at once: two per CU (LDS and registers).
-int64_t tree_slots() {
-  static std::mutex mu;
-  static std::map<int, int64_t> cache;
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return kMaxSlots;
-  std::lock_guard<std::mutex> lock(mu);
-  auto it = cache.find(dev);
-  if (it != cache.end()) return it->second;
-  int cus = 0;
-  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return kMaxSlots;
-  return cache[dev] = std::min<int64_t>(2 * cus, kMaxSlots);
-}
+int64_t tree_slots() { return std::min<int64_t>(2 * device_cus(), kMaxSlots); }
 
 struct TreeShape {
   int64_t row_blocks, max_runs;
