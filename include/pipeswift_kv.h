@@ -425,9 +425,10 @@ int64_t psk_paged_prefill_step_workspace_len(int64_t num_seqs, int64_t total_q, 
  * sees key j < seq_lens[b] - n_b, and key seq_lens[b] - n_b + t, t < n_b, where
  * bit t % 64 of tree_mask[(c_b + i) * tree_mask_stride + t / 64] is set.
  * tree_mask_words words of 64 tokens each hold max_seqlen_q tokens at least.  A
- * token that sees no key writes zeros and lse = -inf.  max_seq_len, a bound on
- * seq_lens, sizes the launch and chooses its form (the results' last bits may
- * differ between forms; a longer sequence is read whole all the same).  P V has
+ * token that sees no key writes zeros and lse = -inf.  max_seqlen_q and
+ * max_seq_len, a bound on seq_lens, size the launch, cut it and choose its form
+ * (the results' last bits may differ between them; a longer sequence is read
+ * whole all the same).  P V has
  * a weight rounded once to fp16 for a bf16 out, and as the sum of two fp16 for a
  * float32 one.  out rows need 4-element alignment.  workspace: device floats,
  * psk_paged_tree_workspace_len() of them (0 where a max_seq_len of at most 1536
@@ -456,7 +457,8 @@ int64_t psk_paged_tree_workspace_len(int64_t num_seqs, int64_t total_q, int64_t 
  *       exp(s_j - lse[hq * lse_head_stride + c_b + i]),
  * s_j and the causal rule as psk_paged_decode_attention, any number of query
  * tokens and heads, in a fixed order of sums.  decay == 0: the old value is not
- * read.  descale_strides: (b, h) of q and k.  max_seq_len only sizes the launch.
+ * read.  descale_strides: (b, h) of q and k.  max_seq_len only sizes the launch;
+ * max_seqlen_q chooses its form and the order of the sums.
  * workspace: psk_attention_weights_workspace_bytes() bytes of device memory (0
  * for at most 32 query rows a kv head, max_seqlen_q * num_q_heads / num_kv_heads,
  * and for an FP8 query; else the queries' e4m3 bytes), no initial contents

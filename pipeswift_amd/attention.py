@@ -387,9 +387,11 @@ def paged_tree_attention(
     to fp16, as in ``paged_prefill_attention``; for a float32 one with P as the
     sum of two fp16 (2^-22 of a weight).
 
-    ``max_seq_len``: a bound on seq_lens where the caller has a closer one than
-    the block table's width; it sizes the launch and chooses its form, and a
-    longer sequence is read whole all the same.  ``workspace``: float32 of
+    ``max_seqlen_q`` and ``max_seq_len`` (a bound on seq_lens where the caller has
+    a closer one than the block table's width) size the launch, cut it and choose
+    its form; sums may be taken in another order under another bound.  A
+    sequence past max_seq_len is read whole all the same; a max_seqlen_q far above
+    the counts costs time.  ``workspace``: float32 of
     ``tree_workspace_floats``, for callers that keep one."""
     B, n = _query_layout(q, cu_seqlens_q, max_seqlen_q, validate)
     _check_paged(q, (k_cache, v_cache), block_table, seq_lens, B)
@@ -474,7 +476,8 @@ def accumulate_attention_weights(
     those queries.  scores: float32 [>= B, Hkv, width], unit last stride;
     entries at or past seq_lens[b] or the width are left as they are, and new
     tokens start from what is there (zeros).  ``decay`` 0 does not read the old
-    sums.  ``max_seq_len`` only sizes the launch.  ``workspace``: uint8 of
+    sums.  ``max_seq_len`` only sizes the launch; ``max_seqlen_q`` chooses its form
+    (and with it the order of the sums).  ``workspace``: uint8 of
     ``weights_workspace_bytes``, for callers that keep one.  Returns ``scores``."""
     B, n = _query_layout(q, cu_seqlens_q, max_seqlen_q, validate)
     _check_paged(q, (k_cache,), block_table, seq_lens, B)

@@ -262,8 +262,9 @@ def evict_tokens(
 
     Returns (kept, new_lens): int32 [L, B, H or 1, budget], each kept token's old
     position (-1 past the last), and int32 [B], the new lengths.  One launch for
-    the choice (five for scores of more than 16384 tokens) and one for each pair
-    of caches of one geometry; no synchronization.
+    the choice -- for scores of more than 16384 tokens four, five in place, and as
+    many again for every 4096 parts of 16384 of all their rows -- and one for each
+    pair of caches of one geometry; no synchronization.
     """
     first = caches if isinstance(caches, torch.Tensor) else caches[0]
     assert first.ndim >= 4, "caches are layered: [L, num_blocks, block_size, heads, ...] or [L, num_blocks, block_size, row]"

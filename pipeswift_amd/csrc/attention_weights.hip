@@ -361,13 +361,16 @@ __device__ __forceinline__ float sum_lanes(float (&v)[16], int lane) {
 }
 
 // The rows go to LDS two tiles ahead, whole 128-byte rows by global_load_lds, so
-// that the loop's registers let four waves share a SIMD: 38 us for the last 64
-// queries of 4 contexts of 8000 to 32000 tokens (32 query heads over 4), 77 % of it
-// VALU time (per score an fma, a quarter-rate exp2 and an addition).  Rows read
+// that the loop's registers let four waves share a SIMD (128 of them, with two spilled
+// outside the loop): 38 us for the last 64 queries of 4 contexts of 8000 to 32000
+// tokens (32 query heads over 4), 77 % of it vector time.  Of the 27 us of that, 14
+// are the scores' (an fma, a quarter-rate exp2 and an addition each), 5 the queries'
+// conversion and 8 a unit's start and end: of 143 vector instructions a tile of 32 x
+// 32, the loop has about 90.  Rows read
 // straight to registers, 64 keys a wave and two waves a SIMD: 48; 64 keys from LDS:
 // 49.  Units go keys first and the CUs take them forwards and backwards in turn, so
 // that under a causal mask a CU's long and short ones add up alike: 28 us for a
-// prompt of 2000 tokens (32 over 8), MANY_FWD.
+// prompt of 2000 tokens (32 over 8).
 //
 // The unit of workgroup w, which runs on XCD w % 8: forwards over the CUs in even
 // rounds, backwards in odd ones.
@@ -389,7 +392,8 @@ __global__ void __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_p
   const uint32_t lse_ring = (uint32_t)(size_t)(lvoid*)s_lse + uint32_t(wave * kManyRing * kRows * 4);
   // As many keys to a workgroup as leave `slots` of them; the fewer keys the step
   // has, the more waves share them (as far as there are row tiles for each).  From
-  // the lengths alone, so that the order of the sums does not depend on a bound.
+  // the lengths and max_seqlen_q, so that the order of the sums does not depend on
+  // max_seq_len.
   SeqWindow seqs;
   JobSpace s = args.s;  // (a step of kTile keys)
   StepRuns step = step_runs(args.a, s, seqs, lane);

@@ -26,10 +26,10 @@ namespace {
 // that the order is kept with ballots and one exchange between the waves.
 //
 //   * rows of at most kChunk: select_row_kernel, everything in one launch, with 64
-//     registers so that two workgroups of 1024 threads share a CU (73 registers,
-//     one of them: 56 us).  512 rows of 12288: 27 us, bound by the histograms'
+//     registers, 8 values spilled, so that two workgroups of 1024 threads share a CU
+//     (73 registers, one of them: 56 us).  512 rows of 12288: 27 us, bound by the histograms'
 //     additions; 8 rows of 1100: 7.8 us, the barriers between the digits.
-//     Rows of at most 4096 take 256 threads, which wait less at them: 512 rows of
+//     Rows of at most 4096 take 256 threads (80 registers, 10 spilled), which wait less at them: 512 rows of
 //     4000 and their moves 29 us against 31 with 1024, 2048 of 2000, 74 against 95.
 //   * longer ones, a workgroup a chunk: three launches of chunk_digit_kernel
 //     leave each chunk's histogram of a digit, and every workgroup of the next

@@ -8,8 +8,8 @@
 // lse = log sum exp s, Q K^T on the bf16 MFMA over exactly converted FP8
 // operands, P V on the fp16 MFMA with V exact, float32 sums.  For a bf16 out P is
 // rounded once (2^-11, below what the output's own rounding leaves); for a float32 one
-// it is the sum of two fp16 (2^-22) and P V runs twice: 102 / 109 us for the 32 trees
-// below, 148 / 201 for four wide ones (prefill_runs.hip).
+// it is the sum of two fp16 (2^-22) and P V runs twice: 110 / 115 us for the 32 trees
+// below, 148 / 197 for four wide ones (prefill_runs.hip).
 //
 // The n G query rows of a kv head (G query heads each) are rows of MFMA tiles,
 // 32 to a workgroup.  Its four waves hold all of them and take the 32-key
@@ -32,13 +32,14 @@
 //
 // The work is cut into equal runs over sequences and kv heads (cached_queries.h).
 // A run's piece that is not all of a job's keys leaves a partial record (maxima,
-// sums, float32 accumulators); merge_tree_kernel joins a job's records in the
-// order of its keys.  Short contexts are not cut (kWholeKeys), and wide trees over
-// much work run in prefill_runs.hip (kWideRows).
+// sums, float32 accumulators); merge_tree_kernel deals a job's records, in the order
+// of their keys, to four waves in turn and joins the four sums.  Short contexts are
+// not cut (kWholeKeys), and wide trees over much work run in prefill_runs.hip
+// (kWideRows).
 //
 // What bounds it, and what it measured: 32 trees of 16 tokens over contexts of 512 to
-// 16384 (32 query heads over 8), 113 us, the loads' latency (3.2 TB/s; the row blocks'
-// second reads come from L2); 48 ragged trees over up to 6000 keys (8 heads over one)
+// 16384 (32 query heads over 8), 113 us, the loads' latency (3.2 TB/s of K and V, each
+// of which goes to LDS once for either row block, the second time from L2); 48 ragged trees over up to 6000 keys (8 heads over one)
 // 27 us and one of 8 over 1000 15 us, the chain lengths - page ids - keys and the
 // merge.  A tile of 32 keys and 32 rows costs 512 matrix cycles and 156 vector
 // instructions, 64 of them the conversion of K and V to bf16 and fp16; the two hardly
@@ -77,8 +78,8 @@ constexpr int kMinRun = 4;
 constexpr int kWholeKeys = 1536;
 // Wide trees over much work go to prefill_runs.hip, whose waves share each key's
 // conversion (here every 32 rows convert it again) at 15 us more for its start and
-// end: from kWideRows rows a sequence on average, and kWideWork query rows x keys at
-// most.  This kernel / that one, us (32 query heads): 4 sequences of 30000 keys over
+// end: from kWideRows rows a sequence on average and kWideWork query rows x keys on,
+// by the bounds of both.  This kernel / that one, us (32 query heads): 4 sequences of 30000 keys over
 // 4 kv heads, 24 tokens each 75 / 80, 32: 88 / 87, 48: 126 / 120, 64: 157 / 134; 16 of
 // 8000 over 8, 32 tokens 95 / 110, 48: 157 / 138; 32 of 2000, 32 tokens 64 / 60, 48:
 // 100 / 74; one of 16000, 64 tokens 38 / 55; uncut (kWholeKeys), 64 of 1500 over 4 kv
@@ -98,7 +99,7 @@ struct TreeArgs {
   double scale_log2;     // softmax_scale * log2(e)
   const int64_t* mask;
   int64_t mask_stride;   // words from a query token's mask to the next one's
-  int32_t row_blocks;    // workgroups that share a run's keys
+  int32_t row_blocks;    // workgroups that share a run's keys, from max_seqlen_q (those past a job's own rows have nothing to do)
   int32_t whole;         // a workgroup takes all of a job's keys, and nothing is merged
   float* records;        // [max_runs][row_blocks][2][kSlab]
 };
