@@ -27,6 +27,7 @@ DTYPE_CODES = {
     torch.bfloat16: 2,
     torch.float8_e4m3fn: 3,
 }
+MXFP4_CODE = 4  # the rows of mxfp4_kv, held as uint8
 
 SWAP_MEMCPY = 0
 SWAP_BLIT = 2
@@ -136,6 +137,21 @@ _SIGNATURES = {
     "psk_commit_draft_tokens": (
         _int,
         [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp],
+    ),
+    "psk_norm_rope": (
+        _int,
+        [_vp, _c_int64_p, _vp, _c_int64_p, _vp, _c_int64_p, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int, ctypes.c_float,
+         _vp, _int, _i64, _i64, _c_int64_p, _vp, _i64, _i64, _i64, _int, _vp, _c_int64_p, _vp, _c_int64_p, _vp, _vp,
+         _c_int64_p, _c_int64_p, _int, _vp, _i64, _i64, _vp, _vp, _vp],
+    ),
+    "psk_mxfp4_entry_bytes": (_i64, [_i64]),
+    "psk_reshape_and_cache_mxfp4": (
+        _int,
+        [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _c_int64_p, _c_int64_p, _c_int64_p, _c_int64_p, _int, _vp],
+    ),
+    "psk_gather_mxfp4": (
+        _int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_int64_p, _i64, _int, _vp],
     ),
     "psk_mla_fp8_tile_entry_bytes": (_i64, [_i64, _i64]),
     "psk_concat_and_cache_mla_fp8_tiles": (

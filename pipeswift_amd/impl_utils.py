@@ -6,7 +6,10 @@ layer's K/V views of ``kv_cache_info.kv_cache`` (GQA) or the layer of
 ``mla_cache_tensor`` with a 1-head axis (MLA), and ``kv_cache_info.slot_mapping``.
 The optional FP8 scales of ``KVCacheInfo`` (one element, or one per layer)
 are passed through.  A uint8 ``mla_cache_tensor`` holds tile-scaled FP8 latent
-entries (``mla_fp8``), which the append quantizes itself (no per-tensor scale).
+entries (``mla_fp8``), which the append quantizes itself (no per-tensor scale), and
+a uint8 ``kv_cache`` holds 4-bit rows (``mxfp4_kv``) likewise.
+``norm_rope_append_kv_cache`` is the append with the layer's norms and rotation of q
+and k in the same pass.
 """
 
 from __future__ import annotations
@@ -15,7 +18,9 @@ import torch
 
 from .metadata import KVCacheInfo, coalesced_to_cuda  # noqa: F401  (re-exported, impl_utils.py:340)
 from .mla_fp8 import concat_and_cache_mla_fp8_tiles
+from .mxfp4_kv import reshape_and_cache_mxfp4
 from .reshape_and_cache import reshape_and_cache_flash, reshape_and_cache_flash_diffkv
+from .rotary import norm_rope_and_cache
 
 
 def _layer_scale(scale, layer_idx):
@@ -27,6 +32,10 @@ def _layer_scale(scale, layer_idx):
 def append_kv_cache(key, value, kv_cache_info: KVCacheInfo = None, layer_idx: int = 0):
     if key.shape[0] == 0:
         return
+    if kv_cache_info.kv_cache[0].dtype == torch.uint8:
+        reshape_and_cache_mxfp4(key, value, kv_cache_info.kv_cache[0][layer_idx], kv_cache_info.kv_cache[1][layer_idx],
+                                kv_cache_info.slot_mapping)
+        return
     reshape_and_cache_flash(
         key,
         value,
@@ -36,6 +45,17 @@ def append_kv_cache(key, value, kv_cache_info: KVCacheInfo = None, layer_idx: in
         _layer_scale(kv_cache_info.k_scale, layer_idx),
         _layer_scale(kv_cache_info.v_scale, layer_idx),
     )
+
+
+def norm_rope_append_kv_cache(query, key, value, positions, cos_sin, q_weight=None, k_weight=None, eps=1e-6, sections=None,
+                              interleaved=False, kv_cache_info: KVCacheInfo = None, layer_idx: int = 0, q_out=None):
+    """query [N, Hq, D] and key [N, Hkv, D] normed and rotated (``rotary.norm_rope``),
+    key and value appended to the layer's cache, whatever its type; returns the query."""
+    k_cache, v_cache = kv_cache_info.kv_cache[0][layer_idx], kv_cache_info.kv_cache[1][layer_idx]
+    return norm_rope_and_cache(
+        query, key, value, k_cache, v_cache, kv_cache_info.slot_mapping, positions, cos_sin, q_weight, k_weight, eps,
+        sections, interleaved, _layer_scale(kv_cache_info.k_scale, layer_idx),
+        _layer_scale(kv_cache_info.v_scale, layer_idx), q_out)
 
 
 def append_mla_kv_cache(ckv, kpe, kv_cache_info: KVCacheInfo = None, layer_idx: int = 0):

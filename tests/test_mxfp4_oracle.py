@@ -1,0 +1,159 @@
+"""The 4-bit oracle against closed forms, and the host-side checks of the C entries
+of the 4-bit cache and of the norms with rotation (no pointer given here could be
+read)."""
+
+import numpy as np
+import pytest
+
+from oracle import mxfp4_oracle as M
+from pipeswift_amd import _lib
+
+FAKE = 1 << 20  # aligned, never dereferenced
+ARG, DTYPE, WORKSPACE = -1, -2, -4
+
+
+def test_row_of_known_values():
+    x = np.zeros((1, 64))
+    x[0, :9] = [6.0, -0.25, 0.75, 1.25, 2.5, -5.0, 0.5, 0.26, 1.75]
+    x[0, 32] = 7.0  # not below 7: the next scale, where it is 3.5 and rounds to 4
+    row = M.quantize(x)[0]
+    assert row.shape == (36,) and list(row[32:]) == [127, 128, 0, 0]
+    assert list(M.dequantize(row, 64)[:9]) == [6.0, -0.0, 1.0, 1.0, 2.0, -4.0, 0.5, 0.5, 2.0]
+    assert M.dequantize(row, 64)[32] == 8.0
+    assert row[0] == 7 | 8 << 4  # the even element low; minus zero keeps its sign
+
+
+def test_scales_at_the_ends():
+    x = np.zeros((5, 32))
+    x[1, 3], x[2, 0], x[3, 0], x[4, 5] = 2.0 ** -149, float.fromhex("0x1.fep127"), np.nan, np.inf
+    rows = M.quantize(x)
+    assert list(rows[:, 16]) == [127, 1, 253, 255, 255]
+    v = M.dequantize(rows, 32)
+    assert (v[0] == 0).all() and (v[1] == 0).all() and v[2, 0] == 2.0 ** 128
+    assert np.isnan(v[3:]).all() and (rows[3:, :16] == 0).all()
+
+
+def test_every_value_is_within_half_a_step():
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((400, 96)) * np.exp(rng.standard_normal((400, 96)) * 3)
+    rows = M.quantize(x)
+    v = M.dequantize(rows, 96)
+    s = np.repeat(np.ldexp(1.0, rows[:, 48:51].astype(int) - 127), 32, -1)
+    assert (np.abs(v - x) <= np.maximum(np.abs(x) / 4, s / 4)).all()
+    assert (np.abs(x) < 7 * s).all() and (np.abs(x).reshape(400, 3, 32).max(-1) >= 3.5 * s[:, ::32]).all()
+
+
+def test_entry_bytes():
+    for d in (32, 64, 96, 128, 256, 512, 4096):
+        assert _lib.lib().psk_mxfp4_entry_bytes(d) == M.entry_bytes(d)
+    assert M.entry_bytes(128) == 68 and M.entry_bytes(64) == 36
+    for d in (0, -32, 48, 4128):
+        assert _lib.lib().psk_mxfp4_entry_bytes(d) == ARG
+
+
+def _call(entry, good, change):
+    assert set(change) <= set(good)
+    return getattr(_lib.lib(), entry)(*{**good, **change}.values())
+
+
+def _refused(entry, good, status, message, change):
+    st = _call(entry, good, change)
+    assert st == status and message in _lib.lib().psk_last_error(), (st, _lib.lib().psk_last_error())
+
+
+ROWS = _lib.i64_array([4 * 128, 128, 1])
+ENTRIES = _lib.i64_array([2 * 16 * 4 * 68, 4 * 68, 68, 1])
+APPEND = dict(k=FAKE, v=FAKE, kc=FAKE, vc=FAKE, slots=FAKE, n=8, H=4, D=128, ps=16, P=10, ks=ROWS, vs=ROWS, kcs=ENTRIES,
+              vcs=ENTRIES, dt=2, stream=None)
+
+
+@pytest.mark.parametrize("status,message,change", [
+    (ARG, b"bad sizes", dict(n=-1)),
+    (ARG, b"bad sizes", dict(H=0)),
+    (ARG, b"bad sizes", dict(D=48)),
+    (ARG, b"bad sizes", dict(ps=0)),
+    (DTYPE, b"bf16, f16 or f32", dict(dt=3)),
+    (ARG, b"NULL", dict(k=None)),
+    (ARG, b"NULL", dict(vc=None)),
+    (ARG, b"NULL", dict(slots=None)),
+    (ARG, b"4-byte", dict(kc=FAKE + 2)),
+    (ARG, b"4-byte", dict(vcs=_lib.i64_array([2 * 16 * 4 * 68, 4 * 68 + 2, 68, 1]))),
+    (ARG, b"shorter", dict(kcs=_lib.i64_array([16 * 4 * 64, 4 * 64, 64, 1]))),
+    (ARG, b"num_tokens", dict(n=1 << 31)),
+])
+def test_append_refuses(status, message, change):
+    _refused("psk_reshape_and_cache_mxfp4", APPEND, status, message, change)
+
+
+GATHER = dict(c=FAKE, cv=FAKE, d=FAKE, dv=FAKE, bt=FAKE, cu=FAKE, starts=None, B=2, bts=10, btw=10, T=8, H=4, D=128, ps=16,
+              P=10, cs=ENTRIES, ds=512, dt=2, stream=None)
+
+
+@pytest.mark.parametrize("status,message,change", [
+    (ARG, b"bad sizes", dict(B=-1)),
+    (ARG, b"bad sizes", dict(D=100)),
+    (ARG, b"bad sizes", dict(T=1 << 31)),
+    (DTYPE, b"read as", dict(dt=3)),
+    (ARG, b"NULL", dict(c=None)),
+    (ARG, b"NULL", dict(cv=None)),
+    (ARG, b"NULL", dict(cu=None)),
+    (ARG, b"4-byte", dict(c=FAKE + 1)),
+    (ARG, b"row stride", dict(ds=511)),
+])
+def test_gather_refuses(status, message, change):
+    _refused("psk_gather_mxfp4", GATHER, status, message, change)
+
+
+SECTIONS = _lib.i64_array([16, 24, 24])
+NORM_ROPE = dict(q=FAKE, qs=ROWS, k=FAKE, ks=ROWS, v=FAKE, vs=ROWS, dt=2, n=8, Hq=4, Hkv=4, D=128, qw=FAKE, kw=FAKE, wdt=2,
+                 eps=1e-6, pos=FAKE, pb=8, pa=8, axes=3, sections=SECTIONS, cs=FAKE, css=128, P=100, rot=128, inter=0, qo=FAKE,
+                 qos=ROWS, ko=None, kos=None, kc=FAKE, vc=FAKE, kcs=ENTRIES, vcs=ENTRIES, cdt=4, slots=FAKE, ps=16, blocks=10,
+                 ksc=None, vsc=None, stream=None)
+
+
+@pytest.mark.parametrize("status,message,change", [
+    (ARG, b"bad sizes", dict(n=-1)),
+    (ARG, b"bad sizes", dict(n=1 << 31)),
+    (ARG, b"bad sizes", dict(Hq=0, Hkv=0)),
+    (ARG, b"head_size", dict(D=132)),
+    (ARG, b"head_size", dict(D=520)),
+    (ARG, b"rot_dim", dict(rot=0)),
+    (ARG, b"rot_dim", dict(rot=144)),
+    (ARG, b"rot_dim", dict(rot=24)),
+    (ARG, b"rot_dim", dict(rot=12, inter=1)),
+    (DTYPE, b"queries and keys", dict(dt=3)),
+    (DTYPE, b"weights", dict(wdt=1)),
+    (ARG, b"axes", dict(axes=5)),
+    (DTYPE, b"positions", dict(pb=2)),
+    (ARG, b"eps", dict(eps=-1.0)),
+    (ARG, b"eps", dict(eps=float("nan"))),
+    (ARG, b"table", dict(P=0)),
+    (ARG, b"table", dict(css=64)),
+    (DTYPE, b"cache dtype", dict(cdt=1)),
+    (ARG, b"multiple of 32", dict(D=80, rot=64)),
+    (ARG, b"geometry", dict(ps=0)),
+    (ARG, b"NULL", dict(q=None)),
+    (ARG, b"NULL", dict(v=None)),
+    (ARG, b"NULL", dict(vc=None)),
+    (ARG, b"NULL", dict(slots=None)),
+    (ARG, b"NULL", dict(sections=None)),
+    (ARG, b"NULL", dict(qo=None)),
+    (ARG, b"NULL", dict(kc=None, vc=None)),
+    (ARG, b"16-byte", dict(q=FAKE + 8)),
+    (ARG, b"16-byte", dict(vs=_lib.i64_array([4 * 128 + 4, 128, 1]))),
+    (ARG, b"4-byte", dict(kc=FAKE + 2)),
+    (ARG, b"8-byte", dict(cdt=3, kc=FAKE + 4)),
+    (ARG, b"16-byte", dict(cdt=2, kc=FAKE + 8)),
+    (ARG, b"scales", dict(ksc=FAKE)),
+    (ARG, b"section", dict(sections=_lib.i64_array([16, -1, 49]))),
+    (ARG, b"sections", dict(sections=_lib.i64_array([16, 24, 23]))),
+])
+def test_norm_rope_refuses(status, message, change):
+    _refused("psk_norm_rope", NORM_ROPE, status, message, change)
+
+
+def test_empty_calls_touch_nothing():
+    assert _call("psk_reshape_and_cache_mxfp4", APPEND, dict(n=0, k=None, v=None, slots=None)) == 0
+    assert _call("psk_gather_mxfp4", GATHER, dict(T=0, d=None, dv=None)) == 0
+    assert _call("psk_gather_mxfp4", GATHER, dict(B=0, bt=None)) == 0
+    assert _call("psk_norm_rope", NORM_ROPE, dict(n=0, q=None, k=None, v=None, qo=None, pos=None, slots=None)) == 0
