@@ -641,6 +641,35 @@ int psk_gather_mxfp4(const void* cache, const void* cache_v, void* dst, void* ds
                      int64_t dst_row_stride, int out_dtype, void* stream);
 
 /*
+ * Attention over that cache (build-defined): for query token i of the n of sequence b
+ * (rows [cu[b], cu[b+1]) of q, its last positions; without cu_seqlens_q max_seqlen_q
+ * rows each) and query head hq of kv head h = hq / (num_q_heads / num_kv_heads), over
+ * the first seq_lens[b] - n + 1 + i keys if causal, else all seq_lens[b]:
+ *   s_j = softmax_scale (q . K[j, h]), out = sum_j softmax(s)_j V[j, h], lse = log sum_j exp s_j
+ * Any number of query tokens and query heads per kv head; head_size 128.  q is bf16, f16
+ * or f32 (16-byte aligned rows), taken to 2^-17 or better; out bf16, f16 or f32, rows
+ * aligned to 4 elements.  Rows without a page are zeros; a query that sees no key gets
+ * zeros and -inf; a NaN in V reaches only the queries that see its token; rows that no
+ * sequence owns are left as they were.  A sequence longer than the block table reads
+ * zeros past it.  max_seq_len and max_seqlen_q (bounds) size and cut the launch.
+ * lse (may be NULL): [hq * lse_head_stride + token].  Caches have BYTE strides of block,
+ * slot and head.  workspace:
+ * psk_paged_mxfp4_workspace_len() floats, no initial contents needed, not shared by
+ * calls that overlap.
+ */
+int psk_paged_mxfp4_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int q_dtype,
+                              const void* k_cache, const void* v_cache, const int64_t* k_strides,
+                              const int64_t* v_strides, const int32_t* block_table, int64_t block_table_stride,
+                              int64_t block_table_width, const int32_t* seq_lens, int64_t num_seqs, int64_t num_q_heads,
+                              int64_t num_kv_heads, int64_t head_size, int64_t block_size, int64_t num_blocks,
+                              int64_t max_seq_len, int64_t total_q, int64_t max_seqlen_q, const int32_t* cu_seqlens_q,
+                              int causal, float softmax_scale, void* out, int64_t out_tok_stride,
+                              int64_t out_head_stride, int out_dtype, float* lse, int64_t lse_head_stride,
+                              float* workspace, int64_t workspace_len, void* stream);
+int64_t psk_paged_mxfp4_workspace_len(int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, int64_t num_q_heads,
+                                      int64_t num_kv_heads, int64_t max_seq_len);
+
+/*
  * Pinned, device-mapped host memory for the L2 mirror and swap staging
  * (hipHostMalloc).  Allocation happens at set-up, never on the hot path.
  */

@@ -144,6 +144,12 @@ _SIGNATURES = {
          _vp, _int, _i64, _i64, _c_int64_p, _vp, _i64, _i64, _i64, _int, _vp, _c_int64_p, _vp, _c_int64_p, _vp, _vp,
          _c_int64_p, _c_int64_p, _int, _vp, _i64, _i64, _vp, _vp, _vp],
     ),
+    "psk_paged_mxfp4_attention": (
+        _int,
+        [_vp, _i64, _i64, _int, _vp, _vp, _c_int64_p, _c_int64_p, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _vp, _int, ctypes.c_float, _vp, _i64, _i64, _int, _vp, _i64, _vp, _i64, _vp],
+    ),
+    "psk_paged_mxfp4_workspace_len": (_i64, [_i64] * 6),
     "psk_mxfp4_entry_bytes": (_i64, [_i64]),
     "psk_reshape_and_cache_mxfp4": (
         _int,

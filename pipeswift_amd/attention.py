@@ -32,6 +32,7 @@ from typing import Optional
 import torch
 
 from ._lib import check, distinct, dtype_code, i64_array, lib, on_device, ptr, stream_handle
+from .mxfp4_kv import check_cache
 
 HEAD_DIM = 128
 MAX_ROWS = 16  # query tokens x query heads per kv head
@@ -39,6 +40,7 @@ MAX_ROWS = 16  # query tokens x query heads per kv head
 _CHECK_ARGS = os.environ.get("PIPESWIFT_AMD_CHECK_ARGS", "0") == "1"
 
 _OUT_CODES = {torch.bfloat16: 2, torch.float32: 0}
+_QUERY_TYPES = (torch.bfloat16, torch.float16, torch.float32)  # queries and outputs over the 4-bit cache
 
 
 def workspace_floats(num_seqs: int, num_q_heads: int, num_kv_heads: int, max_seq_len: int, num_splits: int = 0,
@@ -525,6 +527,95 @@ def weights_workspace_bytes(total_q: int, max_seqlen_q: int, num_q_heads: int, n
     return n
 
 
+def paged_mxfp4_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    max_seqlen_q: int = 1,
+    softmax_scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+    return_softmax_lse: bool = False,
+    causal: bool = True,
+    max_seq_len: Optional[int] = None,
+    workspace: Optional[torch.Tensor] = None,
+    validate: bool = False,
+):
+    """Attention over the 4-bit cache of ``mxfp4_kv``: decode, drafted tokens, prefill.
+
+    q: [total_q, Hq, 128] in bf16, fp16 or fp32 (taken as it is to 2^-17 or better;
+    there is no quantized query and no descale).  Sequence b owns the query rows
+    [cu_seqlens_q[b], cu_seqlens_q[b+1]) (int32 [B+1]; None: max_seqlen_q each), at
+    most ``max_seqlen_q``: its last positions.  With ``causal`` token i of n sees the
+    first seq_lens[b] - n + 1 + i keys, else all.  k_cache, v_cache: uint8 [num_blocks,
+    block_size, Hkv, 68] (views of the fused cache; any strides, rows on 4-byte
+    boundaries).  block_table: int32 [B, W]; seq_lens: int32 [B].  Returns out [total_q,
+    Hq, 128] in q's type (or ``out``, in bf16, fp16 or fp32) and, when asked, lse [Hq,
+    total_q] float32; rows no sequence owns are left as they were, a token that sees
+    no key gets zeros and -inf, a missing page reads as zeros, and a NaN in V reaches
+    only the tokens that see it.
+
+    ``max_seqlen_q`` and ``max_seq_len`` (a bound on seq_lens where the caller has a
+    closer one than the block table's width) size the launch, cut it and choose its
+    form, and with it the order of sums.  ``workspace``: float32 of
+    ``mxfp4_workspace_floats``, for callers that keep one; calls that overlap need one
+    each.  The ragged layout contract, and ``validate``, are ``paged_decode_attention``'s."""
+    B, n = _query_layout(q, cu_seqlens_q, max_seqlen_q, validate)
+    device = q.device
+    assert q.is_cuda and q.dim() == 3 and q.shape[2] == HEAD_DIM and q.stride(2) == 1, \
+        "q must be [T, Hq, 128] with unit last stride"
+    assert q.dtype in _QUERY_TYPES, f"q is bf16, fp16 or fp32, not {q.dtype}"
+    TQ, Hq, _ = q.shape
+    assert k_cache.dim() == 4 and v_cache.shape == k_cache.shape
+    P, ps, Hkv, _ = k_cache.shape
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        check_cache(c, Hkv, HEAD_DIM, name)
+        assert c.device == device, "all tensors must share the query's device"
+    assert Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"{Hq} query heads over {Hkv} kv heads"
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] >= B
+    assert block_table.stride(1) == 1 or block_table.shape[1] <= 1, "block_table needs unit last stride"
+    assert seq_lens.dtype == torch.int32 and seq_lens.is_contiguous() and seq_lens.numel() >= B
+    assert block_table.device == device and seq_lens.device == device, "all tensors must share the query's device"
+    if softmax_scale is None:
+        softmax_scale = HEAD_DIM ** -0.5
+    bound = block_table.shape[1] * ps
+    bound = bound if max_seq_len is None else min(int(max_seq_len), bound)
+    if out is None:
+        out = torch.empty(TQ, Hq, HEAD_DIM, dtype=q.dtype, device=device)
+    else:
+        assert out.dtype in _QUERY_TYPES and out.shape == (TQ, Hq, HEAD_DIM) and out.stride(2) == 1 and out.device == device
+        assert distinct(out), "out is a broadcast"
+    lse = torch.empty(Hq, TQ, dtype=torch.float32, device=device) if return_softmax_lse else None
+    with on_device(device):
+        need = mxfp4_workspace_floats(B, TQ, n, Hq, Hkv, bound)
+        if need and (workspace is None or workspace.numel() < need):
+            workspace = torch.empty(need, dtype=torch.float32, device=device)
+        assert workspace is None or (workspace.dtype == torch.float32 and workspace.device == device
+                                     and workspace.is_contiguous())
+        st = lib().psk_paged_mxfp4_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), dtype_code(q.dtype), k_cache.data_ptr(), v_cache.data_ptr(),
+            i64_array(k_cache.stride()[:3]), i64_array(v_cache.stride()[:3]), block_table.data_ptr(),
+            block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), B, Hq, Hkv, HEAD_DIM, ps, P, bound, TQ, n,
+            ptr(cu_seqlens_q), 1 if causal else 0, float(softmax_scale), out.data_ptr(), out.stride(0), out.stride(1),
+            dtype_code(out.dtype), ptr(lse), TQ if lse is not None else 0, ptr(workspace),
+            0 if workspace is None else workspace.numel(), stream_handle(device),
+        )
+    check(st, "paged_mxfp4_attention")
+    return (out, lse) if return_softmax_lse else out
+
+
+def mxfp4_workspace_floats(num_seqs: int, total_q: int, max_seqlen_q: int, num_q_heads: int, num_kv_heads: int,
+                           max_seq_len: int) -> int:
+    """float32 elements of ``paged_mxfp4_attention``'s workspace."""
+    n = int(lib().psk_paged_mxfp4_workspace_len(num_seqs, total_q, max_seqlen_q, num_q_heads, num_kv_heads,
+                                                 max_seq_len))
+    if n < 0:
+        check(n, "paged mxfp4 workspace")
+    return n
+
+
 def _chunked_queries(cu_seqlens_q, total_q, seqused_k, block_table, chunk, causal, descales):
     """Query tokens of each sequence cut into chunks of at most ``chunk``
     consecutive tokens, each chunk a sequence of its own for the reader, built
@@ -619,13 +710,20 @@ def flash_attn_varlen_func(
     routes through this same entry, attention.py:577-585, or more than 16
     query heads per kv head) the step runs ``paged_prefill_attention``, which
     reads each kv head's keys once per block of 256 query rows; ``num_splits``
-    does not apply there, and ``max_seqlen_k`` only helps to choose the kernel."""
+    does not apply there, and ``max_seqlen_k`` only helps to choose the kernel.
+
+    A uint8 cache is one of 4-bit rows (``mxfp4_kv``) and goes to
+    ``paged_mxfp4_attention``, with an unquantized q and no descales."""
     assert seqused_k is not None and block_table is not None, "paged attention needs seqused_k and block_table"
     B = seqused_k.shape[0]
     assert cu_seqlens_q is not None and cu_seqlens_q.shape[0] == B + 1
     group = q.shape[1] // k.shape[2] if k.shape[2] else 0
     q_len = int(max_seqlen_q)
     ps = k.shape[1]
+    if k.dtype == torch.uint8:
+        assert q_descale is None and k_descale is None and v_descale is None, "a 4-bit cache takes no descales"
+        return paged_mxfp4_attention(q, k, v, block_table, seqused_k, cu_seqlens_q, q_len, softmax_scale, out,
+                                     return_softmax_lse, causal, max_seqlen_k)
     bound = block_table.shape[1] * ps if max_seqlen_k is None else min(int(max_seqlen_k), block_table.shape[1] * ps)
     if q_len * max(group, 1) > MAX_ROWS:
         return paged_prefill_attention(q, k, v, block_table, seqused_k, cu_seqlens_q, q_len, softmax_scale,

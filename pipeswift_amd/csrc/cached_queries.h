@@ -30,7 +30,8 @@ struct CachedQueries {
 
 // PSK_OK with `a` filled in, or the refusal.  Pointers are looked at last, so
 // that an empty step may leave them NULL (*empty).
-inline int check_cached_queries(const CachedQueries& c, DecodeArgs& a, bool* empty) {
+// `align`: bytes that cache rows start on (16 for FP8 rows, 4 for 4-bit ones, which take no FP8 query).
+inline int check_cached_queries(const CachedQueries& c, DecodeArgs& a, bool* empty, int align = 16) {
   *empty = false;
   if (c.num_seqs < 0 || c.num_kv_heads <= 0 || c.num_q_heads <= 0 || c.num_q_heads % c.num_kv_heads)
     return fail(PSK_E_ARG, "bad head counts (q %lld, kv %lld)", (long long)c.num_q_heads, (long long)c.num_kv_heads);
@@ -47,7 +48,7 @@ inline int check_cached_queries(const CachedQueries& c, DecodeArgs& a, bool* emp
   if (c.block_size <= 0 || c.block_size > INT32_MAX || c.num_blocks <= 0 || c.num_blocks > INT32_MAX ||
       c.block_table_width <= 0)
     return fail(PSK_E_ARG, "bad cache geometry");
-  if (c.q_dtype != PSK_DTYPE_FP8_E4M3FN && c.q_dtype != PSK_DTYPE_BF16 && c.q_dtype != PSK_DTYPE_F16 &&
+  if ((c.q_dtype != PSK_DTYPE_FP8_E4M3FN || align < 16) && c.q_dtype != PSK_DTYPE_BF16 && c.q_dtype != PSK_DTYPE_F16 &&
       c.q_dtype != PSK_DTYPE_F32)
     return fail(PSK_E_DTYPE, "query dtype %d", c.q_dtype);
   if (!std::isfinite(c.softmax_scale)) return fail(PSK_E_ARG, "softmax_scale is not finite");
@@ -59,7 +60,8 @@ inline int check_cached_queries(const CachedQueries& c, DecodeArgs& a, bool* emp
     return fail(PSK_E_ARG, "NULL pointer");
   const uint64_t k_align[4] = {uint64_t(uintptr_t(c.k)), uint64_t(c.k_strides[0]), uint64_t(c.k_strides[1]),
                                uint64_t(c.k_strides[2])};
-  if (common_align(k_align, 4, 16) < 16) return fail(PSK_E_ARG, "K/V caches need 16-byte aligned bases and strides");
+  if (common_align(k_align, 4, align) < align)
+    return fail(PSK_E_ARG, "K/V caches need %d-byte aligned bases and strides", align);
   const int qsz = dtype_size(c.q_dtype);
   const uint64_t q_align[3] = {uint64_t(uintptr_t(c.q)), uint64_t(c.q_tok_stride * qsz), uint64_t(c.q_head_stride * qsz)};
   if (common_align(q_align, 3, 16) < 16) return fail(PSK_E_ARG, "query rows need 16-byte alignment");
