@@ -208,6 +208,7 @@ struct JobSpace {
   int32_t min_run;                   // units a run has at least
   int32_t idle;                      // sequences without query tokens are jobs too
   int32_t width;                     // keys past it cost nothing
+  int32_t most = INT32_MAX;          // sequences of more query tokens are no jobs
 };
 
 __device__ __forceinline__ int32_t key_steps(const JobSpace& s, int32_t len) {
@@ -249,7 +250,7 @@ struct SeqWindow {
     if (from + lane < s.num_seqs) {
       const SeqRows r = seq_rows(a, s.total_q, from + lane);
       first = r.first;
-      n = r.n;
+      n = r.n <= s.most ? r.n : 0;
       len = cached_len(a, from + lane);
     }
     price(s, lane);

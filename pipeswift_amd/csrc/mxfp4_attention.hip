@@ -37,8 +37,8 @@
 
 #include <algorithm>
 
-#include "cached_queries.h"
-#include "mxfp4.h"
+#include "mxfp4_attention.h"
+#include "prefill_runs.h"
 
 using namespace psk_detail;
 
@@ -48,13 +48,11 @@ constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kTile = 32;          // keys of a wave's tile
 constexpr int kTileShift = 5;
-constexpr int kCodes = kHead / 2;  // bytes of a row's codes
 constexpr int kPages = 1024;       // page ids a piece stages at a time
 constexpr int kMaxSlots = 512;     // resident workgroups the workspace is sized for
 constexpr int kOver = 2;
 constexpr int kMinRun = 2;
 constexpr int kWholeKeys = 1024;
-constexpr float kLimit = 32768.0f;  // a lane's share of a tile's weights before a row's maximum is raised
 
 struct Mx4Args {
   DecodeArgs a;
@@ -64,73 +62,20 @@ struct Mx4Args {
   int32_t wph_shift;     // log2 of the waves of a head
   int32_t row_blocks;    // workgroups that share a run's keys, 16 kSets query rows each
   int32_t rows;          // query rows of a record
+  int32_t max_rows;      // of a sequence and kv head
   int32_t whole;         // a workgroup takes all of a job's keys, and nothing is merged
   int32_t out_dtype;
   float* records;        // [max_runs][row_blocks][2][hg][rows][kHead + 4]
 };
 
-constexpr int kRecord = kHead + 4;  // floats of a row's record: accumulators, maximum, sum
-
 __device__ __forceinline__ float* record(const Mx4Args& p, int64_t run, int block, int slot, int hl, int row) {
   return p.records + ((((run * p.row_blocks + block) * 2 + slot) * p.hg + hl) * p.rows + row) * kRecord;
-}
-
-typedef u32x4 u32x4_any __attribute__((aligned(4)));
-
-__device__ __forceinline__ void store4(char* dst, int dtype, f32x4 v) {
-  if (dtype == PSK_DTYPE_F32) {
-    *reinterpret_cast<f32x4*>(dst) = v;
-  } else if (dtype == PSK_DTYPE_BF16) {
-    using E = Elt<PSK_DTYPE_BF16>;
-    *reinterpret_cast<u32x2*>(dst) = u32x2{uint32_t(E::from_f32(v[0])) | (uint32_t(E::from_f32(v[1])) << 16),
-                                           uint32_t(E::from_f32(v[2])) | (uint32_t(E::from_f32(v[3])) << 16)};
-  } else {
-    using E = Elt<PSK_DTYPE_F16>;
-    *reinterpret_cast<u32x2*>(dst) = u32x2{uint32_t(E::from_f32(v[0])) | (uint32_t(E::from_f32(v[1])) << 16),
-                                           uint32_t(E::from_f32(v[2])) | (uint32_t(E::from_f32(v[3])) << 16)};
-  }
-}
-
-// Columns col .. col + 3 of a query row, and its lse with the first.
-__device__ __forceinline__ void finish(const Mx4Args& p, const SeqRows& r, int h, int row, int col, f32x4 o, float m,
-                                       float sum) {
-  const DecodeArgs& a = p.a;
-  const int i = row / a.heads, hq = h * a.heads + row - i * a.heads;
-  if (i >= r.n) return;
-  const bool any = sum != 0.0f;  // (a NaN sum counts)
-  const float f = any ? 1.0f / sum : 0.0f;
-  const f32x4 v = any ? o * f : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const int osz = p.out_dtype == PSK_DTYPE_F32 ? 4 : 2;
-  store4(a.out + (int64_t(r.first) + i) * a.out_tok_stride + int64_t(hq) * a.out_head_stride + col * osz, p.out_dtype, v);
-  if (a.lse && col == 0)
-    a.lse[int64_t(hq) * a.lse_head_stride + r.first + i] =
-        any ? (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f : -__builtin_inff();
 }
 
 struct Tile {
   u32x4 k[2], v[2];
   uint32_t ks[2], vs[2];
 };
-
-// Eight elements of a query row as bf16 and, for the wider types, what that leaves.
-template <int Q_DT>
-__device__ __forceinline__ void query8(const char* p, uint32_t sign, bf16x8& hi, bf16x8& lo) {
-  if constexpr (Q_DT == PSK_DTYPE_BF16) {
-    u32x4 x = p ? *reinterpret_cast<const u32x4*>(p) : u32x4(0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] ^= sign;
-    hi = __builtin_bit_cast(bf16x8, x);
-  } else {
-    typename Elt<Q_DT>::Bits e[8] = {};
-    if (p) __builtin_memcpy(e, p, sizeof(e));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = sign ? -Elt<Q_DT>::to_f32(e[i]) : Elt<Q_DT>::to_f32(e[i]);
-      hi[i] = __bf16(x);
-      lo[i] = __bf16(x - float(hi[i]));
-    }
-  }
-}
 
 template <int Q_DT, int kSets>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kSets == 1 && Q_DT == PSK_DTYPE_BF16 ? 4 : 2)))
@@ -219,7 +164,7 @@ mx4_attention_kernel(Mx4Args args) {
                                        : nullptr;
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        query8<Q_DT>(src ? src + (32 * l4 + 8 * q) * Elt<Q_DT>::kSize : nullptr, sl_signed < 0.0f ? 0x80008000u : 0u,
+        query8<Q_DT>(src ? src + (32 * l4 + 8 * q) * Elt<Q_DT>::kSize : nullptr, sl_signed < 0.0f,
                      qop[s][q], qlo[kPairs ? s : 0][q]);
     }
     float m[kSets], l[kSets];
@@ -331,7 +276,7 @@ mx4_attention_kernel(Mx4Args args) {
             }
           };
           weigh();
-          if (__builtin_expect(__any(!(sum <= kLimit)), 0)) {  // (NaN scores come here too)
+          if (__builtin_expect(__any(!(sum <= kShareMost)), 0)) {  // (NaN scores come here too)
             float top = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, sc[e][i]);
@@ -413,7 +358,7 @@ mx4_attention_kernel(Mx4Args args) {
           v = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
         const int row = row0 + 16 * s + l15, col = 16 * d + 4 * l4;
         if (all) {
-          finish(rest, r, h, row, col, v, top, sum);
+          finish(rest.a, rest.out_dtype, r, h, row, col, v, top, sum);
         } else if (row < r.n * rest.a.heads) {
           float* rec = record(rest, j, block, c.from == 0 ? 1 : 0, hl, 16 * s + l15);
           *reinterpret_cast<f32x4*>(rec + col) = v;
@@ -438,14 +383,14 @@ __global__ void __launch_bounds__(kMergeThreads) merge_mx4_kernel(Mx4Args p, int
   __shared__ f32x4 s_o[kParts][32];
   __shared__ float s_m[kParts], s_l[kParts];
   const int tid = int(threadIdx.x), lane = tid & 63, part = tid >> 5, at4 = tid & 31;
-  const int max_rows = a.q_len * a.heads;
+  const int max_rows = p.max_rows;
   const int kv_heads = p.s.heads * p.hg;
   for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
     const int64_t job = uniform_div(task, max_rows);
     const int row = int(task - job * max_rows);
     const int b = int(uniform_div(job, kv_heads)), h = int(job - int64_t(b) * kv_heads);
     const SeqRows r = seq_rows(a, p.s.total_q, b);
-    if (row >= r.n * a.heads) continue;
+    if (r.n > p.s.most || row >= r.n * a.heads) continue;
     SeqWindow seqs;
     const StepRuns cost = step_runs(a, p.s, seqs, lane);
     const int64_t before = units_before(a, p.s, b, seqs, lane);
@@ -496,7 +441,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_mx4_kernel(Mx4Args p, int
         sum += s_l[u] * f;
         o += s_o[u][at4] * f;
       }
-      finish(p, r, h, row, 4 * at4, o, top, sum);
+      finish(a, p.out_dtype, r, h, row, 4 * at4, o, top, sum);
     }
   }
 }
@@ -534,6 +479,21 @@ Mx4Shape mx4_shape(int64_t num_seqs, int64_t max_seqlen_q, int64_t num_q_heads, 
   return s;
 }
 
+// Which kernels a step takes: sequences of at most kFewRows query rows a kv head go by
+// rows, those of more by blocks of 256 (mxfp4_prefill.hip), in one launch each.
+constexpr int kFewRows = 32;
+enum Route { kRows, kBlocks, kBoth };
+Route route(int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, int64_t heads) {
+  if (max_seqlen_q * heads <= kFewRows || heads > kBlockRows) return kRows;
+  // (more sequences than are ordered by their lengths: all by blocks)
+  return num_seqs == 1 || heads > kFewRows || total_q == num_seqs * max_seqlen_q || num_seqs > kOrderMax ? kBlocks : kBoth;
+}
+
+// Query tokens of a sequence that goes by rows, at most.
+int64_t row_tokens(Route r, int64_t max_seqlen_q, int64_t heads) {
+  return r == kBoth ? std::max<int64_t>(kFewRows / heads, 1) : max_seqlen_q;
+}
+
 template <int Q_DT>
 int launch(const Mx4Args& p, const Mx4Shape& s, hipStream_t st) {
   const int64_t jobs = int64_t(p.s.num_seqs) * p.s.heads;
@@ -541,7 +501,7 @@ int launch(const Mx4Args& p, const Mx4Shape& s, hipStream_t st) {
   if (s.sets == 1) hipLaunchKernelGGL((mx4_attention_kernel<Q_DT, 1>), grid, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((mx4_attention_kernel<Q_DT, 2>), grid, dim3(kThreads), 0, st, p);
   if (const int e = check_launch("mx4_attention_kernel launch"); e != PSK_OK || p.whole) return e;
-  const int64_t tasks = int64_t(p.s.num_seqs) * p.s.heads * p.hg * p.a.q_len * p.a.heads;
+  const int64_t tasks = int64_t(p.s.num_seqs) * p.s.heads * p.hg * p.max_rows;
   const dim3 merge{unsigned(std::min<int64_t>(tasks, 1 << 20)), 1u, 1u};
   if (s.sets == 1) hipLaunchKernelGGL((merge_mx4_kernel<16>), merge, dim3(kMergeThreads), 0, st, p, tasks);
   else hipLaunchKernelGGL((merge_mx4_kernel<32>), merge, dim3(kMergeThreads), 0, st, p, tasks);
@@ -557,8 +517,13 @@ int64_t psk_paged_mxfp4_workspace_len(int64_t num_seqs, int64_t total_q, int64_t
   if (num_seqs < 0 || total_q < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
       max_seqlen_q <= 0 || max_seqlen_q > INT32_MAX / (num_q_heads / num_kv_heads) || max_seq_len < 0)
     return PSK_E_ARG;
-  const Mx4Shape s = mx4_shape(num_seqs, max_seqlen_q, num_q_heads, num_kv_heads, max_seq_len, kMaxSlots);
-  return s.whole ? 0 : 4 + s.max_runs * s.row_blocks * 2 * s.hg * s.rows * kRecord;
+  const Route r = route(num_seqs, total_q, max_seqlen_q, num_q_heads / num_kv_heads);
+  const Mx4Shape s = mx4_shape(num_seqs, row_tokens(r, max_seqlen_q, num_q_heads / num_kv_heads), num_q_heads, num_kv_heads,
+                               max_seq_len, kMaxSlots);
+  const int64_t own = s.whole ? 0 : 4 + s.max_runs * s.row_blocks * 2 * s.hg * s.rows * kRecord;
+  if (r == kRows) return own;
+  const int64_t blocks = mx4_prefill_floats(num_seqs, total_q, max_seqlen_q, num_q_heads, num_kv_heads, max_seq_len);
+  return r == kBlocks ? blocks : std::max(own, blocks);  // (one after the other)
 }
 
 int psk_paged_mxfp4_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int q_dtype,
@@ -604,8 +569,18 @@ int psk_paged_mxfp4_attention(const void* q, int64_t q_tok_stride, int64_t q_hea
   a.out_head_stride = out_head_stride * osz;
   a.lse = lse;
   a.lse_head_stride = lse_head_stride;
-  const Mx4Shape s = mx4_shape(num_seqs, max_seqlen_q, num_q_heads, num_kv_heads, max_seq_len, mx4_slots());
   p.scale_log2 = double(softmax_scale) * 1.4426950408889634;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const Route way = route(num_seqs, total_q, max_seqlen_q, a.heads);
+  const int64_t row_q = row_tokens(way, max_seqlen_q, a.heads);
+  if (way != kRows) {
+    const int32_t most = way == kBoth ? int32_t(kFewRows / a.heads) : 0;
+    const Mx4Prefill step{num_seqs, total_q, max_seqlen_q, max_seq_len, most, p.scale_log2, q_dtype, out_dtype};
+    const int e = launch_mx4_prefill(a, step, workspace, st);
+    if (e != PSK_OK || way == kBlocks) return e;
+    p.s.most = most;
+  }
+  const Mx4Shape s = mx4_shape(num_seqs, row_q, num_q_heads, num_kv_heads, max_seq_len, mx4_slots());
   p.s.num_seqs = int32_t(num_seqs);
   p.s.total_q = int32_t(total_q);
   p.s.heads = int32_t(s.groups);
@@ -618,6 +593,7 @@ int psk_paged_mxfp4_attention(const void* q, int64_t q_tok_stride, int64_t q_hea
   p.wph_shift = int32_t(s.wph_shift);
   p.row_blocks = int32_t(s.row_blocks);
   p.rows = int32_t(s.rows);
+  p.max_rows = int32_t(row_q * a.heads);
   p.whole = s.whole;
   p.out_dtype = out_dtype;
   p.records = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
@@ -625,7 +601,6 @@ int psk_paged_mxfp4_attention(const void* q, int64_t q_tok_stride, int64_t q_hea
   if (std::max(num_seqs * s.groups, s.max_runs) > kMost / s.row_blocks)
     return fail(PSK_E_ARG, "too many rows (%lld sequences of up to %lld query tokens)", (long long)num_seqs,
                 (long long)max_seqlen_q);
-  hipStream_t st = static_cast<hipStream_t>(stream);
   switch (q_dtype) {
     case PSK_DTYPE_BF16: return launch<PSK_DTYPE_BF16>(p, s, st);
     case PSK_DTYPE_F16: return launch<PSK_DTYPE_F16>(p, s, st);
