@@ -97,6 +97,20 @@ __device__ __forceinline__ uint32_t mx_quantize8(const typename Elt<DT>::Bits (&
   return byte == kMxNan ? 0u : w;
 }
 
+// Whether any of a group's values (16 code bytes) is NaN or, as 4 and 6 times 2^126 and
+// 2 and more times 2^127 are, past the largest finite one.
+__device__ __forceinline__ bool mx_not_finite(u32x4 codes, uint32_t byte) {
+  if (byte < 253) return false;
+  uint32_t four = 0, six = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t high = codes[i] & 0x44444444u;
+    four |= high;
+    six |= high & (codes[i] << 1);
+  }
+  return byte == kMxNan || (byte == 254 ? four : six) != 0;
+}
+
 // Eight codes -> eight elements.
 __device__ __forceinline__ u32x4 mx_bf16x8(uint32_t w, float s) {
   return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0)),

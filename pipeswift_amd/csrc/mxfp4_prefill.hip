@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
   auto put_stage = [&](auto wide_tag, int st, int t) {
     constexpr bool WIDE = decltype(wide_tag)::value;
     if (is_v) {
-      if (__builtin_expect(byte == kMxNan, 0)) {  // 0 x NaN: zeros here, and at the end for the rows that see it
+      if (__builtin_expect(mx_not_finite(raw, byte), 0)) {  // (0 x NaN) zeros here, NaN at the end for the rows that see it
         atomicMin(&s_nan[sgroup], t * kStage + skey);
         byte = 127;
         raw = u32x4(0);

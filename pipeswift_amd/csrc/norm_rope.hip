@@ -9,15 +9,16 @@
 // axis.  The result is rounded once to the input's type; K then goes to the cache as
 // psk_reshape_and_cache (or its 4-bit form) would write that, V as it is.
 //
-// A workgroup is a token.  A lane holds eight elements of a head (so a head is a
-// power of two of lanes, LPR, and its sum of squares a few DPP steps), and the same
-// eight of every head it takes: the factors of its elements, w c and w s, are made
-// once for the queries and once for the keys.  An element's partner comes from its
+// A token is a wave's, or a workgroup's where the tokens are few.  A lane holds eight
+// elements of a head (so a head is a power of two of lanes, LPR, and its sum of
+// squares a few DPP steps), and the same eight of every head it takes: the factors of
+// its elements, w c and w s, are made once for the queries and once for the keys.  An element's partner comes from its
 // lane by ds_bpermute as it was loaded; its norm is the row's own.
 //
 // C ABI: include/pipeswift_kv.h.  Nothing here allocates or synchronizes.
 
 #include <cmath>
+#include <type_traits>
 
 #include "mxfp4.h"
 
@@ -28,6 +29,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBatch = 4;  // heads of a lane loaded before the first is computed
 constexpr int kAxes = 4;
+constexpr int64_t kManyTokens = 2048;
 
 enum CacheKind { kNoCache = 0, kCopy = 1, kFp8 = 2, kMx4 = 3 };
 
@@ -37,7 +39,9 @@ struct NormRopeArgs {
   char* out[2];                     // q, k; NULL: not written
   int64_t out_tok[2], out_head[2];
   const char* weight[2];            // NULL: no norm
-  int32_t weight_f32;
+  int32_t weight_f32, weight_wide;  // on 16-byte boundaries
+  int32_t tokens_shift;             // log2 of the tokens of a workgroup (of four waves)
+  int64_t num_tokens;
   float eps;
   int32_t num_q, num_kv, head_size, chunks;
   const char* pos;
@@ -153,40 +157,51 @@ __device__ __forceinline__ void put(const Eight<DT>& x, char* row, int chunk, in
 
 template <int DT, int LPR, int KIND>
 __global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRopeArgs a) {
-  const int64_t t = blockIdx.x;
-  const int tid = int(threadIdx.x), lane = tid & 63;
-  const int c = tid & (LPR - 1);           // this lane's eight elements of a head
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = int(threadIdx.x) & 63;
+  const int64_t t = (int64_t(blockIdx.x) << a.tokens_shift) + (wave >> (2 - a.tokens_shift));
+  if (t >= a.num_tokens) return;
+  const int c = lane & (LPR - 1);          // this lane's eight elements of a head
   const bool in_row = c < a.chunks;
-  constexpr int kRows = kThreads / LPR;    // heads a pass takes
-  const int rows = a.num_q + a.num_kv * (KIND == kNoCache ? 1 : 2);
+  constexpr int kRows = 64 / LPR;          // heads of a unit
+  // units of queries, keys and values: a wave takes every `stride`-th
+  const int stride = 4 >> a.tokens_shift, first_unit = wave & (stride - 1);
+  const int q_units = (a.num_q + kRows - 1) / kRows, kv_units = (a.num_kv + kRows - 1) / kRows;
+  const int units = q_units + kv_units * (KIND == kNoCache ? 1 : 2);
   const int d0 = 8 * c;
   const bool turns = d0 < 2 * a.half;
 
+  struct Unit {
+    int which, h;  // uniform; this lane's head
+    bool live;     // the head is there
+  };
+  auto unit_of = [&](int u) {
+    Unit x;
+    x.which = u < q_units ? 0 : u < q_units + kv_units ? 1 : 2;
+    x.h = (u - (x.which == 0 ? 0 : x.which == 1 ? q_units : q_units + kv_units)) * kRows + lane / LPR;
+    x.live = u < units && x.h < (x.which == 0 ? a.num_q : a.num_kv);
+    return x;
+  };
   // the first heads are on their way while the factors are made
   Eight<DT> x[kBatch];
-  auto load = [&](int r0) {
+  auto load = [&](int u0) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int r = r0 + u * kRows + tid / LPR;
-      x[u].zero();
-      if (r < rows && in_row) {
-        const int which = r < a.num_q ? 0 : r < a.num_q + a.num_kv ? 1 : 2;
-        const int h = r - (which == 0 ? 0 : which == 1 ? a.num_q : a.num_q + a.num_kv);
-        x[u].load(a.in[which] + t * a.in_tok[which] + h * a.in_head[which] + d0 * Elt<DT>::kSize);
-      }
+    for (int i = 0; i < kBatch; ++i) {
+      const Unit y = unit_of(u0 + i * stride);
+      x[i].zero();
+      if (y.live && in_row) x[i].load(a.in[y.which] + t * a.in_tok[y.which] + y.h * a.in_head[y.which] + d0 * Elt<DT>::kSize);
     }
   };
-  load(0);
+  load(first_unit);
 
   int64_t slot = -1;
   if constexpr (KIND != kNoCache) slot = a.slots[t];
 
   // cosine and signed sine of each element's pair; a position outside the table gives NaN
   float cs[8], sn[8];
-  int partner = c;  // the chunk that holds the other halves of its pairs
+  const bool first = d0 < a.half;
+  // the chunk that holds the other halves of its pairs
+  const int partner = a.interleaved || !turns ? c : first ? c + a.half / 8 : c - a.half / 8;
   {
-    const bool first = d0 < a.half;
-    if (!a.interleaved && turns) partner = first ? c + a.half / 8 : c - a.half / 8;
     const int i0 = a.interleaved ? d0 / 2 : first ? d0 : d0 - a.half;
     auto position = [&](int axis) {
       const int64_t at = axis * a.pos_axis + t;
@@ -256,16 +271,25 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRopeArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = wp[j] = 1.0f;
     if (a.weight[k] && in_row) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int own = d0 + j, other = a.interleaved ? own ^ 1 : 8 * partner + j;
+      auto get = [&](int at, float (&y)[8]) {
         if (a.weight_f32) {
-          w[j] = reinterpret_cast<const float*>(a.weight[k])[own];
-          wp[j] = reinterpret_cast<const float*>(a.weight[k])[other];
+          typename Elt<PSK_DTYPE_F32>::Bits e[8];
+          load8<PSK_DTYPE_F32>(a.weight[k] + 4 * at, a.weight_wide, e);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = Elt<PSK_DTYPE_F32>::to_f32(e[j]);
         } else {
-          w[j] = Elt<DT>::to_f32(reinterpret_cast<const typename Elt<DT>::Bits*>(a.weight[k])[own]);
-          wp[j] = Elt<DT>::to_f32(reinterpret_cast<const typename Elt<DT>::Bits*>(a.weight[k])[other]);
+          typename Elt<DT>::Bits e[8];
+          load8<DT>(a.weight[k] + Elt<DT>::kSize * at, a.weight_wide, e);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = Elt<DT>::to_f32(e[j]);
         }
+      };
+      get(d0, w);
+      if (a.interleaved) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) wp[j] = w[j ^ 1];
+      } else {
+        get(8 * partner, wp);
       }
     }
 #pragma unroll
@@ -287,50 +311,51 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRopeArgs a) {
     for (int k = 0; k < 2; ++k) qs[k] = make_qscale_uniform(a.scale[k] ? *a.scale[k] : 1.0f);
   }
 
-  for (int r0 = 0; r0 < rows; r0 += kBatch * kRows) {
-    if (r0 > 0) load(r0);
+  // a unit of queries (0) or keys (1)
+  auto turn = [&](auto kind, const Eight<DT>& raw, const Unit& y) {
+    constexpr int K = decltype(kind)::value;
+    float v[8], vp[8];
+    raw.unpack(v);
+    if (a.interleaved) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int r = r0 + u * kRows + tid / LPR;
-      if (r >= rows) continue;  // (whole heads)
-      if (r >= a.num_q + a.num_kv) {
-        const int h = r - a.num_q - a.num_kv;
-        put<DT, KIND>(x[u], a.cache[1] + page * a.blk[1] + off * a.row[1] + h * a.head[1], c, a.head_size, qs[1],
-                      cached && in_row);
-        continue;
-      }
-      const int k = r >= a.num_q;
-      const int h = r - (k ? a.num_q : 0);
-      float v[8], vp[8];
-      x[u].unpack(v);
-      if (a.interleaved) {
+      for (int j = 0; j < 8; ++j) vp[j] = v[j ^ 1];
+    } else {
+      raw.from_lane(from).unpack(vp);
+    }
+    float rstd = 1.0f;
+    if (a.weight[K]) {
+      float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vp[j] = v[j ^ 1];
-      } else {
-        x[u].from_lane(from).unpack(vp);
-      }
-      float rstd = 1.0f;
-      if (a.weight[k]) {
-        float sum = 0.0f;
+      for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(v[j], v[j], sum);
+      rstd = __builtin_amdgcn_rsqf(row_sum<LPR>(sum) / float(a.head_size) + a.eps);
+    }
+    float z[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(v[j], v[j], sum);
-        rstd = __builtin_amdgcn_rsqf(row_sum<LPR>(sum) / float(a.head_size) + a.eps);
-      }
-      float y[8];
+    for (int j = 0; j < 8; ++j) {
+      const float own = v[j] * rstd * wc[K][j];
+      z[j] = turns ? __builtin_fmaf(vp[j] * rstd, ws[K][j], own) : own;
+    }
+    Eight<DT> packed;
+    packed.pack(z);
+    if (a.out[K] && y.live && in_row)
+      packed.store(a.out[K] + t * a.out_tok[K] + y.h * a.out_head[K] + d0 * Elt<DT>::kSize);
+    if constexpr (K == 1 && KIND != kNoCache)
+      put<DT, KIND>(packed, a.cache[0] + page * a.blk[0] + off * a.row[0] + y.h * a.head[0], c, a.head_size, qs[0],
+                    cached && y.live && in_row);
+  };
+  for (int u0 = first_unit; u0 < units; u0 += kBatch * stride) {
+    if (u0 > first_unit) load(u0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float own = v[j] * rstd * (k ? wc[1][j] : wc[0][j]);
-        y[j] = turns ? __builtin_fmaf(vp[j] * rstd, k ? ws[1][j] : ws[0][j], own) : own;
-      }
-      Eight<DT> z;
-      z.pack(y);
-      char* out = k ? a.out[1] : a.out[0];
-      if (out && in_row)
-        z.store(out + t * (k ? a.out_tok[1] : a.out_tok[0]) + h * (k ? a.out_head[1] : a.out_head[0]) + d0 * Elt<DT>::kSize);
-      if constexpr (KIND != kNoCache) {
-        if (k)
-          put<DT, KIND>(z, a.cache[0] + page * a.blk[0] + off * a.row[0] + h * a.head[0], c, a.head_size, qs[0],
-                        cached && in_row);
+    for (int i = 0; i < kBatch; ++i) {
+      if (u0 + i * stride >= units) break;
+      const Unit y = unit_of(u0 + i * stride);
+      if (y.which == 0) {
+        turn(std::integral_constant<int, 0>{}, x[i], y);
+      } else if (y.which == 1) {
+        turn(std::integral_constant<int, 1>{}, x[i], y);
+      } else if constexpr (KIND != kNoCache) {
+        put<DT, KIND>(x[i], a.cache[1] + page * a.blk[1] + off * a.row[1] + y.h * a.head[1], c, a.head_size, qs[1],
+                      cached && y.live && in_row);
       }
     }
   }
@@ -338,7 +363,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRopeArgs a) {
 
 template <int DT, int LPR>
 void launch_kind(const NormRopeArgs& a, int kind, int64_t tokens, hipStream_t st) {
-  const dim3 grid{unsigned(tokens), 1u, 1u};
+  const dim3 grid{unsigned(ceil_div(tokens, int64_t(1) << a.tokens_shift)), 1u, 1u};
   switch (kind) {
     case kNoCache: hipLaunchKernelGGL((norm_rope_kernel<DT, LPR, kNoCache>), grid, dim3(kThreads), 0, st, a); break;
     case kCopy: hipLaunchKernelGGL((norm_rope_kernel<DT, LPR, kCopy>), grid, dim3(kThreads), 0, st, a); break;
@@ -456,6 +481,9 @@ int psk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const 
   a.weight[0] = static_cast<const char*>(q_weight);
   a.weight[1] = static_cast<const char*>(k_weight);
   a.weight_f32 = weight_dtype == PSK_DTYPE_F32;
+  a.weight_wide = ((uint64_t(uintptr_t(q_weight)) | uint64_t(uintptr_t(k_weight))) & 15) == 0;
+  a.num_tokens = num_tokens;
+  a.tokens_shift = num_tokens >= kManyTokens ? 2 : 0;
   a.eps = eps;
   a.num_q = int32_t(num_q_heads);
   a.num_kv = int32_t(num_kv_heads);
