@@ -577,8 +577,10 @@ int psk_gather_mla_fp8_tiles(const void* kv_cache, void* dst, const int32_t* blo
  * append of K and V, in one launch (build-defined; the reference does these as
  * separate layers before append_kv_cache).
  *
- * For head x of token t (q + t * q_strides[0] + h * q_strides[1] elements, k and v
- * alike; D = head_size contiguous elements, 16-byte aligned): y = x * rsqrt(mean
+ * `strides`: 16 of them, token and head of q, k, v, q_out and k_out (elements), then
+ * block, slot and head of key_cache and of value_cache (elements; bytes for a 4-bit
+ * cache); those of absent tensors are not read.
+ * For head x of token t (D = head_size contiguous elements, 16-byte aligned): y = x * rsqrt(mean
  * x^2 + eps) * weight in float32 (weight NULL: y = x), then for pair i < rot_dim /
  * 2, (a, b) = (y_i, y_{i + rot_dim/2}), or (y_2i, y_{2i+1}) if interleaved, becomes
  * (a c - b s, b c + a s) with c = cos_sin[p * cos_sin_stride + i], s = the same row
@@ -591,21 +593,19 @@ int psk_gather_mla_fp8_tiles(const void* kv_cache, void* dst, const int32_t* blo
  * each may be its input itself.  With key_cache and value_cache (both or neither)
  * the rounded keys and the values also go to the caches at slot_mapping, the bytes
  * that psk_reshape_and_cache (cache_dtype = dtype or PSK_DTYPE_FP8_E4M3FN with
- * k_scale and v_scale) or psk_reshape_and_cache_mxfp4 (PSK_DTYPE_MXFP4, strides in
- * bytes) would write; negative and out-of-range slots are skipped.  Cache rows are
+ * k_scale and v_scale) or psk_reshape_and_cache_mxfp4 (PSK_DTYPE_MXFP4) would
+ * write; negative and out-of-range slots are skipped.  Cache rows are
  * aligned to 16, 8 and 4 bytes for these types.
  * head_size: a multiple of 8 up to 512 (of 32 for a 4-bit cache).  rot_dim: a
  * multiple of 16, or of 8 if interleaved.  weight_dtype: dtype or PSK_DTYPE_F32.
  * At most 4 axes.
  */
-int psk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
-                  const int64_t* v_strides, int dtype, int64_t num_tokens, int64_t num_q_heads, int64_t num_kv_heads,
+int psk_norm_rope(const void* q, const void* k, const void* v, void* q_out, void* k_out, void* key_cache, void* value_cache,
+                  const int64_t* strides, int dtype, int64_t num_tokens, int64_t num_q_heads, int64_t num_kv_heads,
                   int64_t head_size, const void* q_weight, const void* k_weight, int weight_dtype, float eps,
                   const void* positions, int position_bytes, int64_t position_axis_stride, int64_t num_axes,
                   const int64_t* sections, const float* cos_sin, int64_t cos_sin_stride, int64_t num_positions,
-                  int64_t rot_dim, int interleaved, void* q_out, const int64_t* q_out_strides, void* k_out,
-                  const int64_t* k_out_strides, void* key_cache, void* value_cache, const int64_t* key_cache_strides,
-                  const int64_t* value_cache_strides, int cache_dtype, const int64_t* slot_mapping, int64_t block_size,
+                  int64_t rot_dim, int interleaved, int cache_dtype, const int64_t* slot_mapping, int64_t block_size,
                   int64_t num_blocks, const float* k_scale, const float* v_scale, void* stream);
 
 /*
@@ -619,9 +619,10 @@ int psk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const 
  * a NaN or an infinity has scale 0xFF and codes 0, and reads as NaN.  D is a multiple
  * of 32 up to 4096; the size entry returns a negative status for others.
  *
- * psk_reshape_and_cache_mxfp4: rows [token, head] of key and value (element strides
- * of token and head, contiguous elements) into the caches at slot_mapping, BYTE
- * strides of block, slot and head, rows 4-byte aligned.
+ * psk_reshape_and_cache_mxfp4: rows [token, head] of key and value (contiguous
+ * elements) into the caches at slot_mapping, rows 4-byte aligned.  `strides`: ten,
+ * token and head of key and of value (elements), then block, slot and head of
+ * key_cache and of value_cache (BYTES).
  *
  * psk_gather_mxfp4: as psk_gather_cache over these rows (BYTE strides, the same for
  * both caches), heads one after the other at dst + t * dst_row_stride (elements), in
@@ -631,9 +632,8 @@ int psk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const 
 int64_t psk_mxfp4_entry_bytes(int64_t head_size);
 int psk_reshape_and_cache_mxfp4(const void* key, const void* value, void* key_cache, void* value_cache,
                                 const int64_t* slot_mapping, int64_t num_tokens, int64_t num_heads, int64_t head_size,
-                                int64_t block_size, int64_t num_blocks, const int64_t* key_strides,
-                                const int64_t* value_strides, const int64_t* k_strides, const int64_t* v_strides,
-                                int in_dtype, void* stream);
+                                int64_t block_size, int64_t num_blocks, const int64_t* strides, int in_dtype,
+                                void* stream);
 int psk_gather_mxfp4(const void* cache, const void* cache_v, void* dst, void* dst_v, const int32_t* block_table,
                      const int32_t* cu_seq_lens, const int32_t* seq_starts, int64_t batch_size,
                      int64_t block_table_stride, int64_t block_table_width, int64_t num_tokens, int64_t num_heads,

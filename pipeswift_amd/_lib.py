@@ -14,6 +14,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 
 import numpy as np
@@ -140,24 +141,23 @@ _SIGNATURES = {
     ),
     "psk_norm_rope": (
         _int,
-        [_vp, _c_int64_p, _vp, _c_int64_p, _vp, _c_int64_p, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int, ctypes.c_float,
-         _vp, _int, _i64, _i64, _c_int64_p, _vp, _i64, _i64, _i64, _int, _vp, _c_int64_p, _vp, _c_int64_p, _vp, _vp,
-         _c_int64_p, _c_int64_p, _int, _vp, _i64, _i64, _vp, _vp, _vp],
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _int, ctypes.c_float, _vp, _int,
+         _i64, _i64, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _i64, _i64, _vp, _vp, _vp],
     ),
     "psk_paged_mxfp4_attention": (
         _int,
-        [_vp, _i64, _i64, _int, _vp, _vp, _c_int64_p, _c_int64_p, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
+        [_vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
          _i64, _i64, _i64, _i64, _vp, _int, ctypes.c_float, _vp, _i64, _i64, _int, _vp, _i64, _vp, _i64, _vp],
     ),
     "psk_paged_mxfp4_workspace_len": (_i64, [_i64] * 6),
     "psk_mxfp4_entry_bytes": (_i64, [_i64]),
     "psk_reshape_and_cache_mxfp4": (
         _int,
-        [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _c_int64_p, _c_int64_p, _c_int64_p, _c_int64_p, _int, _vp],
+        [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _int, _vp],
     ),
     "psk_gather_mxfp4": (
         _int,
-        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_int64_p, _i64, _int, _vp],
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _int, _vp],
     ),
     "psk_mla_fp8_tile_entry_bytes": (_i64, [_i64, _i64]),
     "psk_concat_and_cache_mla_fp8_tiles": (
@@ -247,6 +247,11 @@ def i64_array(values) -> ctypes.Array:
     if n == 3:
         return _I64x3(*values)
     return (_I64x6 if n == 6 else ctypes.c_int64 * n)(*values)
+
+
+# Packed int64 values, for the entries that take strides as one pointer: a bytes
+# object is passed by its address, at a tenth of a ctypes array's cost.
+pack_i64x3, pack_i64x10, pack_i64x16 = (struct.Struct(f"={n}q").pack for n in (3, 10, 16))
 
 
 def _row_starts(t):

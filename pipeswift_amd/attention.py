@@ -31,7 +31,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import check, distinct, dtype_code, i64_array, lib, on_device, ptr, stream_handle
+from ._lib import DTYPE_CODES, check, distinct, dtype_code, i64_array, lib, on_device, pack_i64x3, ptr, stream_handle
 from .mxfp4_kv import check_cache
 
 HEAD_DIM = 128
@@ -563,24 +563,25 @@ def paged_mxfp4_attention(
     ``mxfp4_workspace_floats``, for callers that keep one; calls that overlap need one
     each.  The ragged layout contract, and ``validate``, are ``paged_decode_attention``'s."""
     B, n = _query_layout(q, cu_seqlens_q, max_seqlen_q, validate)
-    device = q.device
-    assert q.is_cuda and q.dim() == 3 and q.shape[2] == HEAD_DIM and q.stride(2) == 1, \
+    device, shape, qs = q.device, q.shape, q.stride()
+    assert q.is_cuda and len(shape) == 3 and shape[2] == HEAD_DIM and qs[2] == 1, \
         "q must be [T, Hq, 128] with unit last stride"
     assert q.dtype in _QUERY_TYPES, f"q is bf16, fp16 or fp32, not {q.dtype}"
-    TQ, Hq, _ = q.shape
-    assert k_cache.dim() == 4 and v_cache.shape == k_cache.shape
+    TQ, Hq, _ = shape
+    assert len(k_cache.shape) == 4 and v_cache.shape == k_cache.shape
     P, ps, Hkv, _ = k_cache.shape
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        check_cache(c, Hkv, HEAD_DIM, name)
-        assert c.device == device, "all tensors must share the query's device"
+    check_cache(k_cache, Hkv, HEAD_DIM, "k_cache")
+    check_cache(v_cache, Hkv, HEAD_DIM, "v_cache")
     assert Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"{Hq} query heads over {Hkv} kv heads"
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] >= B
-    assert block_table.stride(1) == 1 or block_table.shape[1] <= 1, "block_table needs unit last stride"
-    assert seq_lens.dtype == torch.int32 and seq_lens.is_contiguous() and seq_lens.numel() >= B
-    assert block_table.device == device and seq_lens.device == device, "all tensors must share the query's device"
+    rows, width = block_table.shape
+    assert block_table.dtype == torch.int32 and rows >= B, f"block_table must be int32 with {B} rows"
+    assert width <= 1 or block_table.stride(1) == 1, "block_table needs unit last stride"
+    assert seq_lens.dtype == torch.int32 and seq_lens.numel() >= B and seq_lens.is_contiguous()
+    for t in (k_cache, v_cache, block_table, seq_lens):
+        assert t.device == device, "all tensors must share the query's device"
     if softmax_scale is None:
         softmax_scale = HEAD_DIM ** -0.5
-    bound = block_table.shape[1] * ps
+    bound = width * ps
     bound = bound if max_seq_len is None else min(int(max_seq_len), bound)
     if out is None:
         out = torch.empty(TQ, Hq, HEAD_DIM, dtype=q.dtype, device=device)
@@ -595,14 +596,15 @@ def paged_mxfp4_attention(
         assert workspace is None or (workspace.dtype == torch.float32 and workspace.device == device
                                      and workspace.is_contiguous())
         st = lib().psk_paged_mxfp4_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), dtype_code(q.dtype), k_cache.data_ptr(), v_cache.data_ptr(),
-            i64_array(k_cache.stride()[:3]), i64_array(v_cache.stride()[:3]), block_table.data_ptr(),
-            block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), B, Hq, Hkv, HEAD_DIM, ps, P, bound, TQ, n,
-            ptr(cu_seqlens_q), 1 if causal else 0, float(softmax_scale), out.data_ptr(), out.stride(0), out.stride(1),
-            dtype_code(out.dtype), ptr(lse), TQ if lse is not None else 0, ptr(workspace),
-            0 if workspace is None else workspace.numel(), stream_handle(device),
+            q.data_ptr(), qs[0], qs[1], DTYPE_CODES[q.dtype], k_cache.data_ptr(), v_cache.data_ptr(),
+            pack_i64x3(*k_cache.stride()[:3]), pack_i64x3(*v_cache.stride()[:3]), block_table.data_ptr(),
+            block_table.stride(0), width, seq_lens.data_ptr(), B, Hq, Hkv, HEAD_DIM, ps, P, bound, TQ, n,
+            ptr(cu_seqlens_q), 1 if causal else 0, softmax_scale, out.data_ptr(), out.stride(0), out.stride(1),
+            DTYPE_CODES[out.dtype], ptr(lse), TQ, ptr(workspace), 0 if workspace is None else workspace.numel(),
+            stream_handle(device),
         )
-    check(st, "paged_mxfp4_attention")
+    if st:
+        check(st, "paged_mxfp4_attention")
     return (out, lse) if return_softmax_lse else out
 
 

@@ -129,9 +129,8 @@ int64_t psk_mxfp4_entry_bytes(int64_t head_size) {
 
 int psk_reshape_and_cache_mxfp4(const void* key, const void* value, void* key_cache, void* value_cache,
                                 const int64_t* slot_mapping, int64_t num_tokens, int64_t num_heads, int64_t head_size,
-                                int64_t block_size, int64_t num_blocks, const int64_t* key_strides,
-                                const int64_t* value_strides, const int64_t* k_strides, const int64_t* v_strides,
-                                int in_dtype, void* stream) {
+                                int64_t block_size, int64_t num_blocks, const int64_t* strides, int in_dtype,
+                                void* stream) {
   begin_device_call();
   if (bad_head(num_heads, head_size) || num_tokens < 0 || block_size <= 0 || num_blocks < 0)
     return fail(PSK_E_ARG, "bad sizes: num_tokens=%lld num_heads=%lld head_size=%lld block_size=%lld",
@@ -139,9 +138,8 @@ int psk_reshape_and_cache_mxfp4(const void* key, const void* value, void* key_ca
   if (in_dtype != PSK_DTYPE_F32 && in_dtype != PSK_DTYPE_F16 && in_dtype != PSK_DTYPE_BF16)
     return fail(PSK_E_DTYPE, "a 4-bit cache takes bf16, f16 or f32 rows (got %d)", in_dtype);
   if (num_tokens == 0 || num_blocks == 0) return PSK_OK;
-  if (!key || !value || !key_cache || !value_cache || !slot_mapping || !key_strides || !value_strides || !k_strides ||
-      !v_strides)
-    return fail(PSK_E_ARG, "NULL pointer");
+  if (!key || !value || !key_cache || !value_cache || !slot_mapping || !strides) return fail(PSK_E_ARG, "NULL pointer");
+  const int64_t *k_strides = strides + 4, *v_strides = strides + 7;
   const int64_t entry = mx_entry_bytes(head_size);
   const int esz = dtype_size(in_dtype);
   uint64_t align = uint64_t(uintptr_t(key_cache)) | uint64_t(uintptr_t(value_cache));
@@ -158,7 +156,7 @@ int psk_reshape_and_cache_mxfp4(const void* key, const void* value, void* key_ca
   a.slots = slot_mapping;
   a.num_tokens = num_tokens;
   a.num_slots = num_blocks * block_size;
-  const int64_t* in[2] = {key_strides, value_strides};
+  const int64_t* in[2] = {strides, strides + 2};
   const int64_t* ca[2] = {k_strides, v_strides};
   uint64_t in_align = uint64_t(uintptr_t(key)) | uint64_t(uintptr_t(value));
   for (int i = 0; i < 2; ++i) {

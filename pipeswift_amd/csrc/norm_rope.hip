@@ -385,14 +385,12 @@ void launch_rows(const NormRopeArgs& a, int kind, int64_t tokens, hipStream_t st
 
 extern "C" {
 
-int psk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
-                  const int64_t* v_strides, int dtype, int64_t num_tokens, int64_t num_q_heads, int64_t num_kv_heads,
+int psk_norm_rope(const void* q, const void* k, const void* v, void* q_out, void* k_out, void* key_cache, void* value_cache,
+                  const int64_t* strides, int dtype, int64_t num_tokens, int64_t num_q_heads, int64_t num_kv_heads,
                   int64_t head_size, const void* q_weight, const void* k_weight, int weight_dtype, float eps,
                   const void* positions, int position_bytes, int64_t position_axis_stride, int64_t num_axes,
                   const int64_t* sections, const float* cos_sin, int64_t cos_sin_stride, int64_t num_positions,
-                  int64_t rot_dim, int interleaved, void* q_out, const int64_t* q_out_strides, void* k_out,
-                  const int64_t* k_out_strides, void* key_cache, void* value_cache, const int64_t* key_cache_strides,
-                  const int64_t* value_cache_strides, int cache_dtype, const int64_t* slot_mapping, int64_t block_size,
+                  int64_t rot_dim, int interleaved, int cache_dtype, const int64_t* slot_mapping, int64_t block_size,
                   int64_t num_blocks, const float* k_scale, const float* v_scale, void* stream) {
   begin_device_call();
   if (num_tokens < 0 || num_tokens > INT32_MAX || num_q_heads < 0 || num_kv_heads < 0 || num_q_heads + num_kv_heads <= 0 ||
@@ -427,45 +425,41 @@ int psk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const 
     if (block_size <= 0 || num_blocks < 0) return fail(PSK_E_ARG, "bad cache geometry");
   }
   if (num_tokens == 0) return PSK_OK;
-  if ((num_q_heads && (!q || !q_strides || !q_out || !q_out_strides)) || (num_kv_heads && (!k || !k_strides)) || !positions ||
-      !cos_sin || (num_axes > 1 && !sections))
+  if (!strides || (num_q_heads && (!q || !q_out)) || (num_kv_heads && !k) || !positions || !cos_sin ||
+      (num_axes > 1 && !sections))
     return fail(PSK_E_ARG, "NULL pointer");
-  if (cache && (!key_cache || !value_cache || !v || !v_strides || !key_cache_strides || !value_cache_strides || !slot_mapping))
-    return fail(PSK_E_ARG, "NULL pointer");
-  if (!cache && num_kv_heads && (!k_out || !k_out_strides)) return fail(PSK_E_ARG, "NULL pointer");
+  if (cache && (!key_cache || !value_cache || !v || !slot_mapping)) return fail(PSK_E_ARG, "NULL pointer");
+  if (!cache && num_kv_heads && !k_out) return fail(PSK_E_ARG, "NULL pointer");
 
   NormRopeArgs a{};
   const int esz = dtype_size(dtype);
   uint64_t align = 0;
   const void* in[3] = {q, k, v};
-  const int64_t* ins[3] = {q_strides, k_strides, v_strides};
   for (int i = 0; i < (cache ? 3 : 2); ++i) {
     if (i == 0 ? num_q_heads == 0 : num_kv_heads == 0) continue;
     a.in[i] = static_cast<const char*>(in[i]);
-    a.in_tok[i] = ins[i][0] * esz;
-    a.in_head[i] = ins[i][1] * esz;
+    a.in_tok[i] = strides[2 * i] * esz;
+    a.in_head[i] = strides[2 * i + 1] * esz;
     align |= uint64_t(uintptr_t(in[i])) | uint64_t(a.in_tok[i]) | uint64_t(a.in_head[i]);
   }
   void* out[2] = {q_out, k_out};
-  const int64_t* outs[2] = {q_out_strides, k_out_strides};
   for (int i = 0; i < 2; ++i) {
     if (!out[i] || (i == 0 ? num_q_heads == 0 : num_kv_heads == 0)) continue;
     a.out[i] = static_cast<char*>(out[i]);
-    a.out_tok[i] = outs[i][0] * esz;
-    a.out_head[i] = outs[i][1] * esz;
+    a.out_tok[i] = strides[6 + 2 * i] * esz;
+    a.out_head[i] = strides[7 + 2 * i] * esz;
     align |= uint64_t(uintptr_t(out[i])) | uint64_t(a.out_tok[i]) | uint64_t(a.out_head[i]);
   }
   if (align & 15) return fail(PSK_E_ARG, "heads must start on 16-byte boundaries");
   if (cache) {
-    const int64_t* cas[2] = {key_cache_strides, value_cache_strides};
     void* ca[2] = {key_cache, value_cache};
     const int csz = kind == kMx4 ? 1 : dtype_size(cache_dtype);
     uint64_t calign = 0;
     for (int i = 0; i < 2; ++i) {
       a.cache[i] = static_cast<char*>(ca[i]);
-      a.blk[i] = cas[i][0] * csz;
-      a.row[i] = cas[i][1] * csz;
-      a.head[i] = cas[i][2] * csz;
+      a.blk[i] = strides[10 + 3 * i] * csz;
+      a.row[i] = strides[11 + 3 * i] * csz;
+      a.head[i] = strides[12 + 3 * i] * csz;
       calign |= uint64_t(uintptr_t(ca[i])) | uint64_t(a.blk[i]) | uint64_t(a.row[i]) | uint64_t(a.head[i]);
     }
     const uint64_t need = kind == kMx4 ? 4 : kind == kFp8 ? 8 : 16;

@@ -27,25 +27,30 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import check, dtype_code, i64_array, lib, on_device, ptr, stream_handle
+from ._lib import DTYPE_CODES, check, lib, on_device, pack_i64x3, pack_i64x10, ptr, stream_handle
 
 GROUP = 32
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_entries: dict = {}  # bytes of a row, by head size
 
 
 def entry_bytes(head_dim: int) -> int:
     """Bytes of a row: head_dim / 2 codes and head_dim / 32 scales, rounded up to 4."""
-    n = int(lib().psk_mxfp4_entry_bytes(int(head_dim)))
-    check(n if n < 0 else 0, "mxfp4 entry size")
+    n = _entries.get(head_dim)
+    if n is None:
+        n = int(lib().psk_mxfp4_entry_bytes(int(head_dim)))
+        check(n if n < 0 else 0, "mxfp4 entry size")
+        _entries[head_dim] = n
     return n
 
 
 def check_cache(cache: torch.Tensor, num_heads: int, head_dim: int, name: str) -> None:
-    assert cache.dtype == torch.uint8 and cache.ndim == 4, \
+    shape = cache.shape
+    assert cache.dtype == torch.uint8 and len(shape) == 4, \
         f"{name} must be uint8 [num_blocks, block_size, kv_heads, entry_bytes]"
-    entry = entry_bytes(head_dim)
-    assert cache.shape[2] == num_heads and cache.shape[3] == entry, (
-        f"{name} has rows {tuple(cache.shape[2:])}, want ({num_heads}, {entry}) for heads of {head_dim}"
+    entry = _entries.get(head_dim) or entry_bytes(head_dim)
+    assert shape[2] == num_heads and shape[3] == entry, (
+        f"{name} has rows {tuple(shape[2:])}, want ({num_heads}, {entry}) for heads of {head_dim}"
     )
     assert cache.stride(3) == 1, f"{name} needs unit last stride"
 
@@ -61,28 +66,31 @@ def reshape_and_cache_mxfp4(
     key_cache/value_cache, uint8 [num_blocks, block_size, H, entry_bytes(D)]:
     ``reshape_and_cache_flash``'s counterpart for the 4-bit cache.  Token t goes to
     slot ``slot_mapping[t]`` (int64); negative and out-of-range slots are skipped."""
-    assert key.ndim == 3 and value.ndim == 3
-    assert key.is_cuda and value.is_cuda and slot_mapping.is_cuda
-    heads, dim = key.shape[1], key.shape[2]
-    assert value.shape[1:] == key.shape[1:] and value.dtype == key.dtype
-    assert key.dtype in _TYPES, f"a 4-bit cache takes bf16, fp16 or fp32 rows, not {key.dtype}"
-    assert (key.stride(2) == 1 and value.stride(2) == 1) or key.numel() == 0, "heads must have unit inner stride"
+    assert len(key.shape) == 3 and len(value.shape) == 3
+    assert key.is_cuda, "key must be on a GPU"
+    tokens, heads, dim = key.shape
+    dtype, device = key.dtype, key.device
+    assert value.shape[1:] == (heads, dim) and value.dtype == dtype
+    assert dtype in _TYPES, f"a 4-bit cache takes bf16, fp16 or fp32 rows, not {dtype}"
+    ks, vs = key.stride(), value.stride()
+    assert (ks[2] == 1 and vs[2] == 1) or key.numel() == 0, "heads must have unit inner stride"
     check_cache(key_cache, heads, dim, "key_cache")
     check_cache(value_cache, heads, dim, "value_cache")
+    blocks, page = key_cache.shape[:2]
     assert value_cache.shape == key_cache.shape
-    device = key_cache.device
-    assert key.device == device and value.device == device and value_cache.device == device
-    assert slot_mapping.dtype == torch.int64 and slot_mapping.ndim == 1 and slot_mapping.is_contiguous()
-    assert slot_mapping.device == device, "slot_mapping must live on the cache's device"
+    for t in (value, key_cache, value_cache, slot_mapping):
+        assert t.device == device, "all tensors must share the key's device"
     n = slot_mapping.shape[0]
-    assert n <= min(key.shape[0], value.shape[0]), f"slot_mapping has {n} entries for {key.shape[0]} tokens"
+    assert slot_mapping.dtype == torch.int64 and len(slot_mapping.shape) == 1 and (n <= 1 or slot_mapping.stride(0) == 1)
+    assert n <= min(tokens, value.shape[0]), f"slot_mapping has {n} entries for {tokens} tokens"
     with on_device(device):
         st = lib().psk_reshape_and_cache_mxfp4(
-            ptr(key), ptr(value), ptr(key_cache), ptr(value_cache), ptr(slot_mapping), n, heads, dim, key_cache.shape[1],
-            key_cache.shape[0], i64_array(key.stride()), i64_array(value.stride()), i64_array(key_cache.stride()),
-            i64_array(value_cache.stride()), dtype_code(key.dtype), stream_handle(device),
+            key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(), n, heads,
+            dim, page, blocks, pack_i64x10(*ks[:2], *vs[:2], *key_cache.stride()[:3], *value_cache.stride()[:3]),
+            DTYPE_CODES[dtype], stream_handle(device),
         )
-    check(st, "reshape_and_cache_mxfp4")
+    if st:
+        check(st, "reshape_and_cache_mxfp4")
 
 
 def gather_mxfp4(
@@ -102,32 +110,34 @@ def gather_mxfp4(
     block_size``; zeros where there is no such page.  Rows at or past
     cu[batch_size] stay as they were.  ``src_cache_v`` / ``dst_v`` read a second cache
     of the same geometry in the same launch."""
-    assert src_cache.is_cuda and dst.is_cuda and block_table.is_cuda and cu_seq_lens.is_cuda
-    device = src_cache.device
-    assert dst.ndim == 3 and dst.dtype in _TYPES, "dst must be [T, H, D] in bf16, fp16 or fp32"
-    heads, dim = dst.shape[1], dst.shape[2]
+    assert src_cache.is_cuda, "src_cache must be on a GPU"
+    device, dtype = src_cache.device, dst.dtype
+    assert len(dst.shape) == 3 and dtype in _TYPES, "dst must be [T, H, D] in bf16, fp16 or fp32"
+    T, heads, dim = dst.shape
     check_cache(src_cache, heads, dim, "src_cache")
-    assert (dst.stride(2) == 1 and (dst.stride(1) == dim or heads == 1)) or dst.numel() == 0, "dst rows must be contiguous"
-    assert block_table.dtype == torch.int32 and block_table.ndim == 2
-    assert block_table.stride(1) == 1 or block_table.shape[1] <= 1, "block_table needs unit last stride"
-    assert cu_seq_lens.dtype == torch.int32 and cu_seq_lens.ndim == 1 and cu_seq_lens.is_contiguous()
-    B = cu_seq_lens.shape[0] - 1 if batch_size is None else int(batch_size)
-    assert 0 <= B <= cu_seq_lens.shape[0] - 1 and B <= block_table.shape[0]
+    blocks, page = src_cache.shape[:2]
+    ds, cs = dst.stride(), src_cache.stride()
+    assert (ds[2] == 1 and (ds[1] == dim or heads == 1)) or dst.numel() == 0, "dst rows must be contiguous"
+    rows, width = block_table.shape
+    assert block_table.dtype == torch.int32
+    assert width <= 1 or block_table.stride(1) == 1, "block_table needs unit last stride"
+    seqs = cu_seq_lens.shape[0] - 1
+    assert cu_seq_lens.dtype == torch.int32 and len(cu_seq_lens.shape) == 1 and cu_seq_lens.is_contiguous()
+    B = seqs if batch_size is None else int(batch_size)
+    assert 0 <= B <= seqs and B <= rows
     if seq_starts is not None:
         assert seq_starts.dtype == torch.int32 and seq_starts.is_contiguous() and seq_starts.shape[0] >= B
     assert (src_cache_v is None) == (dst_v is None), "a second cache needs a second destination"
     if src_cache_v is not None:
-        assert src_cache_v.shape == src_cache.shape and src_cache_v.stride() == src_cache.stride()
-        assert src_cache_v.dtype == src_cache.dtype
-        assert dst_v.shape == dst.shape and dst_v.stride() == dst.stride() and dst_v.dtype == dst.dtype
+        assert src_cache_v.shape == src_cache.shape and src_cache_v.stride() == cs and src_cache_v.dtype == torch.uint8
+        assert dst_v.shape == dst.shape and dst_v.stride() == ds and dst_v.dtype == dtype
     for t in (dst, block_table, cu_seq_lens, seq_starts, src_cache_v, dst_v):
         assert t is None or t.device == device, "all tensors must share the cache's device"
-    T = dst.shape[0]
     with on_device(device):
         st = lib().psk_gather_mxfp4(
-            ptr(src_cache), ptr(src_cache_v), ptr(dst), ptr(dst_v), ptr(block_table), ptr(cu_seq_lens), ptr(seq_starts), B,
-            block_table.stride(0), block_table.shape[1], T, heads, dim, src_cache.shape[1], src_cache.shape[0],
-            i64_array(src_cache.stride()), max(dst.stride(0), heads * dim) if T <= 1 else dst.stride(0),
-            dtype_code(dst.dtype), stream_handle(device),
+            src_cache.data_ptr(), ptr(src_cache_v), dst.data_ptr(), ptr(dst_v), block_table.data_ptr(), cu_seq_lens.data_ptr(),
+            ptr(seq_starts), B, block_table.stride(0), width, T, heads, dim, page, blocks, pack_i64x3(*cs[:3]),
+            max(ds[0], heads * dim) if T <= 1 else ds[0], DTYPE_CODES[dtype], stream_handle(device),
         )
-    check(st, "gather_mxfp4")
+    if st:
+        check(st, "gather_mxfp4")

@@ -24,7 +24,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import check, distinct, dtype_code, i64_array, lib, on_device, overlap, ptr, stream_handle
+from ._lib import check, distinct, i64_array, lib, on_device, overlap, pack_i64x16, ptr, stream_handle
 from .mxfp4_kv import check_cache
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -54,78 +54,89 @@ def _check_out(out, own, others, name):
             f"{name} must be its input itself or share no element with the inputs and outputs"
 
 
-def _run(q, k, v, positions, cos_sin, q_weight, k_weight, eps, sections, interleaved, q_out, k_out, caches, slot_mapping,
-         scales, what):
-    device = q.device
-    assert q.is_cuda and k.is_cuda, "q and k must be on a GPU"
-    assert q.ndim == 3 and k.ndim == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2], \
-        f"q {tuple(q.shape)} and k {tuple(k.shape)} must be [N, heads, D]"
-    assert q.dtype in _TYPES and k.dtype == q.dtype, f"q and k are bf16, fp16 or fp32, not {q.dtype} and {k.dtype}"
+def _sections(sections, axes, pairs):
+    assert sections is not None and len(sections) == axes, f"positions on {axes} axes need as many sections"
+    sections = [int(x) for x in sections]
+    assert sum(sections) == pairs, f"sections {sections} are not the {pairs} pairs of the rotation"
+    return i64_array(sections) if axes > 1 else None
+
+
+def _run(q, k, v, positions, cos_sin, q_weight, k_weight, eps, sections, interleaved, q_out, k_out, kc, vc, slots, k_scale,
+         v_scale, what):
+    device, dtype = q.device, q.dtype
+    assert q.is_cuda, "q must be on a GPU"
+    assert len(q.shape) == 3 and len(k.shape) == 3, f"q {tuple(q.shape)} and k {tuple(k.shape)} must be [N, heads, D]"
     n, hq, dim = q.shape
     hkv = k.shape[1]
-    for t in (q, k, v):
-        assert t is None or t.stride(2) == 1 or t.numel() == 0, "heads must have unit inner stride"
-    assert cos_sin.dtype == torch.float32 and cos_sin.ndim == 2 and cos_sin.stride(1) == 1, \
-        "cos_sin must be float32 [positions, rot] with unit last stride"
-    assert positions.dtype in (torch.int32, torch.int64) and positions.ndim in (1, 2) and positions.shape[-1] == n, \
-        f"positions must be int32 or int64 [{n}] or [axes, {n}]"
-    assert positions.stride(-1) == 1 or n <= 1, "positions need unit last stride"
-    axes = positions.shape[0] if positions.ndim == 2 else 1
-    if axes > 1 or sections is not None:
-        assert sections is not None and len(sections) == axes, f"positions on {axes} axes need as many sections"
-        assert sum(int(x) for x in sections) * 2 == cos_sin.shape[1], \
-            f"sections {list(sections)} are not the {cos_sin.shape[1] // 2} pairs of the rotation"
-    weight_dtype = q.dtype
+    assert k.shape[0] == n and k.shape[2] == dim, f"q {tuple(q.shape)} and k {tuple(k.shape)} must be [N, heads, D]"
+    assert dtype in _TYPES and k.dtype == dtype, f"q and k are bf16, fp16 or fp32, not {dtype} and {k.dtype}"
+    qs, ks = q.stride(), k.stride()
+    assert (qs[2] == 1 or q.numel() == 0) and (ks[2] == 1 or k.numel() == 0), "heads must have unit inner stride"
+    known, rot = cos_sin.shape
+    table = cos_sin.stride()
+    assert cos_sin.dtype == torch.float32 and table[1] == 1, "cos_sin must be float32 [positions, rot] with unit last stride"
+    dims = len(positions.shape)
+    ps = positions.stride()
+    assert dims in (1, 2) and positions.shape[-1] == n and (ps[-1] == 1 or n <= 1), \
+        f"positions must be [{n}] or [axes, {n}] with unit last stride"
+    assert positions.dtype in (torch.int64, torch.int32), f"positions are int32 or int64, not {positions.dtype}"
+    axes = positions.shape[0] if dims == 2 else 1
+    if axes != 1 or sections is not None:
+        sections = _sections(sections, axes, rot // 2)
+    weight_dtype = dtype
     for w in (q_weight, k_weight):
         if w is not None:
-            assert w.shape == (dim,) and w.is_contiguous() and w.dtype in (q.dtype, torch.float32), \
-                f"a norm's weight is [{dim}] in {q.dtype} or float32"
+            assert w.shape == (dim,) and (w.dtype == dtype or w.dtype == torch.float32) and w.is_contiguous(), \
+                f"a norm's weight is [{dim}] in {dtype} or float32"
             weight_dtype = w.dtype
     assert q_weight is None or k_weight is None or q_weight.dtype == k_weight.dtype, "the weights have one type"
     if q_out is None:
-        q_out = torch.empty((n, hq, dim), dtype=q.dtype, device=device)
+        q_out = torch.empty((n, hq, dim), dtype=dtype, device=device)
     else:
         _check_out(q_out, q, (k, v, k_out), "q_out")
     if k_out is not None:
         _check_out(k_out, k, (q, v), "k_out")
-    elif caches is None:
-        k_out = torch.empty((n, hkv, dim), dtype=q.dtype, device=device)
-    kc = vc = kcs = vcs = slots = None
+    elif kc is None:
+        k_out = torch.empty((n, hkv, dim), dtype=dtype, device=device)
+    vs = os = kcs = vcs = (0, 0, 0)
     code, page, blocks = 0, 1, 0
-    if caches is not None:
-        kc, vc = caches
-        assert v.shape == k.shape and v.dtype == k.dtype, f"v {tuple(v.shape)} must be like k {tuple(k.shape)}"
-        assert kc.ndim == 4 and vc.shape == kc.shape and vc.dtype == kc.dtype
-        if kc.dtype == torch.uint8:
+    if k_out is not None:
+        os = k_out.stride()
+    if kc is not None:
+        assert v.shape == k.shape and v.dtype == dtype, f"v {tuple(v.shape)} must be like k {tuple(k.shape)}"
+        vs = v.stride()
+        assert vs[2] == 1 or v.numel() == 0, "heads must have unit inner stride"
+        shape, ctype = kc.shape, kc.dtype
+        assert len(shape) == 4 and vc.shape == shape and vc.dtype == ctype
+        if ctype == torch.uint8:
             check_cache(kc, hkv, dim, "key_cache")
             check_cache(vc, hkv, dim, "value_cache")
             code = _lib.MXFP4_CODE
         else:
-            assert kc.dtype in (q.dtype, torch.float8_e4m3fn), f"kv cache dtype {kc.dtype} does not match {q.dtype}"
-            assert kc.shape[2:] == (hkv, dim), f"cache rows {tuple(kc.shape[2:])} for keys ({hkv}, {dim})"
+            assert ctype == dtype or ctype == torch.float8_e4m3fn, f"kv cache dtype {ctype} does not match {dtype}"
+            assert shape[2] == hkv and shape[3] == dim, f"cache rows {tuple(shape[2:])} for keys ({hkv}, {dim})"
             assert kc.stride(3) == 1 and vc.stride(3) == 1, "cache rows need unit last stride"
-            code = dtype_code(kc.dtype)
-        slots = slot_mapping
-        assert slots.dtype == torch.int64 and slots.shape == (n,) and slots.is_contiguous(), \
+            code = _lib.DTYPE_CODES[ctype]
+        kcs, vcs = kc.stride(), vc.stride()
+        assert slots.dtype == torch.int64 and slots.shape == (n,) and (n <= 1 or slots.stride(0) == 1), \
             f"slot_mapping must be contiguous int64 [{n}]"
-        for s in scales:
-            assert s is None or s.dtype == torch.float32 and s.numel() == 1 and kc.dtype == torch.float8_e4m3fn, \
+        for s in (k_scale, v_scale):
+            assert s is None or s.dtype == torch.float32 and s.numel() == 1 and ctype == torch.float8_e4m3fn, \
                 "scales are one float32 element each and only apply to an fp8 cache"
-        page, blocks = kc.shape[1], kc.shape[0]
-        kcs, vcs = i64_array(kc.stride()), i64_array(vc.stride())
-    for t in (k, v, positions, cos_sin, q_weight, k_weight, kc, vc, slots, *scales):
+        blocks, page = shape[:2]
+    for t in (k, v, positions, cos_sin, q_weight, k_weight, kc, vc, slots, k_scale, v_scale):
         assert t is None or t.device == device, "all tensors must be on q's device"
     with on_device(device):
         st = lib().psk_norm_rope(
-            ptr(q), i64_array(q.stride()), ptr(k), i64_array(k.stride()), ptr(v), None if v is None else i64_array(v.stride()),
-            dtype_code(q.dtype), n, hq, hkv, dim, ptr(q_weight), ptr(k_weight), dtype_code(weight_dtype), float(eps),
-            ptr(positions), positions.element_size(), positions.stride(0) if axes > 1 else 0, axes,
-            i64_array([int(x) for x in sections]) if axes > 1 else None, ptr(cos_sin), max(cos_sin.stride(0), cos_sin.shape[1]),
-            cos_sin.shape[0], cos_sin.shape[1], 1 if interleaved else 0, ptr(q_out), i64_array(q_out.stride()),
-            ptr(k_out), None if k_out is None else i64_array(k_out.stride()), ptr(kc), ptr(vc), kcs, vcs, code, ptr(slots),
-            page, blocks, ptr(scales[0]), ptr(scales[1]), stream_handle(device),
+            q.data_ptr(), k.data_ptr(), ptr(v), q_out.data_ptr(), ptr(k_out), ptr(kc), ptr(vc),
+            pack_i64x16(*qs[:2], *ks[:2], *vs[:2], *q_out.stride()[:2], *os[:2], *kcs[:3], *vcs[:3]), _lib.DTYPE_CODES[dtype],
+            n, hq, hkv, dim, ptr(q_weight), ptr(k_weight), _lib.DTYPE_CODES[weight_dtype], eps, positions.data_ptr(),
+            8 if positions.dtype == torch.int64 else 4, ps[0] if axes > 1 else 0, axes, sections, cos_sin.data_ptr(),
+            max(table[0], rot), known, rot, 1 if interleaved else 0, code, ptr(slots), page, blocks, ptr(k_scale),
+            ptr(v_scale), stream_handle(device),
         )
-    check(st, what)
+    if st:
+        check(st, what)
     return q_out, k_out
 
 
@@ -147,7 +158,7 @@ def norm_rope(
     may be q and k themselves.  D: a multiple of 8 up to 512; rot: a multiple of 16,
     or of 8 with ``interleaved``.  Returns (q_out, k_out)."""
     return _run(q, k, None, positions, cos_sin, q_weight, k_weight, eps, sections, interleaved, q_out, k_out, None, None,
-                (None, None), "norm_rope")
+                None, None, None, "norm_rope")
 
 
 def norm_rope_and_cache(
@@ -175,5 +186,5 @@ def norm_rope_and_cache(
     cache of k's type or FP8 (with ``k_scale`` / ``v_scale``), of
     ``mxfp4_kv.reshape_and_cache_mxfp4`` for a uint8 one.  The keys are rounded to
     their type first, as there.  ``k_out`` receives them too if given.  Returns q_out."""
-    return _run(q, k, v, positions, cos_sin, q_weight, k_weight, eps, sections, interleaved, q_out, k_out,
-                (key_cache, value_cache), slot_mapping, (k_scale, v_scale), "norm_rope_and_cache")[0]
+    return _run(q, k, v, positions, cos_sin, q_weight, k_weight, eps, sections, interleaved, q_out, k_out, key_cache,
+                value_cache, slot_mapping, k_scale, v_scale, "norm_rope_and_cache")[0]

@@ -61,10 +61,16 @@ def _refused(entry, good, status, message, change):
     assert st == status and message in _lib.lib().psk_last_error(), (st, _lib.lib().psk_last_error())
 
 
-ROWS = _lib.i64_array([4 * 128, 128, 1])
-ENTRIES = _lib.i64_array([2 * 16 * 4 * 68, 4 * 68, 68, 1])
-APPEND = dict(k=FAKE, v=FAKE, kc=FAKE, vc=FAKE, slots=FAKE, n=8, H=4, D=128, ps=16, P=10, ks=ROWS, vs=ROWS, kcs=ENTRIES,
-              vcs=ENTRIES, dt=2, stream=None)
+def _strides(head, **change):
+    """Those of rows [token, 4 heads, 128] for each name of ``head``, and of two caches of 4-bit rows."""
+    s = dict.fromkeys(head, (4 * 128, 128)) | dict(kc=(2 * 16 * 4 * 68, 4 * 68, 68), vc=(2 * 16 * 4 * 68, 4 * 68, 68))
+    assert set(change) <= set(s)
+    return _lib.i64_array([x for t in (s | change).values() for x in t])
+
+
+ENTRIES = _lib.i64_array([2 * 16 * 4 * 68, 4 * 68, 68])
+APPEND = dict(k=FAKE, v=FAKE, kc=FAKE, vc=FAKE, slots=FAKE, n=8, H=4, D=128, ps=16, P=10, strides=_strides("kv"), dt=2,
+              stream=None)
 
 
 @pytest.mark.parametrize("status,message,change", [
@@ -77,8 +83,9 @@ APPEND = dict(k=FAKE, v=FAKE, kc=FAKE, vc=FAKE, slots=FAKE, n=8, H=4, D=128, ps=
     (ARG, b"NULL", dict(vc=None)),
     (ARG, b"NULL", dict(slots=None)),
     (ARG, b"4-byte", dict(kc=FAKE + 2)),
-    (ARG, b"4-byte", dict(vcs=_lib.i64_array([2 * 16 * 4 * 68, 4 * 68 + 2, 68, 1]))),
-    (ARG, b"shorter", dict(kcs=_lib.i64_array([16 * 4 * 64, 4 * 64, 64, 1]))),
+    (ARG, b"NULL", dict(strides=None)),
+    (ARG, b"4-byte", dict(strides=_strides("kv", vc=(2 * 16 * 4 * 68, 4 * 68 + 2, 68)))),
+    (ARG, b"shorter", dict(strides=_strides("kv", kc=(16 * 4 * 64, 4 * 64, 64)))),
     (ARG, b"num_tokens", dict(n=1 << 31)),
 ])
 def test_append_refuses(status, message, change):
@@ -105,10 +112,9 @@ def test_gather_refuses(status, message, change):
 
 
 SECTIONS = _lib.i64_array([16, 24, 24])
-NORM_ROPE = dict(q=FAKE, qs=ROWS, k=FAKE, ks=ROWS, v=FAKE, vs=ROWS, dt=2, n=8, Hq=4, Hkv=4, D=128, qw=FAKE, kw=FAKE, wdt=2,
-                 eps=1e-6, pos=FAKE, pb=8, pa=8, axes=3, sections=SECTIONS, cs=FAKE, css=128, P=100, rot=128, inter=0, qo=FAKE,
-                 qos=ROWS, ko=None, kos=None, kc=FAKE, vc=FAKE, kcs=ENTRIES, vcs=ENTRIES, cdt=4, slots=FAKE, ps=16, blocks=10,
-                 ksc=None, vsc=None, stream=None)
+NORM_ROPE = dict(q=FAKE, k=FAKE, v=FAKE, qo=FAKE, ko=None, kc=FAKE, vc=FAKE, strides=_strides("qkvop"), dt=2, n=8, Hq=4,
+                 Hkv=4, D=128, qw=FAKE, kw=FAKE, wdt=2, eps=1e-6, pos=FAKE, pb=8, pa=8, axes=3, sections=SECTIONS, cs=FAKE,
+                 css=128, P=100, rot=128, inter=0, cdt=4, slots=FAKE, ps=16, blocks=10, ksc=None, vsc=None, stream=None)
 
 
 @pytest.mark.parametrize("status,message,change", [
@@ -140,7 +146,8 @@ NORM_ROPE = dict(q=FAKE, qs=ROWS, k=FAKE, ks=ROWS, v=FAKE, vs=ROWS, dt=2, n=8, H
     (ARG, b"NULL", dict(qo=None)),
     (ARG, b"NULL", dict(kc=None, vc=None)),
     (ARG, b"16-byte", dict(q=FAKE + 8)),
-    (ARG, b"16-byte", dict(vs=_lib.i64_array([4 * 128 + 4, 128, 1]))),
+    (ARG, b"16-byte", dict(strides=_strides("qkvop", v=(4 * 128 + 4, 128)))),
+    (ARG, b"NULL", dict(strides=None)),
     (ARG, b"4-byte", dict(kc=FAKE + 2)),
     (ARG, b"8-byte", dict(cdt=3, kc=FAKE + 4)),
     (ARG, b"16-byte", dict(cdt=2, kc=FAKE + 8)),
