@@ -13,27 +13,35 @@
 // the sum of two bf16 as well (2^-17), since V is only bf16 in general (its scales
 // reach 2^126, past fp16's range).  Maxima, sums and accumulators are float32.
 //
-// A wave takes 32 keys of one kv head at a time (a tile), for 16 kSets query rows (query
-// tokens x heads of the group):
-//   * the rows go to the wave's ring of two LDS slots by global_load_lds, a dword a lane
-//     (a row of 68 bytes lies on 4-byte boundaries only, where wider loads take a cycle
-//     a lane), two tiles ahead.
-//   * lane l reads 16 bytes, a whole group of 32 elements, of key l % 16's row at group
-//     l / 16, and its scale byte, of K and of V, for both halves of the tile.
+// A wave takes 16 keys (32 for two sets of query rows or a wider query) of one kv head at
+// a time (a tile), for 16 kSets query rows (query tokens x heads of the group):
+//   * the workgroup's waves load their tiles together, a stage, 16 bytes a lane by
+//     global_load_lds in the order of memory, into a ring of three, two stages ahead.  A
+//     row of 68 bytes lies on 4-byte boundaries only, where loads of 16 bytes to
+//     registers take a cycle a lane: 64 decode sequences took 223 us with those, 199 with
+//     dword loads to LDS by each wave for itself, and take 157 like this.
+//   * lane l reads a group of 32 elements, 16 bytes, of key l % 16's row at group
+//     l / 16, and its scale byte, of K and of V.
 //   * S^T = K Q^T on v_mfma_f32_16x16x32_bf16: the lane's group is its part of the A
 //     operand of four products as it stands (the query operand has the same order of
-//     elements), and leaves query row l % 16 with keys 4 (l / 16) + r of each half.
-//   * V becomes bf16 rows in the wave's own 8 KiB of LDS, 16-byte chunk c of key t at
-//     c ^ (2 (t & 7)), and comes back transposed by ds_read_b64_tr_b16 as the A operand of
-//     O^T = V^T P^T, whose P^T operand is the lane's weights as they stand.
+//     elements), and leaves query row l % 16 with keys 4 (l / 16) + r of each 16.
+//   * V becomes bf16 rows in the wave's own LDS, half of the columns at a time, and comes
+//     back transposed by ds_read_b64_tr_b16 as the A operand of O^T = V^T P^T, whose P^T
+//     operand is the lane's weights as they stand.
 // The waves of a workgroup take `hg` kv heads of the same tokens, so that the rows of a
 // token, which share cache lines, are read together, and `1 << wph_shift` waves share a
-// head's tiles in turn where the heads are fewer than the waves.  Nothing but the ends of
-// a piece of work waits on a barrier.
+// head's tiles in turn where the heads are fewer than the waves.  Caches that do not allow
+// the joint loads (pages that 8 does not divide, heads apart, other alignments) go to
+// registers row by row (GEN).
 //
 // The work is cut into equal runs over sequences and head groups (cached_queries.h); a
 // piece that is not all of a job's keys leaves a partial record, and merge_mx4_kernel
 // joins a row's records in the order of their keys.  Short contexts are not cut.
+//
+// Bound by memory: 64 sequences of 500 to 32 thousand keys, 8 kv heads of 4 query heads,
+// read 0.67 GB in 157 us, 4.3 TB/s (the loads alone take 138), and 10 us for the merge.  A
+// step of two sequences of 150 and 200 thousand keys takes 57 + 11 us, of which about 23 are the
+// start of a run, its first loads and its end.
 //
 // C ABI: include/pipeswift_kv.h.  Nothing here allocates or synchronizes.
 
@@ -50,16 +58,33 @@ constexpr int kRowBytes = int(mx_entry_bytes(kHead));
 constexpr int kWaves = 8, kThreads = 64 * kWaves;
 constexpr int kUnit = 8;           // keys that are loaded together
 constexpr uint32_t kUnitGap = 16;  // bytes between units in LDS
-constexpr int kSlots = 3;
+constexpr int kSlots = 3;          // stages in LDS
 constexpr int kPages = 512;        // page ids a piece stages at a time
 constexpr int kMaxSlots = 512;     // resident workgroups the workspace is sized for
+// The price of a job's start, in stages of keys: 8 ragged sequences take 32 us at 6, 37 at
+// 0; 256 of 1500 keys 116 and 112, 122 at 16.
 constexpr int kOver = 6;
+// Units of a run, at least: one sequence of 8000 keys takes 25 us at 2, 34 at 1, 27 at 8.
 constexpr int kMinRun = 2;
+// Up to so many keys a workgroup takes all of a job's: no second kernel, but no balance.
+// 1, 64 and 256 sequences of 1024 keys take 15, 25 and 78 us so, 19, 38 and 88 cut; one of
+// 4096 keys 35 and 21.  Twice the keys where the jobs are few: 8, 64, 128 sequences of 2048
+// take 22, 37, 80 us, 29, 52, 82 cut, but 256 of up to 2048 116 and 92; with 32 query rows 16
+// and 64 sequences of 8 kv heads 32 and 62, 46 and 83 cut, but 48 of one kv head 40 and 32.
 constexpr int kWholeKeys = 1024;
+constexpr int kWholeJobs = 128;
+// Workgroups that a step of uncut jobs has, if fewer kv heads a workgroup give them: 128
+// sequences of 1024 keys take 50 us with 256, 41 with 512, 43 with 1024; 512 of 256 keys
+// 43, 43 and 54.
+constexpr int kWholeGroups = 512;
+// Query rows that are joined by half waves, whatever their records: sixteen waves a row
+// take turns on the CUs (24 sequences of 32 rows x 8 heads: 107 us by them, 32 by half waves).
+constexpr int64_t kMergeWide = 1024;
 static_assert(kRowBytes == 68, "the reads and loads below");
 
 // Keys of a wave's tile: 16, whose registers (128) and LDS let two workgroups share a CU,
-// for 16 query rows of bf16; else 32, at one workgroup a CU.
+// for 16 query rows of bf16 (one sequence of 1000 keys 16.5 us, 22.5 with 32; the loads
+// of a long step no faster); else 32, at one workgroup a CU.
 constexpr int tile_shift(int q_dtype, int64_t sets) { return q_dtype == PSK_DTYPE_BF16 && sets == 1 ? 4 : 5; }
 
 struct Mx4Args {
@@ -708,13 +733,14 @@ Mx4Shape mx4_shape(int64_t num_seqs, int64_t max_seqlen_q, int64_t num_q_heads, 
   s.sets = rows <= 16 ? 1 : 2;
   s.row_blocks = ceil_div(rows, 16 * s.sets);
   s.rows = std::min<int64_t>(rows, 16 * s.sets);
-  s.whole = max_seq_len <= kWholeKeys;
   s.hg = 1;
   for (int64_t g = 1; g <= 8; ++g)
     if (num_kv_heads % g == 0) s.hg = g;
+  s.whole = max_seq_len <= kWholeKeys || (max_seq_len <= 2 * kWholeKeys && (s.sets == 1 || num_seqs * num_kv_heads >= kWholeJobs) &&
+             num_seqs * (num_kv_heads / s.hg) * s.row_blocks <= kWholeJobs);
   // uncut: the fewer the jobs, the more waves to a head
   if (s.whole)
-    while (s.hg > 1 && num_seqs * (num_kv_heads / s.hg) * s.row_blocks < 256) {
+    while (s.hg > 1 && num_seqs * (num_kv_heads / s.hg) * s.row_blocks < kWholeGroups) {
       int64_t g = s.hg - 1;
       while (num_kv_heads % g) --g;
       s.hg = g;
@@ -727,19 +753,23 @@ Mx4Shape mx4_shape(int64_t num_seqs, int64_t max_seqlen_q, int64_t num_q_heads, 
   return s;
 }
 
-// Which kernels a step takes: sequences of at most kFewRows query rows a kv head go by
-// rows, those of more by blocks of 256 (mxfp4_prefill.hip), in one launch each.
-constexpr int kFewRows = 32;
-enum Route { kRows, kBlocks, kBoth };
-Route route(int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, int64_t heads) {
-  if (max_seqlen_q * heads <= kFewRows || heads > kBlockRows) return kRows;
+// Which kernels a step takes: sequences of few query rows a kv head go by rows, those of
+// more by blocks of 256 (mxfp4_prefill.hip), in one launch each.  The products of 17 to 32
+// rows take the larger part of a tile's time, and of a block's less than its loads, so
+// that blocks win while they fill no more than the CUs: 32 rows x 8 kv heads of 1, 8, 16,
+// 24, 48 sequences of 2000 to 4000 keys take 35, 48, 32, 33, 60 us by rows and 25, 40, 42, 58, 111
+// by blocks.
+enum Way { kRows, kBlocks, kBoth };
+struct Route {
+  Way way;
+  int64_t row_tokens;  // query tokens of a sequence that goes by rows, at most
+};
+Route route(int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, int64_t heads, int64_t num_kv_heads) {
+  const int64_t few = num_seqs * num_kv_heads >= 128 ? 32 : 16;
+  if (max_seqlen_q * heads <= few || heads > kBlockRows) return {kRows, max_seqlen_q};
   // (more sequences than are ordered by their lengths: all by blocks)
-  return num_seqs == 1 || heads > kFewRows || total_q == num_seqs * max_seqlen_q || num_seqs > kOrderMax ? kBlocks : kBoth;
-}
-
-// Query tokens of a sequence that goes by rows, at most.
-int64_t row_tokens(Route r, int64_t max_seqlen_q, int64_t heads) {
-  return r == kBoth ? std::max<int64_t>(kFewRows / heads, 1) : max_seqlen_q;
+  if (num_seqs == 1 || heads > few || total_q == num_seqs * max_seqlen_q || num_seqs > kOrderMax) return {kBlocks, 0};
+  return {kBoth, few / heads};
 }
 
 // Whether a workgroup's waves load their heads' rows together, 16 bytes a lane: units of 8
@@ -771,7 +801,7 @@ int launch(Mx4Args p, const Mx4Shape& s, hipStream_t st) {
   if (const int e = check_launch("mx4_attention_kernel launch"); e != PSK_OK || p.whole) return e;
   const int64_t tasks = int64_t(p.s.num_seqs) * p.s.heads * p.hg * p.max_rows;
   // records of a row, about
-  const bool few = s.max_runs <= 8 * jobs;
+  const bool few = s.max_runs <= 8 * jobs || tasks > kMergeWide;
   const int64_t groups = ceil_div(tasks, few ? kMergeThreads<2> / 64 : 1);
   if (groups > (1 << 21)) return fail(PSK_E_ARG, "too many rows (%lld)", (long long)tasks);
   const dim3 merge{unsigned(groups), 1u, 1u}, threads{unsigned(few ? kMergeThreads<2> : kMergeThreads<32>)};
@@ -791,13 +821,15 @@ int64_t psk_paged_mxfp4_workspace_len(int64_t num_seqs, int64_t total_q, int64_t
   if (num_seqs < 0 || total_q < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
       max_seqlen_q <= 0 || max_seqlen_q > INT32_MAX / (num_q_heads / num_kv_heads) || max_seq_len < 0)
     return PSK_E_ARG;
-  const Route r = route(num_seqs, total_q, max_seqlen_q, num_q_heads / num_kv_heads);
-  const Mx4Shape s = mx4_shape(num_seqs, row_tokens(r, max_seqlen_q, num_q_heads / num_kv_heads), num_q_heads, num_kv_heads,
-                               max_seq_len, -1);
-  const int64_t own = s.whole ? 0 : 4 + s.max_runs * s.row_blocks * 2 * s.hg * s.rows * kRecord;
-  if (r == kRows) return own;
+  const Route r = route(num_seqs, total_q, max_seqlen_q, num_q_heads / num_kv_heads, num_kv_heads);
+  int64_t own = 0;
+  if (r.way != kBlocks) {
+    const Mx4Shape s = mx4_shape(num_seqs, r.row_tokens, num_q_heads, num_kv_heads, max_seq_len, -1);
+    if (!s.whole) own = 4 + s.max_runs * s.row_blocks * 2 * s.hg * s.rows * kRecord;
+  }
+  if (r.way == kRows) return own;
   const int64_t blocks = mx4_prefill_floats(num_seqs, total_q, max_seqlen_q, num_q_heads, num_kv_heads, max_seq_len);
-  return r == kBlocks ? blocks : std::max(own, blocks);  // (one after the other)
+  return std::max(own, blocks);  // (one after the other)
 }
 
 int psk_paged_mxfp4_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int q_dtype,
@@ -845,13 +877,13 @@ int psk_paged_mxfp4_attention(const void* q, int64_t q_tok_stride, int64_t q_hea
   a.lse_head_stride = lse_head_stride;
   p.scale_log2 = double(softmax_scale) * 1.4426950408889634;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const Route way = route(num_seqs, total_q, max_seqlen_q, a.heads);
-  const int64_t row_q = row_tokens(way, max_seqlen_q, a.heads);
-  if (way != kRows) {
-    const int32_t most = way == kBoth ? int32_t(kFewRows / a.heads) : 0;
+  const Route r = route(num_seqs, total_q, max_seqlen_q, a.heads, num_kv_heads);
+  const int64_t row_q = r.row_tokens;
+  if (r.way != kRows) {
+    const int32_t most = r.way == kBoth ? int32_t(row_q) : 0;
     const Mx4Prefill step{num_seqs, total_q, max_seqlen_q, max_seq_len, most, p.scale_log2, q_dtype, out_dtype};
     const int e = launch_mx4_prefill(a, step, workspace, st);
-    if (e != PSK_OK || way == kBlocks) return e;
+    if (e != PSK_OK || r.way == kBlocks) return e;
     p.s.most = most;
   }
   const Mx4Shape s = mx4_shape(num_seqs, row_q, num_q_heads, num_kv_heads, max_seq_len, q_dtype);

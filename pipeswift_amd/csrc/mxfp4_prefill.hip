@@ -37,7 +37,8 @@ constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kBlock = 32 * kWaves;  // query rows of a workgroup
 constexpr int kStage = 64;           // keys of a stage
-constexpr int kMostSplit = 512;      // workgroups of a step that is split
+constexpr int kMostSplit = 256;      // workgroups of a step that is split: a CU has one at a time (256
+                                     // rows over 8000 keys 59 us, 74 with twice as many)
 constexpr int kSplitKeys = 512;      // keys of a split, at least
 constexpr int kFp16Low = 104, kFp16High = 140;  // scale bytes whose values fp16 holds
 
