@@ -338,3 +338,94 @@ def test_empty_steps_and_refusals(dev):
                    dict(cu_seqlens_q=torch.tensor([0, 3, 3], dtype=torch.int32, device=dev), validate=True)):
         with pytest.raises(AssertionError):
             attention.paged_mxfp4_attention(**{**good, **change})
+
+
+@pytest.mark.parametrize("n", [1, 3])
+@pytest.mark.parametrize("Hq,Hkv,ps,pad,lens", [
+    (16, 16, 16, 0, [600, 40, 1100]),   # two groups of eight heads
+    (32, 32, 8, 0, [2100, 9]),
+    (8, 8, 8, 0, [777, 3000]),          # a page a unit of loads
+    (16, 4, 24, 16, [500, 1300, 2]),    # rows longer than their heads
+    (16, 8, 16, 16, [90, 2500]),
+    (24, 12, 40, 0, [333, 1100]),       # two groups of six heads, that begin off 16-byte boundaries
+    (4, 1, 8, 0, [9000, 17]),           # more pages than are looked up at a time
+    (4, 2, 1, 0, [1700, 3]),
+])
+def test_head_groups_pages_and_padded_rows(dev, n, Hq, Hkv, ps, pad, lens):
+    c = Case(dev, sum(lens) + Hq + n, lens, [n] * len(lens), Hq, Hkv, ps)
+    f = torch.from_numpy(c.fused).to(dev)
+    P, _, _, _, entry = f.shape
+    wide = torch.full((P, 2, ps, Hkv * entry + pad), 255, dtype=torch.uint8, device=dev)
+    wide[..., :Hkv * entry] = f.flatten(3)
+    rows = wide.as_strided(f.shape, (*wide.stride()[:3], entry, 1))
+    c.caches = lambda: (rows[:, 0], rows[:, 1])
+    _both(c)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,n,longest,bound", [
+    (16, 32, 8, 1, 2048, 2048),    # uncut past 1024 keys
+    (16, 32, 8, 8, 2000, 2048),    # 32 rows a head, uncut and cut
+    (16, 32, 8, 8, 2500, 2500),
+    (20, 8, 2, 5, 1500, 4000),     # 20 rows: by blocks
+    (70, 8, 2, 6, 300, 3000),      # by rows, many of them to join
+    (140, 4, 1, 7, 200, 1500),
+])
+def test_many_rows(dev, B, Hq, Hkv, n, longest, bound):
+    lens = [longest if b == 3 else (b * 131) % 400 for b in range(B)]
+    _both(Case(dev, B + n, lens, [n] * B, Hq, Hkv, 16), max_seq_len=bound)
+
+
+@pytest.mark.parametrize("lens,counts", [([1500, 300, 2200, 64], [1, 90, 4, 33]), ([900, 40, 1000, 7], [2, 40, 1, 0])])
+def test_few_and_many_rows_in_one_step_replayed_from_a_graph(dev, lens, counts):
+    c = Case(dev, 19, lens, counts, 8, 2, 16)
+    k, v = c.caches()
+    call = lambda: attention.paged_mxfp4_attention(  # noqa: E731
+        c.qd, k, v, c.btd, c.lensd, c.cud, c.max_q, return_softmax_lse=True)
+    call()
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    got = []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            got.append(call())
+    for lens in (lens, [100, 250, 64, 1], lens[::-1]):
+        c.lensd.copy_(torch.tensor(lens, dtype=torch.int32))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        c.lens = lens
+        want = c.want()
+        for x in got:
+            c.check(x, want)
+        eager = call()
+        assert torch.equal(got[0][0], eager[0]) and torch.equal(got[1][1], eager[1])
+
+
+@pytest.mark.parametrize("byte", [253, 254, 255])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [5, 8, 3], [60, 100, 65]])
+def test_infinite_values_reach_only_what_sees_them(dev, counts, byte):
+    """Codes of 6 under the largest scales, past the largest float, in V of a sequence's last token."""
+    lens = [70, 1200, 100]
+    c = Case(dev, 20, lens, counts, 8, 2, 16)
+    last = lens[1] - 1
+    at = (int(c.bt[1, last // 16]), 1, last % 16, 1)
+    c.fused[at][64 + 2] = 127
+    c.fused[at][32:48] = 0
+    w, wl, most = c.want()
+    tol, tol_lse = c.bounds(most, w, wl, torch.bfloat16)
+    c.fused[at][64 + 2] = byte
+    c.fused[at][32:48] = 0x77
+    out, lse = c.run()
+    got, gl = out.double().cpu().numpy(), lse.double().cpu().numpy().T
+    struck = np.zeros(got.shape, bool)
+    struck[c.cu[2] - 1, 4:, 64:96] = True  # the heads of kv head 1
+    assert not np.isfinite(got[struck]).any()
+    assert (np.abs(got - w) <= tol)[~struck].all() and (np.abs(gl - wl) <= tol_lse).all()
+
+
+def test_sequences_that_share_their_first_pages(dev):
+    c = Case(dev, 21, [1500, 1400, 1500], [1, 1, 1], 8, 2, 16)
+    c.bt[1, :60] = c.bt[0, :60]
+    c.bt[2] = c.bt[0]
+    c.btd = c.bt.to(dev)
+    _both(c)

@@ -218,3 +218,33 @@ def test_python_refusals(dev):
                    dict(key_cache=cache[:, 0].to(torch.uint8), value_cache=cache[:, 1].to(torch.uint8))):
         with pytest.raises(AssertionError):
             rotary.norm_rope_and_cache(**{**good, **change})
+
+
+@pytest.mark.parametrize("kind", ["same", "fp8", "mxfp4"])
+@pytest.mark.parametrize("dtype,N,Hq,Hkv,D,rot,axes,interleaved", [
+    (torch.bfloat16, 2049, 8, 2, 128, 128, 1, False), (torch.float16, 2111, 5, 3, 96, 64, 3, True),
+    (torch.float32, 2050, 2, 2, 32, 32, 1, True), (torch.bfloat16, 2048, 3, 1, 512, 256, 1, False)])
+def test_many_tokens(dev, kind, dtype, N, Hq, Hkv, D, rot, axes, interleaved):
+    """A prompt's worth, with slots that are skipped: results, and the cache as the append would leave it."""
+    x = Inputs(dev, N + D, N, Hq, Hkv, D, rot, dtype, axes)
+    ps = 16
+    P = -(-N // ps) + 2
+    cache, other = (_caches(torch.Generator().manual_seed(1), kind, dtype, P, ps, Hkv, D, dev) for _ in range(2))
+    slots = torch.randperm(P * ps, generator=x.g)[:N]
+    slots[::7] = -1
+    slots[5] = P * ps
+    slots = slots.to(dev)
+    q, k = rotary.norm_rope(x.q, x.k, **x.args, interleaved=interleaved)
+    for i, got in enumerate((q, k)):
+        _check(got, *x.want(i, interleaved=interleaved), dtype)
+    scales = {}
+    if kind == "fp8":
+        scales = dict(k_scale=torch.tensor([0.037], device=dev), v_scale=torch.tensor([0.21], device=dev))
+    got = rotary.norm_rope_and_cache(x.q, x.k, x.v, cache[:, 0], cache[:, 1], slots, **x.args, **scales,
+                                     interleaved=interleaved)
+    v = x.v.contiguous()
+    if kind == "mxfp4":
+        mxfp4_kv.reshape_and_cache_mxfp4(k, v, other[:, 0], other[:, 1], slots)
+    else:
+        reshape_and_cache.reshape_and_cache_flash(k, v, other[:, 0], other[:, 1], slots, **scales)
+    assert torch.equal(_bytes(got), _bytes(q)) and torch.equal(_bytes(cache), _bytes(other))

@@ -164,3 +164,59 @@ def test_empty_calls_touch_nothing():
     assert _call("psk_gather_mxfp4", GATHER, dict(T=0, d=None, dv=None)) == 0
     assert _call("psk_gather_mxfp4", GATHER, dict(B=0, bt=None)) == 0
     assert _call("psk_norm_rope", NORM_ROPE, dict(n=0, q=None, k=None, v=None, qo=None, pos=None, slots=None)) == 0
+
+
+STRIDES = _lib.i64_array([2 * 16 * 4 * 68, 4 * 68, 68])
+ATTENTION = dict(q=FAKE, qt=8 * 128, qh=128, qdt=2, kc=FAKE, vc=FAKE, ks=STRIDES, vs=STRIDES, bt=FAKE, bts=10, btw=10, lens=FAKE,
+                 B=2, Hq=8, Hkv=4, D=128, ps=16, P=10, most=5000, TQ=4, n=2, cu=FAKE, causal=1, scale=0.1, out=FAKE, ot=8 * 128,
+                 oh=128, odt=2, lse=None, ls=0, ws=FAKE, wl=1 << 40, stream=None)
+
+
+@pytest.mark.parametrize("status,message,change", [
+    (ARG, b"", dict(B=-1)),
+    (ARG, b"", dict(TQ=-1)),
+    (ARG, b"", dict(Hq=6)),
+    (ARG, b"", dict(Hkv=0)),
+    (ARG, b"128", dict(D=64)),
+    (ARG, b"max_seqlen_q", dict(n=0)),
+    (ARG, b"max_seqlen_q", dict(n=1 << 31)),
+    (ARG, b"max_seq_len", dict(most=-1)),
+    (ARG, b"without cu_seqlens_q", dict(cu=None, TQ=3)),
+    (DTYPE, b"", dict(qdt=3)),
+    (DTYPE, b"output dtype", dict(odt=3)),
+    (ARG, b"", dict(scale=float("nan"))),
+    (ARG, b"", dict(ps=0)),
+    (ARG, b"NULL", dict(q=None)),
+    (ARG, b"NULL", dict(kc=None)),
+    (ARG, b"NULL", dict(vc=None)),
+    (ARG, b"NULL", dict(vs=None)),
+    (ARG, b"NULL", dict(bt=None)),
+    (ARG, b"NULL", dict(lens=None)),
+    (ARG, b"NULL", dict(out=None)),
+    (ARG, b"align", dict(q=FAKE + 8)),
+    (ARG, b"align", dict(kc=FAKE + 2)),
+    (ARG, b"4-byte", dict(vc=FAKE + 2)),
+    (ARG, b"4-byte", dict(vs=_lib.i64_array([2 * 16 * 4 * 68, 4 * 68, 66]))),
+    (ARG, b"8-byte", dict(out=FAKE + 4)),
+    (ARG, b"16-byte", dict(odt=0, oh=130)),
+    (WORKSPACE, b"need", dict(wl=100)),
+    (WORKSPACE, b"need", dict(ws=None)),
+])
+def test_attention_refuses(status, message, change):
+    _refused("psk_paged_mxfp4_attention", ATTENTION, status, message, change)
+
+
+@pytest.mark.parametrize("change", [dict(B=-1), dict(TQ=-1), dict(n=0), dict(Hq=6), dict(Hkv=0), dict(most=-1), dict(n=1 << 31)])
+def test_workspace_of_a_bad_step(change):
+    good = dict(B=2, TQ=4, n=2, Hq=8, Hkv=4, most=5000)
+    assert _call("psk_paged_mxfp4_workspace_len", good, {}) > 0
+    assert _call("psk_paged_mxfp4_workspace_len", good, change) == ARG
+
+
+def test_empty_attention_touches_nothing():
+    assert _call("psk_paged_mxfp4_attention", ATTENTION, dict(TQ=0, q=None, out=None)) == 0
+    assert _call("psk_paged_mxfp4_attention", ATTENTION, dict(B=0, TQ=0, lens=None, bt=None)) == 0
+
+
+def test_a_short_step_needs_no_workspace():
+    assert _call("psk_paged_mxfp4_workspace_len", dict(B=2, TQ=2, n=1, Hq=8, Hkv=4, most=1024), {}) == 0
