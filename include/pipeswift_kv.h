@@ -649,8 +649,9 @@ int psk_gather_mxfp4(const void* cache, const void* cache_v, void* dst, void* ds
  * Any number of query tokens and query heads per kv head; head_size 128.  q is bf16, f16
  * or f32 (16-byte aligned rows), taken to 2^-17 or better; out bf16, f16 or f32, rows
  * aligned to 4 elements.  Rows without a page are zeros; a query that sees no key gets
- * zeros and -inf; a NaN in V reaches only the queries that see its token; rows that no
- * sequence owns are left as they were.  A sequence longer than the block table reads
+ * zeros and -inf; a NaN in V reaches only the queries that see its token, and so does a
+ * value past the largest finite float, which counts as NaN for its group of 32 columns; rows
+ * that no sequence owns are left as they were.  A sequence longer than the block table reads
  * zeros past it.  max_seq_len and max_seqlen_q (bounds) size and cut the launch.
  * lse (may be NULL): [hq * lse_head_stride + token].  Caches have BYTE strides of block,
  * slot and head.  workspace:

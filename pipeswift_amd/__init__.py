@@ -8,7 +8,9 @@ libpipeswift_kv.so), with the reference's Python cache API on top:
   metadata            KVCacheInfo, prepare_kv_info (slot_mapping, page_table)
   cudagraph           static metadata for graph replay
   cache_ops           gather_cache, copy_blocks, evict_tokens, commit_draft_tokens, compute_kv_scales
-  attention           FP8 paged attention (decode, prefill, drafted trees) and the weights it gave
+  rotary              norm_rope, norm_rope_and_cache: head norms and rotation, with the append
+  mxfp4_kv            the 4-bit cache: reshape_and_cache_mxfp4, gather_mxfp4
+  attention           paged attention over FP8 (decode, prefill, drafted trees) and 4-bit caches, and the weights it gave
   copy_engine         CopyEngine / CopyHandle (DRAM L2 offload, swap_blocks)
   fp8_kv              FP8 constants, flag and scale helpers
 """

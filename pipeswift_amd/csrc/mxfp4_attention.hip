@@ -758,17 +758,19 @@ Mx4Shape mx4_shape(int64_t num_seqs, int64_t max_seqlen_q, int64_t num_q_heads, 
 // rows take the larger part of a tile's time, and of a block's less than its loads, so
 // that blocks win while they fill no more than the CUs: 32 rows x 8 kv heads of 1, 8, 16,
 // 24, 48 sequences of 2000 to 4000 keys take 35, 48, 32, 33, 60 us by rows and 25, 40, 42, 58, 111
-// by blocks.
+// by blocks.  Where the sequences' tokens differ, both kernels would run: 48 sequences of 1 to 4
+// tokens x 8 heads take 27 us by rows, 46 by both.
 enum Way { kRows, kBlocks, kBoth };
 struct Route {
   Way way;
   int64_t row_tokens;  // query tokens of a sequence that goes by rows, at most
 };
 Route route(int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, int64_t heads, int64_t num_kv_heads) {
-  const int64_t few = num_seqs * num_kv_heads >= 128 ? 32 : 16;
+  const bool even = num_seqs == 1 || total_q == num_seqs * max_seqlen_q;
+  const int64_t few = even && num_seqs * num_kv_heads < 128 ? 16 : 32;
   if (max_seqlen_q * heads <= few || heads > kBlockRows) return {kRows, max_seqlen_q};
   // (more sequences than are ordered by their lengths: all by blocks)
-  if (num_seqs == 1 || heads > few || total_q == num_seqs * max_seqlen_q || num_seqs > kOrderMax) return {kBlocks, 0};
+  if (even || heads > few || num_seqs > kOrderMax) return {kBlocks, 0};
   return {kBoth, few / heads};
 }
 

@@ -28,6 +28,8 @@ struct Mx4AppendArgs {
 
 // A lane takes eight elements, a quad of lanes a group: its maximum is two DPP steps
 // away and nothing goes through LDS.  The lanes run over (token, K or V, head, group).
+// Bound by memory: 4096 tokens of 8 heads of 128 in bf16 (16.8 MB in, 4.5 out) take 7.9 us
+// with their launch, 2.7 TB/s, most of it the launch and one round of loads; 17 tokens 3.4.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) mx4_append_kernel(Mx4AppendArgs a) {
   const int per = 2 * a.num_heads * a.chunks;  // lanes of a token (host: below 2^31)
@@ -80,7 +82,11 @@ __device__ __forceinline__ void store8(char* p, bool wide, uint32_t codes, float
   }
 }
 
-// A wave takes a token's rows of K and V, eight elements a lane.
+// A wave takes a token's rows of K and V, eight elements a lane, with a dword of codes a
+// lane: the rows lie on 4-byte boundaries, and a wave's loads side by side all the same.
+// The results are not read again soon and go past the caches.  Bound by memory: 38
+// thousand tokens of 8 heads of 128 (41 MB of K and V into 156 MB of bf16) take 31 us,
+// 6.4 TB/s; 617 tokens 4.8, the chain of a token's sequence, its page id and its rows.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) mx4_gather_kernel(Mx4GatherArgs g) {
   const int lane = int(threadIdx.x) & 63;
