@@ -40,7 +40,7 @@
 //
 // Bound by memory: 64 sequences of 500 to 32 thousand keys, 8 kv heads of 4 query heads,
 // read 0.67 GB in 157 us, 4.3 TB/s (the loads alone take 138), and 10 us for the merge.  A
-// step of two sequences of 150 and 200 thousand keys takes 57 + 11 us, of which about 23 are the
+// step of two sequences of 150 and 200 thousand keys takes 57 + 9 us, of which about 23 are the
 // start of a run, its first loads and its end.
 //
 // C ABI: include/pipeswift_kv.h.  Nothing here allocates or synchronizes.
@@ -168,6 +168,17 @@ mx4_attention_kernel(Mx4Args args) {
   const int w = int(blockIdx.x), idx = (w >> 3) / args.row_blocks, block = (w >> 3) - idx * args.row_blocks;
   int64_t j = 0, x = 0, x_end = 1;  // the run and its units
   int b0 = 0, whole_grp = 0;        // a window of sequences begins with b0
+  int64_t window = 0, before = 0, seq_end = 0;  // units before the window, before the sequence and with it
+  int b = 0, L = 0;
+  SeqRows r{0, 0};
+  // the k-th sequence of a window
+  auto take = [&](const SeqWindow& seqs, int64_t at, int k) {
+    b = b0 + k;
+    before = lane_value(at, k);
+    seq_end = before + lane_value(seqs.cost, k);
+    r = SeqRows{lane_value(seqs.first, k), lane_value(seqs.n, k)};
+    L = lane_value(seqs.len, k);
+  };
   if (args.whole) {                 // a workgroup a job: x follows with its sequence
     const int jobs = args.s.num_seqs * args.s.heads, per = (jobs + 7) >> 3;
     const int job = (w & 7) * per + idx;
@@ -181,6 +192,7 @@ mx4_attention_kernel(Mx4Args args) {
     x = j * step_run.run;
     if (x >= step_run.total) return;
     x_end = min(x + step_run.run, step_run.total);
+    if (args.s.num_seqs <= 64) take(seqs, seqs.before, __builtin_ctzll(__ballot(seqs.before <= x && x < seqs.before + seqs.cost)));
   }
 
   char* const vt = s_lds + kSlots * kSlot + wave * kTile * kHead;
@@ -194,9 +206,6 @@ mx4_attention_kernel(Mx4Args args) {
   const uint32_t rd_v = uint32_t(128 * vkey + 16 * (((l15 & 3) >> 1) ^ (vkey >> 3)) + 8 * (l15 & 1));
   const uint32_t rd_sw = 32 * ((vkey >> 1) & 3);
 
-  int64_t window = 0, before = 0, seq_end = 0;  // units before the window, before the sequence and with it
-  int b = 0, L = 0;
-  SeqRows r{0, 0};
   while (x < x_end) {  // over the run's jobs
     const Mx4Args& p = args_again<Mx4Args>();
     const DecodeArgs& a = p.a;
@@ -211,12 +220,7 @@ mx4_attention_kernel(Mx4Args args) {
         b0 += 64;
         continue;
       }
-      const int k = __builtin_ctzll(here);
-      b = b0 + k;
-      before = lane_value(at, k);
-      seq_end = before + lane_value(seqs.cost, k);
-      r = SeqRows{lane_value(seqs.first, k), lane_value(seqs.n, k)};
-      L = lane_value(seqs.len, k);
+      take(seqs, at, __builtin_ctzll(here));
     }
     const int steps = key_steps(p.s, L);
     const int64_t job_cost = p.s.over + steps;
@@ -706,17 +710,23 @@ __global__ void __launch_bounds__(kMergeThreads<kParts>) merge_mx4_kernel(Mx4Arg
       s_l[part] = sum;
     }
     __syncthreads();
-    if (part > 0) return;
-#pragma unroll 1
-    for (int u = 1; u < kParts; ++u) top = __builtin_fmaxf(top, s_m[u]);
-    sum = 0.0f;
+    if (part > 1) return;
+    // half a wave every other part: lane i has part i's weight
+    static_assert(kParts == 32, "");
+    const float m = s_m[at4];
+    top = m;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
+    const float f = __builtin_amdgcn_exp2f(m - top);
+    sum = s_l[at4] * f;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor(sum, x);
     o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-    for (int u = 0; u < kParts; ++u) {
-      const float f = __builtin_amdgcn_exp2f(s_m[u] - top);
-      sum += s_l[u] * f;
-      o += s_o[u][at4] * f;
-    }
+#pragma unroll
+    for (int u = 0; u < 16; ++u) o += s_o[2 * u + part][at4] * __shfl(f, 2 * u + part);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], 32);
+    if (part > 0) return;
     finish(a, p.out_dtype, r, h, row, 4 * at4, o, top, sum);
   }
 }
