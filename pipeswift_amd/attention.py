@@ -573,8 +573,9 @@ def paged_mxfp4_attention(
     check_cache(k_cache, Hkv, HEAD_DIM, "k_cache")
     check_cache(v_cache, Hkv, HEAD_DIM, "v_cache")
     assert Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"{Hq} query heads over {Hkv} kv heads"
+    assert len(block_table.shape) == 2 and block_table.dtype == torch.int32, "block_table must be int32 [sequences, pages]"
     rows, width = block_table.shape
-    assert block_table.dtype == torch.int32 and rows >= B, f"block_table must be int32 with {B} rows"
+    assert rows >= B, f"block_table has {rows} rows for {B} sequences"
     assert width <= 1 or block_table.stride(1) == 1, "block_table needs unit last stride"
     assert seq_lens.dtype == torch.int32 and seq_lens.numel() >= B and seq_lens.is_contiguous()
     for t in (k_cache, v_cache, block_table, seq_lens):
@@ -599,7 +600,7 @@ def paged_mxfp4_attention(
             q.data_ptr(), qs[0], qs[1], DTYPE_CODES[q.dtype], k_cache.data_ptr(), v_cache.data_ptr(),
             pack_i64x3(*k_cache.stride()[:3]), pack_i64x3(*v_cache.stride()[:3]), block_table.data_ptr(),
             block_table.stride(0), width, seq_lens.data_ptr(), B, Hq, Hkv, HEAD_DIM, ps, P, bound, TQ, n,
-            ptr(cu_seqlens_q), 1 if causal else 0, softmax_scale, out.data_ptr(), out.stride(0), out.stride(1),
+            ptr(cu_seqlens_q), 1 if causal else 0, float(softmax_scale), out.data_ptr(), out.stride(0), out.stride(1),
             DTYPE_CODES[out.dtype], ptr(lse), TQ, ptr(workspace), 0 if workspace is None else workspace.numel(),
             stream_handle(device),
         )

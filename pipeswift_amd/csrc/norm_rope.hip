@@ -473,6 +473,10 @@ int psk_norm_rope(const void* q, const void* k, const void* v, void* q_out, void
     }
     const uint64_t need = kind == kMx4 ? 4 : kind == kFp8 ? 8 : 16;
     if (calign & (need - 1)) return fail(PSK_E_ARG, "cache rows must start on %d-byte boundaries", int(need));
+    const int64_t row_bytes = kind == kMx4 ? mx_entry_bytes(head_size) : head_size * csz;
+    for (int i = 0; i < 2; ++i)
+      if ((num_kv_heads > 1 && a.head[i] < row_bytes) || (block_size > 1 && a.row[i] < row_bytes))
+        return fail(PSK_E_ARG, "cache strides are shorter than the %lld-byte row", (long long)row_bytes);
     if (kind != kFp8 && (k_scale || v_scale)) return fail(PSK_E_ARG, "scales only apply to an fp8 cache");
     a.slots = slot_mapping;
     a.block_size = block_size;

@@ -80,8 +80,9 @@ def reshape_and_cache_mxfp4(
     assert value_cache.shape == key_cache.shape
     for t in (value, key_cache, value_cache, slot_mapping):
         assert t.device == device, "all tensors must share the key's device"
+    assert slot_mapping.dtype == torch.int64 and len(slot_mapping.shape) == 1, "slot_mapping must be int64 [tokens]"
     n = slot_mapping.shape[0]
-    assert slot_mapping.dtype == torch.int64 and len(slot_mapping.shape) == 1 and (n <= 1 or slot_mapping.stride(0) == 1)
+    assert n <= 1 or slot_mapping.stride(0) == 1, "slot_mapping needs unit stride"
     assert n <= min(tokens, value.shape[0]), f"slot_mapping has {n} entries for {tokens} tokens"
     with on_device(device):
         st = lib().psk_reshape_and_cache_mxfp4(
@@ -118,11 +119,11 @@ def gather_mxfp4(
     blocks, page = src_cache.shape[:2]
     ds, cs = dst.stride(), src_cache.stride()
     assert (ds[2] == 1 and (ds[1] == dim or heads == 1)) or dst.numel() == 0, "dst rows must be contiguous"
+    assert len(block_table.shape) == 2 and block_table.dtype == torch.int32, "block_table must be int32 [sequences, pages]"
     rows, width = block_table.shape
-    assert block_table.dtype == torch.int32
     assert width <= 1 or block_table.stride(1) == 1, "block_table needs unit last stride"
-    seqs = cu_seq_lens.shape[0] - 1
     assert cu_seq_lens.dtype == torch.int32 and len(cu_seq_lens.shape) == 1 and cu_seq_lens.is_contiguous()
+    seqs = cu_seq_lens.shape[0] - 1
     B = seqs if batch_size is None else int(batch_size)
     assert 0 <= B <= seqs and B <= rows
     if seq_starts is not None:

@@ -72,6 +72,7 @@ def _run(q, k, v, positions, cos_sin, q_weight, k_weight, eps, sections, interle
     assert dtype in _TYPES and k.dtype == dtype, f"q and k are bf16, fp16 or fp32, not {dtype} and {k.dtype}"
     qs, ks = q.stride(), k.stride()
     assert (qs[2] == 1 or q.numel() == 0) and (ks[2] == 1 or k.numel() == 0), "heads must have unit inner stride"
+    assert len(cos_sin.shape) == 2, "cos_sin must be [positions, rot]"
     known, rot = cos_sin.shape
     table = cos_sin.stride()
     assert cos_sin.dtype == torch.float32 and table[1] == 1, "cos_sin must be float32 [positions, rot] with unit last stride"
@@ -130,7 +131,7 @@ def _run(q, k, v, positions, cos_sin, q_weight, k_weight, eps, sections, interle
         st = lib().psk_norm_rope(
             q.data_ptr(), k.data_ptr(), ptr(v), q_out.data_ptr(), ptr(k_out), ptr(kc), ptr(vc),
             pack_i64x16(*qs[:2], *ks[:2], *vs[:2], *q_out.stride()[:2], *os[:2], *kcs[:3], *vcs[:3]), _lib.DTYPE_CODES[dtype],
-            n, hq, hkv, dim, ptr(q_weight), ptr(k_weight), _lib.DTYPE_CODES[weight_dtype], eps, positions.data_ptr(),
+            n, hq, hkv, dim, ptr(q_weight), ptr(k_weight), _lib.DTYPE_CODES[weight_dtype], float(eps), positions.data_ptr(),
             8 if positions.dtype == torch.int64 else 4, ps[0] if axes > 1 else 0, axes, sections, cos_sin.data_ptr(),
             max(table[0], rot), known, rot, 1 if interleaved else 0, code, ptr(slots), page, blocks, ptr(k_scale),
             ptr(v_scale), stream_handle(device),
@@ -186,5 +187,7 @@ def norm_rope_and_cache(
     cache of k's type or FP8 (with ``k_scale`` / ``v_scale``), of
     ``mxfp4_kv.reshape_and_cache_mxfp4`` for a uint8 one.  The keys are rounded to
     their type first, as there.  ``k_out`` receives them too if given.  Returns q_out."""
+    assert v is not None and key_cache is not None and value_cache is not None and slot_mapping is not None, \
+        "the append needs v, both caches and slot_mapping"
     return _run(q, k, v, positions, cos_sin, q_weight, k_weight, eps, sections, interleaved, q_out, k_out, key_cache,
                 value_cache, slot_mapping, k_scale, v_scale, "norm_rope_and_cache")[0]

@@ -148,6 +148,8 @@ NORM_ROPE = dict(q=FAKE, k=FAKE, v=FAKE, qo=FAKE, ko=None, kc=FAKE, vc=FAKE, str
     (ARG, b"16-byte", dict(q=FAKE + 8)),
     (ARG, b"16-byte", dict(strides=_strides("qkvop", v=(4 * 128 + 4, 128)))),
     (ARG, b"NULL", dict(strides=None)),
+    (ARG, b"shorter", dict(strides=_strides("qkvop", kc=(2 * 16 * 4 * 68, 0, 68)))),
+    (ARG, b"shorter", dict(strides=_strides("qkvop", vc=(2 * 16 * 4 * 68, 4 * 68, 64)))),
     (ARG, b"4-byte", dict(kc=FAKE + 2)),
     (ARG, b"8-byte", dict(cdt=3, kc=FAKE + 4)),
     (ARG, b"16-byte", dict(cdt=2, kc=FAKE + 8)),
