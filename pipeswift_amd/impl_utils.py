@@ -32,15 +32,15 @@ def _layer_scale(scale, layer_idx):
 def append_kv_cache(key, value, kv_cache_info: KVCacheInfo = None, layer_idx: int = 0):
     if key.shape[0] == 0:
         return
-    if kv_cache_info.kv_cache[0].dtype == torch.uint8:
-        reshape_and_cache_mxfp4(key, value, kv_cache_info.kv_cache[0][layer_idx], kv_cache_info.kv_cache[1][layer_idx],
-                                kv_cache_info.slot_mapping)
+    k_cache, v_cache = kv_cache_info.kv_cache[0][layer_idx], kv_cache_info.kv_cache[1][layer_idx]
+    if k_cache.dtype == torch.uint8:
+        reshape_and_cache_mxfp4(key, value, k_cache, v_cache, kv_cache_info.slot_mapping)
         return
     reshape_and_cache_flash(
         key,
         value,
-        kv_cache_info.kv_cache[0][layer_idx],
-        kv_cache_info.kv_cache[1][layer_idx],
+        k_cache,
+        v_cache,
         kv_cache_info.slot_mapping,
         _layer_scale(kv_cache_info.k_scale, layer_idx),
         _layer_scale(kv_cache_info.v_scale, layer_idx),
@@ -52,10 +52,12 @@ def norm_rope_append_kv_cache(query, key, value, positions, cos_sin, q_weight=No
     """query [N, Hq, D] and key [N, Hkv, D] normed and rotated (``rotary.norm_rope``),
     key and value appended to the layer's cache, whatever its type; returns the query."""
     k_cache, v_cache = kv_cache_info.kv_cache[0][layer_idx], kv_cache_info.kv_cache[1][layer_idx]
+    scales = None, None
+    if k_cache.dtype != torch.uint8:  # (4-bit rows have their own)
+        scales = _layer_scale(kv_cache_info.k_scale, layer_idx), _layer_scale(kv_cache_info.v_scale, layer_idx)
     return norm_rope_and_cache(
         query, key, value, k_cache, v_cache, kv_cache_info.slot_mapping, positions, cos_sin, q_weight, k_weight, eps,
-        sections, interleaved, _layer_scale(kv_cache_info.k_scale, layer_idx),
-        _layer_scale(kv_cache_info.v_scale, layer_idx), q_out)
+        sections, interleaved, *scales, q_out)
 
 
 def append_mla_kv_cache(ckv, kpe, kv_cache_info: KVCacheInfo = None, layer_idx: int = 0):

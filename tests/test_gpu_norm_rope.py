@@ -248,3 +248,22 @@ def test_many_tokens(dev, kind, dtype, N, Hq, Hkv, D, rot, axes, interleaved):
     else:
         reshape_and_cache.reshape_and_cache_flash(k, v, other[:, 0], other[:, 1], slots, **scales)
     assert torch.equal(_bytes(got), _bytes(q)) and torch.equal(_bytes(cache), _bytes(other))
+
+
+@pytest.mark.parametrize("kind", ["same", "fp8", "mxfp4"])
+def test_layer_calls_over_a_list_of_layers(dev, kind):
+    """The layer's calls with each layer's cache a tensor of its own, and scales where 4-bit rows have no use for them."""
+    x = Inputs(dev, 4, 9, 8, 2, 128, 128, torch.bfloat16)
+    layers, other = ([_caches(torch.Generator().manual_seed(i), kind, torch.bfloat16, 3, 16, 2, 128, dev) for i in range(2)]
+                     for _ in range(2))
+    info = metadata.KVCacheInfo.__new__(metadata.KVCacheInfo)
+    info.slot_mapping = torch.arange(9, device=dev) * 5
+    info.k_scale = info.v_scale = None if kind == "same" else torch.tensor([0.5, 0.25], device=dev)
+    info.kv_cache = [[c[:, 0] for c in layers], [c[:, 1] for c in layers]]
+    q = impl_utils.norm_rope_append_kv_cache(x.q, x.k, x.v, **x.args, kv_cache_info=info, layer_idx=1)
+    want, k = rotary.norm_rope(x.q, x.k, **x.args)
+    info.kv_cache = [[c[:, 0] for c in other], [c[:, 1] for c in other]]
+    impl_utils.append_kv_cache(k, x.v, info, 1)
+    assert torch.equal(_bytes(q), _bytes(want))
+    assert all(torch.equal(_bytes(a), _bytes(b)) for a, b in zip(layers, other))
+    assert not torch.equal(_bytes(layers[1]), _bytes(_caches(torch.Generator().manual_seed(1), kind, torch.bfloat16, 3, 16, 2, 128, dev)))
