@@ -648,7 +648,10 @@ int psk_gather_mxfp4(const void* cache, const void* cache_v, void* dst, void* ds
  *   s_j = softmax_scale (q . K[j, h]), out = sum_j softmax(s)_j V[j, h], lse = log sum_j exp s_j
  * Any number of query tokens and query heads per kv head; head_size 128.  q is bf16, f16
  * or f32 (16-byte aligned rows), taken to 2^-17 or better; out bf16, f16 or f32, rows
- * aligned to 4 elements.  Rows without a page are zeros; a query that sees no key gets
+ * aligned to 4 elements.  The weights meet V to 2^-17 or better; but into a bf16 out, in steps that
+ * go by blocks of query rows (more than 32 query rows a kv head, and from 17 on by the
+ * step's other sequences), rounded once to 2^-11, below that out's own 2^-8.  Rows without
+ * a page are zeros; a query that sees no key gets
  * zeros and -inf; a NaN in V reaches only the queries that see its token, and so does a
  * value past the largest finite float, which counts as NaN for its group of 32 columns; rows
  * that no sequence owns are left as they were.  A sequence longer than the block table reads

@@ -546,7 +546,10 @@ def paged_mxfp4_attention(
     """Attention over the 4-bit cache of ``mxfp4_kv``: decode, drafted tokens, prefill.
 
     q: [total_q, Hq, 128] in bf16, fp16 or fp32 (taken as it is to 2^-17 or better;
-    there is no quantized query and no descale).  Sequence b owns the query rows
+    there is no quantized query and no descale).  The softmax weights meet V to 2^-17 or
+    better, but in the form for many query rows a bf16 ``out`` has them rounded once to
+    2^-11, below its own 2^-8: which form a sequence takes can depend on the others of its
+    step.  Sequence b owns the query rows
     [cu_seqlens_q[b], cu_seqlens_q[b+1]) (int32 [B+1]; None: max_seqlen_q each), at
     most ``max_seqlen_q``: its last positions.  With ``causal`` token i of n sees the
     first seq_lens[b] - n + 1 + i keys, else all.  k_cache, v_cache: uint8 [num_blocks,

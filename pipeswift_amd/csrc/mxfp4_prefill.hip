@@ -10,9 +10,12 @@
 //     writes and both kinds of reads over the banks;
 //   * S^T = K Q^T is eight v_mfma_f32_32x32x16_bf16 for 32 keys and a wave's 32 query
 //     rows, and leaves each lane one row (l % 32) and keys 8 (i / 4) + 4 (l / 32) + i % 4;
-//   * O^T = V^T P^T is eight v_mfma_f32_32x32x16_f16: the lane's weights, rounded once to
-//     fp16 (2^-11), are the P^T operand as they stand, and ds_read_b64_tr_b16 gives V^T.
-//     Into a float32 out P is the sum of two fp16 (2^-22) and P V runs twice.
+//   * O^T = V^T P^T is eight v_mfma_f32_32x32x16_f16: the lane's weights are the P^T operand
+//     as they stand, and ds_read_b64_tr_b16 gives V^T.  Into an fp16 or float32 out P is the sum
+//     of two fp16 (2^-22) and P V runs twice.  Into a bf16 out P is rounded once (2^-11): the
+//     error against 64 bits is 1.669e-3 of the values so, 1.658e-3 by the output's rounding
+//     alone, and the second product would take 1470 us instead of 1060 for the chunk below.
+//     (One rounding into fp16 left 2.8e-4 where the output's own is 2.1e-4.)
 // V is exact in fp16 where its scales lie in [2^-23, 2^13]; a block that meets another
 // one is computed again with V as bf16 and P as the sum of two bf16 (2^-17).
 // A row's maximum is raised only when a tile's weights pass 2^15, to kHeadRoom below the
@@ -411,7 +414,7 @@ int launch_mx4_prefill(const DecodeArgs& a, const Mx4Prefill& s, float* workspac
   hipLaunchKernelGGL(mx4_order_kernel, dim3(1), dim3(1024), 0, st, a, int(s.num_seqs), int(s.total_q), p.tq, s.most, order,
                      order + s.num_seqs + 1);
   if (const int e = check_launch("mx4_order_kernel launch"); e != PSK_OK) return e;
-  const bool pairs = s.out_dtype == PSK_DTYPE_F32;
+  const bool pairs = s.out_dtype != PSK_DTYPE_BF16;
   switch (s.q_dtype) {
     case PSK_DTYPE_BF16:
       return pairs ? launch<PSK_DTYPE_BF16, true>(p, jobs, st) : launch<PSK_DTYPE_BF16, false>(p, jobs, st);

@@ -429,3 +429,35 @@ def test_sequences_that_share_their_first_pages(dev):
     c.bt[2] = c.bt[0]
     c.btd = c.bt.to(dev)
     _both(c)
+
+
+class ExactScores(Case):
+    """Queries of small whole numbers, so that every q K and every sum of them is exact, and
+    V of 6 at the first token, 0 at all others: out is 6 times the first token's weight."""
+
+    def __init__(self, dev, seed, lens, counts, Hq, Hkv, ps, dtype, k_byte=127):
+        super().__init__(dev, seed, lens, counts, Hq, Hkv, ps, dtype)
+        self.q = torch.randint(-2, 3, self.q.shape, generator=self.g).to(dtype)
+        self.qd = self.q.to(dev)
+        self.fused[:, 0, ..., 64:] = k_byte
+        self.fused[:, 1, ..., :64], self.fused[:, 1, ..., 64:] = 0, 127
+        for b in range(len(lens)):
+            self.fused[self.bt[b, 0], 1, 0, :, :64] = 0x77
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("counts", [[300, 40], [1, 1]])
+def test_weights_under_an_fp16_output_are_finer_than_it(dev, dtype, counts):
+    """The scores are exact but for their scaling, an error d of 4 e of the largest; a weight is off by
+    2 (exp(d) - 1) of itself, 2^-17 of it as a sum of two 16-bit parts, (K + 64) 2 e by the sums; what
+    is left is the output's own rounding, 2^-11 (2^-25 below its normal range), and what the parts
+    lose of weights 2^-33 of the largest."""
+    c = ExactScores(dev, 31, [300, 700], counts, 8, 2, 16, dtype)
+    out = torch.empty(c.q.shape, dtype=torch.float16, device=dev)
+    c.run(out=out)
+    w, _, most = c.want()
+    d = 4 * EPS * max(most, 1.0) * 2
+    fine = np.abs(w) * (2 * np.expm1(d) + 2.0 ** -17 + (700 + 64) * 2 * EPS) + 6 * 2.0 ** -33
+    err = np.abs(out.double().cpu().numpy() - w)
+    tol = fine + 2.0 ** -11 * (np.abs(w) + fine) + 2.0 ** -25
+    assert (err <= tol).all(), f"off by {(err / tol).max():.3f} of the bound"
