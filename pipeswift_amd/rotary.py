@@ -76,6 +76,7 @@ def _run(q, k, v, positions, cos_sin, q_weight, k_weight, eps, sections, interle
     known, rot = cos_sin.shape
     table = cos_sin.stride()
     assert cos_sin.dtype == torch.float32 and table[1] == 1, "cos_sin must be float32 [positions, rot] with unit last stride"
+    assert table[0] >= rot or known <= 1, f"cos_sin has rows of {rot} that are {table[0]} apart"
     dims = len(positions.shape)
     ps = positions.stride()
     assert dims in (1, 2) and positions.shape[-1] == n and (ps[-1] == 1 or n <= 1), \
@@ -133,7 +134,7 @@ def _run(q, k, v, positions, cos_sin, q_weight, k_weight, eps, sections, interle
             pack_i64x16(*qs[:2], *ks[:2], *vs[:2], *q_out.stride()[:2], *os[:2], *kcs[:3], *vcs[:3]), _lib.DTYPE_CODES[dtype],
             n, hq, hkv, dim, ptr(q_weight), ptr(k_weight), _lib.DTYPE_CODES[weight_dtype], float(eps), positions.data_ptr(),
             8 if positions.dtype == torch.int64 else 4, ps[0] if axes > 1 else 0, axes, sections, cos_sin.data_ptr(),
-            max(table[0], rot), known, rot, 1 if interleaved else 0, code, ptr(slots), page, blocks, ptr(k_scale),
+            table[0] if known > 1 else rot, known, rot, 1 if interleaved else 0, code, ptr(slots), page, blocks, ptr(k_scale),
             ptr(v_scale), stream_handle(device),
         )
     if st:

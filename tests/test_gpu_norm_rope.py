@@ -267,3 +267,15 @@ def test_layer_calls_over_a_list_of_layers(dev, kind):
     assert torch.equal(_bytes(q), _bytes(want))
     assert all(torch.equal(_bytes(a), _bytes(b)) for a, b in zip(layers, other))
     assert not torch.equal(_bytes(layers[1]), _bytes(_caches(torch.Generator().manual_seed(1), kind, torch.bfloat16, 3, 16, 2, 128, dev)))
+
+
+def test_tables_that_are_broadcasts_or_single_rows(dev):
+    """A broadcast table is refused; a table of one row has whatever stride it likes."""
+    x = Inputs(dev, 9, 4, 3, 1, 64, 64, torch.bfloat16, P=1)
+    with pytest.raises(AssertionError):
+        rotary.norm_rope(x.q, x.k, **{**x.args, "cos_sin": x.args["cos_sin"].expand(500, 64)})
+    for stride in (0, 3, 64, 1000):
+        one = x.args["cos_sin"].as_strided((1, 64), (stride, 1))
+        q, k = rotary.norm_rope(x.q, x.k, **{**x.args, "cos_sin": one})
+        for i, got in enumerate((q, k)):
+            _check(got, *x.want(i), torch.bfloat16)
