@@ -39,7 +39,7 @@ def _span(t):
 
 
 def _check_out(out, own, others, name):
-    """An output is its input itself, or shares no element with any input."""
+    """An output is its input itself, or shares no element with any input, other output or cache."""
     assert out.shape == own.shape and out.dtype == own.dtype and out.device == own.device, \
         f"{name} must have the shape and type of its input"
     assert out.stride(2) == 1 or out.shape[2] <= 1, f"{name} needs unit last stride"
@@ -51,7 +51,7 @@ def _check_out(out, own, others, name):
             continue
         a, b = _span(t)
         assert b < lo or hi < a or t.element_size() == out.element_size() and not overlap(out, t), \
-            f"{name} must be its input itself or share no element with the inputs and outputs"
+            f"{name} must be its input itself or share no element with the inputs, outputs and caches"
 
 
 def _sections(sections, axes, pairs):
@@ -95,9 +95,9 @@ def _run(q, k, v, positions, cos_sin, q_weight, k_weight, eps, sections, interle
     if q_out is None:
         q_out = torch.empty((n, hq, dim), dtype=dtype, device=device)
     else:
-        _check_out(q_out, q, (k, v, k_out), "q_out")
+        _check_out(q_out, q, (k, v, k_out, kc, vc), "q_out")
     if k_out is not None:
-        _check_out(k_out, k, (q, v), "k_out")
+        _check_out(k_out, k, (q, v, kc, vc), "k_out")
     elif kc is None:
         k_out = torch.empty((n, hkv, dim), dtype=dtype, device=device)
     vs = os = kcs = vcs = (0, 0, 0)

@@ -31,3 +31,20 @@ def test_tables_whose_rows_overlap(stride):
     x["cos_sin"] = _gpu(torch.zeros(500 * 64).as_strided((500, 64), (stride, 1)))
     with pytest.raises(AssertionError, match="cos_sin"):
         rotary.norm_rope(**x)
+
+
+@pytest.mark.parametrize("kind", ["same", "fp8", "mxfp4"])
+@pytest.mark.parametrize("name,side", [("q_out", 0), ("q_out", 1), ("k_out", 0), ("k_out", 1)])
+def test_outputs_that_lie_in_a_cache(kind, name, side):
+    """Where the append writes, whatever the cache's type; beside it they are no concern."""
+    x = _inputs()
+    heads, D = (4, 64) if name == "q_out" else (2, 64)
+    store = torch.zeros(1 << 16, dtype=torch.uint8)
+    entry, dtype, size = {"same": (64, torch.bfloat16, 2), "fp8": (64, torch.float8_e4m3fn, 1), "mxfp4": (36, torch.uint8, 1)}[kind]
+    fused = store[:3 * 2 * 16 * 2 * entry * size].view(dtype).view(3, 2, 16, 2, entry)
+    at = side * 16 * 2 * entry * size  # where that cache begins
+    out = store[at:at + 4 * heads * D * 2].view(torch.bfloat16).view(4, heads, D)
+    x |= dict(v=_gpu(torch.zeros(4, 2, D, dtype=torch.bfloat16)), key_cache=_gpu(fused[:, 0]), value_cache=_gpu(fused[:, 1]),
+              slot_mapping=_gpu(torch.arange(4)))
+    with pytest.raises(AssertionError, match=f"{name} must be its input itself or share no element"):
+        rotary.norm_rope_and_cache(**x, **{name: _gpu(out)})
