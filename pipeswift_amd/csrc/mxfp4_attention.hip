@@ -800,11 +800,18 @@ bool loads_together(Mx4Args& p) {
   return (align & 15) == 0;
 }
 
+// How a cut step's rows are joined (by the records of a row, about), and by how many workgroups.
+bool joins_by_halves(const Mx4Shape& s, int64_t jobs, int64_t tasks) { return s.max_runs <= 8 * jobs || tasks > kMergeWide; }
+int64_t merge_groups(bool few, int64_t tasks) { return ceil_div(tasks, few ? kMergeThreads<2> / 64 : 1); }
+
+// Workgroups of the rows' kernel.
+int64_t row_groups(const Mx4Shape& s, int64_t jobs) { return (s.whole ? ceil_div(jobs, 8) * 8 : s.max_runs) * s.row_blocks; }
+
 template <int Q_DT>
 int launch(Mx4Args p, const Mx4Shape& s, hipStream_t st) {
   const bool general = !loads_together(p);
   const int64_t jobs = int64_t(p.s.num_seqs) * p.s.heads;
-  const dim3 grid{unsigned((p.whole ? ceil_div(jobs, 8) * 8 : s.max_runs) * s.row_blocks), 1u, 1u};
+  const dim3 grid{unsigned(row_groups(s, jobs)), 1u, 1u};
   const dim3 block(kThreads);
   if (s.sets == 1 && general) hipLaunchKernelGGL((mx4_attention_kernel<Q_DT, 1, true>), grid, block, 0, st, p);
   else if (s.sets == 1) hipLaunchKernelGGL((mx4_attention_kernel<Q_DT, 1, false>), grid, block, 0, st, p);
@@ -812,11 +819,8 @@ int launch(Mx4Args p, const Mx4Shape& s, hipStream_t st) {
   else hipLaunchKernelGGL((mx4_attention_kernel<Q_DT, 2, false>), grid, block, 0, st, p);
   if (const int e = check_launch("mx4_attention_kernel launch"); e != PSK_OK || p.whole) return e;
   const int64_t tasks = int64_t(p.s.num_seqs) * p.s.heads * p.hg * p.max_rows;
-  // records of a row, about
-  const bool few = s.max_runs <= 8 * jobs || tasks > kMergeWide;
-  const int64_t groups = ceil_div(tasks, few ? kMergeThreads<2> / 64 : 1);
-  if (groups > (1 << 21)) return fail(PSK_E_ARG, "too many rows (%lld)", (long long)tasks);
-  const dim3 merge{unsigned(groups), 1u, 1u}, threads{unsigned(few ? kMergeThreads<2> : kMergeThreads<32>)};
+  const bool few = joins_by_halves(s, jobs, tasks);
+  const dim3 merge{unsigned(merge_groups(few, tasks)), 1u, 1u}, threads{unsigned(few ? kMergeThreads<2> : kMergeThreads<32>)};
   if (s.sets == 1 && few) hipLaunchKernelGGL((merge_mx4_kernel<16, 2>), merge, threads, 0, st, p, tasks);
   else if (s.sets == 1) hipLaunchKernelGGL((merge_mx4_kernel<16, 32>), merge, threads, 0, st, p, tasks);
   else if (few) hipLaunchKernelGGL((merge_mx4_kernel<32, 2>), merge, threads, 0, st, p, tasks);
@@ -891,6 +895,15 @@ int psk_paged_mxfp4_attention(const void* q, int64_t q_tok_stride, int64_t q_hea
   hipStream_t st = static_cast<hipStream_t>(stream);
   const Route r = route(num_seqs, total_q, max_seqlen_q, a.heads, num_kv_heads);
   const int64_t row_q = r.row_tokens;
+  Mx4Shape s{};
+  if (r.way != kBlocks) {  // refused before the first launch, which may be the blocks'
+    s = mx4_shape(num_seqs, row_q, num_q_heads, num_kv_heads, max_seq_len, q_dtype);
+    const int64_t jobs = num_seqs * s.groups, tasks = num_seqs * num_kv_heads * row_q * a.heads;
+    constexpr int64_t kMost = (int64_t(1) << 32) / kThreads - 1;  // a launch has fewer than 2^32 threads
+    if (row_groups(s, jobs) > kMost || (!s.whole && merge_groups(joins_by_halves(s, jobs, tasks), tasks) > 1 << 21))
+      return fail(PSK_E_ARG, "too many rows (%lld sequences of up to %lld query tokens)", (long long)num_seqs,
+                  (long long)row_q);
+  }
   if (r.way != kRows) {
     const int32_t most = r.way == kBoth ? int32_t(row_q) : 0;
     const Mx4Prefill step{num_seqs, total_q, max_seqlen_q, max_seq_len, most, p.scale_log2, q_dtype, out_dtype};
@@ -898,7 +911,6 @@ int psk_paged_mxfp4_attention(const void* q, int64_t q_tok_stride, int64_t q_hea
     if (e != PSK_OK || r.way == kBlocks) return e;
     p.s.most = most;
   }
-  const Mx4Shape s = mx4_shape(num_seqs, row_q, num_q_heads, num_kv_heads, max_seq_len, q_dtype);
   p.s.num_seqs = int32_t(num_seqs);
   p.s.total_q = int32_t(total_q);
   p.s.heads = int32_t(s.groups);
@@ -915,10 +927,6 @@ int psk_paged_mxfp4_attention(const void* q, int64_t q_tok_stride, int64_t q_hea
   p.whole = s.whole;
   p.out_dtype = out_dtype;
   p.records = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
-  constexpr int64_t kMost = (int64_t(1) << 24) - 8;  // workgroups of a launch
-  if (std::max(num_seqs * s.groups, s.max_runs) > kMost / s.row_blocks)
-    return fail(PSK_E_ARG, "too many rows (%lld sequences of up to %lld query tokens)", (long long)num_seqs,
-                (long long)max_seqlen_q);
   switch (q_dtype) {
     case PSK_DTYPE_BF16: return launch<PSK_DTYPE_BF16>(p, s, st);
     case PSK_DTYPE_F16: return launch<PSK_DTYPE_F16>(p, s, st);

@@ -222,3 +222,12 @@ def test_empty_attention_touches_nothing():
 
 def test_a_short_step_needs_no_workspace():
     assert _call("psk_paged_mxfp4_workspace_len", dict(B=2, TQ=2, n=1, Hq=8, Hkv=4, most=1024), {}) == 0
+
+
+@pytest.mark.parametrize("change", [
+    dict(B=65537, TQ=65537, n=1, Hq=256, Hkv=8),               # 2^24 rows and more to join
+    dict(B=1024, TQ=1024 * 32, n=33, Hq=1024, Hkv=1024),       # the same, behind the launch for the longer sequences
+    dict(B=9 << 20, TQ=9 << 20, n=1, Hq=1, Hkv=1, most=100),   # uncut, 2^32 threads
+])
+def test_attention_refuses_too_many_rows_before_any_launch(change):
+    _refused("psk_paged_mxfp4_attention", ATTENTION, ARG, b"too many rows", change)
