@@ -651,8 +651,8 @@ int psk_gather_mxfp4(const void* cache, const void* cache_v, void* dst, void* ds
  * aligned to 4 elements.  The weights meet V to 2^-17 or better; but into a bf16 out, in steps that
  * go by blocks of query rows (more than 32 query rows a kv head, and from 17 on by the
  * step's other sequences), rounded once to 2^-11, below that out's own 2^-8.  Rows without
- * a page are zeros; a query that sees no key gets
- * zeros and -inf; a NaN in V reaches only the queries that see its token, and so does a
+ * a page are zeros; a query that sees no key gets zeros and -inf (one whose scores are all
+ * infinite, past the largest float among them, NaN); a NaN in V reaches only the queries that see its token, and so does a
  * value past the largest finite float, which counts as NaN for its group of 32 columns; rows
  * that no sequence owns are left as they were.  A sequence longer than the block table reads
  * zeros past it.  max_seq_len and max_seqlen_q (bounds) size and cut the launch.

@@ -242,8 +242,6 @@ mx4_attention_kernel(Mx4Args args) {
     auto limit = [&](int i) { return a.causal ? min(max(base + i, 0), L) : L; };
     const int key_hi = limit(min((row0 + kRows - 1) / a.heads, r.n - 1)), key_open = limit(row0 / a.heads);
     const float sl_signed = float(p.scale_log2);
-    // a negative scale is applied as -q (exact); a scale of 0 stays above it, for a hidden key's -inf
-    const float sl = __builtin_fmaxf(__builtin_fabsf(sl_signed), 0x1p-126f);
     int row_lim[kSets];
     bf16x8 qop[kSets][4], qlo[kPairs ? kSets : 1][4];
 #pragma unroll
@@ -260,10 +258,13 @@ mx4_attention_kernel(Mx4Args args) {
                      qop[s][q], qlo[kPairs ? s : 0][q]);
     }
     float m[kSets], l[kSets];
+    // once a row's maximum is_far, the wave's tiles take the masked way, where the scale is applied first
+    bool far = false;
+    float mul = scale_size(p.scale_log2);  // or 1
     f32x4 o[kSets][8];
 #pragma unroll
     for (int s = 0; s < kSets; ++s) {
-      m[s] = kNegBig;
+      m[s] = kNoScore;
       l[s] = 0.0f;
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[s][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -321,6 +322,7 @@ mx4_attention_kernel(Mx4Args args) {
 
       const int t_end = min(s1 << wph_shift, (key_hi + kTile - 1) / kTile);
       const int s_end = (t_end + wph - 1) >> wph_shift;
+      int t_mask = far ? 0 : key_open / kTile;  // tiles from here on need masks
       // What is not cached loads from the first page and is dropped by attend().  Unless
       // GEN, a unit's keys share a page: lane units k + u holds where unit u of stage win + k
       // begins, for 64 / units stages at a time.
@@ -425,6 +427,7 @@ mx4_attention_kernel(Mx4Args args) {
           }
         };
         put_v(0);
+        const bool was_far = far;
         float sc[kSets][4 * kHalves];
 #pragma unroll
         for (int u = 0; u < kHalves; ++u) {
@@ -453,13 +456,18 @@ mx4_attention_kernel(Mx4Args args) {
 #pragma unroll
             for (int i = 0; i < 4 * kHalves; ++i)
               sc[e][i] = t * kTile + 16 * (i >> 2) + 4 * l4 + (i & 3) < row_lim[e] ? sc[e][i] : -__builtin_inff();
+            if (was_far) {
+              const float sl = scale_size(args_again<Mx4Args>().scale_log2);
+#pragma unroll
+              for (int i = 0; i < 4 * kHalves; ++i) sc[e][i] *= sl;
+            }
           }
           float pv[4 * kHalves], sum = 0.0f;
           auto weigh = [&] {
             sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4 * kHalves; ++i) {
-              pv[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e][i], sl, -m[e]));
+              pv[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e][i], mul, -m[e]));
               sum += pv[i];
             }
           };
@@ -468,7 +476,7 @@ mx4_attention_kernel(Mx4Args args) {
             float top = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < 4 * kHalves; ++i) top = __builtin_fmaxf(top, sc[e][i]);
-            top *= sl;
+            top *= mul;
             top = __builtin_fmaxf(top, __shfl_xor(top, 16));
             top = __builtin_fmaxf(top, __shfl_xor(top, 32));
             const float mn = __builtin_fmaxf(m[e], top);
@@ -477,6 +485,16 @@ mx4_attention_kernel(Mx4Args args) {
             l[e] *= f;
 #pragma unroll
             for (int d = 0; d < 8; ++d) o[e][d] *= f;
+            if (!far && __any(is_far(mn))) {  // (this set's scores and those of the sets that follow)
+              far = true;
+              t_mask = 0;
+#pragma unroll
+              for (int x = e; x < kSets; ++x) {
+#pragma unroll
+                for (int i = 0; i < 4 * kHalves; ++i) sc[x][i] *= mul;
+              }
+              mul = 1.0f;
+            }
             weigh();
           }
           l[e] += sum;
@@ -521,7 +539,6 @@ mx4_attention_kernel(Mx4Args args) {
         }
       };
 
-      const int t_mask = key_open / kTile;  // tiles from here on need masks
       const int stage_loads = segs * ((chunks + 63) >> 6);
       // (the builtin would wait for the loads too, which the compiler does not see)
       auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
@@ -585,7 +602,7 @@ mx4_attention_kernel(Mx4Args args) {
       const int first = hl << rest.wph_shift;
       float top = m[s];
       if (wph > 1) {
-        top = kNegBig;
+        top = kNoScore;
 #pragma unroll 1
         for (int v = 0; v < wph; ++v) top = __builtin_fmaxf(top, s_m[first + v][16 * s + l15]);
       }
@@ -602,7 +619,7 @@ mx4_attention_kernel(Mx4Args args) {
         const int g = (i >> 3) & 3, at = ((i >> 1) - (GEN ? 0 : g)) & 3;
         const int from = 64 * (2 * g + (at >> 1)) + 16 * (2 * (at & 1) + (i & 1)) + row16;
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        float high = kNegBig, sum = 0.0f;
+        float high = kNoScore, sum = 0.0f;
 #pragma unroll 1
         for (int u = 0; u < wph; ++u) {
           v += s_o[512 * (v0 + u) + from];
@@ -614,7 +631,7 @@ mx4_attention_kernel(Mx4Args args) {
         if (__builtin_expect(s_nan[head][g] < lim, 0)) v = f32x4(__builtin_nanf(""));
         const int col = 4 * (i & 31);
         if (all) {
-          finish(rest.a, rest.out_dtype, r, grp * rest.hg + head, row0 + row, col, v, high, sum);
+          finish(rest.a, rest.out_dtype, r, grp * rest.hg + head, row0 + row, col, v, high, sum, lim > 0);
         } else {
           float* rec = record(rest, j, block, c.from == 0 ? 1 : 0, head, row);
           *reinterpret_cast<f32x4*>(rec + col) = v;
@@ -670,8 +687,9 @@ __global__ void __launch_bounds__(kMergeThreads<kParts>) merge_mx4_kernel(Mx4Arg
   const int64_t j0 = uniform_div(at, run), j1 = steps > 0 ? uniform_div(at + steps - 1, run) : j0 - 1;
   if (j0 == j1) return;  // one run had all the keys and wrote the row
   const int block = row / kRows, in_block = row - block * kRows;
+  const bool sees = (a.causal ? L - r.n + 1 + row / a.heads : L) > 0;
 
-  float top = kNegBig, sum = 0.0f;
+  float top = kNoScore, sum = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int kAhead = kParts == 2 ? 4 : 8;  // records read together
 #pragma unroll 1
@@ -702,7 +720,7 @@ __global__ void __launch_bounds__(kMergeThreads<kParts>) merge_mx4_kernel(Mx4Arg
     f32x4 other;
 #pragma unroll
     for (int i = 0; i < 4; ++i) other[i] = __shfl_xor(o[i], 32);
-    if (part == 0) finish(a, p.out_dtype, r, h, row, 4 * at4, o * f0 + other * f1, up, sum * f0 + l1 * f1);
+    if (part == 0) finish(a, p.out_dtype, r, h, row, 4 * at4, o * f0 + other * f1, up, sum * f0 + l1 * f1, sees);
   } else {
     s_o[part][at4] = o;
     if (at4 == 0) {
@@ -727,7 +745,7 @@ __global__ void __launch_bounds__(kMergeThreads<kParts>) merge_mx4_kernel(Mx4Arg
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], 32);
     if (part > 0) return;
-    finish(a, p.out_dtype, r, h, row, 4 * at4, o, top, sum);
+    finish(a, p.out_dtype, r, h, row, 4 * at4, o, top, sum, sees);
   }
 }
 

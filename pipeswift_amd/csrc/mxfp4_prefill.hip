@@ -144,8 +144,6 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
   const int w_open = limit(w.i0 + wave * 32 / G), w_end = wave_live ? limit(w.i0 + min((wave * 32 + 31) / G, w.ni - 1)) : 0;
 
   const float sl_signed = float(p.scale_log2);
-  // a negative scale is applied as -q (exact); a scale of 0 stays above it, for a hidden key's -inf
-  const float sl = __builtin_fmaxf(__builtin_fabsf(sl_signed), 0x1p-126f);
   bf16x8 qop[8], qlo[kPairs ? 8 : 1];
   {
     const char* src = live ? a.q + (int64_t(w.r.first) + w.i0 + ti) * a.q_tok_stride +
@@ -201,6 +199,10 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
   };
 
   float m, l;
+  // once a row's maximum is_far, the wave's tiles take the masked way, where the scale is applied first
+  bool far;
+  float mul;  // the scale, or 1
+  int open;  // keys that all of the wave's rows see
   f32x16 o[4];
   // V^T reads: in each 16 lanes lane r addresses key r / 4 (of the four from 4 half) and columns 4 (r % 4)
   const int vr = lane & 15, vkey = 4 * half + (vr >> 2), vg = (lane >> 4) & 1;
@@ -219,13 +221,14 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     if (masked) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) y[i] = key0 + 8 * (i >> 2) + 4 * half + (i & 3) < row_lim ? y[i] : -__builtin_inff();
+      if (far) y *= scale_size(args_again<PrefillArgs>().scale_log2);
     }
     float e[16], sum = 0.0f;
     auto weigh = [&] {
       sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[i], sl, -m));
+        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[i], mul, -m));
         sum += e[i];
       }
     };
@@ -234,14 +237,21 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
       float top = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, y[i]);
-      top *= sl;
-      top = __builtin_fmaxf(top, __shfl_xor(top, 32)) - kHeadRoom;
+      top *= mul;
+      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+      if (!is_far(top)) top -= kHeadRoom;  // (a far one's steps may be wider than that)
       const float mn = __builtin_fmaxf(m, top);
       const float f = __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= f;
 #pragma unroll
       for (int d = 0; d < 4; ++d) o[d] *= f;
+      if (!far && __any(is_far(mn))) {
+        far = true;
+        open = 0;
+        y *= mul;
+        mul = 1.0f;
+      }
       weigh();
     }
     l += sum;
@@ -282,8 +292,11 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 
   // The loads of stage t + 1 fly while stage t is computed, and the page ids of t + 2.
   auto stream = [&](auto wide_tag) {
-    m = kNegBig;
+    m = kNoScore;
     l = 0.0f;
+    far = false;
+    mul = scale_size(p.scale_log2);
+    open = w_open;
 #pragma unroll
     for (int d = 0; d < 4; ++d) o[d] = f32x16{};
     if (t_from >= t_to) return;
@@ -300,7 +313,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
       for (int kb = 0; kb < kStage / 32; ++kb) {
         const int key0 = t * kStage + 32 * kb;
-        if (key0 < w_end) tile(wide_tag, t & 1, key0, kb, key0 + 32 > w_open);
+        if (key0 < w_end) tile(wide_tag, t & 1, key0, kb, key0 + 32 > open);
       }
       if (more) put_stage(wide_tag, (t + 1) & 1, t + 1);
       __syncthreads();
@@ -331,7 +344,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
           rec[kHead + 1] = sum;
         }
       } else {
-        finish(a, p.out_dtype, SeqRows{w.r.first + w.i0, w.ni}, h, row, col, v, m, sum);
+        finish(a, p.out_dtype, SeqRows{w.r.first + w.i0, w.ni}, h, row, col, v, m, sum, row_lim > 0);
       }
     }
   }
@@ -348,7 +361,7 @@ __global__ void __launch_bounds__(256) mx4_prefill_merge_kernel(PrefillArgs p) {
   if (!block_of(p, idx, lane, w) || row >= w.ni * a.heads) return;
   const int at4 = lane & 31;
   const float* rec = p.records + (int64_t(job) * p.splits * kBlock + row) * kRecord;
-  float top = kNegBig, sum = 0.0f;
+  float top = kNoScore, sum = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int s = 0; s < p.splits; ++s, rec += int64_t(kBlock) * kRecord) {
     const float m = rec[kHead], l = rec[kHead + 1];
@@ -359,7 +372,9 @@ __global__ void __launch_bounds__(256) mx4_prefill_merge_kernel(PrefillArgs p) {
     sum = sum * f0 + l * f1;
     o = o * f0 + v * f1;
   }
-  finish(a, p.out_dtype, SeqRows{w.r.first + w.i0, w.ni}, h, row, 4 * at4, o, top, sum);
+  const int L = cached_len(a, w.b);
+  const bool sees = (a.causal ? L - w.r.n + 1 + w.i0 + row / a.heads : L) > 0;
+  finish(a, p.out_dtype, SeqRows{w.r.first + w.i0, w.ni}, h, row, 4 * at4, o, top, sum, sees);
 }
 
 // Blocks at most: whole ones, and a partial one a sequence.

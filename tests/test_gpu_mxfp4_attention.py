@@ -461,3 +461,41 @@ def test_weights_under_an_fp16_output_are_finer_than_it(dev, dtype, counts):
     err = np.abs(out.double().cpu().numpy() - w)
     tol = fine + 2.0 ** -11 * (np.abs(w) + fine) + 2.0 ** -25
     assert (err <= tol).all(), f"off by {(err / tol).max():.3f} of the bound"
+
+
+@pytest.mark.parametrize("k_byte", [150, 170, 238])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [50, 3, 9], [100, 200, 40]])
+def test_scores_far_from_zero(dev, counts, dtype, sign, k_byte):
+    """Finite scores of one sign, up to 5 10^35, exact but for their scaling: the largest takes all,
+    equal ones share.  Values of 1 to 6 under one scale 2^(byte - 127) and queries of 1 and 2 make
+    scores of 2^(byte - 123) to 2^(byte - 119) in the exponent of 2, half a scale apart, which is
+    2^(byte - 131) there; their rounding is 2^(byte - 144) at most.  So from byte 150 on all but the
+    largest have weight 0, and equal scores equal weights: out is off by a sum's division, 4 e of the
+    largest |V|, and its own rounding; lse by 6 e of itself (scale, products, log 2, sum)."""
+    c = ExactScores(dev, 32, [1500, 70, 200], counts, 8, 2, 16, dtype, k_byte)
+    c.q = (torch.randint(1, 3, c.q.shape, generator=c.g) * sign).to(dtype)
+    c.qd = c.q.to(dev)
+    c.fused[:, 0, ..., :64] = (c.fused[:, 0, ..., :64] & 0x77) | 0x22  # codes 2, 3, 6 and 7
+    c.fused[:, 1] = M.quantize(np.random.default_rng(1).standard_normal((*c.fused[:, 1].shape[:-1], 128)))
+    (out, lse), (w, wl, _) = c.run(), c.want()
+    got, gl = out.double().cpu().numpy(), lse.double().cpu().numpy().T
+    see = np.isfinite(wl)
+    assert (np.sign(wl[see]) == sign).all() and (np.abs(wl[see]) > 2.0 ** (k_byte - 124)).all()
+    tol = STEP[out.dtype] * np.abs(w) + 4 * EPS * np.abs(M.dequantize(c.fused[:, 1], 128)).max()
+    assert np.array_equal(np.isneginf(gl), ~see)
+    assert (np.abs(got - w) <= tol).all(), f"off by {np.nanmax(np.abs(got - w) / tol):.3f} of the bound"
+    assert (np.abs(gl[see] - wl[see]) <= 6 * EPS * np.abs(wl[see])).all()
+
+
+@pytest.mark.parametrize("counts", [[1, 1], [40, 3], [1, 90]])
+def test_scores_past_the_largest_float_are_not_taken_for_no_keys(dev, counts):
+    """All of a row's scores minus infinity: NaN, where a row that sees no key is zeros."""
+    c = ExactScores(dev, 33, [1300, 50], counts, 8, 2, 16, torch.bfloat16, 254)
+    c.qd = torch.full_like(c.qd, -2.0)
+    c.fused[:, 0, ..., :64] = 0x77
+    out, lse = c.run()
+    see = np.concatenate([[L - n + 1 + i > 0 for i in range(n)] for L, n in zip(c.lens, counts)])
+    assert torch.isnan(out[torch.from_numpy(see)]).all() and (out[torch.from_numpy(~see)] == 0).all()
+    assert torch.isneginf(lse).all()
