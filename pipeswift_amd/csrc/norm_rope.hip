@@ -86,6 +86,12 @@ __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
+// 1 / sqrt(x); v_rsq_f32 takes a subnormal x (a small row without an eps) for zero.
+__device__ __forceinline__ float rsqrt_any(float x) {
+  const bool small = x < 0x1p-100f;
+  return __builtin_amdgcn_rsqf(small ? x * 0x1p64f : x) * (small ? 0x1p32f : 1.0f);
+}
+
 // Eight elements as they were loaded.
 template <int DT>
 struct Eight {
@@ -336,7 +342,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRopeArgs a) {
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(v[j], v[j], sum);
-      rstd = __builtin_amdgcn_rsqf(row_sum<LPR>(sum) / float(a.head_size) + a.eps);
+      rstd = rsqrt_any(row_sum<LPR>(sum) / float(a.head_size) + a.eps);
     }
     float z[8];
 #pragma unroll

@@ -279,3 +279,18 @@ def test_tables_that_are_broadcasts_or_single_rows(dev):
         q, k = rotary.norm_rope(x.q, x.k, **{**x.args, "cos_sin": one})
         for i, got in enumerate((q, k)):
             _check(got, *x.want(i), torch.bfloat16)
+
+
+@pytest.mark.parametrize("N", [6, 2050])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_whose_squares_are_subnormal_without_an_eps(dev, dtype, N):
+    """Squares of about 2^-130: each is off by 2^-150 and so is each of their sums, the mean by 2^-149
+    with its division, and the reciprocal root by no more than the mean's share of that."""
+    x = Inputs(dev, 10, N, 4, 2, 128, 64, dtype)
+    for t in (x.on_dev, x.qkv):
+        t *= 2.0 ** -66
+    for i, got in enumerate(rotary.norm_rope(x.q, x.k, **x.args, eps=0.0)):
+        want, size = x.want(i, eps=0.0)
+        mean = (x.host[i].double().numpy() ** 2).mean(-1, keepdims=True)
+        assert (mean < 2.0 ** -126).any() and (mean > 2.0 ** -131).all()
+        _check(got, want, size * (1 + 2.0 ** -149 / mean / (18 * 2.0 ** -24)), dtype)
