@@ -499,3 +499,17 @@ def test_scores_past_the_largest_float_are_not_taken_for_no_keys(dev, counts):
     see = np.concatenate([[L - n + 1 + i > 0 for i in range(n)] for L, n in zip(c.lens, counts)])
     assert torch.isnan(out[torch.from_numpy(see)]).all() and (out[torch.from_numpy(~see)] == 0).all()
     assert torch.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_blocks_of_more_sequences_than_are_ordered(dev, causal):
+    """1100 sequences, among them some without query tokens, of up to 46 rows a kv head: blocks in batch order."""
+    lens = [(37 * i) % 90 for i in range(1100)]
+    _both(Case(dev, 34, lens, [(5 * i) % 24 for i in range(1100)], 4, 2, 16, spare_rows=2), causal=causal, max_seq_len=90)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("Hq,Hkv,lens,counts", [
+    (300, 1, [700, 40], [1, 3]), (520, 2, [1500, 0, 90], [2, 1, 2]), (257, 1, [5], [1]), (1000, 1, [2100], [20])])
+def test_more_query_heads_than_a_block_has_rows(dev, dtype, Hq, Hkv, lens, counts):
+    _both(Case(dev, Hq, lens, counts, Hq, Hkv, 16, dtype))
