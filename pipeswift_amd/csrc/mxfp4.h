@@ -16,8 +16,8 @@
 // that holds an infinity or a NaN has no scale: it reads as NaN.
 //
 // v_cvt_scalef32_pk_fp4_* and *_pk_*_fp4 compute exactly this for every scale byte
-// (round to nearest even, denormals kept, NaN for 0xFF): checked on all bf16 values
-// and all codes.
+// (round to nearest even, denormals kept, NaN for 0xFF, and 2^-127 for byte 0, which is handed
+// to them as 0.0): checked on all bf16 values and on all codes under all scale bytes.
 #pragma once
 
 #include "psk_common.h"

@@ -14,7 +14,7 @@ rot/2 pairs, then their sines.  ``positions`` is [N], or [axes, N] for several a
 (time, height, width): then ``sections`` says how many pairs, in order, go by each.
 A weight that counts from one (``1 + w``) is passed with the one added.
 Results are rounded once, to the input's type.  A position outside the table turns
-its head to NaN.
+the pairs that go by it to NaN, and no other element.
 """
 
 from __future__ import annotations

@@ -239,3 +239,25 @@ def test_python_refusals(dev):
                  (kc, dst, bt, cu, 2), (kc, dst, bt, cu, 1, None, vc, None), (kc, dst.transpose(0, 1), bt, cu)):
         with pytest.raises(AssertionError):
             mxfp4_kv.gather_mxfp4(*args)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_code_under_every_scale_byte(dev, dtype):
+    """Scales from 2^-127 to past the largest finite value, which is infinity, and NaN: exact in bf16 and
+    f32, subnormal results included; rounded to nearest even in fp16."""
+    cache = np.zeros((1, 256, 1, 20), np.uint8)  # row s: every code, twice, under scale byte s
+    cache[0, :, 0, :16] = np.tile(np.arange(8) * 2 | (np.arange(8) * 2 + 1) << 4, 2)
+    cache[0, :, 0, 16] = np.arange(256)
+    out = torch.zeros(256, 1, 32, dtype=dtype, device=dev)
+    mxfp4_kv.gather_mxfp4(torch.from_numpy(cache).to(dev), out, torch.zeros(1, 1, dtype=torch.int32, device=dev),
+                          torch.tensor([0, 256], dtype=torch.int32, device=dev))
+    want = M.dequantize(cache[0], 32)
+    with np.errstate(over="ignore", invalid="ignore"):
+        if dtype == torch.float16:
+            want = want.astype(np.float16).astype(np.float64)
+        else:  # (bf16 holds all of these values that float32 does)
+            want = np.where(np.abs(want) > np.finfo(np.float32).max, np.sign(want) * np.inf, want)
+    got = out.double().cpu().numpy()
+    assert np.array_equal(got, want, equal_nan=True)
+    known = ~np.isnan(want)
+    assert np.array_equal(np.signbit(got)[known], np.signbit(want)[known])
