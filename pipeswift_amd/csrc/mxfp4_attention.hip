@@ -148,8 +148,6 @@ mx4_attention_kernel(Mx4Args args) {
   constexpr int kTileShift = tile_shift(Q_DT, kSets), kTile = 1 << kTileShift, kHalves = kTile / 16;  // keys of a wave's tile
   constexpr int kStageKeys = kWaves * kTile;                                       // of a stage, a tile a wave
   constexpr uint32_t kSlot = 2 * kStageKeys * kRowBytes + 2 * kStageKeys / kUnit * kUnitGap;  // bytes of a stage
-  constexpr uint32_t kTileBytes = kTile * kRowBytes;
-  constexpr int kOwnLoads = int(kTileBytes / 4 + 63) / 64;  // dword loads of a wave's own rows of K, or of V
   constexpr int kMostChunks = kHalves == 1 ? 3 : 5;         // 16-byte loads of a wave's part of a unit
   // the stages, and half of a tile's V as bf16 a wave; at the end of a piece the waves' accumulators
   __shared__ __attribute__((aligned(1024))) char s_lds[kSlots * kSlot + kStageKeys * kHead];
