@@ -234,15 +234,7 @@ __device__ __forceinline__ int64_t wave_uniform(int64_t x) { return lane_value(x
 // x / y for 0 <= x, 0 < y, short where both fit 31 bits (they do, but for a huge step).
 __device__ __forceinline__ int64_t uniform_div(int64_t x, int64_t y) {
   if (((x | y) >> 31) == 0) return int64_t(wave_uniform(int32_t(uint32_t(x) / uint32_t(y))));
-  uint64_t q = 0, rest = 0;  // bit by bit: the compiler's division would be most of a short kernel's code
-#pragma unroll 1
-  for (int i = 62; i >= 0; --i) {
-    rest = rest << 1 | (uint64_t(x) >> i & 1);
-    const bool in = rest >= uint64_t(y);
-    rest -= in ? uint64_t(y) : 0;
-    q = q << 1 | uint64_t(in);
-  }
-  return wave_uniform(int64_t(q));
+  return wave_uniform(x / y);
 }
 
 // 64 consecutive sequences, one a lane: the lane's query rows and length, its
