@@ -75,9 +75,9 @@ struct Mx4Prefill {
   int q_dtype, out_dtype;
 };
 
-// Floats of workspace, and the launch (`a` filled in).
+// Floats of workspace (rows: `most`), and the launch (`a` filled in).
 int64_t mx4_prefill_floats(int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, int64_t num_q_heads,
-                           int64_t num_kv_heads, int64_t max_seq_len);
+                           int64_t num_kv_heads, int64_t max_seq_len, int64_t rows);
 int launch_mx4_prefill(const DecodeArgs& a, const Mx4Prefill& s, float* workspace, hipStream_t st);
 
 }  // namespace psk_detail

@@ -860,7 +860,8 @@ int64_t psk_paged_mxfp4_workspace_len(int64_t num_seqs, int64_t total_q, int64_t
     if (!s.whole) own = 4 + s.max_runs * s.row_blocks * 2 * s.hg * s.rows * kRecord;
   }
   if (r.way == kRows) return own;
-  const int64_t blocks = mx4_prefill_floats(num_seqs, total_q, max_seqlen_q, num_q_heads, num_kv_heads, max_seq_len);
+  const int64_t blocks = mx4_prefill_floats(num_seqs, total_q, max_seqlen_q, num_q_heads, num_kv_heads, max_seq_len,
+                                            r.way == kBoth ? r.row_tokens : 0);
   return std::max(own, blocks);  // (one after the other)
 }
 

@@ -58,11 +58,25 @@ struct PrefillArgs {
   const int32_t* order;   // [num_seqs]: the sequence at launch position k
   int32_t num_seqs, total_q;
   int32_t tq;             // query tokens of a block
-  int32_t splits;
+  int32_t max_blocks;
+  int32_t splits;         // workgroups that share a block's keys; 0: by the blocks that there are,
+  int32_t most_splits;    // at most so many
   int32_t out_dtype;
   double scale_log2;
   float* records;         // [blocks][kv heads][splits][kBlock][kRecord]
 };
+
+// The splits of a step of `jobs` blocks and kv heads whose longest sequence can be cut into `most`.
+__host__ __device__ constexpr int64_t splits_of(int64_t jobs, int64_t most) {
+  const int64_t n = jobs < kMostSplit ? kMostSplit / int32_t(jobs > 0 ? jobs : 1) : 1;
+  return n < most ? n : most > 1 ? most : 1;
+}
+
+// The step's blocks (max_blocks at most, whatever cu_seqlens_q says) and their splits.
+__device__ __forceinline__ int blocks_here(const PrefillArgs& p) { return min(p.blocks[p.num_seqs], p.max_blocks); }
+__device__ __forceinline__ int splits_here(const PrefillArgs& p) {
+  return p.splits > 0 ? p.splits : int(splits_of(int64_t(blocks_here(p)) * p.a.num_kv_heads, p.most_splits));
+}
 
 // The launch order of the blocks of sequences with more than `most` query tokens.
 __global__ void __launch_bounds__(1024) mx4_order_kernel(DecodeArgs a, int num_seqs, int total_q, int tq, int most,
@@ -103,7 +117,7 @@ struct Where {
   SeqRows r;
 };
 __device__ __forceinline__ bool block_of(const PrefillArgs& p, int idx, int lane, Where& w) {
-  if (idx >= p.blocks[p.num_seqs]) return false;
+  if (idx >= blocks_here(p)) return false;
   const int k = __builtin_amdgcn_readfirstlane(position_of(p.blocks, p.num_seqs, idx, lane));
   w.b = __builtin_amdgcn_readfirstlane(p.order[k]);
   // a sequence's blocks from its last (the most keys, when causal) to its first
@@ -124,7 +138,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int Hkv = a.num_kv_heads, G = a.heads;
   const int v0 = int(blockIdx.x) / Hkv, h = int(blockIdx.x) - v0 * Hkv;
-  const int idx = v0 / p.splits, split = v0 - idx * p.splits;
+  const int splits = splits_here(p), idx = v0 / splits, split = v0 - idx * splits;
   Where w;
   w.h = h;
   if (!block_of(p, idx, lane, w)) return;
@@ -134,7 +148,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
   const int key_end = limit(w.i0 + w.ni - 1);
   // this split's stages
   const int stages = (key_end + kStage - 1) / kStage;
-  const int t_from = int(int64_t(stages) * split / p.splits), t_to = int(int64_t(stages) * (split + 1) / p.splits);
+  const int t_from = int(int64_t(stages) * split / splits), t_to = int(int64_t(stages) * (split + 1) / splits);
 
   // the wave's rows: which there are, what all and any of them see
   const int row = wave * 32 + l31, ti = row / G;
@@ -327,7 +341,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 
   if (!wave_live) return;
   const float sum = l + __shfl_xor(l, 32);
-  float* rec = p.splits > 1 ? p.records + (((int64_t(idx) * Hkv + h) * p.splits + split) * kBlock + row) * kRecord : nullptr;
+  float* rec = splits > 1 ? p.records + (((int64_t(idx) * Hkv + h) * splits + split) * kBlock + row) * kRecord : nullptr;
 #pragma unroll
   for (int d = 0; d < 4; ++d) {
     const bool nan = s_nan[d] < row_lim;
@@ -356,14 +370,14 @@ __global__ void __launch_bounds__(256) mx4_prefill_merge_kernel(PrefillArgs p) {
   const int lane = int(threadIdx.x) & 63;
   const int Hkv = a.num_kv_heads;
   const int job = int(blockIdx.x) / (kBlock / 8), row = (int(blockIdx.x) - job * (kBlock / 8)) * 8 + (int(threadIdx.x) >> 5);
-  const int idx = job / Hkv, h = job - idx * Hkv;
+  const int idx = job / Hkv, h = job - idx * Hkv, splits = splits_here(p);
   Where w;
-  if (!block_of(p, idx, lane, w) || row >= w.ni * a.heads) return;
+  if (splits == 1 || !block_of(p, idx, lane, w) || row >= w.ni * a.heads) return;
   const int at4 = lane & 31;
-  const float* rec = p.records + (int64_t(job) * p.splits * kBlock + row) * kRecord;
+  const float* rec = p.records + (int64_t(job) * splits * kBlock + row) * kRecord;
   float top = kNoScore, sum = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < p.splits; ++s, rec += int64_t(kBlock) * kRecord) {
+  for (int s = 0; s < splits; ++s, rec += int64_t(kBlock) * kRecord) {
     const float m = rec[kHead], l = rec[kHead + 1];
     const f32x4 v = *reinterpret_cast<const f32x4*>(rec + 4 * at4);
     const float up = __builtin_fmaxf(top, m);
@@ -382,18 +396,44 @@ int64_t most_blocks(int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, int
   return std::min(ceil_div(total_q, tq) + num_seqs - (num_seqs > 0 ? 1 : 0), num_seqs * ceil_div(max_seqlen_q, tq));
 }
 
-int64_t splits_of(int64_t blocks, int64_t num_kv_heads, int64_t max_seq_len) {
-  const int64_t jobs = std::max<int64_t>(blocks * num_kv_heads, 1);
-  return std::max<int64_t>(1, std::min(kMostSplit / jobs, max_seq_len / kSplitKeys));
+// How a step's blocks are split.  The host's bound on the blocks counts one for each
+// sequence, also for those that go by rows (of up to `rows` query tokens); where fewer blocks
+// could be split further, their number decides on the device (splits 0): a chunk of 256
+// tokens over 32000 keys beside 31 decode sequences is 4 blocks of up to 36.
+struct Splits {
+  int64_t blocks, most, splits;
+  int64_t groups;   // workgroups of the step
+  int64_t joined;   // blocks and kv heads whose splits are joined, at most
+  int64_t records;  // of blocks and kv heads, a split each
+};
+Splits splits_for(int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, int64_t heads, int64_t num_kv_heads,
+                  int64_t max_seq_len, int64_t rows) {
+  const int64_t tq = kBlock / heads;
+  Splits s;
+  s.blocks = most_blocks(num_seqs, total_q, max_seqlen_q, tq);
+  s.most = std::min<int64_t>(max_seq_len / kSplitKeys, kMostSplit);
+  const int64_t jobs = s.blocks * num_kv_heads;
+  s.splits = splits_of(jobs, s.most);
+  s.groups = jobs * s.splits;
+  s.joined = s.splits > 1 ? jobs : 0;
+  s.records = s.splits > 1 ? s.groups : 0;
+  const int64_t least = std::max<int64_t>(ceil_div(total_q - num_seqs * rows, tq), 1) * num_kv_heads;
+  if (rows > 0 && splits_of(least, s.most) > s.splits) {
+    s.splits = 0;
+    s.records = std::min<int64_t>(jobs * s.most, kMostSplit);
+    s.groups = std::max(jobs, s.records);
+    s.joined = std::min<int64_t>(jobs, kMostSplit / 2);
+  }
+  return s;
 }
 
 int64_t order_floats(int64_t num_seqs) { return (2 * num_seqs + 1 + 3) / 4 * 4; }
 
 template <int Q_DT, bool P_PAIRS>
-int launch(const PrefillArgs& p, int64_t jobs, hipStream_t st) {
-  hipLaunchKernelGGL((mx4_prefill_kernel<Q_DT, P_PAIRS>), dim3(unsigned(jobs * p.splits)), dim3(kThreads), 0, st, p);
-  if (const int e = check_launch("mx4_prefill_kernel launch"); e != PSK_OK || p.splits == 1) return e;
-  hipLaunchKernelGGL(mx4_prefill_merge_kernel, dim3(unsigned(jobs * (kBlock / 8))), dim3(256), 0, st, p);
+int launch(const PrefillArgs& p, const Splits& s, hipStream_t st) {
+  hipLaunchKernelGGL((mx4_prefill_kernel<Q_DT, P_PAIRS>), dim3(unsigned(s.groups)), dim3(kThreads), 0, st, p);
+  if (const int e = check_launch("mx4_prefill_kernel launch"); e != PSK_OK || s.joined == 0) return e;
+  hipLaunchKernelGGL(mx4_prefill_merge_kernel, dim3(unsigned(s.joined * (kBlock / 8))), dim3(256), 0, st, p);
   return check_launch("mx4_prefill_merge_kernel launch");
 }
 
@@ -402,10 +442,9 @@ int launch(const PrefillArgs& p, int64_t jobs, hipStream_t st) {
 namespace psk_detail {
 
 int64_t mx4_prefill_floats(int64_t num_seqs, int64_t total_q, int64_t max_seqlen_q, int64_t num_q_heads,
-                           int64_t num_kv_heads, int64_t max_seq_len) {
-  const int64_t blocks = most_blocks(num_seqs, total_q, max_seqlen_q, kBlock / (num_q_heads / num_kv_heads));
-  const int64_t splits = splits_of(blocks, num_kv_heads, max_seq_len);
-  return 4 + order_floats(num_seqs) + (splits > 1 ? blocks * num_kv_heads * splits * kBlock * kRecord : 0);
+                           int64_t num_kv_heads, int64_t max_seq_len, int64_t rows) {
+  const Splits s = splits_for(num_seqs, total_q, max_seqlen_q, num_q_heads / num_kv_heads, num_kv_heads, max_seq_len, rows);
+  return 4 + order_floats(num_seqs) + s.records * kBlock * kRecord;
 }
 
 int launch_mx4_prefill(const DecodeArgs& a, const Mx4Prefill& s, float* workspace, hipStream_t st) {
@@ -416,11 +455,12 @@ int launch_mx4_prefill(const DecodeArgs& a, const Mx4Prefill& s, float* workspac
   p.tq = kBlock / a.heads;
   p.out_dtype = s.out_dtype;
   p.scale_log2 = s.scale_log2;
-  const int64_t blocks = most_blocks(s.num_seqs, s.total_q, s.max_seqlen_q, p.tq);
-  p.splits = int32_t(splits_of(blocks, a.num_kv_heads, s.max_seq_len));
-  const int64_t jobs = blocks * a.num_kv_heads;
-  if (jobs > INT32_MAX / kBlock)
-    return fail(PSK_E_ARG, "too many query blocks (%lld x %d kv heads)", (long long)blocks, int(a.num_kv_heads));
+  const Splits n = splits_for(s.num_seqs, s.total_q, s.max_seqlen_q, a.heads, a.num_kv_heads, s.max_seq_len, s.most);
+  if (n.groups > INT32_MAX / kBlock)
+    return fail(PSK_E_ARG, "too many query blocks (%lld x %d kv heads)", (long long)n.blocks, int(a.num_kv_heads));
+  p.max_blocks = int32_t(n.blocks);
+  p.splits = int32_t(n.splits);
+  p.most_splits = int32_t(n.most);
   float* ws = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
   int32_t* order = reinterpret_cast<int32_t*>(ws);
   p.blocks = order;
@@ -432,9 +472,9 @@ int launch_mx4_prefill(const DecodeArgs& a, const Mx4Prefill& s, float* workspac
   const bool pairs = s.out_dtype != PSK_DTYPE_BF16;
   switch (s.q_dtype) {
     case PSK_DTYPE_BF16:
-      return pairs ? launch<PSK_DTYPE_BF16, true>(p, jobs, st) : launch<PSK_DTYPE_BF16, false>(p, jobs, st);
-    case PSK_DTYPE_F16: return pairs ? launch<PSK_DTYPE_F16, true>(p, jobs, st) : launch<PSK_DTYPE_F16, false>(p, jobs, st);
-    default: return pairs ? launch<PSK_DTYPE_F32, true>(p, jobs, st) : launch<PSK_DTYPE_F32, false>(p, jobs, st);
+      return pairs ? launch<PSK_DTYPE_BF16, true>(p, n, st) : launch<PSK_DTYPE_BF16, false>(p, n, st);
+    case PSK_DTYPE_F16: return pairs ? launch<PSK_DTYPE_F16, true>(p, n, st) : launch<PSK_DTYPE_F16, false>(p, n, st);
+    default: return pairs ? launch<PSK_DTYPE_F32, true>(p, n, st) : launch<PSK_DTYPE_F32, false>(p, n, st);
   }
 }
 

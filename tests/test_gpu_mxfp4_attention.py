@@ -513,3 +513,30 @@ def test_blocks_of_more_sequences_than_are_ordered(dev, causal):
     (300, 1, [700, 40], [1, 3]), (520, 2, [1500, 0, 90], [2, 1, 2]), (257, 1, [5], [1]), (1000, 1, [2100], [20])])
 def test_more_query_heads_than_a_block_has_rows(dev, dtype, Hq, Hkv, lens, counts):
     _both(Case(dev, Hq, lens, counts, Hq, Hkv, 16, dtype))
+
+
+@pytest.mark.parametrize("L,n", [(3000, 200), (2600, 20)])
+def test_a_chunk_is_cut_the_same_beside_decode_sequences(dev, L, n):
+    """The bits of a chunk alone, whose blocks' keys are split over the CUs, and of the same chunk beside
+    sequences that go by rows; replayed from one graph as the step turns into other ones of its bounds."""
+    lens, counts = [L, *[40 + 13 * i for i in range(31)]], [n] + [1] * 31
+    c = Case(dev, 35, lens, counts, 8, 2, 16)
+    k, v = c.caches()
+    call = lambda: attention.paged_mxfp4_attention(c.qd, k, v, c.btd, c.lensd, c.cud, n, return_softmax_lse=True)  # noqa: E731
+    out, lse = call()
+    one, one_lse = attention.paged_mxfp4_attention(c.qd[:n], k, v, c.btd[:1], c.lensd[:1], c.cud[:2], n,
+                                                   return_softmax_lse=True)
+    assert torch.equal(out[:n], one) and torch.equal(lse[:, :n], one_lse)
+    c.check((out, lse), c.want())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for counts in ([n] + [1] * 31, [1] * 32, [n // 2 + 1] + [1] * 31, [9] * (n // 9) + [1] * (32 - n // 9)):
+        c.cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        c.rows = int(c.cu[-1])
+        c.cud.copy_(torch.from_numpy(c.cu))
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(got, c.want())
+        eager = call()
+        assert torch.equal(got[0][:c.rows], eager[0][:c.rows]) and torch.equal(got[1][:, :c.rows], eager[1][:, :c.rows])
