@@ -38,6 +38,17 @@ def _span(t):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size() - 1
 
 
+def _side_by_side(a, b):
+    """Whether [N, heads, D] tensors of one type and token stride are columns of a projection that do not
+    meet (False where it takes ``overlap`` to say)."""
+    s, size = a.stride(0), a.element_size()
+    off, rest = divmod(b.data_ptr() - a.data_ptr(), size)
+    if rest or s <= 0 or b.dim() != 3 or b.stride(0) != s:
+        return False
+    at = off % s
+    return at >= (a.shape[1] - 1) * a.stride(1) + a.shape[2] and at + (b.shape[1] - 1) * b.stride(1) + b.shape[2] <= s
+
+
 def _check_out(out, own, others, name):
     """An output is its input itself, or shares no element with any input, other output or cache."""
     assert out.shape == own.shape and out.dtype == own.dtype and out.device == own.device, \
@@ -50,7 +61,7 @@ def _check_out(out, own, others, name):
         if t is None:
             continue
         a, b = _span(t)
-        assert b < lo or hi < a or t.element_size() == out.element_size() and not overlap(out, t), \
+        assert b < lo or hi < a or t.element_size() == out.element_size() and (_side_by_side(out, t) or not overlap(out, t)), \
             f"{name} must be its input itself or share no element with the inputs, outputs and caches"
 
 

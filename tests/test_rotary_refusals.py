@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from pipeswift_amd import rotary
+from pipeswift_amd._lib import overlap
 
 
 class OnGpu(torch.Tensor):
@@ -48,3 +49,26 @@ def test_outputs_that_lie_in_a_cache(kind, name, side):
               slot_mapping=_gpu(torch.arange(4)))
     with pytest.raises(AssertionError, match=f"{name} must be its input itself or share no element"):
         rotary.norm_rope_and_cache(**x, **{name: _gpu(out)})
+
+
+def test_columns_side_by_side_do_not_overlap():
+    """What is taken for columns beside each other shares no element, and a projection's columns are."""
+    g = torch.Generator().manual_seed(1)
+    draw = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))  # noqa: E731
+    store = torch.zeros(4000, dtype=torch.bfloat16)
+    found = 0
+    for _ in range(3000):
+        s, pair = draw(8, 90), []
+        for _ in range(2):
+            n, heads, dim, gap = draw(1, 5), draw(1, 4), draw(1, 9), draw(0, 20)
+            pair.append(store[draw(0, 300):].as_strided((n, heads, dim), (s, gap, 1), store[draw(0, 300):].storage_offset()))
+        a, b = pair
+        if rotary._side_by_side(a, b):
+            found += 1
+            assert not overlap(a, b)
+    assert found > 300
+    q, k, v = torch.zeros(6, 48 * 64).split([32 * 64, 8 * 64, 8 * 64], 1)
+    q, k, v = (x.unflatten(1, (-1, 64)) for x in (q, k, v))
+    for a in (q, k, v):
+        for b in (q, k, v):
+            assert rotary._side_by_side(a, b) == (a is not b)
