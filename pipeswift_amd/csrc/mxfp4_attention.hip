@@ -19,7 +19,7 @@
 //     global_load_lds in the order of memory, into a ring of three, two stages ahead.  A
 //     row of 68 bytes lies on 4-byte boundaries only, where loads of 16 bytes to
 //     registers take a cycle a lane: 64 decode sequences took 223 us with those, 199 with
-//     dword loads to LDS by each wave for itself, and take 157 like this.
+//     dword loads to LDS by each wave for itself, and take 155-160 like this.
 //   * lane l reads a group of 32 elements, 16 bytes, of key l % 16's row at group
 //     l / 16, and its scale byte, of K and of V.
 //   * S^T = K Q^T on v_mfma_f32_16x16x32_bf16: the lane's group is its part of the A
@@ -39,7 +39,8 @@
 // joins a row's records in the order of their keys.  Short contexts are not cut.
 //
 // Bound by memory: 64 sequences of 500 to 32 thousand keys, 8 kv heads of 4 query heads,
-// read 0.67 GB in 157 us, 4.3 TB/s (the loads alone take 138), and 10 us for the merge.  A
+// read 0.67 GB in a step of 155-160 us, its merge included, 4.2-4.3 TB/s (the loads alone take 138;
+// a trace has 158 for this kernel and 9 for the merge).  A
 // step of two sequences of 150 and 200 thousand keys takes 57 + 9 us, of which about 23 are the
 // start of a run, its first loads and its end.
 //

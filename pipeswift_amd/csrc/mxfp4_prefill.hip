@@ -14,7 +14,7 @@
 //     as they stand, and ds_read_b64_tr_b16 gives V^T.  Into an fp16 or float32 out P is the sum
 //     of two fp16 (2^-22) and P V runs twice.  Into a bf16 out P is rounded once (2^-11): the
 //     error against 64 bits is 1.669e-3 of the values so, 1.658e-3 by the output's rounding
-//     alone, and the second product would take 1470 us instead of 1060 for the chunk below.
+//     alone, and the second product takes 1410 us instead of 1050 for the chunk below.
 //     (One rounding into fp16 left 2.8e-4 where the output's own is 2.1e-4.)
 // V is exact in fp16 where its scales lie in [2^-23, 2^13]; a block that meets another
 // one is computed again with V as bf16 and P as the sum of two bf16 (2^-17).
@@ -22,8 +22,8 @@
 // largest, so that the common path has no rescale.
 //
 // Bound by the matrix cores and the softmax's vector work in turn: a chunk of 2048 tokens over
-// 30000 keys (32 heads over 8) takes 1040 us, 1.0 PFLOP/s of the 1.2 of a large product; 8 prompts of 100 to
-// 4000 tokens 472 us, 790 TFLOP/s.  Both halves of a stage at once need more registers than there
+// 30000 keys (32 heads over 8) takes 1050 us, 1.0 PFLOP/s where large products reach 1.2 (8192^3) to
+// 1.35 (16384^3); 8 prompts of 100 to 4000 tokens 474 us, 790 TFLOP/s.  Both halves of a stage at once need more registers than there
 // are (1640 us); wave priorities around the products gain nothing.
 //
 // Where the blocks are fewer than the CUs, a block's keys are split over several
